@@ -1,4 +1,4 @@
-"""Build the HIP C-ABI library ``libmi355_fa.so`` in-tree for gfx950.
+"""Build the HIP C-ABI libraries ``libmi355_fa.so`` and ``libmi355_serve.so`` in-tree for gfx950.
 
 hipcc cross-compiles without a GPU, so this runs on any host with ROCm.
 Usage: ``python -m custom_ops_amd.build`` (or ``__graft_entry__.build()``).
@@ -49,14 +49,18 @@ def hipcc() -> str:
     raise RuntimeError("hipcc not found (expected /opt/rocm/bin/hipcc)")
 
 
-def compile_checked(out_path: str, flags=None, verbose: bool = False) -> str:
-    """Compile SRC into ``out_path`` (atomically) after checking the device
+SERVE_SRC = os.path.join(PKG_DIR, "csrc", "serve.hip")   # the serving operators' library
+SERVE_LIB_PATH = os.path.join(PKG_DIR, "libmi355_serve.so")
+
+
+def compile_checked(out_path: str, flags=None, verbose: bool = False, src: str = SRC) -> str:
+    """Compile ``src`` into ``out_path`` (atomically) after checking the device
     assembly of that same compilation; raise RuntimeError on either failure."""
     from .isa_check import missed_occupancy, violations
     flags = list(HIPCC_FLAGS if flags is None else flags)
     with tempfile.TemporaryDirectory(prefix="mi355fa-build-") as tmp:
         product = os.path.join(tmp, os.path.basename(out_path))
-        cmd = [hipcc(), *flags, f"-I{INCLUDE}", SRC, "-o", product, "-save-temps=obj"]
+        cmd = [hipcc(), *flags, f"-I{INCLUDE}", src, "-o", product, "-save-temps=obj"]
         if verbose:
             print(" ".join(cmd), flush=True)
         res = subprocess.run(cmd, capture_output=True, text=True, cwd=tmp)
@@ -90,12 +94,17 @@ TORCH_BINDING_PATH = os.path.join(PKG_DIR, "libmi355_fa_torch.so")
 OPS_PATH = os.path.join(PKG_DIR, "libmi355_fa_ops.so")   # the same source, implementation only
 
 
-def ops_stamp() -> str:
+SERVE_BINDING_SRC = os.path.join(PKG_DIR, "csrc", "serve_binding.cpp")
+SERVE_OPS_PATH = os.path.join(PKG_DIR, "libmi355_serve_ops.so")
+_BINDING_HEADER = {TORCH_BINDING_SRC: "mi355_fa.h", SERVE_BINDING_SRC: "mi355_serve.h"}
+
+
+def ops_stamp(binding: str = TORCH_BINDING_SRC) -> str:
     """What a compiled operator implementation has to be built from: its sources
     and the PyTorch it runs in. The file holds this text (csrc/torch_binding.cpp)."""
     import torch
     h = hashlib.sha256()
-    for src in (TORCH_BINDING_SRC, os.path.join(INCLUDE, "mi355_fa.h")):
+    for src in (binding, os.path.join(INCLUDE, _BINDING_HEADER[binding])):
         with open(src, "rb") as f:
             h.update(f.read())
     return f"mi355-ops {h.hexdigest()} torch {torch.__version__};"
@@ -112,15 +121,15 @@ def ops_stamp_of(path: str) -> str | None:
     return found.group().decode(errors="replace") if found else None
 
 
-def ops_current(path: str) -> bool:
+def ops_current(path: str, binding: str = TORCH_BINDING_SRC) -> bool:
     """Whether the file was built from the present sources for this PyTorch."""
     try:
-        return ops_stamp_of(path) == ops_stamp()
+        return ops_stamp_of(path) == ops_stamp(binding)
     except OSError:      # no sources to compare with
         return False
 
 
-def _compile_binding(path: str, extra: list, verbose: bool) -> str:
+def _compile_binding(path: str, extra: list, verbose: bool, src: str = TORCH_BINDING_SRC) -> str:
     import torch
     tdir = os.path.dirname(torch.__file__)
     abi = int(torch.compiled_with_cxx11_abi())
@@ -128,7 +137,7 @@ def _compile_binding(path: str, extra: list, verbose: bool) -> str:
     cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__",
            f"-D_GLIBCXX_USE_CXX11_ABI={abi}", f"-I{tdir}/include",
            f"-I{tdir}/include/torch/csrc/api/include", "-I/opt/rocm/include", f"-I{INCLUDE}",
-           TORCH_BINDING_SRC, "-o", path + ".tmp",
+           src, "-o", path + ".tmp",
            f"-L{tdir}/lib", "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip",
            "-L/opt/rocm/lib", "-lamdhip64", *extra]
     if verbose:
@@ -156,11 +165,25 @@ def build_torch_binding(verbose: bool = False) -> str:
     return TORCH_BINDING_PATH
 
 
+def build_serve_ops(path: str = SERVE_OPS_PATH, verbose: bool = False) -> str:
+    """Compile the serving operators' implementation over their library's C ABI."""
+    return _compile_binding(path, [f'-DMI355_OPS_STAMP="{ops_stamp(SERVE_BINDING_SRC)}"', "-ldl"], verbose,
+                            SERVE_BINDING_SRC)
+
+
+def build_serve(verbose: bool = False) -> str:
+    """Compile the serving operators' library and its binding; return the library's path."""
+    out = compile_checked(SERVE_LIB_PATH, verbose=verbose, src=SERVE_SRC)
+    build_serve_ops(verbose=verbose)
+    return out
+
+
 def build(verbose: bool = False) -> str:
-    """Compile the library (always recompiles) and the C++ torch binding over
-    it; return the library's path."""
+    """Compile the libraries (always recompiles) and the C++ torch bindings over
+    them; return the attention library's path."""
     out = compile_checked(LIB_PATH, verbose=verbose)
     build_torch_binding(verbose=verbose)
+    build_serve(verbose=verbose)
     return out
 
 

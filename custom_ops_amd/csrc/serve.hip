@@ -1,0 +1,321 @@
+// serve.hip — the serving operators for MI355X (gfx950 / CDNA4): attention over
+// packed sequences, one-token attention over a paged key-value cache, rotary
+// positions with the write into that cache, and the cache's layout. C ABI in
+// include/mi355_serve.h; each operator's kernels and their reasons in its header.
+
+#include <hip/hip_runtime.h>
+
+#include <limits.h>
+#include <math.h>
+#include <stdarg.h>
+#include <stdint.h>
+#include <stdio.h>
+#include <string.h>
+
+#include <algorithm>
+#include <mutex>
+#include <type_traits>
+
+#include "mi355_serve.h"
+#include "gfx950.h"
+
+namespace mi355fa {
+namespace {
+
+#include "packed_fwd.h"
+#include "paged_decode.h"
+#include "rope_store.h"
+#include "paged_layout.h"
+
+// ── host side ─────────────────────────────────────────────────────────────────
+
+struct Err {
+  char* text;
+  size_t len;
+  __attribute__((format(printf, 3, 4))) int fail(int rc, const char* fmt, ...) const {
+    if (text && len) {
+      va_list ap;
+      va_start(ap, fmt);
+      vsnprintf(text, len, fmt, ap);
+      va_end(ap);
+    }
+    return rc;
+  }
+};
+
+struct Device {
+  int cus = 0;
+  bool gfx950 = false;
+};
+
+Device device_info() {
+  static Device known[64];
+  static std::mutex mu;
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) {
+    (void)hipGetLastError();
+    return Device{256, false};
+  }
+  std::lock_guard<std::mutex> lk(mu);
+  Device& d = known[dev];
+  if (!d.cus) {
+    int n = 0;
+    d.cus = hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && n > 0 ? n : 256;
+    hipDeviceProp_t prop;
+    d.gfx950 = hipGetDeviceProperties(&prop, dev) == hipSuccess && strncmp(prop.gcnArchName, "gfx950", 6) == 0;
+    (void)hipGetLastError();
+  }
+  return d;
+}
+
+// Restores the launch error state around one launch and names what failed.
+int launched(const Err& err, const char* what) {
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return err.fail(MI355_SERVE_ELAUNCH, "%s: launch failed: %s", what, hipGetErrorString(e));
+  return MI355_SERVE_OK;
+}
+
+bool rows_ok(const void* p, std::initializer_list<int64_t> strides) {
+  int64_t x = (int64_t)(uintptr_t)p & 15;
+  for (int64_t s : strides) x |= s & 7;
+  return x == 0;
+}
+
+bool window_ok(int w) { return w >= 0; }
+constexpr int kNoWindow = 1 << 30;
+int window_of(int w) { return w == 0 ? kNoWindow : std::min(w, kNoWindow); }
+
+// The factors of a call's scores (PackedArgs, DecodeArgs); false where scale or
+// softcap is none the kernels can work with.
+constexpr float kMaxSoftcap = 1000.f;   // above, 2·softcap·2^-24 of a score is lost to the tanh's rounding
+template <class A> bool score_factors(A& a, float scale, float softcap) {
+  if (!(scale > 0.f) || isinf(scale) || !(softcap >= 0.f) || softcap > kMaxSoftcap) return false;
+  const bool cap = softcap > 0.f;
+  a.u_scale = cap ? 2.f * kLog2e * scale / softcap : 0.f;
+  a.c2 = cap ? 2.f * softcap * kLog2e : scale * kLog2e;
+  a.bias = cap ? -0.5f / softcap : -1.f / scale;
+  return std::isfinite(a.u_scale) && std::isfinite(a.c2) && a.c2 > 0.f && std::isfinite(a.bias) &&
+         std::isfinite(kSlackLog2 / a.c2);
+}
+
+const char* kScoresText = "scale must be positive and finite, softcap 0 (none) or in (0, 1000]";
+
+// f(integral_constant...) for the runtime values of (d, bf16, cap, bias)
+template <class F> void by_type(int d, bool bf16, F f) {
+  typedef std::integral_constant<int, 64> D64;
+  typedef std::integral_constant<int, 128> D128;
+  if (d == 64) bf16 ? f(D64{}, std::true_type{}) : f(D64{}, std::false_type{});
+  else bf16 ? f(D128{}, std::true_type{}) : f(D128{}, std::false_type{});
+}
+template <class F> void by_scores(bool cap, bool bias, F f) {
+  if (cap) bias ? f(std::true_type{}, std::true_type{}) : f(std::true_type{}, std::false_type{});
+  else bias ? f(std::false_type{}, std::true_type{}) : f(std::false_type{}, std::false_type{});
+}
+
+int check_heads(const Err& err, int h, int hk, int d, int dtype) {
+  if (dtype != MI355_SERVE_FP16 && dtype != MI355_SERVE_BF16)
+    return err.fail(MI355_SERVE_EINVAL, "q must be float16 or bfloat16");
+  if (d != 64 && d != 128) return err.fail(MI355_SERVE_EINVAL, "Only head_dim=64 or head_dim=128 is supported");
+  if (hk <= 0 || h < 0 || h % hk) return err.fail(MI355_SERVE_EINVAL, "n_heads must be divisible by n_kv_heads (GQA)");
+  return MI355_SERVE_OK;
+}
+
+constexpr int kMaxRows = 1 << 30;
+constexpr int64_t kMaxRowStride = 1 << 24;   // 64 rows of it stay below 2^31 bytes
+
+int packed_fwd(const mi355_packed_params* p, hipStream_t st, const Err& err) {
+  if (!p) return err.fail(MI355_SERVE_EINVAL, "params must not be NULL");
+  if (int rc = check_heads(err, p->h, p->h_k, p->d, p->dtype)) return rc;
+  if (p->total_q < 0 || p->total_k < 0 || p->n_seqs < 0 || p->total_q > kMaxRows || p->total_k > kMaxRows || p->n_seqs > kMaxRows)
+    return err.fail(MI355_SERVE_EINVAL, "total_q, total_k and n_seqs must be in 0 .. 2^30");
+  if (!window_ok(p->window)) return err.fail(MI355_SERVE_EINVAL, "window must be 0 (none) or positive");
+  PackedArgs a{};
+  if (!score_factors(a, p->scale, p->softcap)) return err.fail(MI355_SERVE_EINVAL, "%s", kScoresText);
+  if (p->total_q == 0 || p->h == 0) return MI355_SERVE_OK;
+  if (!p->q || !p->o || !p->cu_q || !p->cu_k || (p->total_k > 0 && (!p->k || !p->v)))
+    return err.fail(MI355_SERVE_EINVAL, "tensor pointer is NULL");
+  if (!rows_ok(p->q, {p->q_token_stride, p->q_head_stride}) || !rows_ok(p->k, {p->k_token_stride, p->k_head_stride}) ||
+      !rows_ok(p->v, {p->v_token_stride, p->v_head_stride}) || !rows_ok(p->o, {p->o_token_stride, p->o_head_stride}))
+    return err.fail(MI355_SERVE_EINVAL, "q/k/v/o must be 16-byte aligned with strides that are multiples of 8 elements");
+  for (int64_t s : {p->q_token_stride, p->k_token_stride, p->v_token_stride, p->o_token_stride})
+    if (s < 0 || s >= kMaxRowStride) return err.fail(MI355_SERVE_EINVAL, "token strides must be in 0 .. 2^24 elements");
+  const Device dev = device_info();
+  if (!dev.gfx950) return err.fail(MI355_SERVE_EDEVICE, "mi355_serve: current HIP device is not gfx950 (MI355X)");
+
+  a.q = (const uint16_t*)p->q; a.k = (const uint16_t*)p->k; a.v = (const uint16_t*)p->v; a.o = (uint16_t*)p->o;
+  a.cu_q = p->cu_q; a.cu_k = p->cu_k; a.prefix = p->prefix_lens; a.slopes = p->slopes;
+  a.q_ts = p->q_token_stride; a.q_hs = p->q_head_stride; a.k_ts = p->k_token_stride; a.k_hs = p->k_head_stride;
+  a.v_ts = p->v_token_stride; a.v_hs = p->v_head_stride; a.o_ts = p->o_token_stride; a.o_hs = p->o_head_stride;
+  a.tq = p->total_q; a.tk = p->total_k; a.n = p->n_seqs; a.h = p->h; a.ratio = p->h / p->h_k;
+  a.causal = p->causal != 0; a.window = window_of(p->window);
+  // 256 rows a workgroup where those fill the chip, else 128
+  const int waves = ((int64_t)p->total_q / 256 + 1) * p->h >= dev.cus ? 8 : 4;
+  const int64_t blocks = (int64_t)p->total_q / (32 * waves) + p->n_seqs + 2, total = blocks * p->h;
+  if (total >= (1LL << 31)) return err.fail(MI355_SERVE_EINVAL, "problem too large: %lld workgroups", (long long)total);
+  a.blocks = (int)blocks;
+  by_type(p->d, p->dtype == MI355_SERVE_BF16, [&](auto d, auto bf) {
+    by_scores(p->softcap > 0.f, p->slopes != nullptr, [&](auto cap, auto bias) {
+      constexpr int D = decltype(d)::value;
+      if (waves == 8) packed_fwd_kernel<D, decltype(bf)::value, decltype(cap)::value, decltype(bias)::value, 8><<<dim3((unsigned)total), dim3(512), 0, st>>>(a);
+      else packed_fwd_kernel<D, decltype(bf)::value, decltype(cap)::value, decltype(bias)::value, 4><<<dim3((unsigned)total), dim3(256), 0, st>>>(a);
+    });
+  });
+  return launched(err, "mha_packed_fwd");
+}
+
+struct DecodePlan {
+  int groups, splits;
+  size_t bytes;
+};
+
+DecodePlan decode_plan(const mi355_decode_params* p, int cus) {
+  DecodePlan pl{};
+  const int ratio = p->h / p->h_k;
+  pl.groups = (ratio + kDecHeads - 1) / kDecHeads;
+  const int64_t units = (int64_t)p->b * p->h_k * pl.groups;
+  const int64_t tiles = ((int64_t)p->table_cols * p->page_size + kDecTile - 1) / kDecTile;
+  // two workgroups of four waves run on a CU; a split of its own for every 4 tiles at least
+  const int64_t most = std::max<int64_t>(1, tiles / kDecWaves);
+  pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>({most, 2LL * cus / std::max<int64_t>(1, units), 128}));
+  if (pl.splits > 1) pl.bytes = (size_t)pl.splits * p->b * p->h * (p->d + 2) * 4;
+  return pl;
+}
+
+int decode_check(const mi355_decode_params* p, const Err& err) {
+  if (!p) return err.fail(MI355_SERVE_EINVAL, "params must not be NULL");
+  if (int rc = check_heads(err, p->h, p->h_k, p->d, p->dtype)) return rc;
+  if (p->b < 0 || p->num_pages < 0 || p->table_cols < 0) return err.fail(MI355_SERVE_EINVAL, "negative dimension");
+  if (p->page_size < 8 || p->page_size > 1024 || (p->page_size & (p->page_size - 1)))
+    return err.fail(MI355_SERVE_EINVAL, "page_size must be a power of two in 8 .. 1024");
+  if (!window_ok(p->window)) return err.fail(MI355_SERVE_EINVAL, "window must be 0 (none) or positive");
+  return MI355_SERVE_OK;
+}
+
+int paged_decode(const mi355_decode_params* p, hipStream_t st, const Err& err) {
+  if (int rc = decode_check(p, err)) return rc;
+  DecodeArgs a{};
+  if (!score_factors(a, p->scale, p->softcap)) return err.fail(MI355_SERVE_EINVAL, "%s", kScoresText);
+  if (p->b == 0 || p->h == 0) return MI355_SERVE_OK;
+  if (!p->q || !p->o || !p->kv_lens || (p->table_cols > 0 && !p->block_table) || (p->num_pages > 0 && (!p->k_cache || !p->v_cache)))
+    return err.fail(MI355_SERVE_EINVAL, "tensor pointer is NULL");
+  if (!rows_ok(p->q, {p->q_batch_stride, p->q_head_stride}) || !rows_ok(p->o, {}) ||
+      !rows_ok(p->k_cache, {p->k_page_stride, p->k_head_stride, p->k_row_stride}) ||
+      !rows_ok(p->v_cache, {p->v_page_stride, p->v_head_stride, p->v_row_stride}))
+    return err.fail(MI355_SERVE_EINVAL, "q and the caches must be 16-byte aligned with strides that are multiples of 8 elements");
+  const Device dev = device_info();
+  if (!dev.gfx950) return err.fail(MI355_SERVE_EDEVICE, "mi355_serve: current HIP device is not gfx950 (MI355X)");
+  const DecodePlan pl = decode_plan(p, dev.cus);
+  if (pl.bytes && (!p->workspace || p->workspace_bytes < pl.bytes || ((uintptr_t)p->workspace & 15)))
+    return err.fail(MI355_SERVE_EWORKSPACE, "workspace of %zu bytes needed (16-byte aligned), got %zu", pl.bytes, p->workspace_bytes);
+  a.q = (const uint16_t*)p->q; a.k = (const uint16_t*)p->k_cache; a.v = (const uint16_t*)p->v_cache; a.o = (uint16_t*)p->o;
+  a.table = p->block_table; a.lens = p->kv_lens; a.slopes = p->slopes;
+  a.q_bs = p->q_batch_stride; a.q_hs = p->q_head_stride; a.o_bs = p->o_batch_stride; a.o_hs = p->o_head_stride;
+  a.kp = p->k_page_stride; a.kh = p->k_head_stride; a.kr = p->k_row_stride;
+  a.vp = p->v_page_stride; a.vh = p->v_head_stride; a.vr = p->v_row_stride; a.ts = p->table_stride;
+  a.b = p->b; a.h = p->h; a.hk = p->h_k; a.ratio = p->h / p->h_k; a.groups = pl.groups;
+  a.pages = p->num_pages; a.shift = __builtin_ctz((unsigned)p->page_size);
+  a.cols = p->num_pages > 0 ? p->table_cols : 0;   // no pages: nothing is seen
+  a.window = window_of(p->window); a.splits = pl.splits;
+  a.part_o = (float*)p->workspace;
+  a.part_ml = a.part_o + (size_t)pl.splits * p->b * p->h * p->d;
+  const int64_t total = (int64_t)p->b * p->h_k * pl.groups * pl.splits;
+  if (total >= (1LL << 31) || (int64_t)p->b * p->h >= (1LL << 31))
+    return err.fail(MI355_SERVE_EINVAL, "problem too large: %lld workgroups", (long long)total);
+  by_type(p->d, p->dtype == MI355_SERVE_BF16, [&](auto d, auto bf) {
+    constexpr int D = decltype(d)::value;
+    by_scores(p->softcap > 0.f, p->slopes != nullptr, [&](auto cap, auto bias) {
+      paged_decode_kernel<D, decltype(bf)::value, decltype(cap)::value, decltype(bias)::value><<<dim3((unsigned)total), dim3(64 * kDecWaves), 0, st>>>(a);
+    });
+    if (pl.splits > 1) paged_join_kernel<D, decltype(bf)::value><<<dim3((unsigned)(p->b * p->h)), dim3(D), 0, st>>>(a);
+  });
+  return launched(err, "mha_paged_decode");
+}
+
+int rope_store(const mi355_rope_params* p, hipStream_t st, const Err& err) {
+  if (!p) return err.fail(MI355_SERVE_EINVAL, "params must not be NULL");
+  if (int rc = check_heads(err, p->h, p->h_k, p->d, p->dtype)) return rc;
+  if (p->t < 0 || p->num_pages < 0 || p->t > kMaxRows) return err.fail(MI355_SERVE_EINVAL, "t and num_pages must be in 0 .. 2^30");
+  if (p->rot < 0 || p->rot > p->d || p->rot % 16) return err.fail(MI355_SERVE_EINVAL, "rot must be a multiple of 16 in 0 .. head_dim");
+  if (p->page_size < 1) return err.fail(MI355_SERVE_EINVAL, "page_size must be positive");
+  if (!std::isfinite(p->amplitude)) return err.fail(MI355_SERVE_EINVAL, "amplitude must be finite");
+  if (p->t == 0) return MI355_SERVE_OK;
+  if (!p->q || !p->k || !p->v || !p->q_out || !p->k_out || !p->positions || !p->slot_map || (p->rot > 0 && !p->inv_freq) ||
+      (p->num_pages > 0 && (!p->k_cache || !p->v_cache)))
+    return err.fail(MI355_SERVE_EINVAL, "tensor pointer is NULL");
+  if (!rows_ok(p->q, {p->q_token_stride, p->q_head_stride}) || !rows_ok(p->k, {p->k_token_stride, p->k_head_stride}) ||
+      !rows_ok(p->v, {p->v_token_stride, p->v_head_stride}) || !rows_ok(p->q_out, {p->qo_token_stride, p->qo_head_stride}) ||
+      !rows_ok(p->k_out, {p->ko_token_stride, p->ko_head_stride}) ||
+      !rows_ok(p->k_cache, {p->kc_page_stride, p->kc_head_stride, p->kc_row_stride}) ||
+      !rows_ok(p->v_cache, {p->vc_page_stride, p->vc_head_stride, p->vc_row_stride}))
+    return err.fail(MI355_SERVE_EINVAL, "q/k/v, outputs and caches must be 16-byte aligned with strides that are multiples of 8 elements");
+  if (!device_info().gfx950) return err.fail(MI355_SERVE_EDEVICE, "mi355_serve: current HIP device is not gfx950 (MI355X)");
+  RopeArgs a{};
+  a.q = (const uint16_t*)p->q; a.k = (const uint16_t*)p->k; a.v = (const uint16_t*)p->v;
+  a.qo = (uint16_t*)p->q_out; a.ko = (uint16_t*)p->k_out; a.kc = (uint16_t*)p->k_cache; a.vc = (uint16_t*)p->v_cache;
+  a.positions = p->positions; a.inv_freq = p->inv_freq; a.slots = p->slot_map;
+  a.q_ts = p->q_token_stride; a.q_hs = p->q_head_stride; a.k_ts = p->k_token_stride; a.k_hs = p->k_head_stride;
+  a.v_ts = p->v_token_stride; a.v_hs = p->v_head_stride; a.qo_ts = p->qo_token_stride; a.qo_hs = p->qo_head_stride;
+  a.ko_ts = p->ko_token_stride; a.ko_hs = p->ko_head_stride;
+  a.kc_ps = p->kc_page_stride; a.kc_hs = p->kc_head_stride; a.kc_rs = p->kc_row_stride;
+  a.vc_ps = p->vc_page_stride; a.vc_hs = p->vc_head_stride; a.vc_rs = p->vc_row_stride;
+  a.num_slots = (int64_t)p->num_pages * p->page_size;
+  a.t = p->t; a.h = p->h; a.hk = p->h_k; a.rot = p->rot; a.page = p->page_size; a.amplitude = p->amplitude;
+  by_type(p->d, p->dtype == MI355_SERVE_BF16, [&](auto d, auto bf) {
+    constexpr int D = decltype(d)::value;
+    constexpr bool BF = decltype(bf)::value;
+    if (p->interleaved) rope_store_kernel<D, BF, true, 1><<<dim3((unsigned)p->t), dim3(256), 0, st>>>(a);
+    else rope_store_kernel<D, BF, false, 1><<<dim3((unsigned)p->t), dim3(256), 0, st>>>(a);
+  });
+  return launched(err, "rope_paged_store");
+}
+
+int paged_layout(const mi355_layout_params* p, hipStream_t st, const Err& err) {
+  if (!p) return err.fail(MI355_SERVE_EINVAL, "params must not be NULL");
+  if (p->n < 0 || p->n > MI355_SERVE_MAX_REQUESTS) return err.fail(MI355_SERVE_EINVAL, "at most %d requests", MI355_SERVE_MAX_REQUESTS);
+  if (p->table_cols < 0 || p->n_free < 0 || p->max_tokens < 0) return err.fail(MI355_SERVE_EINVAL, "negative dimension");
+  if (p->page_size < 1) return err.fail(MI355_SERVE_EINVAL, "page_size must be positive");
+  if (!p->cu_new || !p->counts || (p->n > 0 && (!p->seq_lens || !p->new_lens || !p->kv_lens)) ||
+      (p->n > 0 && p->table_cols > 0 && (!p->block_table || !p->table)) || (p->n_free > 0 && !p->free_pages) ||
+      (p->max_tokens > 0 && (!p->positions || !p->slot_map)))
+    return err.fail(MI355_SERVE_EINVAL, "tensor pointer is NULL");
+  const Device dev = device_info();
+  if (!dev.gfx950) return err.fail(MI355_SERVE_EDEVICE, "mi355_serve: current HIP device is not gfx950 (MI355X)");
+  LayoutArgs a{};
+  a.seq = p->seq_lens; a.fresh = p->new_lens; a.table_in = p->block_table; a.free_pages = p->free_pages;
+  a.kv_lens = p->kv_lens; a.cu = p->cu_new; a.positions = p->positions; a.slots = p->slot_map; a.table = p->table; a.counts = p->counts;
+  a.ts = p->table_stride; a.n = p->n; a.cols = p->table_cols; a.n_free = p->n_free; a.page = p->page_size; a.max_tokens = p->max_tokens;
+  const int64_t items = std::max((int64_t)p->n * p->table_cols, (int64_t)p->max_tokens);
+  const int64_t wgs = std::max<int64_t>(1, std::min<int64_t>((items + kLayoutThreads - 1) / kLayoutThreads, 2LL * dev.cus));
+  paged_layout_kernel<<<dim3((unsigned)wgs), dim3(kLayoutThreads), (size_t)(2 * p->n + 1) * 4, st>>>(a);
+  return launched(err, "paged_layout");
+}
+
+}  // namespace
+}  // namespace mi355fa
+
+extern "C" {
+
+int mi355_serve_abi_version(void) { return MI355_SERVE_ABI_VERSION; }
+
+int mi355_packed_fwd(const mi355_packed_params* p, void* stream, char* err, size_t errlen) {
+  return mi355fa::packed_fwd(p, (hipStream_t)stream, {err, errlen});
+}
+
+size_t mi355_paged_decode_workspace_bytes(const mi355_decode_params* p) {
+  if (mi355fa::decode_check(p, {nullptr, 0}) || p->b == 0 || p->h == 0) return 0;
+  return mi355fa::decode_plan(p, mi355fa::device_info().cus).bytes;
+}
+
+int mi355_paged_decode(const mi355_decode_params* p, void* stream, char* err, size_t errlen) {
+  return mi355fa::paged_decode(p, (hipStream_t)stream, {err, errlen});
+}
+
+int mi355_rope_paged_store(const mi355_rope_params* p, void* stream, char* err, size_t errlen) {
+  return mi355fa::rope_store(p, (hipStream_t)stream, {err, errlen});
+}
+
+int mi355_paged_layout(const mi355_layout_params* p, void* stream, char* err, size_t errlen) {
+  return mi355fa::paged_layout(p, (hipStream_t)stream, {err, errlen});
+}
+
+}  // extern "C"

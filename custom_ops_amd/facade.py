@@ -28,11 +28,17 @@ from typing import Optional
 
 import torch
 
-from .loader import CustomOpsError, FAOps
+from . import serve
+from .loader import CustomOpsError, FAOps, ServeOps
 
 # group name -> loader class; operator name -> group name
-GROUP_LOADERS = {"fa": FAOps}
-OP_GROUPS = {"mha_fwd_with_mask": "fa"}
+GROUP_LOADERS = {"fa": FAOps, "serve": ServeOps}
+OP_GROUPS = {"mha_fwd_with_mask": "fa", **{name: "serve" for name in serve.SCHEMAS}}
+
+# Groups that calls naming no group stand for: the reference's. The others load by
+# name or at their operators' first call, and appear in ``ops.groups`` from then on,
+# so a program that uses the attention alone deploys and reports it alone.
+_DEFAULT_GROUPS = ("fa",)
 
 _BACKENDS = ("auto", "cuda", "hip")
 
@@ -83,7 +89,7 @@ class _Slot:
 
 
 class RecsysOps:
-    """Facade over the operator groups (one group, ``fa``, in this build)."""
+    """Facade over the operator groups: the reference's ``fa``, and ``serve``."""
 
     def __init__(self, *, allow_jit: bool = True) -> None:
         self._mu = threading.RLock()
@@ -154,12 +160,12 @@ class RecsysOps:
         return self
 
     def ensure_loaded(self, *groups: str) -> "RecsysOps":
-        """Load the named groups (all when none is named). Unknown names are
-        rejected before anything loads."""
+        """Load the named groups (the reference's when none is named). Unknown names
+        are rejected before anything loads."""
         with self._mu:
             for g in groups:
                 self._slot(g)
-            for g in groups or tuple(self._slots):
+            for g in groups or _DEFAULT_GROUPS:
                 self._acquire(g)
         return self
 
@@ -168,9 +174,11 @@ class RecsysOps:
 
     @property
     def groups(self) -> dict:
-        """``{group: "loaded" | "failed" | "not_loaded"}``."""
+        """``{group: "loaded" | "failed" | "not_loaded"}``, of the reference's groups and
+        those beside them that were asked for."""
         with self._mu:
-            return {name: slot.state for name, slot in self._slots.items()}
+            return {name: slot.state for name, slot in self._slots.items()
+                    if name in _DEFAULT_GROUPS or slot.loader is not None}
 
     def is_available(self, group: Optional[str] = None) -> bool:
         """Whether the named group (else the facade as a whole) can run.
@@ -225,6 +233,73 @@ class RecsysOps:
         if not slot.ready:
             self._acquire("fa")
         return torch.ops.recsys_ops.mha_fwd_with_mask(q, k, v, mask)
+
+    def _serve(self, backend: Optional[str]):
+        """The dispatcher's operators, with the group ``serve`` loaded."""
+        if backend is not None or "CUSTOM_OPS_BACKEND" in os.environ:
+            resolve_backend(backend)
+        slot = self._slots["serve"]
+        if not slot.ready:
+            self._acquire("serve")
+        return torch.ops.recsys_ops
+
+    def mha_packed_fwd(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor,
+                       causal: bool = True, scale: Optional[float] = None, softcap: float = 0.0, window: int = 0,
+                       slopes: Optional[torch.Tensor] = None, prefix_lens: Optional[torch.Tensor] = None,
+                       backend: Optional[str] = None) -> torch.Tensor:
+        """Attention over packed sequences; rows of different sequences do not see each other.
+
+        q [Tq,H,d], k/v [Tk,Hk,d] (fp16/bf16, H % Hk == 0, d in {64, 128}; views whose
+        strides are multiples of 8 elements do); cu_q/cu_k [N+1] int32: sequence n's
+        rows and keys, ascending. Position: the last row stands at the last key. Row i sees key j
+        if j <= i (causal) and |i - j| < window (window > 0), and sees the first
+        prefix_lens[n] keys in any case. Scores: scale·q·k (default 1/sqrt(d)), then
+        softcap·tanh(s/softcap), then - slopes[h]·|i - j| (slopes [H] float32). A row
+        that sees no key, and one of no sequence, gives 0. Returns [Tq,H,d]."""
+        return self._serve(backend).mha_packed_fwd(q, k, v, cu_q, cu_k, causal, scale, softcap, window, slopes, prefix_lens)
+
+    def mha_paged_decode(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                         kv_lens: torch.Tensor, scale: Optional[float] = None, softcap: float = 0.0, window: int = 0,
+                         slopes: Optional[torch.Tensor] = None, backend: Optional[str] = None) -> torch.Tensor:
+        """Attention of one new token per request over a paged cache that holds it.
+
+        q [B,H,d]; caches [pages,Hk,page_size,d], page_size a power of two in 8 .. 1024;
+        block_table [B,M] int32; kv_lens [B] int32, the new token among them. Scores as
+        in ``mha_packed_fwd``, for the row at the last key. A page number outside the
+        cache hides its keys; a request that sees no key gives 0. Returns [B,H,d]."""
+        return self._serve(backend).mha_paged_decode(q, k_cache, v_cache, block_table, kv_lens, scale, softcap, window, slopes)
+
+    def rope_paged_store(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+                         inv_freq: torch.Tensor, slot_map: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                         interleaved: bool = False, amplitude: float = 1.0, backend: Optional[str] = None):
+        """Rotary positions of q and k, and the turned k and v into a paged cache.
+
+        q [T,H,d], k/v [T,Hk,d] (views do, as above); positions [T] int32; inv_freq
+        [rot/2] float64 radians per position (see ``rotary_frequencies``), rot a multiple
+        of 16 up to d; slot_map [T] int64, slot = page·page_size + row, one outside the
+        cache (-1) stores nothing, two tokens of a call may not share one. Pairs are
+        elements (i, i + rot/2), or (2i, 2i + 1) if interleaved. Writes the caches
+        [pages,Hk,page_size,d] in place; returns the turned (q, k), contiguous."""
+        return self._serve(backend).rope_paged_store(q, k, v, positions, inv_freq, slot_map, k_cache, v_cache, interleaved,
+                                                     amplitude)
+
+    def paged_layout(self, seq_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor,
+                     free_pages: torch.Tensor, page_size: int, max_tokens: int, backend: Optional[str] = None):
+        """Page tables, slots and positions of a step, from the requests' lengths.
+
+        seq_lens/new_lens [N] int32 (N <= 8192): tokens cached and to add; block_table
+        [N,M] int32: the pages held; free_pages [F] int32: requests take the pages they
+        lack from its front, in order. Returns ``(kv_lens [N], cu_new [N+1], positions
+        [max_tokens], slot_map [max_tokens] int64, table [N,M], counts [3])``: lengths
+        after the step, offsets, position and slot of each new token (0 and -1 behind the
+        last), the new table (-1 where there is no page) and {new tokens, pages taken,
+        pages wanted and not had}. Tokens without a page have the slot -1."""
+        return self._serve(backend).paged_layout(seq_lens, new_lens, block_table, free_pages, page_size, max_tokens)
+
+    @staticmethod
+    def rotary_frequencies(*args, **kwargs):
+        """``(inv_freq, amplitude)`` for ``rope_paged_store``: see serve.rotary_frequencies."""
+        return serve.rotary_frequencies(*args, **kwargs)
 
     def __getattr__(self, name: str):
         if name.startswith("_"):

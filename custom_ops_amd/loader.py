@@ -1,4 +1,4 @@
-"""Deployment loading for the ``fa`` op group.
+"""Deployment loading for the op groups ``fa`` and ``serve``.
 
 Contract kept from the reference facade (``CustomOps.build`` /
 ``load_precompiled`` / ``load``, __init__.py:654-1011, and ``FAOps``,
@@ -46,7 +46,7 @@ from typing import Callable, Optional
 
 import torch
 
-from . import _lib, build as _build, fa
+from . import _lib, build as _build, fa, serve
 
 ARTIFACT_FORMAT = "custom_ops_amd.artifact/2"
 GROUP_VERSION = "1"
@@ -268,7 +268,33 @@ class FAOps:
     so_name = "libmi355_fa"
     ops = {fa.OP_NAME: fa.SCHEMA}
     meta_ops = (fa.OP_NAME,)
+    abi = _lib.ABI_VERSION
     default_targets = ("gfx950",)
+
+    # what the group's library is built from, and how it is opened
+    def _source(self) -> str:
+        return _build.SRC
+
+    def _compile(self, product: str, flags: list, verbose: bool) -> None:
+        _build.compile_checked(product, flags, verbose=verbose)
+
+    def _compile_ops(self, product: str, verbose: bool) -> None:
+        _build.build_ops(product, verbose=verbose)
+
+    def _open(self, library: Path, native: Optional[Path]) -> None:
+        """Open the library and register its operators, with the compiled
+        implementation at ``native`` (None: the Python one)."""
+        _lib.load(str(library))
+        fa.native_path = None if native is None else str(native)
+        fa.register()
+
+    def _tree(self) -> tuple:
+        """The in-tree library, compiled if it is missing, and the in-tree operator
+        implementation if it is of the present sources."""
+        path = Path(_build.lib_path())
+        if not path.exists():
+            _build.build()
+        return path.resolve(strict=True), Path(fa.OPS_PATH) if _build.ops_current(fa.OPS_PATH) else None
 
     def __init__(self, *, allow_jit: bool = True) -> None:
         self._allow_jit = True
@@ -320,7 +346,7 @@ class FAOps:
                 "schemas": {f"{self.namespace}::{op}": f"{self.namespace}::{schema}"
                             for op, schema in sorted(self.ops.items())},
                 "meta_ops": sorted(self.meta_ops),
-                "abi": _lib.ABI_VERSION,
+                "abi": self.abi,
                 "group_version": GROUP_VERSION}
 
     def _expectation(self) -> _Expectation:
@@ -329,8 +355,8 @@ class FAOps:
     # offline build
     def _provenance(self, targets: list, extra: list) -> dict:
         h = hashlib.sha256()
-        csrc = Path(_build.SRC).parent
-        for src in [Path(_build.SRC), *sorted(csrc.glob("*.h")), *sorted(csrc.glob("*.inc")),
+        csrc = Path(self._source()).parent
+        for src in [Path(self._source()), *sorted(csrc.glob("*.h")), *sorted(csrc.glob("*.inc")),
                     *sorted(Path(_build.INCLUDE).glob("*.h"))]:
             h.update(src.name.encode() + b"\0" + src.read_bytes())
         flags = [f for f in _build.HIPCC_FLAGS if not f.startswith("--offload-arch=")] + extra
@@ -372,9 +398,9 @@ class FAOps:
                 with tempfile.TemporaryDirectory(prefix=".build-", dir=out) as tmp:
                     product = Path(tmp) / library.name
                     try:   # compiles and checks the device assembly (isa_check)
-                        _build.compile_checked(
+                        self._compile(
                             str(product), [*before["flags"], *[f"--offload-arch={t}" for t in targets]],
-                            verbose=verbose)
+                            verbose)
                     except RuntimeError as e:
                         raise CustomOpsError(str(e)) from e
                     if self._provenance(targets, extra) != before:
@@ -388,7 +414,7 @@ class FAOps:
                     ops = out / f"{self.so_name}_ops.so"
                     ops_product = Path(tmp) / ops.name
                     try:
-                        _build.build_ops(str(ops_product), verbose=verbose)
+                        self._compile_ops(str(ops_product), verbose)
                     except RuntimeError as e:
                         raise CustomOpsError(str(e)) from e
                     manifest["companion"] = {"file": ops.name, "bytes": ops_product.stat().st_size,
@@ -438,9 +464,7 @@ class FAOps:
         if all(c.state == "live" for c in claims):
             return
         try:
-            _lib.load(str(library))
-            fa.native_path = None if native is None else str(native)
-            fa.register()
+            self._open(library, native)
             self._verify_registered()
         except Exception as e:
             for c in claims:
@@ -477,7 +501,7 @@ class FAOps:
                 self._library, self._sidecar, self._error = library, sidecar, None
             except Exception as e:
                 self._error = str(e)
-                raise CustomOpsError(f"[FAOps] precompiled load failed (JIT disabled): {e}") from e
+                raise CustomOpsError(f"[{type(self).__name__}] precompiled load failed (JIT disabled): {e}") from e
         return self
 
     def load(self) -> "FAOps":
@@ -488,18 +512,50 @@ class FAOps:
             if self._library is not None:
                 return self
             if not self._allow_jit:
-                self._error = ("JIT is disabled for FAOps; call load_precompiled("
+                self._error = (f"JIT is disabled for {type(self).__name__}; call load_precompiled("
                                "library_path, metadata_path=None) before load()")
                 raise CustomOpsError(self._error)
             try:
-                path = Path(_build.lib_path())
-                if not path.exists():
-                    _build.build()
-                path = path.resolve(strict=True)
-                self._bind(path, Path(fa.OPS_PATH) if _build.ops_current(fa.OPS_PATH) else None,
-                           lambda: None)
+                path, native = self._tree()
+                self._bind(path, native, lambda: None)
                 self._library, self._sidecar, self._error = path, None, None
             except Exception as e:
                 self._error = str(e)
-                raise CustomOpsError(f"[FAOps] load failed: {e}") from e
+                raise CustomOpsError(f"[{type(self).__name__}] load failed: {e}") from e
         return self
+
+
+class ServeOps(FAOps):
+    """The ``serve`` op group (serve.py): no counterpart in the reference. Its compiled
+    implementation is not optional: there is no Python one."""
+
+    so_name = "libmi355_serve"
+    ops = dict(serve.SCHEMAS)
+    meta_ops = tuple(sorted(serve.SCHEMAS))
+    abi = serve.ABI_VERSION
+
+    def _source(self) -> str:
+        return _build.SERVE_SRC
+
+    def _compile(self, product: str, flags: list, verbose: bool) -> None:
+        _build.compile_checked(product, flags, verbose=verbose, src=_build.SERVE_SRC)
+
+    def _compile_ops(self, product: str, verbose: bool) -> None:
+        _build.build_serve_ops(product, verbose=verbose)
+
+    def _validate(self, library: Path, sidecar: Path) -> Path:
+        native = super()._validate(library, sidecar)
+        if native is None:
+            raise CustomOpsError(f"{self.so_name}_ops.so was not deployed with {library.name} for torch {torch.__version__}")
+        return native
+
+    def _open(self, library: Path, native: Optional[Path]) -> None:
+        serve.register(str(library), str(native))
+
+    def _tree(self) -> tuple:
+        path, native = Path(_build.SERVE_LIB_PATH), Path(_build.SERVE_OPS_PATH)
+        if not path.exists():
+            _build.build_serve()
+        if not _build.ops_current(str(native), _build.SERVE_BINDING_SRC):
+            _build.build_serve_ops()
+        return path.resolve(strict=True), native
