@@ -13,8 +13,11 @@
 //    the join of the waves at the end.
 //  * K and V of the next tile are in flight, in registers, while a tile computes;
 //    the page numbers of the one behind it too.
-//  * The length is split over workgroups; their parts (O, max, sum, fp32) are joined
-//    by a second kernel.
+//  * Sequences are split by their own lengths, which only the device knows: every
+//    workgroup sums the tiles of all requests, takes the part size that makes about
+//    `target` parts of them, and finds its own part by a scan. So a long sequence
+//    in a ragged batch is shared by many workgroups and a short one is not split.
+//    Parts (O, max, sum, fp32) of a shared sequence are joined by a second kernel.
 
 constexpr int kDecTile = 32;    // keys per wave tile
 constexpr int kDecWaves = 4;
@@ -28,11 +31,15 @@ struct DecodeArgs {
   const int* table;
   const int* lens;
   const float* slopes;
-  float* part_o;   // [splits][b·h][D]
-  float* part_ml;  // [splits][b·h][2]: max in log2 units, sum
+  int* rec;        // [b][hk·groups][2]: first part, parts
+  float* part_ml;  // [parts][16][2]: max in log2 units, sum
+  float* part_o;   // [parts][16][D]
   int64_t q_bs, q_hs, o_bs, o_hs, kp, kh, kr, vp, vh, vr, ts;
   int b, h, hk, ratio, groups;   // groups: 16-head groups per KV head
-  int pages, shift, cols, window, splits;
+  int pages, shift, cols, window;
+  int split;       // 0: a workgroup per (request, head group)
+  int target;      // parts to make, about
+  int least;       // tiles of a part at least
   float u_scale, c2, bias;       // as in PackedArgs
 };
 
@@ -42,30 +49,79 @@ __device__ __forceinline__ f32x4 mfma16(typename Elt<BF16>::v8 a, typename Elt<B
   else return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-template <int D, bool BF16, bool CAP, bool BIAS>
-__global__ __launch_bounds__(64 * kDecWaves) __attribute__((amdgpu_waves_per_eu(2, 2)))
+// The tiles that a request's keys span: its first seen tile, and their number.
+struct Keys {
+  int len, first, tile0, tiles;
+};
+__device__ __forceinline__ Keys keys_of(const DecodeArgs& a, int b) {
+  Keys k;
+  k.len = max(0, (int)min((int64_t)a.lens[b], (int64_t)a.cols << a.shift));
+  k.first = max(0, k.len - a.window);
+  k.tile0 = k.first / kDecTile;
+  k.tiles = (k.len + kDecTile - 1) / kDecTile - k.tile0;
+  return k;
+}
+
+// Part w: request, head group, place among the request's parts. All waves of the
+// workgroup find the same, each for itself: two passes over the lengths, 64 at a time.
+struct Part {
+  int b, hg, part, parts, slot;   // slot: of part 0
+};
+__device__ __forceinline__ bool find_part(const DecodeArgs& a, int w, Part& p) {
+  const int hgs = a.hk * a.groups, lane = threadIdx.x & 63;
+  if (!a.split) {
+    p = Part{w / hgs, w % hgs, 0, 1, 0};
+    return true;
+  }
+  // (a request counts for 2^20 tiles at most, 2^25 keys, so that sums stay below 2^31)
+  int sum = 0;
+  for (int i = lane; i < a.b; i += 64) sum += min(keys_of(a, i).tiles, 1 << 20);
+  sum = __builtin_amdgcn_readlane(wave_scan(sum), 63);
+  const int per = (int)max((int64_t)a.least, ((int64_t)sum * hgs + a.target - 1) / a.target);
+  int run = 0;
+  for (int base = 0; base < a.b; base += 64) {
+    const int i = base + lane;
+    const int n = i < a.b ? max(1, (min(keys_of(a, i).tiles, 1 << 20) + per - 1) / per) : 0;
+    const int incl = wave_scan(n * hgs);
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(run + incl > w);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      p.b = base + l;
+      p.parts = __builtin_amdgcn_readlane(n, l);
+      const int start = run + (int)__builtin_amdgcn_readlane(incl, l) - p.parts * hgs;
+      p.hg = (w - start) / p.parts;
+      p.part = (w - start) % p.parts;
+      p.slot = w - p.part;
+      return true;
+    }
+    run += __builtin_amdgcn_readlane(incl, 63);
+  }
+  return false;
+}
+
+template <int D, bool BF16, bool CAP, bool BIAS, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2)))
 void paged_decode_kernel(const DecodeArgs a) {
   typedef typename Elt<BF16>::v8 V8;
   constexpr int KD = D / 32, DB = D / 16;
   constexpr int kRow = D * 2 + 32;   // LDS bytes per V row: transposed reads of 16 rows touch all banks alike
-  __shared__ __align__(16) uint8_t sV[kDecWaves][kDecTile * kRow];
-  __shared__ float sM[kDecWaves][kDecHeads], sL[kDecWaves][kDecHeads];
+  __shared__ __align__(16) uint8_t sV[WAVES][kDecTile * kRow];
+  __shared__ float sM[WAVES][kDecHeads], sL[WAVES][kDecHeads];
 
-  const int split = blockIdx.x % a.splits;
-  const int rest = blockIdx.x / a.splits;
-  const int hg = rest % (a.hk * a.groups), b = rest / (a.hk * a.groups);
+  Part pt;
+  if (!find_part(a, blockIdx.x, pt)) return;
+  const int b = pt.b, hg = pt.hg;
   const int hk = hg / a.groups, h0 = hk * a.ratio + (hg % a.groups) * kDecHeads;
   const int heads = min(kDecHeads, (hk + 1) * a.ratio - h0);
   const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
   const int l16 = lane & 15, g = lane >> 4;
 
   const int page_size = 1 << a.shift;
-  const int len = uni(max(0, (int)min((int64_t)a.lens[b], (int64_t)a.cols << a.shift)));
-  const int first = max(0, len - a.window);
-  // tiles of this split, this wave: t_lo + wave, + kDecWaves, ...
-  const int tile0 = first / kDecTile, tiles = (len + kDecTile - 1) / kDecTile - tile0;
-  const int per = (tiles + a.splits - 1) / a.splits;
-  const int t_lo = tile0 + min(tiles, split * per), t_hi = tile0 + min(tiles, (split + 1) * per);
+  const Keys ks = keys_of(a, b);
+  const int len = uni(ks.len), first = uni(ks.first), tile0 = uni(ks.tile0), tiles = uni(ks.tiles);
+  // tiles of this part, this wave: t_lo + wave, + WAVES, ...
+  const int per = (tiles + pt.parts - 1) / pt.parts;
+  const int t_lo = tile0 + min(tiles, pt.part * per), t_hi = tile0 + min(tiles, (pt.part + 1) * per);
 
   // Q of the wave's heads: B operand, column l16, d = 8·(4·kd + g)
   V8 qreg[KD];
@@ -86,12 +142,16 @@ void paged_decode_kernel(const DecodeArgs a) {
   const int* table = a.table + (int64_t)b * a.ts;
   const uint16_t* kbase = a.k + (int64_t)hk * a.kh + g * 8;
   const uint16_t* vbase = a.v + (int64_t)hk * a.vh + g * 8;
-  // page numbers of the lane's keys l16 and 16 + l16 of a tile (-1: not seen)
+  // Page numbers of the lane's keys l16 and 16 + l16 of a tile (-1: not seen). No load
+  // of the loop is conditional, or the compiler would wait for all loads in flight where
+  // the paths meet: what is behind the part's end reads what is there anyway.
+  const int last = max(len - 1, 0);
   auto entries = [&](int t, int (&e)[2]) __attribute__((always_inline)) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int key = t * kDecTile + r * 16 + l16;
-      e[r] = (t < t_hi && key >= first && key < len) ? table[key >> a.shift] : -1;
+      const int x = table[min(key, last) >> a.shift];
+      e[r] = (t < t_hi && key >= first && key < len) ? x : -1;
     }
   };
   struct Tile { u32x4 k[2][KD], v[2][KD]; bool ok[2]; };
@@ -100,7 +160,7 @@ void paged_decode_kernel(const DecodeArgs a) {
     for (int r = 0; r < 2; ++r) {
       x.ok[r] = e[r] >= 0 && e[r] < a.pages;
       const int64_t page = x.ok[r] ? e[r] : 0;
-      const int64_t in = (t * kDecTile + r * 16 + l16) & (page_size - 1);
+      const int64_t in = x.ok[r] ? (t * kDecTile + r * 16 + l16) & (page_size - 1) : 0;
       const uint16_t* kp = kbase + page * a.kp + in * a.kr;
       const uint16_t* vp = vbase + page * a.vp + in * a.vr;
 #pragma unroll
@@ -169,23 +229,22 @@ void paged_decode_kernel(const DecodeArgs a) {
     }
   };
 
-  {
+  if (t_lo + wave < t_hi) {
     int t = t_lo + wave;
     int e0[2], e1[2];
     Tile x0, x1;
     entries(t, e0);
-    entries(t + kDecWaves, e1);
-    if (t < t_hi) fetch(t, e0, x0);
-    for (; t < t_hi; t += 2 * kDecWaves) {
-      entries(t + 2 * kDecWaves, e0);
-      if (t + kDecWaves < t_hi) fetch(t + kDecWaves, e1, x1);
+    entries(t + WAVES, e1);
+    fetch(t, e0, x0);
+    for (; t + WAVES < t_hi; t += 2 * WAVES) {
+      entries(t + 2 * WAVES, e0);
+      fetch(t + WAVES, e1, x1);
       compute(t, x0);
-      if (t + kDecWaves < t_hi) {
-        entries(t + 3 * kDecWaves, e1);
-        if (t + 2 * kDecWaves < t_hi) fetch(t + 2 * kDecWaves, e0, x0);
-        compute(t + kDecWaves, x1);
-      }
+      entries(t + 3 * WAVES, e1);
+      fetch(t + 2 * WAVES, e0, x0);
+      compute(t + WAVES, x1);
     }
+    if (t < t_hi) compute(t, x0);
   }
 
   // join the waves: O in its own slice as fp32, [D][16 heads] (the slices are free)
@@ -202,54 +261,110 @@ void paged_decode_kernel(const DecodeArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) so[l16 * (D + 2) + db * 16 + 4 * g + i] = oacc[db][i];
   __syncthreads();
-  for (int x = tid; x < heads * D; x += 64 * kDecWaves) {
+  for (int x = tid; x < heads * D; x += 64 * WAVES) {
     const int n = x / D, d = x % D;
     float m = sM[0][n];
 #pragma unroll
-    for (int w = 1; w < kDecWaves; ++w) m = fmaxf(m, sM[w][n]);
+    for (int w = 1; w < WAVES; ++w) m = fmaxf(m, sM[w][n]);
     float acc = 0.f, l = 0.f;
 #pragma unroll
-    for (int w = 0; w < kDecWaves; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       const float f = sM[w][n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sM[w][n] - m);
       // a wave that saw nothing adds nothing; NaN sums stay
       l += sL[w][n] == 0.f ? 0.f : sL[w][n] * (sM[w][n] == -INFINITY ? 1.f : f);
       const float y = reinterpret_cast<const float*>(sV[w])[n * (D + 2) + d];
       acc += sL[w][n] == 0.f ? 0.f : y * (sM[w][n] == -INFINITY ? 1.f : f);
     }
-    if (a.splits == 1) {
+    if (pt.parts == 1) {
       const float r = l == 0.f ? 0.f : acc / l;
       uint16_t out;
       if constexpr (BF16) out = bitcast<uint16_t>((__bf16)r);
       else out = bitcast<uint16_t>((_Float16)r);
       a.o[(int64_t)b * a.o_bs + (int64_t)(h0 + n) * a.o_hs + d] = out;
     } else {
-      const int64_t bh = (int64_t)split * a.b * a.h + (int64_t)b * a.h + h0 + n;
-      a.part_o[bh * D + d] = acc;
+      const int64_t at = (int64_t)(pt.slot + pt.part) * kDecHeads + n;
+      a.part_o[at * D + d] = acc;
       if (d == 0) {
-        a.part_ml[bh * 2] = m;
-        a.part_ml[bh * 2 + 1] = l;
+        a.part_ml[at * 2] = m;
+        a.part_ml[at * 2 + 1] = l;
       }
     }
   }
+  if (a.split && pt.part == 0 && tid == 0) {
+    int* rec = a.rec + ((int64_t)b * a.hk * a.groups + hg) * 2;
+    rec[0] = pt.slot;
+    rec[1] = pt.parts;
+  }
 }
 
-// One workgroup per (request, head): the splits' parts, weighted by 2^(m_s − m).
+// One workgroup per (request, head): the parts, weighted by 2^(m_s − m). Its 256
+// threads are 1024 / D rows of D / 4 threads; a row takes every so many parts, 8 of
+// them in flight, with a running max, and the rows' sums are joined in LDS.
 template <int D, bool BF16>
-__global__ __launch_bounds__(D) void paged_join_kernel(const DecodeArgs a) {
-  const int bh = blockIdx.x, d = threadIdx.x;
-  const int64_t n = (int64_t)a.b * a.h;
-  float m = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[(s * n + bh) * 2]);
-  float acc = 0.f, l = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float ms = a.part_ml[(s * n + bh) * 2], ls = a.part_ml[(s * n + bh) * 2 + 1];
-    const float f = ms == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ms - m);
-    l += ls == 0.f ? 0.f : ls * f;
-    acc += ls == 0.f ? 0.f : a.part_o[(s * n + bh) * D + d] * f;
+__global__ __launch_bounds__(256) void paged_join_kernel(const DecodeArgs a) {
+  constexpr int TPR = D / 4, ROWS = 256 / TPR, J = 8;
+  __shared__ float sAcc[ROWS][D], sMax[ROWS], sSum[ROWS];
+  const int b = blockIdx.x / a.h, h = blockIdx.x % a.h, tid = threadIdx.x;
+  const int hk = h / a.ratio, n = (h - hk * a.ratio) % kDecHeads, hg = hk * a.groups + (h - hk * a.ratio) / kDecHeads;
+  const int* rec = a.rec + ((int64_t)b * a.hk * a.groups + hg) * 2;
+  const int slot = uni(rec[0]), parts = uni(rec[1]);
+  if (parts <= 1) return;   // written by its one part
+  const float* ml = a.part_ml + ((int64_t)slot * kDecHeads + n) * 2;
+  const float* po = a.part_o + ((int64_t)slot * kDecHeads + n) * D;
+  const int row = tid / TPR, c = tid % TPR;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  for (int s0 = row; s0 < parts; s0 += ROWS * J) {
+    float ms[J], ls[J];
+    f32x4 x[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int s = min(s0 + j * ROWS, parts - 1);
+      ms[j] = ml[(int64_t)s * kDecHeads * 2];
+      ls[j] = ml[(int64_t)s * kDecHeads * 2 + 1];
+      x[j] = *reinterpret_cast<const f32x4*>(po + (int64_t)s * kDecHeads * D + c * 4);
+    }
+    float top = m;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      if (s0 + j * ROWS >= parts) ls[j] = 0.f;   // a copy of the last part
+      top = fmaxf(top, ls[j] == 0.f ? -INFINITY : ms[j]);
+    }
+    const float old = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);
+    l *= old;
+    acc *= old;
+    m = top;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      // a part that saw nothing adds nothing; NaN sums stay
+      const float f = ms[j] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ms[j] - top);
+      l += ls[j] == 0.f ? 0.f : ls[j] * f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] += ls[j] == 0.f ? 0.f : x[j][i] * f;
+    }
   }
-  const float r = l == 0.f ? 0.f : acc / l;
-  uint16_t out;
-  if constexpr (BF16) out = bitcast<uint16_t>((__bf16)r);
-  else out = bitcast<uint16_t>((_Float16)r);
-  a.o[(int64_t)(bh / a.h) * a.o_bs + (int64_t)(bh % a.h) * a.o_hs + d] = out;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sAcc[row][c * 4 + i] = acc[i];
+  if (c == 0) {
+    sMax[row] = m;
+    sSum[row] = l;
+  }
+  __syncthreads();
+  if (tid < D) {
+    float top = sMax[0];
+#pragma unroll
+    for (int r = 1; r < ROWS; ++r) top = fmaxf(top, sMax[r]);
+    float y = 0.f, t = 0.f;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const float f = sMax[r] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(sMax[r] - top);
+      y += sSum[r] == 0.f ? 0.f : sAcc[r][tid] * f;
+      t += sSum[r] == 0.f ? 0.f : sSum[r] * f;
+    }
+    const float r = t == 0.f ? 0.f : y / t;
+    uint16_t out;
+    if constexpr (BF16) out = bitcast<uint16_t>((__bf16)r);
+    else out = bitcast<uint16_t>((_Float16)r);
+    a.o[(int64_t)b * a.o_bs + (int64_t)h * a.o_hs + tid] = out;
+  }
 }

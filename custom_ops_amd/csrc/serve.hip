@@ -163,9 +163,12 @@ int packed_fwd(const mi355_packed_params* p, hipStream_t st, const Err& err) {
   return launched(err, "mha_packed_fwd");
 }
 
+constexpr int kDecMaxScan = 1024;
+
 struct DecodePlan {
-  int groups, splits;
-  size_t bytes;
+  int groups, split, target, least;
+  int64_t grid;   // workgroups, and parts at most
+  size_t ml, o, bytes;   // offsets of the parts' statistics and sums in the workspace
 };
 
 DecodePlan decode_plan(const mi355_decode_params* p, int cus) {
@@ -174,10 +177,25 @@ DecodePlan decode_plan(const mi355_decode_params* p, int cus) {
   pl.groups = (ratio + kDecHeads - 1) / kDecHeads;
   const int64_t units = (int64_t)p->b * p->h_k * pl.groups;
   const int64_t tiles = ((int64_t)p->table_cols * p->page_size + kDecTile - 1) / kDecTile;
-  // two workgroups of four waves run on a CU; a split of its own for every 4 tiles at least
-  const int64_t most = std::max<int64_t>(1, tiles / kDecWaves);
-  pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>({most, 2LL * cus / std::max<int64_t>(1, units), 128}));
-  if (pl.splits > 1) pl.bytes = (size_t)pl.splits * p->b * p->h * (p->d + 2) * 4;
+  // Parts to make: two workgroups of 4 waves are resident on a CU. With many units
+  // their remainders would leave a half-empty second round, so twice as many, smaller
+  // parts ([32 x <= 8192, 16/4, 128]: 47 us against 55); with few, each part more costs
+  // the join ([131072, 32/4, 128]: 51 against 55).
+  pl.target = (int)std::clamp<int64_t>(8 * units, 2 * cus, 4 * cus);
+  // A CU alone reads about 40 GB/s, so even short sequences are shared once that pays
+  // for the join's launch, about 5 us: [1000 keys, 16/4, 128] 18.3 us whole, 10.3 in
+  // parts of 4 tiles; [500, 8/8, 64] (16 tiles) 7.1 whole, 8.9 in parts.
+  pl.least = p->d == 128 ? 4 : 8;
+  // (beyond kDecMaxScan requests the scan of their lengths is no longer small)
+  pl.split = tiles > 3 * pl.least && p->b <= kDecMaxScan;
+  pl.grid = units;
+  if (pl.split) {
+    pl.grid += pl.target;
+    auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+    pl.ml = up((size_t)units * 8);
+    pl.o = pl.ml + up((size_t)pl.grid * kDecHeads * 8);
+    pl.bytes = pl.o + (size_t)pl.grid * kDecHeads * p->d * 4;
+  }
   return pl;
 }
 
@@ -215,18 +233,20 @@ int paged_decode(const mi355_decode_params* p, hipStream_t st, const Err& err) {
   a.b = p->b; a.h = p->h; a.hk = p->h_k; a.ratio = p->h / p->h_k; a.groups = pl.groups;
   a.pages = p->num_pages; a.shift = __builtin_ctz((unsigned)p->page_size);
   a.cols = p->num_pages > 0 ? p->table_cols : 0;   // no pages: nothing is seen
-  a.window = window_of(p->window); a.splits = pl.splits;
-  a.part_o = (float*)p->workspace;
-  a.part_ml = a.part_o + (size_t)pl.splits * p->b * p->h * p->d;
-  const int64_t total = (int64_t)p->b * p->h_k * pl.groups * pl.splits;
+  a.window = window_of(p->window);
+  a.split = pl.split; a.target = pl.target; a.least = pl.least;
+  a.rec = (int*)p->workspace;
+  a.part_ml = (float*)((char*)p->workspace + pl.ml);
+  a.part_o = (float*)((char*)p->workspace + pl.o);
+  const int64_t total = pl.grid;
   if (total >= (1LL << 31) || (int64_t)p->b * p->h >= (1LL << 31))
     return err.fail(MI355_SERVE_EINVAL, "problem too large: %lld workgroups", (long long)total);
   by_type(p->d, p->dtype == MI355_SERVE_BF16, [&](auto d, auto bf) {
     constexpr int D = decltype(d)::value;
     by_scores(p->softcap > 0.f, p->slopes != nullptr, [&](auto cap, auto bias) {
-      paged_decode_kernel<D, decltype(bf)::value, decltype(cap)::value, decltype(bias)::value><<<dim3((unsigned)total), dim3(64 * kDecWaves), 0, st>>>(a);
+      paged_decode_kernel<D, decltype(bf)::value, decltype(cap)::value, decltype(bias)::value, kDecWaves><<<dim3((unsigned)total), dim3(64 * kDecWaves), 0, st>>>(a);
     });
-    if (pl.splits > 1) paged_join_kernel<D, decltype(bf)::value><<<dim3((unsigned)(p->b * p->h)), dim3(D), 0, st>>>(a);
+    if (pl.split) paged_join_kernel<D, decltype(bf)::value><<<dim3((unsigned)((int64_t)p->b * p->h)), dim3(256), 0, st>>>(a);
   });
   return launched(err, "mha_paged_decode");
 }

@@ -9,6 +9,7 @@
 //
 // Every check is of shapes, types and strides, on the host; lengths, offsets, page
 // and slot numbers stay on the device, where the kernels hold them to their ranges.
+#include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <ATen/ATen.h>
@@ -35,11 +36,23 @@ decltype(&mi355_paged_layout) g_layout = nullptr;
 using at::Tensor;
 typedef std::optional<Tensor> Maybe;
 
+// A fresh tensor on x's GPU, straight from the caching allocator (the dispatcher's
+// at::empty costs another 0.5 us, six times for the layout)
+Tensor fresh(const Tensor& x, at::IntArrayRef sizes, at::ScalarType type) {
+  return at::detail::empty_cuda(sizes, type, x.device(), std::nullopt);
+}
+
 void* stream_of(const Tensor& x) {
   return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(x.device().index()).stream();
 }
 
 void finish(int rc, const char* err) { TORCH_CHECK(rc == 0, err); }
+
+// There is no backward pass: a call that autograd would have to follow is refused.
+void check_no_grad(std::initializer_list<const Tensor*> xs) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor* x : xs) TORCH_CHECK(!x->requires_grad(), "forward only: call it under torch.no_grad() or on detached tensors");
+}
 
 void check_gpu(const Tensor& x, const Tensor& like, const char* name) {
   TORCH_CHECK(x.is_cuda(), name, " must be a CUDA tensor");
@@ -96,6 +109,7 @@ void check_head_dim(int64_t d) { TORCH_CHECK(d == 64 || d == 128, "Only head_dim
 Tensor mha_packed_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu_q, const Tensor& cu_k, bool causal,
                       std::optional<double> scale, double softcap, int64_t window, const Maybe& slopes, const Maybe& prefix_lens) {
   check_half(q);
+  check_no_grad({&q, &k, &v});
   check_rows(q, q, "q", 3);
   check_rows(k, q, "k", 3);
   check_rows(v, q, "v", 3);
@@ -117,7 +131,7 @@ Tensor mha_packed_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const T
   p.slopes = slopes_of(slopes, q, H);
 
   c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
-  Tensor out = at::empty({Tq, H, d}, q.options());
+  Tensor out = fresh(q, {Tq, H, d}, q.scalar_type());
   if (out.numel() == 0) return out;
   p.q = q.data_ptr(); p.k = k.data_ptr(); p.v = v.data_ptr(); p.o = out.data_ptr();
   p.cu_q = cu_q.data_ptr<int>(); p.cu_k = cu_k.data_ptr<int>();
@@ -139,6 +153,7 @@ Tensor mha_packed_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const T
 Tensor mha_paged_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table, const Tensor& kv_lens,
                         std::optional<double> scale, double softcap, int64_t window, const Maybe& slopes) {
   check_half(q);
+  check_no_grad({&q, &k_cache, &v_cache});
   check_rows(q, q, "q", 3);
   check_rows(k_cache, q, "k_cache", 4);
   check_rows(v_cache, q, "v_cache", 4);
@@ -160,7 +175,7 @@ Tensor mha_paged_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_
   p.slopes = slopes_of(slopes, q, H);
 
   c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
-  Tensor out = at::empty({B, H, d}, q.options());
+  Tensor out = fresh(q, {B, H, d}, q.scalar_type());
   if (out.numel() == 0) return out;
   p.q = q.data_ptr(); p.k_cache = k_cache.data_ptr(); p.v_cache = v_cache.data_ptr(); p.o = out.data_ptr();
   p.block_table = block_table.numel() ? block_table.data_ptr<int>() : nullptr;
@@ -177,7 +192,7 @@ Tensor mha_paged_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_
   p.softcap = (float)softcap;
   Tensor ws;
   if (const size_t n = g_decode_bytes(&p)) {
-    ws = at::empty({(int64_t)n}, q.options().dtype(at::kByte));
+    ws = fresh(q, {(int64_t)n}, at::kByte);
     p.workspace = ws.data_ptr();
     p.workspace_bytes = n;
   }
@@ -190,6 +205,7 @@ std::tuple<Tensor, Tensor> rope_paged_store(const Tensor& q, const Tensor& k, co
                                             const Tensor& slot_map, const Tensor& k_cache, const Tensor& v_cache, bool interleaved,
                                             double amplitude) {
   check_half(q);
+  check_no_grad({&q, &k, &v, &k_cache, &v_cache});
   check_rows(q, q, "q", 3);
   check_rows(k, q, "k", 3);
   check_rows(v, q, "v", 3);
@@ -216,7 +232,7 @@ std::tuple<Tensor, Tensor> rope_paged_store(const Tensor& q, const Tensor& k, co
   TORCH_CHECK(std::isfinite(amplitude) && std::isfinite((float)amplitude), "amplitude must be finite");
 
   c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
-  Tensor qo = at::empty({T, H, d}, q.options()), ko = at::empty({T, Hk, d}, q.options());
+  Tensor qo = fresh(q, {T, H, d}, q.scalar_type()), ko = fresh(q, {T, Hk, d}, q.scalar_type());
   if (T == 0) return {qo, ko};
   mi355_rope_params p{};
   p.q = q.data_ptr(); p.k = k.data_ptr(); p.v = v.data_ptr(); p.q_out = qo.data_ptr(); p.k_out = ko.data_ptr();
@@ -259,9 +275,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> paged_layout(const Te
   TORCH_CHECK(M <= INT_MAX && free_pages.size(0) <= INT_MAX, "too many pages");
 
   c10::hip::HIPGuardMasqueradingAsCUDA guard(seq_lens.device());
-  const auto opt = seq_lens.options();
-  Tensor kv_lens = at::empty({n}, opt), cu = at::empty({n + 1}, opt), positions = at::empty({max_tokens}, opt);
-  Tensor slots = at::empty({max_tokens}, opt.dtype(at::kLong)), table = at::empty({n, M}, opt), counts = at::empty({3}, opt);
+  auto make = [&](at::IntArrayRef sizes) { return fresh(seq_lens, sizes, at::kInt); };
+  Tensor kv_lens = make({n}), cu = make({n + 1}), positions = make({max_tokens}), table = make({n, M}), counts = make({3});
+  Tensor slots = fresh(seq_lens, {max_tokens}, at::kLong);
   mi355_layout_params p{};
   auto ints = [](const Tensor& x) { return x.numel() ? x.data_ptr<int>() : nullptr; };
   p.seq_lens = ints(seq_lens); p.new_lens = ints(new_lens); p.block_table = ints(block_table); p.free_pages = ints(free_pages);
@@ -295,7 +311,16 @@ extern "C" int mi355_serve_connect(void* handle) {
     static torch::Library lib(torch::Library::IMPL, "recsys_ops", c10::DispatchKey::CUDA, __FILE__, __LINE__);
     static const bool once = (lib.impl("mha_packed_fwd", &mha_packed_fwd), lib.impl("mha_paged_decode", &mha_paged_decode),
                               lib.impl("rope_paged_store", &rope_paged_store), lib.impl("paged_layout", &paged_layout), true);
+    // nothing to record: without this every call goes through autograd's boxed
+    // fallback (check_no_grad refuses what would need it)
+    static torch::Library autograd(torch::Library::IMPL, "recsys_ops", c10::DispatchKey::Autograd, __FILE__, __LINE__);
+    static const bool once_more = [] {
+      for (const char* name : {"mha_packed_fwd", "mha_paged_decode", "rope_paged_store", "paged_layout"})
+        autograd.impl(name, torch::CppFunction::makeFallthrough());
+      return true;
+    }();
     (void)once;
+    (void)once_more;
   } catch (const std::exception&) {
     return 1;
   }
