@@ -13,12 +13,11 @@
 //    scores. No mask is read: a row's seen keys are [lo, hi) and [0, prefix), and
 //    only key tiles that a border crosses compare keys with them.
 //  * Key tiles that no row of the workgroup sees are not visited.
-//  * Offsets stay on the device: the workgroup finds its sequence by a scan over
-//    cu_q, so the grid holds total_q / BM + n_seqs + 2 blocks per head, the most
+//  * Offsets stay on the device: the workgroup finds its rows by a scan over the
+//    sequences, the longest blocks first, so the grid holds total_q / BM + n_seqs + 2 blocks per head, the most
 //    that any split of the rows can need.
 //  * K and V tiles come HBM → LDS by DMA, two stages, one barrier per tile.
 
-constexpr int kTile = 64;   // keys per tile
 constexpr float kSlackLog2 = 8.f;   // the running max moves when a score passes it by this (P <= 2^8)
 
 struct PackedArgs {
@@ -33,16 +32,18 @@ struct PackedArgs {
   int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs;
   int tq, tk, n, h, ratio;
   int causal, window;   // window: 2^30 where there is none
-  int blocks;           // row blocks per head in the grid
+  int pack;             // heads of one KV head that share a workgroup: divides ratio, 1, 2 or 4
+  int bm_shift;         // log2 of a block's rows: 32·RW / pack
+  int levels;           // classes of block lengths (find_block)
   float u_scale;        // capped: 2·log2(e)·scale / softcap
   float c2;             // scores u to log2 units: scale·log2(e), capped 2·softcap·log2(e)
   float bias;           // slopes to u: −1/scale, capped −1/(2·softcap)
 };
 
-// A row block: rows m0 .. of the sequence's lq, which start at global row q0.
+// A row block: rows m0 .. of the sequence's lq, which start at global row q0, its lk
+// keys, which start at global key k0, and the prefix that all rows see.
 struct RowBlock {
-  int seq;   // -1: rows of no sequence
-  int q0, lq, m0;
+  int q0, lq, m0, k0, lk, pre;
 };
 
 // Inclusive sum over the wave's lanes: rows of 16 by shifts, then the rows' sums.
@@ -55,69 +56,112 @@ __device__ __forceinline__ int wave_scan(int x) {
   x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);   // row_bcast:31 into rows 2 and 3
   return x;
 }
+__device__ __forceinline__ int wave_max(int x) {   // of values >= 0, over the wave's lanes
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(x, 63);
+}
 
-// Block t of the rows, counted from the last sequence's last rows (with a causal
-// mask the longest blocks run first). Segment e = 0 .. n + 1 holds the rows from
-// cu[e − 1] to cu[e] (0 before the first, tq behind the last): sequence e − 1, or
-// rows of none. Offsets are held to 0 .. tq.
-template <int BM>
+// Row block t of a head, the blocks with the most key tiles first: in a.levels classes,
+// each of half the tiles of the one before, so that no long block starts last. Segment
+// e = 0 .. n + 1 holds the rows from cu[e − 1] to cu[e] (0 before the first, tq behind
+// the last): sequence e − 1, or rows of none, which have no keys. Offsets are held to
+// 0 .. tq. All waves find the same, each for itself, 64 segments at a time; of more
+// than 62 sequences (short ones, then) there is one class.
 __device__ __forceinline__ bool find_block(const PackedArgs& a, int t, RowBlock& rb) {
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, BM = 1 << a.bm_shift;
+  const int iters = (a.n + 2 + 63) / 64;
+  struct Seg { int c0, rows, k0, lk, pre, blocks; };
+  auto segment = [&](int it) __attribute__((always_inline)) {
+    const int e = it * 64 + lane;
+    Seg x{0, 0, 0, 0, 0, 0};
+    if (e <= a.n + 1) {
+      const bool real = e >= 1 && e <= a.n;
+      const int c1 = e == a.n + 1 ? a.tq : a.cu_q[e], k1 = real ? a.cu_k[e] : 0;
+      const int c0 = e == 0 ? 0 : a.cu_q[e - 1], k0 = real ? a.cu_k[e - 1] : 0;
+      const int pre = real && a.prefix ? a.prefix[e - 1] : 0;
+      x.c0 = min(max(c0, 0), a.tq);
+      x.rows = max(0, min(max(c1, 0), a.tq) - x.c0);
+      x.k0 = min(max(k0, 0), a.tk);
+      x.lk = real ? max(0, min(max(k1, 0), a.tk) - x.k0) : 0;
+      x.pre = min(max(pre, 0), x.lk);
+      x.blocks = (x.rows + BM - 1) >> a.bm_shift;
+    }
+    return x;
+  };
+  // keys that block b of a segment spans, about; more for later blocks, or the same
+  auto span_of = [&](const Seg& x, int b) {
+    if (!a.causal) return a.window > x.lk / 2 ? x.lk : 2 * a.window;
+    const int hi = min(x.lk, (b + 1) * BM + x.lk - x.rows);
+    return max(0, min(hi, a.window));
+  };
+  Seg x = segment(0);
+  const int levels = iters == 1 ? a.levels : 1;
+  const int most = levels > 1 ? wave_max(x.blocks ? span_of(x, x.blocks - 1) : 0) : 0;
   int run = 0;
-  for (int base = 0; base < a.n + 2; base += 64) {
-    const int e = a.n + 1 - (base + lane);
-    int c0 = 0, c1 = 0;
-    if (e >= 0) {
-      c0 = e == 0 ? 0 : min(max(a.cu_q[e - 1], 0), a.tq);
-      c1 = e == a.n + 1 ? a.tq : min(max(a.cu_q[e], 0), a.tq);
+#pragma unroll 1
+  for (int level = 0; level < levels; ++level) {
+    const int above = level == levels - 1 ? -1 : most >> (level + 1);   // blocks that span more
+    const int below = level == 0 ? INT_MAX : most >> level;              // and at most this
+    auto first_over = [&](const Seg& s, int lim) {   // of a segment's blocks, the first that spans more than lim
+      if (s.blocks == 0 || span_of(s, s.blocks - 1) <= lim) return s.blocks;
+      if (span_of(s, 0) > lim) return 0;
+      return min(s.blocks, (lim - (s.lk - s.rows)) >> a.bm_shift);   // causal: (b + 1)·BM + lk − rows > lim
+    };
+    for (int it = 0; it < iters; ++it) {
+      if (iters > 1) x = segment(it);
+      const int b0 = first_over(x, above), b1 = first_over(x, below), cnt = b1 - b0;
+      const int incl = wave_scan(cnt);
+      const uint64_t hit = __builtin_amdgcn_ballot_w64(run + incl > t);
+      if (hit) {
+        const int l = __builtin_ctzll(hit);
+        const int left = run + (int)__builtin_amdgcn_readlane(incl, l) - 1 - t;   // blocks of the class behind t in its segment
+        rb.m0 = ((int)__builtin_amdgcn_readlane(b0, l) + left) * BM;
+        rb.q0 = __builtin_amdgcn_readlane(x.c0, l);
+        rb.lq = __builtin_amdgcn_readlane(x.rows, l);
+        rb.k0 = __builtin_amdgcn_readlane(x.k0, l);
+        rb.lk = __builtin_amdgcn_readlane(x.lk, l);
+        rb.pre = __builtin_amdgcn_readlane(x.pre, l);
+        return true;
+      }
+      run += __builtin_amdgcn_readlane(incl, 63);
     }
-    const int cnt = c1 > c0 ? (c1 - c0 + BM - 1) / BM : 0;
-    const int incl = wave_scan(cnt);
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(run + incl > t);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
-      const int es = uni(__builtin_amdgcn_readlane(e, l));
-      const int ends = run + (int)__builtin_amdgcn_readlane(incl, l);
-      rb.q0 = __builtin_amdgcn_readlane(c0, l);
-      rb.lq = (int)__builtin_amdgcn_readlane(c1, l) - rb.q0;
-      rb.m0 = (ends - 1 - t) * BM;
-      rb.seq = es >= 1 && es <= a.n ? es - 1 : -1;
-      return true;
-    }
-    run += __builtin_amdgcn_readlane(incl, 63);
   }
   return false;
 }
 
-template <int D, bool BF16, bool CAP, bool BIAS, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2)))
+template <int D, bool BF16, bool CAP, bool BIAS, int RW, int KG>
+__global__ __launch_bounds__(64 * RW * KG) __attribute__((amdgpu_waves_per_eu(D == 64 && KG < 4 ? 4 : 2)))
 void packed_fwd_kernel(const PackedArgs a) {
   typedef typename Elt<BF16>::v8 V8;
-  constexpr int BM = 32 * WAVES, UPR = D / 8, KD = D / 16, DB = D / 32;
-  constexpr int kElems = kTile * D, kLoads = kTile * UPR / 64 / WAVES;
-  __shared__ __align__(16) uint16_t sK[2][kElems];
-  __shared__ __align__(16) uint16_t sV[2][kElems];
+  constexpr int WAVES = RW * KG, NKB = KG * D > 256 ? 1 : 2, kTile = 32 * NKB;   // keys per tile
+  constexpr int UPR = D / 8, KD = D / 16, DB = D / 32;
+  constexpr int kElems = kTile * D, kWaveLoads = kTile * UPR / 64;   // of a K or V tile
+  constexpr int kLoads = (kWaveLoads + WAVES - 1) / WAVES;
+  __shared__ __align__(16) uint16_t sKV[4][KG * kElems];   // two K stages, two V stages
 
-  const int id = xcd_remap(blockIdx.x, gridDim.x);
-  const int h = id / a.blocks;
+  // Head groups fastest, KV heads before the groups of one: workgroup i runs on XCD
+  // i % 8, so a KV head's keys stay on few XCDs' L2
   RowBlock rb;
-  if (!find_block<BM>(a, id - h * a.blocks, rb)) return;
-  const int hk = h / a.ratio;
+  const int groups = a.h / a.pack, hks = a.h / a.ratio;
+  if (!find_block(a, blockIdx.x / groups, rb)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
+  const int rw = wave % RW, kg = wave / RW;
   const int l32 = lane & 31, g = lane >> 5;
+  const int hg = blockIdx.x % groups, hk = hg % hks;
+  const int h = hk * a.ratio + hg / hks * a.pack + rw % a.pack;
 
-  int k0 = 0, lk = 0, pre = 0;
-  if (rb.seq >= 0) {
-    k0 = uni(min(max(a.cu_k[rb.seq], 0), a.tk));
-    lk = uni(min(max(a.cu_k[rb.seq + 1], k0), a.tk)) - k0;
-    if (a.prefix) pre = uni(min(max(a.prefix[rb.seq], 0), lk));
-  }
+  const int k0 = rb.k0, lk = rb.lk, pre = rb.pre;
   const int off = lk - rb.lq;   // row r is at key position r + off
   auto hi_of = [&](int i) { return a.causal ? min(lk, i + 1) : min(lk, i + a.window); };
   auto lo_of = [&](int i) { return max(0, i - a.window + 1); };
 
   // key tiles that some row of the block sees: those of the prefix, then a range
-  const int i0 = rb.m0 + off, i1 = min(rb.m0 + BM, rb.lq) - 1 + off;
+  const int i0 = rb.m0 + off, i1 = min(rb.m0 + (1 << a.bm_shift), rb.lq) - 1 + off;
   const int np = (pre + kTile - 1) / kTile;
   const int hi_b = max(0, hi_of(i1)), lo_b = lo_of(i0);
   const int t0 = max(np, lo_b / kTile);
@@ -126,7 +170,7 @@ void packed_fwd_kernel(const PackedArgs a) {
   auto tile_at = [&](int i) { return i < np ? i : i - np + t0; };
 
   // this wave's rows, and this lane's
-  const int w0 = rb.m0 + wave * 32, w1 = min(w0 + 31, rb.lq - 1);
+  const int w0 = rb.m0 + rw / a.pack * 32, w1 = min(w0 + 31, rb.lq - 1);
   const int row = w0 + l32;
   const bool mine = row < rb.lq;
   const int ia = row + off;
@@ -151,22 +195,25 @@ void packed_fwd_kernel(const PackedArgs a) {
     const i32x4 r = make_rsrc_words(base + (int64_t)first * ts, span(min(kTile, lk - first), ts));
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
-      bload16_lds(r, lds_addr(dst) + (uint32_t)((i * WAVES + wave) * 64 * 16), offs[i]);
+      if (kWaveLoads % WAVES == 0 || i * WAVES + wave < kWaveLoads)
+        bload16_lds(r, lds_addr(dst) + (uint32_t)((i * WAVES + wave) * 64 * 16), offs[i]);
+  };
+  auto issue_step = [&](int i, int st) __attribute__((always_inline)) {   // tiles i·KG .. into stage st
+#pragma unroll
+    for (int j = 0; j < KG; ++j)
+      if (i * KG + j < cnt) {
+        issue(kb, a.k_ts, k_off, tile_at(i * KG + j), sKV[st] + j * kElems);
+        issue(vb, a.v_ts, v_off, tile_at(i * KG + j), sKV[2 + st] + j * kElems);
+      }
   };
 
   // A tile that the sequence ends inside leaves V rows unwritten, whose P is 0:
   // they hold 0, or an earlier tile's values
   if (lk % kTile != 0) {
-    for (int i = tid; i < kElems / 8; i += 64 * WAVES) {
-      reinterpret_cast<u32x4*>(sV[0])[i] = u32x4{0u, 0u, 0u, 0u};
-      reinterpret_cast<u32x4*>(sV[1])[i] = u32x4{0u, 0u, 0u, 0u};
-    }
+    for (int i = tid; i < 2 * KG * kElems / 8; i += 64 * WAVES) reinterpret_cast<u32x4*>(sKV[2])[i] = u32x4{0u, 0u, 0u, 0u};
     __syncthreads();
   }
-  if (cnt > 0) {
-    issue(kb, a.k_ts, k_off, tile_at(0), sK[0]);
-    issue(vb, a.v_ts, v_off, tile_at(0), sV[0]);
-  }
+  issue_step(0, 0);
   V8 qreg[KD];
   {
     const rsrc_t rq = make_rsrc(a.q + (int64_t)(rb.q0 + w0) * a.q_ts + (int64_t)h * a.q_hs,
@@ -195,56 +242,61 @@ void packed_fwd_kernel(const PackedArgs a) {
   float m_run = -INFINITY, mlog2 = 0.f, l_run = 0.f;
   wait_vmcnt<0>();
 
-  auto body = [&](int base, const uint16_t* tK, const uint16_t* tV) __attribute__((always_inline)) {
-    const uint8_t* k8 = reinterpret_cast<const uint8_t*>(tK);
-    const uint8_t* v8 = reinterpret_cast<const uint8_t*>(tV);
-    constexpr int kWin = 2;   // LDS operand reads in flight
-    f32x16 s[2] = {f32x16{}, f32x16{}};
-    {
-      auto rd = [&](int i) {
-        return bitcast<V8>(*reinterpret_cast<const u32x4*>(k8 + (i / KD) * 32 * D * 2 + k_rd[i % KD]));
-      };
-      V8 win[kWin];
+  constexpr int kWin = 2;   // LDS operand reads in flight (4 and 8 measured the same)
+  f32x16 s[NKB];
+  auto qk = [&](int base, const uint16_t* tK) __attribute__((always_inline)) {
+    // the distance bias is where the sums start from; keys that are all behind the wave's
+    // rows take one operation each
+    constexpr bool START = BIAS && !CAP;
+    if constexpr (START) {
+      const float x0 = (float)(ia - base - g * 16), bx = bco * x0;
+      if (base + kTile <= w0 + off + 1) {
 #pragma unroll
-      for (int i = 0; i < kWin; ++i) win[i] = rd(i);
+        for (int c = 0; c < 16 * NKB; ++c) s[c / 16][c % 16] = __builtin_fmaf(-bco, (float)(c / 16 * 32 + c % 16), bx);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 2 * KD; ++i) {
-        const V8 x = win[i % kWin];
-        if (i + kWin < 2 * KD) win[i % kWin] = rd(i + kWin);
-        s[i / KD] = Elt<BF16>::mfma(x, qreg[i % KD], s[i / KD]);
+        for (int c = 0; c < 16 * NKB; ++c) s[c / 16][c % 16] = bco * __builtin_fabsf(x0 - (float)(c / 16 * 32 + c % 16));
       }
     }
+    const uint8_t* k8 = reinterpret_cast<const uint8_t*>(tK);
+    auto rd = [&](int i) {
+      return bitcast<V8>(*reinterpret_cast<const u32x4*>(k8 + (i / KD) * 32 * D * 2 + k_rd[i % KD]));
+    };
+    V8 win[kWin];
+#pragma unroll
+    for (int i = 0; i < kWin; ++i) win[i] = rd(i);
+#pragma unroll
+    for (int i = 0; i < NKB * KD; ++i) {
+      const V8 x = win[i % kWin];
+      if (i + kWin < NKB * KD) win[i % kWin] = rd(i + kWin);
+      s[i / KD] = Elt<BF16>::mfma(x, qreg[i % KD], i % KD == 0 && !START ? f32x16{} : s[i / KD]);
+    }
+  };
+  auto softmax_pv = [&](int base, const uint16_t* tV) __attribute__((always_inline)) {
+    const uint8_t* v8 = reinterpret_cast<const uint8_t*>(tV);
     // u: scores up to the factor c2. Capped: tanh z = 1 − 2 / (e^{2z} + 1), and the
     // 1 cancels in the softmax, so u = −1 / (e^{2z} + 1) with c2 = 2·softcap·log2(e)
-    if constexpr (CAP || BIAS) {
-      const float x0 = (float)(ia - base - g * 16);
+    float u[16 * NKB];   // key 32·(c / 16) + c % 16, from the lane's first
+    const float x0 = (float)(ia - base - g * 16);
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float u = s[b][i];
-          if constexpr (CAP) u = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(u * a.u_scale));
-          if constexpr (BIAS) u = __builtin_fmaf(bco, __builtin_fabsf(x0 - (float)(b * 32 + i)), u);
-          s[b][i] = u;
-        }
+    for (int c = 0; c < 16 * NKB; ++c) {
+      u[c] = s[c / 16][c % 16];
+      if constexpr (CAP) u[c] = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(u[c] * a.u_scale));
+      if constexpr (BIAS && CAP) u[c] = __builtin_fmaf(bco, __builtin_fabsf(x0 - (float)(c / 16 * 32 + c % 16)), u[c]);
     }
+    // only a tile that a border crosses compares
     const bool full = base + kTile <= pre || (base + kTile <= w_hi0 && base >= w_lo1);
     if (!full) {
       const int h_r = hi - base - g * 16, l_r = lo - base - g * 16, p_r = pl - base - g * 16;
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int c = b * 32 + i;
-          const bool seen = (c < h_r && c >= l_r) || c < p_r;
-          s[b][i] = seen ? s[b][i] : -INFINITY;
-        }
+      for (int c = 0; c < 16 * NKB; ++c) {
+        const int k = c / 16 * 32 + c % 16;
+        u[c] = (k < h_r && k >= l_r) || k < p_r ? u[c] : -INFINITY;
+      }
     }
     float mx = -INFINITY;
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
+    for (int c = 0; c < 16 * NKB; ++c) mx = fmaxf(mx, u[c]);
     mx = xhalf_max(mx);
     const bool need = mx > m_run + slack;
     if (__builtin_amdgcn_ballot_w64(need)) {
@@ -257,7 +309,7 @@ void packed_fwd_kernel(const PackedArgs a) {
       for (int db = 0; db < DB; ++db) oacc[db] *= alpha;
     }
     {
-      constexpr int N = 4 * DB;
+      constexpr int N = 2 * NKB * DB;
       auto rd = [&](int i) {
         const int j = i / DB, db = i % DB;
         const int o = ((j / 2) * 32 + (j % 2) * 8) * D * 2;
@@ -272,15 +324,15 @@ void packed_fwd_kernel(const PackedArgs a) {
         f32x8 pf;
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          pf[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j / 2][(j % 2) * 8 + e], c2, -mlog2));
+          pf[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(u[j * 8 + e], c2, -mlog2));
         return __builtin_convertvector(pf, V8);
       };
       V8 pcur = pstep(0);
       l_run = psum8<BF16>(pcur, l_run);   // of the rounded P: the weights that V meets
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 2 * NKB; ++j) {
         V8 pnext;
-        if (j < 3) pnext = pstep(j + 1);
+        if (j < 2 * NKB - 1) pnext = pstep(j + 1);
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
           const int i = j * DB + db;
@@ -288,40 +340,75 @@ void packed_fwd_kernel(const PackedArgs a) {
           if (i + kWin < N) win[i % kWin] = rd(i + kWin);
           oacc[db] = Elt<BF16>::mfma(x, pcur, oacc[db]);
         }
-        if (j < 3) {
+        if (j < 2 * NKB - 1) {
           l_run = psum8<BF16>(pnext, l_run);
           pcur = pnext;
         }
       }
     }
   };
+  // Step i: tiles i·KG .., one for each key group
+  const int steps = (cnt + KG - 1) / KG;
   auto iter = [&](auto stc, int i) __attribute__((always_inline)) {
-    constexpr int ST = decltype(stc)::value;
-    wait_vmcnt<0>();   // tile i has landed
-    wg_barrier();      // for every wave; and all have left tile i − 1's stage
-    if (i + 1 < cnt) {
-      issue(kb, a.k_ts, k_off, tile_at(i + 1), sK[ST ^ 1]);
-      issue(vb, a.v_ts, v_off, tile_at(i + 1), sV[ST ^ 1]);
-    }
-    const int base = tile_at(i) * kTile;
-    // a tile that none of the wave's rows sees
-    const bool dead = w0 >= rb.lq || (base >= pre && (base >= w_hi1 || base + kTile <= w_lo0));
-    if (!dead) body(base, sK[ST], sV[ST]);
+    constexpr int ST = decltype(stc)::value;   // i % 2
+    wait_vmcnt<0>();   // the wave's loads of step i have landed
+    wg_barrier();      // all waves' have, and all have left the stage of step i − 1
+    issue_step(i + 1, ST ^ 1);
+    if (i * KG + kg >= cnt || w0 >= rb.lq) return;
+    const int base = tile_at(i * KG + kg) * kTile;
+    if (base >= pre && (base >= w_hi1 || base + kTile <= w_lo0)) return;   // no row of the wave sees it
+    qk(base, sKV[ST] + kg * kElems);
+
+    softmax_pv(base, sKV[2 + ST] + kg * kElems);
   };
   int i = 0;
-  for (; i + 1 < cnt; i += 2) {
+  for (; i + 1 < steps; i += 2) {
     iter(std::integral_constant<int, 0>{}, i);
     iter(std::integral_constant<int, 1>{}, i + 1);
   }
-  if (i < cnt) iter(std::integral_constant<int, 0>{}, i);
+  if (i < steps) iter(std::integral_constant<int, 0>{}, i);
 
-  // O through LDS, each wave in its own slice of the stages, so that a store
-  // instruction writes whole rows
   wait_vmcnt<0>();
-  wg_barrier();
-  uint8_t* stg = (wave < 4 ? reinterpret_cast<uint8_t*>(sK[0]) : reinterpret_cast<uint8_t*>(sV[0])) + (wave & 3) * 32 * D * 2;
-  static_assert(4 * 32 * D * 2 <= 2 * kElems * 2, "staging fits");
-  const float l = xhalf_sum(l_run);
+  wg_barrier();   // the stages are free
+  l_run = xhalf_sum(l_run);
+  // the key groups' sums of the same rows, in the lanes that hold them
+  constexpr int kJoin = (DB * 16 + 2) * 64;   // floats of one wave
+  float* sj = reinterpret_cast<float*>(sKV[0]);
+  if constexpr (KG > 1) {
+    static_assert(RW * (KG - 1) * kJoin * 4 <= (int)sizeof(sKV), "joined sums fit");
+    if (kg > 0) {
+      float* at = sj + (rw * (KG - 1) + kg - 1) * kJoin + lane;
+      at[0] = m_run;
+      at[64] = l_run;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) at[(2 + db * 16 + e) * 64] = oacc[db][e];
+    }
+    __syncthreads();
+    if (kg > 0) return;
+#pragma unroll 1
+    for (int k = 1; k < KG; ++k) {
+      const float* at = sj + (rw * (KG - 1) + k - 1) * kJoin + lane;
+      const float mk = at[0], lk2 = at[64];
+      const float top = fmaxf(m_run, mk);
+      // a group that saw nothing has sums of 0 (or NaN, which stay)
+      const float f0 = m_run == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_run - top) * c2);
+      const float f1 = mk == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mk - top) * c2);
+      l_run = l_run * f0 + lk2 * f1;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) oacc[db][e] = oacc[db][e] * f0 + at[(2 + db * 16 + e) * 64] * f1;
+      m_run = top;
+    }
+  }
+
+  // O through LDS, each wave in a slice of its own (which no other wave reads), so that
+  // a store instruction writes whole rows
+  uint8_t* stg = KG > 1 ? reinterpret_cast<uint8_t*>(sj + rw * (KG - 1) * kJoin) : reinterpret_cast<uint8_t*>(sKV[0]) + wave * 32 * D * 2;
+  static_assert(RW * 32 * D * 2 <= (int)sizeof(sKV) && 32 * D * 2 <= kJoin * 4, "staging fits");
+  const float l = l_run;
   const float inv = (l == 0.f || l != l) ? 1.f : 1.f / l;
   constexpr int CH = D / 8, RPI = 64 / CH;
   typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
