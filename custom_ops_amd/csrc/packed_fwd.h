@@ -202,17 +202,16 @@ void packed_fwd_kernel(const PackedArgs a) {
 #pragma unroll
     for (int j = 0; j < KG; ++j)
       if (i * KG + j < cnt) {
-        issue(kb, a.k_ts, k_off, tile_at(i * KG + j), sKV[st] + j * kElems);
-        issue(vb, a.v_ts, v_off, tile_at(i * KG + j), sKV[2 + st] + j * kElems);
+        const int tile = tile_at(i * KG + j), left = lk - tile * kTile;
+        issue(kb, a.k_ts, k_off, tile, sKV[st] + j * kElems);
+        issue(vb, a.v_ts, v_off, tile, sKV[2 + st] + j * kElems);
+        // V rows behind the last key, which the DMA leaves as they are, meet a P of 0
+        if (left < kTile)
+          for (int x = left * UPR + tid; x < kTile * UPR; x += 64 * WAVES)
+            reinterpret_cast<u32x4*>(sKV[2 + st] + j * kElems)[x] = u32x4{0u, 0u, 0u, 0u};
       }
   };
 
-  // A tile that the sequence ends inside leaves V rows unwritten, whose P is 0:
-  // they hold 0, or an earlier tile's values
-  if (lk % kTile != 0) {
-    for (int i = tid; i < 2 * KG * kElems / 8; i += 64 * WAVES) reinterpret_cast<u32x4*>(sKV[2])[i] = u32x4{0u, 0u, 0u, 0u};
-    __syncthreads();
-  }
   issue_step(0, 0);
   V8 qreg[KD];
   {
@@ -410,6 +409,7 @@ void packed_fwd_kernel(const PackedArgs a) {
   static_assert(RW * 32 * D * 2 <= (int)sizeof(sKV) && 32 * D * 2 <= kJoin * 4, "staging fits");
   const float l = l_run;
   const float inv = (l == 0.f || l != l) ? 1.f : 1.f / l;
+  bool odd = false;   // a value that is not finite
   constexpr int CH = D / 8, RPI = 64 / CH;
   typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
   typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
@@ -419,7 +419,10 @@ void packed_fwd_kernel(const PackedArgs a) {
     for (int q4 = 0; q4 < 4; ++q4) {
       f32x4 x;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = oacc[db][q4 * 4 + e] * inv;
+      for (int e = 0; e < 4; ++e) {
+        x[e] = oacc[db][q4 * 4 + e] * inv;
+        odd |= !(__builtin_fabsf(x[e]) < INFINITY);
+      }
       u32x2 packed;
       if constexpr (BF16) packed = bitcast<u32x2>(__builtin_convertvector(x, bf16x4));
       else packed = bitcast<u32x2>(__builtin_convertvector(x, f16x4));
@@ -434,5 +437,88 @@ void packed_fwd_kernel(const PackedArgs a) {
     const int r = r0 + k * RPI;
     const u32x4 x = *reinterpret_cast<const u32x4*>(stg + r * D * 2 + ((ch ^ (r & (CH - 1))) * 16));
     __builtin_amdgcn_raw_buffer_store_b128(x, ro, (uint32_t)(r * (int)a.o_ts + ch * 8) * 2u, 0, 0);
+  }
+
+  // A tile that a border crosses multiplies the V of its unseen keys by a P of 0, which
+  // makes NaN of what is not finite. So rows of finite weights with such values look at
+  // the unseen keys of those tiles, and where one of them, and no seen one, holds a value
+  // that is not finite in a column, that column is formed again from the seen keys alone.
+  const uint64_t odds = __builtin_amdgcn_ballot_w64(odd && mine && l < INFINITY);
+  uint32_t rows = (uint32_t)(odds | odds >> 32);
+  if (rows) {
+    wait_vmcnt<0>();   // the rows are stored
+    constexpr int C = D / 64;   // columns lane, lane + 64 of a row
+    auto num = [](uint16_t x) {
+      if constexpr (BF16) return __uint_as_float((uint32_t)x << 16);
+      else return (float)bitcast<_Float16>(x);
+    };
+    while (rows) {
+      const int r = __builtin_ctz(rows);
+      rows &= rows - 1;
+      const int at = w0 + r + off, r_hi = hi_of(at), r_lo = lo_of(at);
+      auto sees = [&](int j) { return (j < r_hi && j >= r_lo) || j < pre; };
+      bool out[C], unseen[C] = {}, known[C] = {}, again[C], any = false;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int d = lane + 64 * c;
+        const float x = num(*reinterpret_cast<const uint16_t*>(stg + r * D * 2 + (((d / 8) ^ (r & (CH - 1))) * 16) + d % 8 * 2));
+        out[c] = !(__builtin_fabsf(x) < INFINITY);
+      }
+      for (int t = 0; t < cnt; ++t) {
+        const int base = tile_at(t) * kTile;
+        if (base + kTile <= pre || (base + kTile <= r_hi && base >= r_lo)) continue;   // all seen
+        for (int j = base; j < min(base + kTile, lk); ++j)
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            const bool wild = !(__builtin_fabsf(num(vb[(int64_t)j * a.v_ts + lane + 64 * c])) < INFINITY);
+            unseen[c] |= wild && !sees(j);
+            known[c] |= wild && sees(j);
+          }
+      }
+#pragma unroll
+      for (int c = 0; c < C; ++c) any |= again[c] = out[c] && unseen[c] && !known[c];
+      if (!__builtin_amdgcn_ballot_w64(any)) continue;
+      const uint16_t* q = a.q + (int64_t)(rb.q0 + w0 + r) * a.q_ts + (int64_t)h * a.q_hs;
+      const float bc = BIAS ? a.slopes[h] * a.bias : 0.f;
+      float m = -INFINITY, sum = 0.f, acc[C] = {};
+      for (int t = 0; t < cnt; ++t) {
+        const int base = tile_at(t) * kTile, j = base + lane;   // a key each lane
+        const bool seen = lane < kTile && j < lk && sees(j);
+        float u = -INFINITY;
+        if (seen) {
+          u = 0.f;
+          for (int d = 0; d < D; ++d) u = __builtin_fmaf(num(q[d]), num(kb[(int64_t)j * a.k_ts + d]), u);
+          if constexpr (CAP) u = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(u * a.u_scale));
+          if constexpr (BIAS) u = __builtin_fmaf(bc, __builtin_fabsf((float)(at - j)), u);
+        }
+        float top = u;
+#pragma unroll
+        for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
+        top = fmaxf(top, m);
+        if (top == -INFINITY) continue;
+        const float old = __builtin_amdgcn_exp2f((m - top) * c2), w = seen ? __builtin_amdgcn_exp2f((u - top) * c2) : 0.f;
+        m = top;
+        sum = sum * old + w;   // of the lane's keys
+#pragma unroll
+        for (int c = 0; c < C; ++c) acc[c] *= old;
+        for (uint64_t left = __builtin_amdgcn_ballot_w64(seen); left; left &= left - 1) {
+          const int x = __builtin_ctzll(left);
+          const float p = __shfl(w, x);
+#pragma unroll
+          for (int c = 0; c < C; ++c) acc[c] = __builtin_fmaf(p, num(vb[(int64_t)(base + x) * a.v_ts + lane + 64 * c]), acc[c]);
+        }
+      }
+#pragma unroll
+      for (int x = 1; x < 64; x *= 2) sum += __shfl_xor(sum, x);
+      uint16_t* o = a.o + (int64_t)(rb.q0 + w0 + r) * a.o_ts + (int64_t)h * a.o_hs;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const float y = acc[c] / sum;
+        if (again[c]) {
+          if constexpr (BF16) o[lane + 64 * c] = bitcast<uint16_t>((__bf16)y);
+          else o[lane + 64 * c] = bitcast<uint16_t>((_Float16)y);
+        }
+      }
+    }
   }
 }

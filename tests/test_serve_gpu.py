@@ -386,3 +386,356 @@ def test_layout_table_slice(ops):
     a = ops.paged_layout(i32([20, 0, 33]), i32([1, 2, 3]), table[:, 2:6], i32([90, 91, 92]), 16, 10)
     b = ops.paged_layout(i32([20, 0, 33]), i32([1, 2, 3]), table[:, 2:6].contiguous(), i32([90, 91, 92]), 16, 10)
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+# ── what a row does not see ───────────────────────────────────────────────────
+
+@pytest.mark.parametrize("wild", [NAN, math.inf, -math.inf])
+@pytest.mark.parametrize("d,H,lens,kw", [
+    (64, 2, [70, 200], {}),                                                    # 128 rows a workgroup
+    (128, 2, [300, 65], dict(window=50)),
+    (128, 4, [600], dict(window=33, prefix=[20])),                            # 64 rows
+    (64, 4, [600], dict(softcap=9.0)),
+    (128, 16, [1500, 3000, 1100], dict(window=700, slopes=True)),             # 256 rows
+    (64, 2, [129], dict(causal=False, window=10)),
+])
+def test_packed_unseen_keys_reach_nothing(ops, wild, d, H, lens, kw):
+    """Values that are not finite, in keys and values, reach only the rows that see them."""
+    kw = dict(kw)
+    slopes = slopes_of(H) if kw.pop("slopes", False) else None
+    prefix = kw.pop("prefix", None)
+    cu, Hk = cu_of(lens), max(1, H // 2)
+    T = cu[-1] + 9
+    q, k, v = randn(T, H, d, seed=1), randn(T, Hk, d, seed=2), randn(T, Hk, d, seed=3)
+    v[cu[-1]:], k[cu[-1]:] = wild, wild             # behind the last sequence
+    for c, n in zip(cu, lens):
+        v[c + n // 2, 0, 5] = wild                  # one element in the middle of each sequence
+        v[c + n - 1, -1] = wild                     # the last key's
+        k[c + n - 2, 0, 7] = NAN
+    got = ops.mha_packed_fwd(q, k, v, i32(cu), i32(cu), slopes=slopes, prefix_lens=i32(prefix) if prefix else None, **kw)
+    want, tol = ref.packed(q, k, v, cu, cu, slopes=slopes, prefix_lens=prefix, **kw)
+    fine = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(got), fine)
+    ref.check(torch.where(fine, got.double(), 0), torch.where(fine, want, 0), torch.where(fine, tol, 1), f"{lens} {kw}")
+
+
+def test_decode_unseen_keys_reach_nothing(ops):
+    """Keys before the window, in the tile where it starts, hold NaN."""
+    q, k, v = randn(2, 4, 128, seed=1), randn(40, 2, 16, 128, seed=2), randn(40, 2, 16, 128, seed=3)
+    t = torch.arange(40, dtype=torch.int32, device="cuda").view(2, 20)
+    lens = [300, 111]
+    for b, n in enumerate(lens):
+        for j in range(max(0, n - 45)):
+            k[b * 20 + j // 16, :, j % 16] = NAN
+            v[b * 20 + j // 16, :, j % 16] = math.inf
+    got = ops.mha_paged_decode(q, k, v, t, i32(lens), window=45)
+    want, tol = ref.decode(q, k, v, t, lens, window=45)
+    assert torch.isfinite(got).all()
+    ref.check(got, want, tol)
+
+
+def test_seen_nan_stays(ops):
+    q, k, v = randn(80, 2, 64, seed=1), randn(80, 2, 64, seed=2), randn(80, 2, 64, seed=3)
+    v[3] = NAN
+    out = ops.mha_packed_fwd(q, k, v, i32([0, 80]), i32([0, 80]))
+    assert torch.isfinite(out[:3]).all() and out[3:].isnan().all()
+    q[50, 0] = NAN
+    v[3] = 0
+    out = ops.mha_packed_fwd(q, k, v, i32([0, 80]), i32([0, 80]))
+    assert out[50, 0].isnan().all() and torch.isfinite(out[:50]).all() and torch.isfinite(out[51:]).all()
+    kc, vc = randn(3, 1, 16, 64, seed=4), randn(3, 1, 16, 64, seed=5)
+    kc[1, 0, 2] = NAN
+    out = ops.mha_paged_decode(randn(2, 2, 64, seed=6), kc, vc, i32([[0, 1, 2], [0, 2, 1]]), i32([48, 20]))
+    assert out[0].isnan().all() and torch.isfinite(out[1]).all()
+
+
+# ── streams, graphs, far offsets, a whole step ────────────────────────────────
+
+def test_other_stream(ops):
+    """The calls run on the current stream: inputs made there are seen without a wait."""
+    side = torch.cuda.Stream()
+    k, v = randn(64, 2, 16, 128, seed=1), randn(64, 2, 16, 128, seed=2)
+    t = torch.arange(64, dtype=torch.int32, device="cuda").view(1, 64)
+    q0 = randn(1, 4, 128, seed=3)
+    want = ops.mha_paged_decode(q0 * 2, k, v, t, i32([1000]))
+    lens = i32([1000])
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(10 ** 7)
+        got = ops.mha_paged_decode(q0 * 2, k, v, t, lens)
+    side.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_results_do_not_depend_on_the_run(ops):
+    """Twenty calls, and calls on two streams at once, give the same bits."""
+    q, k, v = randn(3, 16, 128, seed=1), randn(600, 4, 16, 128, seed=2), randn(600, 4, 16, 128, seed=3)
+    t = torch.arange(600, dtype=torch.int32, device="cuda").view(3, 200)
+    lens = i32([3200, 17, 1500])
+    want = ops.mha_paged_decode(q, k, v, t, lens)
+    for _ in range(20):
+        assert torch.equal(ops.mha_paged_decode(q, k, v, t, lens), want)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(10):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append(ops.mha_paged_decode(q, k, v, t, lens))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
+class Model:
+    """One attention block's state and a step of it: the operators as a program runs them."""
+
+    def __init__(self, ops, H=8, Hk=2, d=128, page=16, pages=80, N=3, M=20, dtype=torch.bfloat16, softcap=0.0, rot=64):
+        self.ops, self.H, self.Hk, self.d, self.page = ops, H, Hk, d, page
+        self.kc, self.vc = (torch.full((pages, Hk, page, d), NAN, dtype=dtype, device="cuda") for _ in range(2))
+        self.table = torch.full((N, M), -1, dtype=torch.int32, device="cuda")
+        self.lens = torch.zeros(N, dtype=torch.int32, device="cuda")
+        g = torch.Generator().manual_seed(5)
+        self.free = torch.randperm(pages, generator=g).int().cuda()
+        self.freq, self.amp = ops.rotary_frequencies(rot, scaling="yarn", factor=4.0, original_len=64, device="cuda")
+        self.softcap = softcap
+
+    def store(self, qkv, new, max_tokens):
+        o, H, Hk = self.ops, self.H, self.Hk
+        lens, cu, pos, slots, table, counts = o.paged_layout(self.lens, new, self.table, self.free, self.page, max_tokens)
+        q, k = o.rope_paged_store(qkv[:, :H], qkv[:, H:H + Hk], qkv[:, H + Hk:], pos, self.freq, slots, self.kc, self.vc, amplitude=self.amp)
+        return q, k, qkv[:, H + Hk:], lens, cu, table, counts
+
+    def prompt(self, qkv, new):
+        q, k, v, lens, cu, table, counts = self.store(qkv, new, qkv.shape[0])
+        out = self.ops.mha_packed_fwd(q, k, v, cu, cu, softcap=self.softcap)
+        self.lens, self.table, self.free = lens, table, self.free[int(counts[1]):].contiguous()
+        return out
+
+    def token(self, qkv, new):
+        q, _, _, lens, _, table, counts = self.store(qkv, new, qkv.shape[0])
+        return self.ops.mha_paged_decode(q, self.kc, self.vc, table, lens, softcap=self.softcap), lens, table, counts
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("softcap", [0.0, 20.0])
+def test_prompt_and_tokens_together(ops, dtype, softcap):
+    """Prompts, then tokens one by one, against attention in 64 bits over everything seen so far:
+    positions, slots, pages and lengths all have to agree for it to match."""
+    m = Model(ops, dtype=dtype, softcap=softcap)
+    H, Hk, d = m.H, m.Hk, m.d
+    lens = [37, 1, 90]
+    seen_q, seen_k, seen_v = ([[] for _ in lens] for _ in range(3))
+
+    def rotated(qkv, at):
+        pos = torch.tensor(at, device="cuda")
+        y, tol = ref.rotate(qkv[:, :H + Hk], pos, m.freq, False, m.amp)
+        return y.to(dtype), tol    # rounded as the operator rounds (ties apart, see below)
+
+    def compare(got, qkv, rows):
+        """rows: (request, position) of each row of got."""
+        turned, _ = rotated(qkv, [p for _, p in rows])
+        for i, (r, p) in enumerate(rows):
+            seen_k[r].append(turned[i, H:])
+            seen_v[r].append(qkv[i, H + Hk:])
+        for i, (r, p) in enumerate(rows):
+            k, v = torch.stack(seen_k[r])[:p + 1], torch.stack(seen_v[r])[:p + 1]
+            for h in range(H):
+                want, tol = ref.attend(turned[i, h:h + 1], k[:, h // (H // Hk)], v[:, h // (H // Hk)], ref.seen_mask(1, p + 1, True, 0, 0, "cuda"),
+                                       scale=d ** -0.5, softcap=softcap, dtype=dtype)
+                # a turned value may round the other way (its fp32 sum is off by 2^-20): a step of
+                # q or k in one of d products, d times at most, moves a score by u·Σ|q·k|·2^-7
+                u = ref.HALF_STEP[dtype]
+                slack = 2 * (u * 2.0 ** -7) * float((turned[i, h].double().abs() @ k[:, h // (H // Hk)].double().abs().T).max()) * d ** -0.5
+                ref.check(got[i, h:h + 1], want, tol + slack * (want.abs() + v.abs().double().amax()), f"request {r} position {p} head {h}")
+
+    qkv = randn(sum(lens), H + 2 * Hk, d, seed=9, dtype=dtype)
+    out = m.prompt(qkv, i32(lens))
+    compare(out, qkv, [(r, p) for r, n in enumerate(lens) for p in range(n)])
+    for step in range(4):
+        qkv = randn(3, H + 2 * Hk, d, seed=20 + step, dtype=dtype)
+        out, lens_t, table, counts = m.token(qkv, i32([1, 1, 1]))
+        m.lens, m.table, m.free = lens_t, table, m.free[int(counts[1]):].contiguous()
+        compare(out, qkv, [(r, n + step) for r, n in enumerate(lens)])
+    assert m.lens.tolist() == [n + 4 for n in lens]
+
+
+def test_step_in_a_graph(ops):
+    """A captured step, replayed with other lengths, tables and tokens in its inputs, between eager
+    work of the same kind and of a second graph that shares the memory pool: each replay is the
+    eager result."""
+    def inputs(seed):
+        qkv = randn(3, 12, 128, seed=seed)
+        lens = i32([100 + seed, 3 * seed, 33])
+        return qkv, lens
+
+    def fresh():
+        m = Model(ops)
+        m.kc.normal_()
+        m.vc.normal_()
+        m.table.copy_(torch.arange(60, dtype=torch.int32, device="cuda").view(3, 20))
+        return m
+
+    def eager(seed):
+        torch.manual_seed(3)
+        m = fresh()
+        qkv, lens = inputs(seed)
+        m.lens = lens
+        return (*m.token(qkv, i32([1, 1, 1])), m.kc.clone(), m.vc.clone())
+
+    torch.manual_seed(3)
+    m = fresh()
+    base_k, base_v = m.kc.clone(), m.vc.clone()
+    qkv, lens = inputs(1)
+    m.lens = lens
+    one = i32([1, 1, 1])
+    warm = torch.cuda.Stream()
+    warm.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(warm):
+        m.token(qkv, one)
+    torch.cuda.current_stream().wait_stream(warm)
+    graphs, outs = [], []
+    pool = torch.cuda.graph_pool_handle()
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            outs.append(m.token(qkv, one))
+        graphs.append(g)
+    for round_, seed in enumerate([1, 4, 2, 7, 4, 1]):
+        want = eager(seed)
+        q2, l2 = inputs(seed)
+        qkv.copy_(q2)
+        lens.copy_(l2)
+        m.kc.copy_(base_k)
+        m.vc.copy_(base_v)
+        i = round_ % 2
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        for a, b in zip((*outs[i], m.kc, m.vc), want):
+            assert torch.equal(a, b), (round_, seed)
+
+
+def test_cache_offsets_past_32_bits(ops):
+    """A cache of more than 2^32 elements: pages at its far end are written and read."""
+    P, Hk, page, d = 2 ** 32 // (2 * 16 * 128) + 40, 2, 16, 128
+    kc, vc = (torch.empty(P, Hk, page, d, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    T, H = 100, 4
+    far = [P - 1 - i * 2 for i in range(7)]
+    slots = torch.tensor([far[t // page] * page + t % page for t in range(T)], device="cuda")
+    q, k, v = randn(T, H, d, seed=1), randn(T, Hk, d, seed=2), randn(T, Hk, d, seed=3)
+    freq = ops.rotary_frequencies(d, device="cuda")[0]
+    qo, ko = ops.rope_paged_store(q, k, v, i32(list(range(T))), freq, slots, kc, vc)
+    small = torch.stack([kc[p] for p in far]), torch.stack([vc[p] for p in far])
+    assert torch.equal(small[0].transpose(1, 2).reshape(-1, Hk, d)[:T], ko)
+    got = ops.mha_paged_decode(qo[-1:], kc, vc, i32([far]), i32([T]))
+    assert torch.equal(got, ops.mha_paged_decode(qo[-1:], *small, i32([list(range(7))]), i32([T])))
+    del kc, vc
+    torch.cuda.empty_cache()
+
+
+def test_packed_offsets_past_32_bits(ops):
+    """Rows so far apart that their offsets pass 2^32 elements."""
+    d, H, Hk, T, step = 64, 2, 1, 1100, 2 ** 22 + 64
+    raw = torch.empty(T * step, dtype=torch.bfloat16, device="cuda")
+    x = raw.as_strided((T, H + 2 * Hk, d), (step, d, 1))
+    x.copy_(randn(T, H + 2 * Hk, d, seed=3))
+    cu = i32([0, 30, T])
+    far = ops.mha_packed_fwd(x[:, :H], x[:, H:H + Hk], x[:, H + Hk:], cu, cu)
+    y = x.contiguous()
+    assert torch.equal(far, ops.mha_packed_fwd(y[:, :H], y[:, H:H + Hk], y[:, H + Hk:], cu, cu))
+    del raw, x
+    torch.cuda.empty_cache()
+
+
+# ── refusals ──────────────────────────────────────────────────────────────────
+
+def refused(text, f, *args, **kw):
+    with pytest.raises(RuntimeError, match=text):
+        f(*args, **kw)
+
+
+def test_refusals_packed(ops):
+    q, k, cu = randn(8, 4, 64), randn(8, 2, 64), i32([0, 8])
+    f = ops.mha_packed_fwd
+    refused("float16 or bfloat16", f, q.float(), k.float(), k.float(), cu, cu)
+    refused("k dtype must match q", f, q, k.half(), k, cu, cu)
+    refused("k must be a CUDA tensor", f, q, k.cpu(), k, cu, cu)
+    refused("q must be 3D", f, q[0], k, k, cu, cu)
+    refused("head_dim mismatch", f, q, randn(8, 2, 128), k, cu, cu)
+    refused("token count mismatch", f, q, k, k[:7], cu, cu)
+    refused("n_kv_heads mismatch", f, q, k, randn(8, 1, 64), cu, cu)
+    refused("divisible", f, randn(8, 3, 64), k, k, cu, cu)
+    refused("Only head_dim", f, randn(8, 4, 96), randn(8, 2, 96), randn(8, 2, 96), cu, cu)
+    refused("innermost stride", f, randn(8, 64, 4).transpose(1, 2), k, k, cu, cu)
+    refused("multiples of 8", f, randn(8, 4, 65)[..., :64], k, k, cu, cu)
+    refused("16-byte aligned", f, randn(8 * 4 * 64 + 8)[4:-4].view(8, 4, 64), k, k, cu, cu)
+    refused("cu_q must be", f, q, k, k, cu.long(), cu)
+    refused("cu_k must have", f, q, k, k, cu, i32([0, 4, 8]))
+    refused("cu_q must be 1D", f, q, k, k, i32([]), i32([]))
+    refused("prefix_lens must have", f, q, k, k, cu, cu, prefix_lens=i32([1, 2]))
+    refused("slopes must be float32", f, q, k, k, cu, cu, slopes=slopes_of(4).double())
+    refused("slopes must be contiguous with 4", f, q, k, k, cu, cu, slopes=slopes_of(3))
+    for bad in (0.0, -1.0, math.inf, NAN):
+        refused("scale", f, q, k, k, cu, cu, scale=bad)
+    for bad in (-1.0, 1000.5, math.inf, NAN):
+        refused("softcap", f, q, k, k, cu, cu, softcap=bad)
+    refused("window", f, q, k, k, cu, cu, window=-1)
+    refused("forward only", f, q.clone().requires_grad_(), k, k, cu, cu)
+    with torch.no_grad():
+        f(q.clone().requires_grad_(), k, k, cu, cu)
+
+
+def test_refusals_decode(ops):
+    q, k, t, n = randn(2, 4, 64), randn(5, 2, 16, 64), i32([[0, 1], [2, 3]]), i32([20, 30])
+    f = ops.mha_paged_decode
+    refused("float16 or bfloat16", f, q.float(), k, k, t, n)
+    refused("v_cache dtype", f, q, k, k.half(), t, n)
+    refused("k_cache must be 4D", f, q, k[0], k, t, n)
+    refused("same shape", f, q, k, k[:4], t, n)
+    refused("head_dim mismatch", f, q, randn(5, 2, 16, 128), randn(5, 2, 16, 128), t, n)
+    refused("divisible", f, randn(2, 3, 64), k, k, t, n)
+    for page in (4, 24, 2048):
+        refused("page_size", f, q, randn(5, 2, page, 64), randn(5, 2, page, 64), t, n)
+    refused("block_table must be int32", f, q, k, k, t.long(), n)
+    refused("block_table must be int32", f, q, k, k, t[:1], n)
+    refused("block_table must have an innermost", f, q, k, k, i32([[0, 2], [1, 3]]).t(), n)
+    refused("kv_lens must be", f, q, k, k, t, n.long())
+    refused("kv_lens must have", f, q, k, k, t, i32([1]))
+    refused("window", f, q, k, k, t, n, window=2 ** 31)
+    refused("slopes", f, q, k, k, t, n, slopes=slopes_of(4).half())
+    refused("forward only", f, q, k.clone().requires_grad_(), k, t, n)
+
+
+def test_refusals_rope(ops):
+    T = 5
+    q, k, pos, slots = randn(T, 4, 64), randn(T, 2, 64), i32(range(T)), torch.arange(T, device="cuda")
+    freq, kc, vc = ops.rotary_frequencies(64, device="cuda")[0], randn(3, 2, 16, 64), randn(3, 2, 16, 64)
+    f = ops.rope_paged_store
+    refused("positions must be", f, q, k, k, pos.long(), freq, slots, kc, vc)
+    refused("slot_map must be", f, q, k, k, pos, freq, slots.int(), kc, vc)
+    refused("slot_map must have", f, q, k, k, pos, freq, slots[:4], kc, vc)
+    refused("inv_freq must be", f, q, k, k, pos, freq.float(), slots, kc, vc)
+    refused("inv_freq must be 1D", f, q, k, k, pos, freq[:12], slots, kc, vc)
+    refused("inv_freq must be 1D", f, q, k, k, pos, torch.cat([freq, freq]), slots, kc, vc)
+    refused("token count", f, q, k[:4], k, pos, freq, slots, kc, vc)
+    refused("k_cache must be", f, q, k, k, pos, freq, slots, randn(3, 1, 16, 64), vc)
+    refused("same shape", f, q, k, k, pos, freq, slots, kc, vc[:2])
+    refused("single memory location", f, q, k, k, pos, freq, slots, kc[:1].expand(3, 2, 16, 64), vc)
+    refused("overlap|same memory|single memory", f, q, k, k, pos, freq, slots, kc, kc)
+    refused("amplitude", f, q, k, k, pos, freq, slots, kc, vc, amplitude=NAN)
+    refused("forward only", f, q, k.clone().requires_grad_(), k, pos, freq, slots, kc, vc)
+
+
+def test_refusals_layout(ops):
+    a, t, fr = i32([1, 2]), i32([[0, 1], [2, 3]]), i32([4, 5])
+    f = ops.paged_layout
+    refused("seq_lens must be a CUDA", f, a.cpu(), a, t, fr, 16, 8)
+    refused("new_lens must have", f, a, a[:1], t, fr, 16, 8)
+    refused("new_lens must be", f, a, a.long(), t, fr, 16, 8)
+    refused("block_table", f, a, a, t.long(), fr, 16, 8)
+    refused("block_table", f, a, a, t[:1], fr, 16, 8)
+    refused("free_pages", f, a, a, t, fr.long(), 16, 8)
+    refused("free_pages", f, a, a, t, t, 16, 8)
+    refused("page_size", f, a, a, t, fr, 0, 8)
+    refused("max_tokens", f, a, a, t, fr, 16, -1)
+    many = torch.zeros(8193, dtype=torch.int32, device="cuda")
+    refused("at most 8192", f, many, many, many.view(-1, 1), fr, 16, 8)
