@@ -320,8 +320,9 @@ int paged_layout(const mi355_layout_params* p, hipStream_t st, const Err& err) {
   a.seq = p->seq_lens; a.fresh = p->new_lens; a.table_in = p->block_table; a.free_pages = p->free_pages;
   a.kv_lens = p->kv_lens; a.cu = p->cu_new; a.positions = p->positions; a.slots = p->slot_map; a.table = p->table; a.counts = p->counts;
   a.ts = p->table_stride; a.n = p->n; a.cols = p->table_cols; a.n_free = p->n_free; a.page = p->page_size; a.max_tokens = p->max_tokens;
-  const int64_t items = std::max((int64_t)p->n * p->table_cols, (int64_t)p->max_tokens);
-  const int64_t wgs = std::max<int64_t>(1, std::min<int64_t>((items + kLayoutThreads - 1) / kLayoutThreads, 2LL * dev.cus));
+  // a wave for each row of the table, a thread for each token
+  const int64_t items = std::max((int64_t)p->n * 64, (int64_t)p->max_tokens);
+  const int64_t wgs = std::max<int64_t>(1, std::min<int64_t>((items + kLayoutThreads - 1) / kLayoutThreads, dev.cus));
   paged_layout_kernel<<<dim3((unsigned)wgs), dim3(kLayoutThreads), (size_t)(2 * p->n + 1) * 4, st>>>(a);
   return launched(err, "paged_layout");
 }
