@@ -73,12 +73,12 @@ __device__ __forceinline__ int wave_max(int x) {   // of values >= 0, over the w
 // 0 .. tq. All waves find the same, each for itself, 64 segments at a time; of more
 // than 62 sequences (short ones, then) there is one class.
 __device__ __forceinline__ bool find_block(const PackedArgs& a, int t, RowBlock& rb) {
-  const int lane = threadIdx.x & 63, BM = 1 << a.bm_shift;
+  const int lane = threadIdx.x & 63;
   const int iters = (a.n + 2 + 63) / 64;
-  struct Seg { int c0, rows, k0, lk, pre, blocks; };
+  struct Seg { int c0, rows, k0, lk, pre; };
   auto segment = [&](int it) __attribute__((always_inline)) {
     const int e = it * 64 + lane;
-    Seg x{0, 0, 0, 0, 0, 0};
+    Seg x{0, 0, 0, 0, 0};
     if (e <= a.n + 1) {
       const bool real = e >= 1 && e <= a.n;
       const int c1 = e == a.n + 1 ? a.tq : a.cu_q[e], k1 = real ? a.cu_k[e] : 0;
@@ -89,38 +89,30 @@ __device__ __forceinline__ bool find_block(const PackedArgs& a, int t, RowBlock&
       x.k0 = min(max(k0, 0), a.tk);
       x.lk = real ? max(0, min(max(k1, 0), a.tk) - x.k0) : 0;
       x.pre = min(max(pre, 0), x.lk);
-      x.blocks = (x.rows + BM - 1) >> a.bm_shift;
     }
     return x;
   };
-  // keys that block b of a segment spans, about; more for later blocks, or the same
-  auto span_of = [&](const Seg& x, int b) {
-    if (!a.causal) return a.window > x.lk / 2 ? x.lk : 2 * a.window;
-    const int hi = min(x.lk, (b + 1) * BM + x.lk - x.rows);
-    return max(0, min(hi, a.window));
-  };
+  const RowSpans rs{a.causal, a.window, a.bm_shift};
   Seg x = segment(0);
   const int levels = iters == 1 ? a.levels : 1;
-  const int most = levels > 1 ? wave_max(x.blocks ? span_of(x, x.blocks - 1) : 0) : 0;
+  int most = 0;
+  if (levels > 1) {
+    const int n = block_count(rs, x.rows);
+    most = wave_max(n ? block_span(rs, x.rows, x.lk, n - 1) : 0);
+  }
   int run = 0;
 #pragma unroll 1
   for (int level = 0; level < levels; ++level) {
-    const int above = level == levels - 1 ? -1 : most >> (level + 1);   // blocks that span more
-    const int below = level == 0 ? INT_MAX : most >> level;              // and at most this
-    auto first_over = [&](const Seg& s, int lim) {   // of a segment's blocks, the first that spans more than lim
-      if (s.blocks == 0 || span_of(s, s.blocks - 1) <= lim) return s.blocks;
-      if (span_of(s, 0) > lim) return 0;
-      return min(s.blocks, (lim - (s.lk - s.rows)) >> a.bm_shift);   // causal: (b + 1)·BM + lk − rows > lim
-    };
     for (int it = 0; it < iters; ++it) {
       if (iters > 1) x = segment(it);
-      const int b0 = first_over(x, above), b1 = first_over(x, below), cnt = b1 - b0;
+      const int b0 = first_over(rs, x.rows, x.lk, class_floor(most, level, levels));
+      const int cnt = first_over(rs, x.rows, x.lk, class_ceil(most, level)) - b0;
       const int incl = wave_scan(cnt);
       const uint64_t hit = __builtin_amdgcn_ballot_w64(run + incl > t);
       if (hit) {
         const int l = __builtin_ctzll(hit);
         const int left = run + (int)__builtin_amdgcn_readlane(incl, l) - 1 - t;   // blocks of the class behind t in its segment
-        rb.m0 = ((int)__builtin_amdgcn_readlane(b0, l) + left) * BM;
+        rb.m0 = ((int)__builtin_amdgcn_readlane(b0, l) + left) << a.bm_shift;
         rb.q0 = __builtin_amdgcn_readlane(x.c0, l);
         rb.lq = __builtin_amdgcn_readlane(x.rows, l);
         rb.k0 = __builtin_amdgcn_readlane(x.k0, l);

@@ -19,7 +19,6 @@
 //    in a ragged batch is shared by many workgroups and a short one is not split.
 //    Parts (O, max, sum, fp32) of a shared sequence are joined by a second kernel.
 
-constexpr int kDecTile = 32;    // keys per wave tile
 constexpr int kDecWaves = 4;
 constexpr int kDecHeads = 16;   // heads of a group per workgroup
 
@@ -49,17 +48,8 @@ __device__ __forceinline__ f32x4 mfma16(typename Elt<BF16>::v8 a, typename Elt<B
   else return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// The tiles that a request's keys span: its first seen tile, and their number.
-struct Keys {
-  int len, first, tile0, tiles;
-};
-__device__ __forceinline__ Keys keys_of(const DecodeArgs& a, int b) {
-  Keys k;
-  k.len = max(0, (int)min((int64_t)a.lens[b], (int64_t)a.cols << a.shift));
-  k.first = max(0, k.len - a.window);
-  k.tile0 = k.first / kDecTile;
-  k.tiles = (k.len + kDecTile - 1) / kDecTile - k.tile0;
-  return k;
+__device__ __forceinline__ KeySpan keys_of(const DecodeArgs& a, int b) {
+  return key_span(a.lens[b], (int64_t)a.cols << a.shift, a.window);
 }
 
 // Part w: request, head group, place among the request's parts. All waves of the
@@ -73,15 +63,14 @@ __device__ __forceinline__ bool find_part(const DecodeArgs& a, int w, Part& p) {
     p = Part{w / hgs, w % hgs, 0, 1, 0};
     return true;
   }
-  // (a request counts for 2^20 tiles at most, 2^25 keys, so that sums stay below 2^31)
   int sum = 0;
-  for (int i = lane; i < a.b; i += 64) sum += min(keys_of(a, i).tiles, 1 << 20);
+  for (int i = lane; i < a.b; i += 64) sum += weighed(keys_of(a, i).tiles);
   sum = __builtin_amdgcn_readlane(wave_scan(sum), 63);
-  const int per = (int)max((int64_t)a.least, ((int64_t)sum * hgs + a.target - 1) / a.target);
+  const int per = part_size(sum, hgs, a.target, a.least);
   int run = 0;
   for (int base = 0; base < a.b; base += 64) {
     const int i = base + lane;
-    const int n = i < a.b ? max(1, (min(keys_of(a, i).tiles, 1 << 20) + per - 1) / per) : 0;
+    const int n = i < a.b ? part_count(keys_of(a, i).tiles, per) : 0;
     const int incl = wave_scan(n * hgs);
     const uint64_t hit = __builtin_amdgcn_ballot_w64(run + incl > w);
     if (hit) {
@@ -117,11 +106,10 @@ void paged_decode_kernel(const DecodeArgs a) {
   const int l16 = lane & 15, g = lane >> 4;
 
   const int page_size = 1 << a.shift;
-  const Keys ks = keys_of(a, b);
+  const KeySpan ks = keys_of(a, b);
   const int len = uni(ks.len), first = uni(ks.first), tile0 = uni(ks.tile0), tiles = uni(ks.tiles);
   // tiles of this part, this wave: t_lo + wave, + WAVES, ...
-  const int per = (tiles + pt.parts - 1) / pt.parts;
-  const int t_lo = tile0 + min(tiles, pt.part * per), t_hi = tile0 + min(tiles, (pt.part + 1) * per);
+  const int t_lo = tile0 + part_start(tiles, pt.parts, pt.part), t_hi = tile0 + part_start(tiles, pt.parts, pt.part + 1);
 
   // Q of the wave's heads: B operand, column l16, d = 8·(4·kd + g)
   V8 qreg[KD];

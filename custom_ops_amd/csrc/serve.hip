@@ -18,6 +18,7 @@
 
 #include "mi355_serve.h"
 #include "gfx950.h"
+#include "serve_sched.h"
 
 namespace mi355fa {
 namespace {
@@ -82,7 +83,6 @@ bool rows_ok(const void* p, std::initializer_list<int64_t> strides) {
 }
 
 bool window_ok(int w) { return w >= 0; }
-constexpr int kNoWindow = 1 << 30;
 int window_of(int w) { return w == 0 ? kNoWindow : std::min(w, kNoWindow); }
 
 // The factors of a call's scores (PackedArgs, DecodeArgs); false where scale or
@@ -179,8 +179,6 @@ int packed_fwd(const mi355_packed_params* p, hipStream_t st, const Err& err) {
   return launched(err, "mha_packed_fwd");
 }
 
-constexpr int kDecMaxScan = 1024;
-
 struct DecodePlan {
   int groups, split, target, least;
   int64_t grid;   // workgroups, and parts at most
@@ -221,6 +219,7 @@ int decode_check(const mi355_decode_params* p, const Err& err) {
   if (p->b < 0 || p->num_pages < 0 || p->table_cols < 0) return err.fail(MI355_SERVE_EINVAL, "negative dimension");
   if (p->page_size < 8 || p->page_size > 1024 || (p->page_size & (p->page_size - 1)))
     return err.fail(MI355_SERVE_EINVAL, "page_size must be a power of two in 8 .. 1024");
+  if ((int64_t)p->table_cols * p->page_size > kMaxRows) return err.fail(MI355_SERVE_EINVAL, "block_table must span at most 2^30 keys");
   if (!window_ok(p->window)) return err.fail(MI355_SERVE_EINVAL, "window must be 0 (none) or positive");
   return MI355_SERVE_OK;
 }

@@ -168,7 +168,7 @@ Tensor mha_paged_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_
   TORCH_CHECK(block_table.scalar_type() == at::kInt && block_table.dim() == 2 && block_table.size(0) == B,
               "block_table must be int32 of shape (batch, pages)");
   TORCH_CHECK(block_table.size(1) <= 1 || block_table.stride(1) == 1, "block_table must have an innermost stride of 1");
-  TORCH_CHECK(block_table.size(1) * page <= INT_MAX, "block_table must span fewer than 2^31 keys");
+  TORCH_CHECK(block_table.size(1) <= (1 << 30) / page, "block_table must span at most 2^30 keys");
   check_ints(kv_lens, q, "kv_lens", at::kInt, B);
   check_scores(scale, softcap, window);
   mi355_decode_params p{};

@@ -84,7 +84,7 @@ int mi355_packed_fwd(const mi355_packed_params* p, void* stream, char* err, size
  * row j % page_size of page block_table[n][j / page_size], j < kv_lens[n]; its row
  * is at the last key. Layouts: q, o [b, h, d]; caches [num_pages, h_k, page_size, d]
  * (strides as above); block_table [b, table_cols]. A page number outside the cache
- * hides that page's keys; kv_lens past table_cols·page_size count as that.
+ * hides that page's keys; kv_lens past table_cols·page_size (2^30 at most) count as that.
  */
 typedef struct mi355_decode_params {
   const void* q;
