@@ -8,9 +8,10 @@
 // core; the vector unit's exponentials (one per pair, three with a cap) run
 // beside them.
 //
-//  * A workgroup serves BM = 32·WAVES rows of one sequence and one head; each
-//    wave owns 32 of them and computes Sᵀ = K·Qᵀ, so that a lane holds one row's
-//    scores. No mask is read: a row's seen keys are [lo, hi) and [0, prefix), and
+//  * A workgroup is RW·KG waves: RW of 32 rows each, of one sequence and `pack` heads
+//    of one KV head, and KG groups of them that take every KG-th key tile and join
+//    their sums in LDS at the end. A wave computes Sᵀ = K·Qᵀ, so that a lane holds one
+//    row's scores. No mask is read: a row's seen keys are [lo, hi) and [0, prefix), and
 //    only key tiles that a border crosses compare keys with them.
 //  * Key tiles that no row of the workgroup sees are not visited.
 //  * Offsets stay on the device: the workgroup finds its rows by a scan over the
@@ -126,11 +127,15 @@ __device__ __forceinline__ bool find_block(const PackedArgs& a, int t, RowBlock&
   return false;
 }
 
+// Keys of a tile; and waves per SIMD: of two workgroups on a CU where their LDS allows it
+template <int D, int KG> constexpr int kKeys = KG * D > 256 ? 32 : 64;
+template <int D, int RW, int KG> constexpr int kWavesPerEu = RW * KG / 4 * (2 * 4 * KG * kKeys<D, KG> * D * 2 <= 160 * 1024 ? 2 : 1);
+
 template <int D, bool BF16, bool CAP, bool BIAS, int RW, int KG>
-__global__ __launch_bounds__(64 * RW * KG) __attribute__((amdgpu_waves_per_eu(D == 64 && KG < 4 ? 4 : 2)))
+__global__ __launch_bounds__(64 * RW * KG) __attribute__((amdgpu_waves_per_eu(kWavesPerEu<D, RW, KG>)))
 void packed_fwd_kernel(const PackedArgs a) {
   typedef typename Elt<BF16>::v8 V8;
-  constexpr int WAVES = RW * KG, NKB = KG * D > 256 ? 1 : 2, kTile = 32 * NKB;   // keys per tile
+  constexpr int WAVES = RW * KG, kTile = kKeys<D, KG>, NKB = kTile / 32;
   constexpr int UPR = D / 8, KD = D / 16, DB = D / 32;
   constexpr int kElems = kTile * D, kWaveLoads = kTile * UPR / 64;   // of a K or V tile
   constexpr int kLoads = (kWaveLoads + WAVES - 1) / WAVES;

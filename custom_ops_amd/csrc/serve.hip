@@ -148,32 +148,39 @@ int packed_fwd(const mi355_packed_params* p, hipStream_t st, const Err& err) {
   a.v_ts = p->v_token_stride; a.v_hs = p->v_head_stride; a.o_ts = p->o_token_stride; a.o_hs = p->o_head_stride;
   a.tq = p->total_q; a.tk = p->total_k; a.n = p->n_seqs; a.h = p->h; a.ratio = p->h / p->h_k;
   a.causal = p->causal != 0; a.window = window_of(p->window);
-  // Rows a workgroup: 256, one wave each 32; 128 with two groups of waves that take every
-  // other key tile; 64 with four. Fewer rows make more workgroups with shorter chains of
-  // tiles, and read K and V more often. By the workgroups that 256 rows would make
-  // (us for 256 / 128 / 64 rows, bf16, 16/4 heads, d = 128 unless noted):
-  //   many: 8192 tokens 250 / 277 / 410; 24 documents, 8000 tokens 46 / 61 / 105
-  //   about one a CU: 4000 tokens 103 / 80 / 117; 2000 tokens 55 / 37 / 44
-  //   a quarter of that: 1000 tokens 31 / 22 / 20; 4000 tokens, 4 heads 97 / 60 / 51
-  // d = 64 has two workgroups of 128 on a CU: 8000 tokens 174 / 157 / 240.
+  // A workgroup's shape: 4 waves of 32 rows (two workgroups on a CU); 8 waves, 4 of rows
+  // by 2 groups that take every other key tile; 2 by 4; or 2 by 2. More groups make
+  // shorter chains of tiles, fewer rows more workgroups, which read K and V more often.
+  // By the workgroups that 256 rows each would make (us for the four shapes, bf16, 16/4
+  // heads, d = 128; * chosen):
+  //   more than CUs: 8192 tokens 266* / 290 / 419 / 457; 24 documents, 8000 tokens
+  //     42* / 63 / 107 / 102; 8 documents, 4000 tokens 35* / 42 / 68 / 66
+  //   up to CUs: 4000 tokens 95 / 82* / 121 / 127; 2000 tokens 46 / 38* / 45 / 44
+  //   a quarter: 4000 tokens, 4 heads 79 / 61 / 52* / 55; 500 tokens 16 / 16 / 14 / 14*;
+  //     100 tokens, 8 heads 9.0 / 9.9 / 9.9 / 8.9*
+  // d = 64 keeps two 8-wave workgroups on a CU: 8000 tokens 162 / 163* / 248 / 198, 24
+  // documents of 8 heads 28 / 24* / 44 / 27.
   const int64_t full = (((int64_t)p->total_q + 255) / 256 + p->n_seqs / 2) * p->h;
-  const bool long_keys = p->total_k / std::max(p->n_seqs, 1) > 256;   // more than the four groups take at once
-  const int rows = full <= dev.cus / 4 && long_keys ? 64 : p->d == 64 || full <= dev.cus + dev.cus / 4 ? 128 : 256;
+  enum { k4x1, k4x2, k2x4, k2x2 };
+  const int shape = full <= dev.cus / 4 ? (p->total_k / std::max(p->n_seqs, 1) > 512 ? k2x4 : k2x2)
+                    : p->d == 64 || full <= dev.cus ? k4x2 : k4x1;
+  const int rows = shape == k4x1 || shape == k4x2 ? 128 : 64;
   // Heads that share a KV head share a workgroup: the same keys for fewer rows of a
-  // sequence, so short ones waste less (100 documents, 8000 tokens: 68 us, packed 36).
+  // sequence, so short ones waste less (100 documents, 8000 tokens: 68 us, together 32).
   a.pack = std::min(a.ratio % 4 == 0 ? 4 : a.ratio % 2 == 0 ? 2 : 1, rows / 32);
   a.bm_shift = __builtin_ctz((unsigned)(rows / a.pack));
   const int64_t blocks = ((int64_t)p->total_q >> a.bm_shift) + p->n_seqs + 2, total = blocks * (p->h / a.pack);
-  a.levels = total > dev.cus ? 4 : 1;   // the order matters once workgroups wait for others
+  a.levels = total > 2 * dev.cus ? 4 : 1;   // the order matters once workgroups wait for others
   if (total >= (1LL << 31)) return err.fail(MI355_SERVE_EINVAL, "problem too large: %lld workgroups", (long long)total);
   by_type(p->d, p->dtype == MI355_SERVE_BF16, [&](auto d, auto bf) {
     by_scores(p->softcap > 0.f, p->slopes != nullptr, [&](auto cap, auto bias) {
       constexpr int D = decltype(d)::value;
       constexpr bool BF = decltype(bf)::value, CAP = decltype(cap)::value, BIAS = decltype(bias)::value;
-      const dim3 grid((unsigned)total), wg(512);
-      if (rows == 256) packed_fwd_kernel<D, BF, CAP, BIAS, 8, 1><<<grid, wg, 0, st>>>(a);
-      else if (rows == 128) packed_fwd_kernel<D, BF, CAP, BIAS, 4, 2><<<grid, wg, 0, st>>>(a);
-      else packed_fwd_kernel<D, BF, CAP, BIAS, 2, 4><<<grid, wg, 0, st>>>(a);
+      const dim3 grid((unsigned)total);
+      if (shape == k4x2) packed_fwd_kernel<D, BF, CAP, BIAS, 4, 2><<<grid, dim3(512), 0, st>>>(a);
+      else if (shape == k2x4) packed_fwd_kernel<D, BF, CAP, BIAS, 2, 4><<<grid, dim3(512), 0, st>>>(a);
+      else if (shape == k2x2) packed_fwd_kernel<D, BF, CAP, BIAS, 2, 2><<<grid, dim3(256), 0, st>>>(a);
+      else if constexpr (D == 128) packed_fwd_kernel<D, BF, CAP, BIAS, 4, 1><<<grid, dim3(256), 0, st>>>(a);
     });
   });
   return launched(err, "mha_packed_fwd");
