@@ -171,6 +171,20 @@ __device__ __forceinline__ float psum8(typename Elt<BF16>::v8 v, float acc) {
 // readfirstlane of a value the caller knows to be uniform
 __device__ __forceinline__ int uni(int x) { return (int)__builtin_amdgcn_readfirstlane((uint32_t)x); }
 
+// The kernel's parameter struct, read again from the kernarg segment (scalar loads, behind
+// an empty asm statement) where an epilogue needs it: held from the kernel's entry across
+// a tile loop its fields would spill.
+template <class T> using kernarg = const __attribute__((address_space(4))) T;
+template <class T> __device__ __forceinline__ kernarg<T>& reload_kernarg(const T& host) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  kernarg<T>* q = (kernarg<T>*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(q));
+  return *q;
+#else
+  return *(kernarg<T>*)&host;   // host pass only: never runs
+#endif
+}
+
 // XOR swizzle of V's 16-byte chunks by LDS row, for conflict-free transposed reads
 template <int D> __device__ __forceinline__ int v_swz(int r) {
   return (D == 128) ? 4 * (r & 3) : 4 * ((r >> 1) & 1);

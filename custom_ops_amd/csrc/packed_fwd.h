@@ -37,6 +37,7 @@ struct PackedArgs {
   int bm_shift;         // log2 of a block's rows: 32·RW / pack
   int levels;           // classes of block lengths (find_block)
   float u_scale;        // capped: 2·log2(e)·scale / softcap
+  float tanh_lim, tanh_p[4];   // capped: scores up to which tanh is the polynomial, and its factors
   float c2;             // scores u to log2 units: scale·log2(e), capped 2·softcap·log2(e)
   float bias;           // slopes to u: −1/scale, capped −1/(2·softcap)
 };
@@ -271,23 +272,52 @@ void packed_fwd_kernel(const PackedArgs a) {
   auto softmax_pv = [&](int base, const uint16_t* tV) __attribute__((always_inline)) {
     const uint8_t* v8 = reinterpret_cast<const uint8_t*>(tV);
     // u: scores up to the factor c2. Capped: tanh z = 1 − 2 / (e^{2z} + 1), and the
-    // 1 cancels in the softmax, so u = −1 / (e^{2z} + 1) with c2 = 2·softcap·log2(e)
+    // 1 cancels in the softmax, so u = −1 / (e^{2z} + 1) with c2 = 2·softcap·log2(e).
+    // Where all of the wave's |z| are below 1/2 it is (tanh z − 1) / 2 with tanh z / z as
+    // a polynomial in z² (least squares in Chebyshev nodes, off by 6·10^-7): 5 operations
+    // of 4 cycles a score, where the two transcendental ones take 16 each.
     float u[16 * NKB];   // key 32·(c / 16) + c % 16, from the lane's first
-    const float x0 = (float)(ia - base - g * 16);
 #pragma unroll
-    for (int c = 0; c < 16 * NKB; ++c) {
-      u[c] = s[c / 16][c % 16];
-      if constexpr (CAP) u[c] = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(u[c] * a.u_scale));
-      if constexpr (BIAS && CAP) u[c] = __builtin_fmaf(bco, __builtin_fabsf(x0 - (float)(c / 16 * 32 + c % 16)), u[c]);
+    for (int c = 0; c < 16 * NKB; ++c) u[c] = s[c / 16][c % 16];
+    if constexpr (CAP) {
+      const float x0 = (float)(ia - base - g * 16);
+      auto biased = [&](int c, float x) {
+        return BIAS ? __builtin_fmaf(bco, __builtin_fabsf(x0 - (float)(c / 16 * 32 + c % 16)), x) : x;
+      };
+      bool small = false;
+      if constexpr (D == 128) {   // (d = 64 has no registers for the choice at 4 waves a SIMD)
+        float big = 0.f;
+#pragma unroll
+        for (int c = 0; c < 16 * NKB; ++c) big = fmaxf(big, __builtin_fabsf(u[c]));
+        small = __builtin_amdgcn_ballot_w64(big > a.tanh_lim) == 0;
+      }
+      if (small) {
+#pragma unroll
+        for (int c = 0; c < 16 * NKB; ++c) {
+          const float t = u[c] * u[c];
+          const float p = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(a.tanh_p[3], t, a.tanh_p[2]), t, a.tanh_p[1]), t, a.tanh_p[0]);
+          u[c] = biased(c, __builtin_fmaf(u[c], p, -0.5f));
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 16 * NKB; ++c) u[c] = biased(c, __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(u[c] * a.u_scale)));
+      }
     }
-    // only a tile that a border crosses compares
+    // Only a tile that a border crosses hides scores: a bit for each key of the lane, and
+    // two operations a score (a compare with each border takes four and the scalar unit's)
     const bool full = base + kTile <= pre || (base + kTile <= w_hi0 && base >= w_lo1);
     if (!full) {
-      const int h_r = hi - base - g * 16, l_r = lo - base - g * 16, p_r = pl - base - g * 16;
 #pragma unroll
-      for (int c = 0; c < 16 * NKB; ++c) {
-        const int k = c / 16 * 32 + c % 16;
-        u[c] = (k < h_r && k >= l_r) || k < p_r ? u[c] : -INFINITY;
+      for (int b = 0; b < NKB; ++b) {
+        const int first = base + b * 32 + g * 16;   // the lane's 16 keys
+        auto below = [&](int x) { return (1u << min(max(x - first, 0), 16)) - 1u; };   // keys before x
+        const int hidden = (int)~((below(hi) & ~below(lo)) | below(pl));
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint32_t h = (uint32_t)__builtin_amdgcn_sbfe(hidden, i, 1);   // all ones where hidden
+          float& x = u[b * 16 + i];
+          x = __uint_as_float((h & 0xff800000u) | (~h & __float_as_uint(x)));
+        }
       }
     }
     float mx = -INFINITY;
@@ -400,6 +430,7 @@ void packed_fwd_kernel(const PackedArgs a) {
     }
   }
 
+  kernarg<PackedArgs>& z = reload_kernarg(a);
   // O through LDS, each wave in a slice of its own (which no other wave reads), so that
   // a store instruction writes whole rows
   uint8_t* stg = KG > 1 ? reinterpret_cast<uint8_t*>(sj + rw * (KG - 1) * kJoin) : reinterpret_cast<uint8_t*>(sKV[0]) + wave * 32 * D * 2;
@@ -426,14 +457,14 @@ void packed_fwd_kernel(const PackedArgs a) {
       const int c = db * 4 + q4;
       *reinterpret_cast<u32x2*>(stg + l32 * D * 2 + ((c ^ (l32 & (CH - 1))) * 16) + g * 8) = packed;
     }
-  const rsrc_t ro = make_rsrc(a.o + (int64_t)(rb.q0 + w0) * a.o_ts + (int64_t)h * a.o_hs,
-                              span(min(32, rb.lq - w0), a.o_ts));
+  const rsrc_t ro = make_rsrc(z.o + (int64_t)(rb.q0 + w0) * z.o_ts + (int64_t)h * z.o_hs,
+                              span(min(32, rb.lq - w0), z.o_ts));
   const int ch = lane % CH, r0 = lane / CH;
 #pragma unroll
   for (int k = 0; k < 32 / RPI; ++k) {
     const int r = r0 + k * RPI;
     const u32x4 x = *reinterpret_cast<const u32x4*>(stg + r * D * 2 + ((ch ^ (r & (CH - 1))) * 16));
-    __builtin_amdgcn_raw_buffer_store_b128(x, ro, (uint32_t)(r * (int)a.o_ts + ch * 8) * 2u, 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b128(x, ro, (uint32_t)(r * (int)z.o_ts + ch * 8) * 2u, 0, 0);
   }
 
   // A tile that a border crosses multiplies the V of its unseen keys by a P of 0, which
@@ -445,6 +476,8 @@ void packed_fwd_kernel(const PackedArgs a) {
   if (rows) {
     wait_vmcnt<0>();   // the rows are stored
     constexpr int C = D / 64;   // columns lane, lane + 64 of a row
+    const uint16_t* kz = z.k + (int64_t)k0 * z.k_ts + (int64_t)hk * z.k_hs;
+    const uint16_t* vz = z.v + (int64_t)k0 * z.v_ts + (int64_t)hk * z.v_hs;
     auto num = [](uint16_t x) {
       if constexpr (BF16) return __uint_as_float((uint32_t)x << 16);
       else return (float)bitcast<_Float16>(x);
@@ -452,7 +485,7 @@ void packed_fwd_kernel(const PackedArgs a) {
     while (rows) {
       const int r = __builtin_ctz(rows);
       rows &= rows - 1;
-      const int at = w0 + r + off, r_hi = hi_of(at), r_lo = lo_of(at);
+      const int at = w0 + r + off, r_hi = min(lk, z.causal ? at + 1 : at + z.window), r_lo = max(0, at - z.window + 1);
       auto sees = [&](int j) { return (j < r_hi && j >= r_lo) || j < pre; };
       bool out[C], unseen[C] = {}, known[C] = {}, again[C], any = false;
 #pragma unroll
@@ -467,7 +500,7 @@ void packed_fwd_kernel(const PackedArgs a) {
         for (int j = base; j < min(base + kTile, lk); ++j)
 #pragma unroll
           for (int c = 0; c < C; ++c) {
-            const bool wild = !(__builtin_fabsf(num(vb[(int64_t)j * a.v_ts + lane + 64 * c])) < INFINITY);
+            const bool wild = !(__builtin_fabsf(num(vz[(int64_t)j * z.v_ts + lane + 64 * c])) < INFINITY);
             unseen[c] |= wild && !sees(j);
             known[c] |= wild && sees(j);
           }
@@ -475,8 +508,8 @@ void packed_fwd_kernel(const PackedArgs a) {
 #pragma unroll
       for (int c = 0; c < C; ++c) any |= again[c] = out[c] && unseen[c] && !known[c];
       if (!__builtin_amdgcn_ballot_w64(any)) continue;
-      const uint16_t* q = a.q + (int64_t)(rb.q0 + w0 + r) * a.q_ts + (int64_t)h * a.q_hs;
-      const float bc = BIAS ? a.slopes[h] * a.bias : 0.f;
+      const uint16_t* q = z.q + (int64_t)(rb.q0 + w0 + r) * z.q_ts + (int64_t)h * z.q_hs;
+      const float bc = BIAS ? z.slopes[h] * z.bias : 0.f;
       float m = -INFINITY, sum = 0.f, acc[C] = {};
       for (int t = 0; t < cnt; ++t) {
         const int base = tile_at(t) * kTile, j = base + lane;   // a key each lane
@@ -484,8 +517,8 @@ void packed_fwd_kernel(const PackedArgs a) {
         float u = -INFINITY;
         if (seen) {
           u = 0.f;
-          for (int d = 0; d < D; ++d) u = __builtin_fmaf(num(q[d]), num(kb[(int64_t)j * a.k_ts + d]), u);
-          if constexpr (CAP) u = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(u * a.u_scale));
+          for (int d = 0; d < D; ++d) u = __builtin_fmaf(num(q[d]), num(kz[(int64_t)j * z.k_ts + d]), u);
+          if constexpr (CAP) u = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(u * z.u_scale));
           if constexpr (BIAS) u = __builtin_fmaf(bc, __builtin_fabsf((float)(at - j)), u);
         }
         float top = u;
@@ -502,12 +535,12 @@ void packed_fwd_kernel(const PackedArgs a) {
           const int x = __builtin_ctzll(left);
           const float p = __shfl(w, x);
 #pragma unroll
-          for (int c = 0; c < C; ++c) acc[c] = __builtin_fmaf(p, num(vb[(int64_t)(base + x) * a.v_ts + lane + 64 * c]), acc[c]);
+          for (int c = 0; c < C; ++c) acc[c] = __builtin_fmaf(p, num(vz[(int64_t)(base + x) * z.v_ts + lane + 64 * c]), acc[c]);
         }
       }
 #pragma unroll
       for (int x = 1; x < 64; x *= 2) sum += __shfl_xor(sum, x);
-      uint16_t* o = a.o + (int64_t)(rb.q0 + w0 + r) * a.o_ts + (int64_t)h * a.o_hs;
+      uint16_t* o = z.o + (int64_t)(rb.q0 + w0 + r) * z.o_ts + (int64_t)h * z.o_hs;
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         const float y = acc[c] / sum;

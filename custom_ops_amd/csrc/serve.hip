@@ -143,6 +143,12 @@ int packed_fwd(const mi355_packed_params* p, hipStream_t st, const Err& err) {
   if (!dev.gfx950) return err.fail(MI355_SERVE_EDEVICE, "mi355_serve: current HIP device is not gfx950 (MI355X)");
 
   a.q = (const uint16_t*)p->q; a.k = (const uint16_t*)p->k; a.v = (const uint16_t*)p->v; a.o = (uint16_t*)p->o;
+  if (p->softcap > 0.f) {
+    // (tanh z) / 2 = k·u·(c0 + c1·z² + ..) / 2 with z = k·u; powers of a k below 10^-5 would underflow
+    const double c[4] = {0.999999464, -0.3332637607, 0.1319091244, -0.04441858165}, k = (double)p->scale / p->softcap;
+    for (int i = 0; i < 4; ++i) a.tanh_p[i] = (float)(0.5 * c[i] * pow(k, 2 * i + 1));
+    a.tanh_lim = k >= 1e-5 && k <= 1e5 ? (float)(0.5 / k) : -1.f;
+  }
   a.cu_q = p->cu_q; a.cu_k = p->cu_k; a.prefix = p->prefix_lens; a.slopes = p->slopes;
   a.q_ts = p->q_token_stride; a.q_hs = p->q_head_stride; a.k_ts = p->k_token_stride; a.k_hs = p->k_head_stride;
   a.v_ts = p->v_token_stride; a.v_hs = p->v_head_stride; a.o_ts = p->o_token_stride; a.o_hs = p->o_head_stride;
