@@ -69,11 +69,14 @@ Device device_info() {
   return d;
 }
 
-// Restores the launch error state around one launch and names what failed.
-int launched(const Err& err, const char* what) {
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return err.fail(MI355_SERVE_ELAUNCH, "%s: launch failed: %s", what, hipGetErrorString(e));
-  return MI355_SERVE_OK;
+// Launches; the error is the launch's own, whatever an earlier call left behind.
+template <class A>
+int run(const Err& err, const char* what, void (*kernel)(const A), int64_t grid, int threads, size_t lds, hipStream_t st, A& a) {
+  void* args[] = {&a};
+  const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(kernel), dim3((unsigned)grid), dim3((unsigned)threads), args, lds, st);
+  if (e == hipSuccess) return MI355_SERVE_OK;
+  (void)hipGetLastError();
+  return err.fail(MI355_SERVE_ELAUNCH, "%s: launch failed: %s", what, hipGetErrorString(e));
 }
 
 bool rows_ok(const void* p, std::initializer_list<int64_t> strides) {
@@ -178,18 +181,19 @@ int packed_fwd(const mi355_packed_params* p, hipStream_t st, const Err& err) {
   const int64_t blocks = ((int64_t)p->total_q >> a.bm_shift) + p->n_seqs + 2, total = blocks * (p->h / a.pack);
   a.levels = total > 2 * dev.cus ? 4 : 1;   // the order matters once workgroups wait for others
   if (total >= (1LL << 31)) return err.fail(MI355_SERVE_EINVAL, "problem too large: %lld workgroups", (long long)total);
+  int rc = MI355_SERVE_OK;
   by_type(p->d, p->dtype == MI355_SERVE_BF16, [&](auto d, auto bf) {
     by_scores(p->softcap > 0.f, p->slopes != nullptr, [&](auto cap, auto bias) {
       constexpr int D = decltype(d)::value;
       constexpr bool BF = decltype(bf)::value, CAP = decltype(cap)::value, BIAS = decltype(bias)::value;
-      const dim3 grid((unsigned)total);
-      if (shape == k4x2) packed_fwd_kernel<D, BF, CAP, BIAS, 4, 2><<<grid, dim3(512), 0, st>>>(a);
-      else if (shape == k2x4) packed_fwd_kernel<D, BF, CAP, BIAS, 2, 4><<<grid, dim3(512), 0, st>>>(a);
-      else if (shape == k2x2) packed_fwd_kernel<D, BF, CAP, BIAS, 2, 2><<<grid, dim3(256), 0, st>>>(a);
-      else if constexpr (D == 128) packed_fwd_kernel<D, BF, CAP, BIAS, 4, 1><<<grid, dim3(256), 0, st>>>(a);
+      auto go = [&](void (*kernel)(const PackedArgs), int waves) { rc = run(err, "mha_packed_fwd", kernel, total, 64 * waves, 0, st, a); };
+      if (shape == k4x2) go(packed_fwd_kernel<D, BF, CAP, BIAS, 4, 2>, 8);
+      else if (shape == k2x4) go(packed_fwd_kernel<D, BF, CAP, BIAS, 2, 4>, 8);
+      else if (shape == k2x2) go(packed_fwd_kernel<D, BF, CAP, BIAS, 2, 2>, 4);
+      else if constexpr (D == 128) go(packed_fwd_kernel<D, BF, CAP, BIAS, 4, 1>, 4);
     });
   });
-  return launched(err, "mha_packed_fwd");
+  return rc;
 }
 
 struct DecodePlan {
@@ -269,14 +273,16 @@ int paged_decode(const mi355_decode_params* p, hipStream_t st, const Err& err) {
   const int64_t total = pl.grid;
   if (total >= (1LL << 31) || (int64_t)p->b * p->h >= (1LL << 31))
     return err.fail(MI355_SERVE_EINVAL, "problem too large: %lld workgroups", (long long)total);
+  int rc = MI355_SERVE_OK;
   by_type(p->d, p->dtype == MI355_SERVE_BF16, [&](auto d, auto bf) {
     constexpr int D = decltype(d)::value;
+    constexpr bool BF = decltype(bf)::value;
     by_scores(p->softcap > 0.f, p->slopes != nullptr, [&](auto cap, auto bias) {
-      paged_decode_kernel<D, decltype(bf)::value, decltype(cap)::value, decltype(bias)::value, kDecWaves><<<dim3((unsigned)total), dim3(64 * kDecWaves), 0, st>>>(a);
+      rc = run(err, "mha_paged_decode", paged_decode_kernel<D, BF, decltype(cap)::value, decltype(bias)::value, kDecWaves>, total, 64 * kDecWaves, 0, st, a);
     });
-    if (pl.split) paged_join_kernel<D, decltype(bf)::value><<<dim3((unsigned)((int64_t)p->b * p->h)), dim3(256), 0, st>>>(a);
+    if (rc == MI355_SERVE_OK && pl.split) rc = run(err, "mha_paged_decode (join)", paged_join_kernel<D, BF>, (int64_t)p->b * p->h, 256, 0, st, a);
   });
-  return launched(err, "mha_paged_decode");
+  return rc;
 }
 
 int rope_store(const mi355_rope_params* p, hipStream_t st, const Err& err) {
@@ -308,13 +314,13 @@ int rope_store(const mi355_rope_params* p, hipStream_t st, const Err& err) {
   a.vc_ps = p->vc_page_stride; a.vc_hs = p->vc_head_stride; a.vc_rs = p->vc_row_stride;
   a.num_slots = (int64_t)p->num_pages * p->page_size;
   a.t = p->t; a.h = p->h; a.hk = p->h_k; a.rot = p->rot; a.page = p->page_size; a.amplitude = p->amplitude;
+  int rc = MI355_SERVE_OK;
   by_type(p->d, p->dtype == MI355_SERVE_BF16, [&](auto d, auto bf) {
     constexpr int D = decltype(d)::value;
     constexpr bool BF = decltype(bf)::value;
-    if (p->interleaved) rope_store_kernel<D, BF, true, 1><<<dim3((unsigned)p->t), dim3(256), 0, st>>>(a);
-    else rope_store_kernel<D, BF, false, 1><<<dim3((unsigned)p->t), dim3(256), 0, st>>>(a);
+    rc = run(err, "rope_paged_store", p->interleaved ? rope_store_kernel<D, BF, true, 1> : rope_store_kernel<D, BF, false, 1>, p->t, 256, 0, st, a);
   });
-  return launched(err, "rope_paged_store");
+  return rc;
 }
 
 int paged_layout(const mi355_layout_params* p, hipStream_t st, const Err& err) {
@@ -335,8 +341,7 @@ int paged_layout(const mi355_layout_params* p, hipStream_t st, const Err& err) {
   // a wave for each row of the table, a thread for each token
   const int64_t items = std::max((int64_t)p->n * 64, (int64_t)p->max_tokens);
   const int64_t wgs = std::max<int64_t>(1, std::min<int64_t>((items + kLayoutThreads - 1) / kLayoutThreads, dev.cus));
-  paged_layout_kernel<<<dim3((unsigned)wgs), dim3(kLayoutThreads), (size_t)(2 * p->n + 1) * 4, st>>>(a);
-  return launched(err, "paged_layout");
+  return run(err, "paged_layout", paged_layout_kernel, wgs, kLayoutThreads, (size_t)(2 * p->n + 1) * 4, st, a);
 }
 
 }  // namespace

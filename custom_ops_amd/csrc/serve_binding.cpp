@@ -90,6 +90,7 @@ void check_ints(const Tensor& x, const Tensor& q, const char* name, at::ScalarTy
 const float* slopes_of(const Maybe& s, const Tensor& q, int64_t heads) {
   if (!s.has_value()) return nullptr;
   check_gpu(*s, q, "slopes");
+  check_no_grad({&*s});
   TORCH_CHECK(s->scalar_type() == at::kFloat, "slopes must be float32");
   TORCH_CHECK(s->dim() == 1 && s->size(0) == heads && s->is_contiguous(), "slopes must be contiguous with ", heads, " elements");
   return s->data_ptr<float>();
@@ -99,7 +100,7 @@ int type_of(const Tensor& q) { return q.scalar_type() == at::kBFloat16 ? MI355_S
 
 void check_scores(std::optional<double> scale, double softcap, int64_t window) {
   TORCH_CHECK(!scale.has_value() || (*scale > 0 && std::isfinite(*scale)), "scale must be positive and finite");
-  TORCH_CHECK(softcap >= 0 && softcap <= 1000, "softcap must be 0 (none) or in (0, 1000]");
+  TORCH_CHECK(softcap >= 0 && softcap <= 1000 && (softcap == 0 || (float)softcap > 0), "softcap must be 0 (none) or in (0, 1000]");
   TORCH_CHECK(window >= 0 && window <= INT_MAX, "window must be 0 (none) or positive");
 }
 
@@ -205,7 +206,7 @@ std::tuple<Tensor, Tensor> rope_paged_store(const Tensor& q, const Tensor& k, co
                                             const Tensor& slot_map, const Tensor& k_cache, const Tensor& v_cache, bool interleaved,
                                             double amplitude) {
   check_half(q);
-  check_no_grad({&q, &k, &v, &k_cache, &v_cache});
+  check_no_grad({&q, &k, &v, &k_cache, &v_cache, &inv_freq});
   check_rows(q, q, "q", 3);
   check_rows(k, q, "k", 3);
   check_rows(v, q, "v", 3);

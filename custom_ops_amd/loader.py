@@ -554,8 +554,14 @@ class ServeOps(FAOps):
 
     def _tree(self) -> tuple:
         path, native = Path(_build.SERVE_LIB_PATH), Path(_build.SERVE_OPS_PATH)
-        if not path.exists():
-            _build.build_serve()
-        if not _build.ops_current(str(native), _build.SERVE_BINDING_SRC):
-            _build.build_serve_ops()
+
+        def missing():
+            return not path.exists() or not _build.ops_current(str(native), _build.SERVE_BINDING_SRC)
+        if missing():   # one process of several builds
+            with open(path.parent / f".{self.so_name}.build.lock", "a") as lockf:
+                fcntl.flock(lockf, fcntl.LOCK_EX)
+                if not path.exists():
+                    _build.build_serve()
+                elif missing():
+                    _build.build_serve_ops()
         return path.resolve(strict=True), native

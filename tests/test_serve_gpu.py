@@ -739,3 +739,8 @@ def test_refusals_layout(ops):
     refused("max_tokens", f, a, a, t, fr, 16, -1)
     many = torch.zeros(8193, dtype=torch.int32, device="cuda")
     refused("at most 8192", f, many, many, many.view(-1, 1), fr, 16, 8)
+
+
+def test_decode_more_requests_than_are_scanned(ops):
+    """Beyond 1024 requests a workgroup serves a request each, whatever its length."""
+    decode_case(ops, [(i * 7) % 50 for i in range(1100)] + [900], H=2, Hk=1, d=64)
