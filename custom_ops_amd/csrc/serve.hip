@@ -208,11 +208,12 @@ DecodePlan decode_plan(const mi355_decode_params* p, int cus) {
   pl.groups = (ratio + kDecHeads - 1) / kDecHeads;
   const int64_t units = (int64_t)p->b * p->h_k * pl.groups;
   const int64_t tiles = ((int64_t)p->table_cols * p->page_size + kDecTile - 1) / kDecTile;
-  // Parts to make: two workgroups of 4 waves are resident on a CU. With many units
-  // their remainders would leave a half-empty second round, so twice as many, smaller
-  // parts ([32 x <= 8192, 16/4, 128]: 47 us against 55); with few, each part more costs
-  // the join ([131072, 32/4, 128]: 51 against 55).
-  pl.target = (int)std::clamp<int64_t>(8 * units, 2 * cus, 4 * cus);
+  // Parts to make, beside a remainder for each unit. Two workgroups of 4 waves are
+  // resident on a CU. Few units: all parts at once, one a CU or two (any count between
+  // leaves CUs unequal: [131072 keys, 32/4, 128] 256 parts 57.6 us, 320 72.4, 512 59.4;
+  // [6 x <= 39725, 16/8] 464 + 48 parts 124 us, 512 + 48 146). More: several rounds of
+  // small parts ([32 x <= 8192, 16/4] 384 + 128: 56.6 us, 1024 + 128: 55.0).
+  pl.target = (int)(units <= 16 ? cus - units : units <= cus / 4 ? 2 * cus - units : 4 * cus);
   // A CU alone reads about 40 GB/s, so even short sequences are shared once that pays
   // for the join's launch, about 5 us: [1000 keys, 16/4, 128] 18.3 us whole, 10.3 in
   // parts of 4 tiles; [500, 8/8, 64] (16 tiles) 7.1 whole, 8.9 in parts.
