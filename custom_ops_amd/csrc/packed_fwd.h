@@ -36,6 +36,7 @@ struct PackedArgs {
   int pack;             // heads of one KV head that share a workgroup: divides ratio, 1, 2 or 4
   int bm_shift;         // log2 of a block's rows: 32·RW / pack
   int levels;           // classes of block lengths (find_block)
+  int fold;             // see folded
   float u_scale;        // capped: 2·log2(e)·scale / softcap
   float tanh_lim, tanh_p[4];   // capped: scores up to which tanh is the polynomial, and its factors
   float c2;             // scores u to log2 units: scale·log2(e), capped 2·softcap·log2(e)
@@ -146,7 +147,7 @@ void packed_fwd_kernel(const PackedArgs a) {
   // i % 8, so a KV head's keys stay on few XCDs' L2
   RowBlock rb;
   const int groups = a.h / a.pack, hks = a.h / a.ratio;
-  if (!find_block(a, blockIdx.x / groups, rb)) return;
+  if (!find_block(a, folded(blockIdx.x / groups, a.fold, gridDim.x / groups), rb)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
   const int rw = wave % RW, kg = wave / RW;
   const int l32 = lane & 31, g = lane >> 5;

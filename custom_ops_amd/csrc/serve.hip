@@ -180,6 +180,14 @@ int packed_fwd(const mi355_packed_params* p, hipStream_t st, const Err& err) {
   a.bm_shift = __builtin_ctz((unsigned)(rows / a.pack));
   const int64_t blocks = ((int64_t)p->total_q >> a.bm_shift) + p->n_seqs + 2, total = blocks * (p->h / a.pack);
   a.levels = total > 2 * dev.cus ? 4 : 1;   // the order matters once workgroups wait for others
+  // Two workgroups on a CU: the second ones in reverse order, so that the longest block
+  // shares its CU with the shortest (24 documents, 16/4 heads, d = 128: 43.6 -> 41.2 us;
+  // 4000 tokens, d = 64: 54.6 -> 50.6).
+  const int heads = p->h / a.pack;
+  if (shape == k4x1 || (shape == k4x2 && p->d == 64)) {
+    a.fold = dev.cus % heads == 0 && total > dev.cus ? dev.cus / heads : 0;
+    if (a.fold) a.levels = 4;
+  }
   if (total >= (1LL << 31)) return err.fail(MI355_SERVE_EINVAL, "problem too large: %lld workgroups", (long long)total);
   int rc = MI355_SERVE_OK;
   by_type(p->d, p->dtype == MI355_SERVE_BF16, [&](auto d, auto bf) {

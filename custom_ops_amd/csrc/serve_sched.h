@@ -42,6 +42,13 @@ MI355_HD inline int first_over(const RowSpans& s, int rows, int lk, int lim) {
 MI355_HD inline int class_floor(int most, int level, int levels) { return level == levels - 1 ? -1 : most >> (level + 1); }
 MI355_HD inline int class_ceil(int most, int level) { return level == 0 ? INT_MAX : most >> level; }
 
+// Workgroups of ranks [fold, 2·fold) of `ranks` take their blocks in reverse order (fold 0:
+// none): the first `fold` ranks give every CU its first workgroup.
+MI355_HD inline int folded(int rank, int fold, int ranks) {
+  const int end = imin(2 * fold, ranks);
+  return rank >= fold && rank < end ? fold + end - 1 - rank : rank;
+}
+
 // ── paged decode: parts of requests ──────────────────────────────────────────
 constexpr int kDecTile = 32;   // keys per tile
 

@@ -113,6 +113,12 @@ def test_packed_eight_wave_grid(ops):
     packed_case(ops, [2100, 2000], H=16, Hk=16, d=64, window=700, softcap=30.0, slopes=True, prefix=[100, 3], dtype=torch.float16)
 
 
+@pytest.mark.parametrize("T", [4300, 5000, 7900, 8300])
+def test_packed_between_one_and_two_workgroups_a_cu(ops, T):
+    packed_case(ops, [T], H=8, Hk=8, d=64, window=300)
+    packed_case(ops, [T // 2, 33, T // 3], H=4, Hk=1, d=64)
+
+
 def test_packed_many_sequences(ops):
     """More sequences than a wave has lanes, empty ones among them."""
     packed_case(ops, [(i * 7) % 40 for i in range(200)], H=2, Hk=1, d=64)

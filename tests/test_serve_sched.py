@@ -61,6 +61,15 @@ int main() {
       REQUIRE((int)seen.size() == blocks);
     }
   }
+  for (int round = 0; round < 2000; ++round) {   // every rank has a block of its own
+    const int ranks = pick(1, 300), fold = pick(0, 200);
+    std::set<int> seen;
+    for (int r = 0; r < ranks; ++r) {
+      const int b = folded(r, fold, ranks);
+      REQUIRE(b >= 0 && b < ranks && seen.insert(b).second);
+      REQUIRE((b < fold) == (r < fold) && (b < 2 * fold) == (r < 2 * fold));
+    }
+  }
   // the largest sizes
   {
     RowSpans s{1, kNoWindow, 5};
