@@ -48,34 +48,38 @@ __device__ __forceinline__ f32x4 mfma16(typename Elt<BF16>::v8 a, typename Elt<B
   else return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-__device__ __forceinline__ KeySpan keys_of(const DecodeArgs& a, int b) {
-  return key_span(a.lens[b], (int64_t)a.cols << a.shift, a.window);
+__device__ __forceinline__ KeySpan keys_of(const DecodeArgs& a, int len) {
+  return key_span(len, (int64_t)a.cols << a.shift, a.window);
 }
 
 // Part w: request, head group, place among the request's parts. All waves of the
 // workgroup find the same, each for itself: two passes over the lengths, 64 at a time.
 struct Part {
   int b, hg, part, parts, slot;   // slot: of part 0
+  int len;                        // the request's keys
 };
 __device__ __forceinline__ bool find_part(const DecodeArgs& a, int w, Part& p) {
   const int hgs = a.hk * a.groups, lane = threadIdx.x & 63;
   if (!a.split) {
-    p = Part{w / hgs, w % hgs, 0, 1, 0};
+    p = Part{w / hgs, w % hgs, 0, 1, 0, 0};
+    p.len = a.lens[p.b];
     return true;
   }
   int sum = 0;
-  for (int i = lane; i < a.b; i += 64) sum += weighed(keys_of(a, i).tiles);
+  for (int i = lane; i < a.b; i += 64) sum += weighed(keys_of(a, a.lens[i]).tiles);
   sum = __builtin_amdgcn_readlane(wave_scan(sum), 63);
   const int per = part_size(sum, hgs, a.target, a.least);
   int run = 0;
   for (int base = 0; base < a.b; base += 64) {
     const int i = base + lane;
-    const int n = i < a.b ? part_count(keys_of(a, i).tiles, per) : 0;
+    const int len = i < a.b ? a.lens[i] : 0;
+    const int n = i < a.b ? part_count(keys_of(a, len).tiles, per) : 0;
     const int incl = wave_scan(n * hgs);
     const uint64_t hit = __builtin_amdgcn_ballot_w64(run + incl > w);
     if (hit) {
       const int l = __builtin_ctzll(hit);
       p.b = base + l;
+      p.len = __builtin_amdgcn_readlane(len, l);
       p.parts = __builtin_amdgcn_readlane(n, l);
       const int start = run + (int)__builtin_amdgcn_readlane(incl, l) - p.parts * hgs;
       p.hg = (w - start) / p.parts;
@@ -106,7 +110,7 @@ void paged_decode_kernel(const DecodeArgs a) {
   const int l16 = lane & 15, g = lane >> 4;
 
   const int page_size = 1 << a.shift;
-  const KeySpan ks = keys_of(a, b);
+  const KeySpan ks = keys_of(a, pt.len);
   const int len = uni(ks.len), first = uni(ks.first), tile0 = uni(ks.tile0), tiles = uni(ks.tiles);
   // tiles of this part, this wave: t_lo + wave, + WAVES, ...
   const int t_lo = tile0 + part_start(tiles, pt.parts, pt.part), t_hi = tile0 + part_start(tiles, pt.parts, pt.part + 1);
@@ -205,6 +209,8 @@ void paged_decode_kernel(const DecodeArgs a) {
     f32x8 pf;
 #pragma unroll
     for (int e = 0; e < 8; ++e) pf[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e / 4][e % 4], c2, -mlog2));
+    // P rounded for the second product, and its sum of the rounded: normalised by their
+    // own sum, the weights' errors are independent and O's about that of its own rounding
     const V8 p = __builtin_convertvector(pf, V8);
     l_run = psum8<BF16>(p, l_run);
     // Vᵀ: lane s of a 16-lane group reads 4 columns of row 4·g + s/4 (and 16 + that)
