@@ -544,7 +544,7 @@ void packed_fwd_kernel(const PackedArgs a) {
       uint16_t* o = z.o + (int64_t)(rb.q0 + w0 + r) * z.o_ts + (int64_t)h * z.o_hs;
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        const float y = acc[c] / sum;
+        const float y = sum == 0.f ? 0.f : acc[c] / sum;
         if (again[c]) {
           if constexpr (BF16) o[lane + 64 * c] = bitcast<uint16_t>((__bf16)y);
           else o[lane + 64 * c] = bitcast<uint16_t>((_Float16)y);

@@ -425,6 +425,20 @@ def test_packed_unseen_keys_reach_nothing(ops, wild, d, H, lens, kw):
     ref.check(torch.where(fine, got.double(), 0), torch.where(fine, want, 0), torch.where(fine, tol, 1), f"{lens} {kw}")
 
 
+@pytest.mark.parametrize("wild", [NAN, math.inf])
+@pytest.mark.parametrize("d,H,lens_q,lens_k", [(64, 2, [40], [10]), (128, 4, [300], [70]), (128, 16, [1500, 3000, 1100], [700, 2900, 1])])
+def test_packed_rows_that_see_nothing_stay_0(ops, wild, d, H, lens_q, lens_k):
+    """Rows in front of the first key share tiles with rows that see keys; no value reaches them."""
+    cq, ck = cu_of(lens_q), cu_of(lens_k)
+    q, k, v = randn(cq[-1], H, d, seed=1), randn(ck[-1], H // 2, d, seed=2), randn(ck[-1], H // 2, d, seed=3)
+    for c, n in zip(ck, lens_k):
+        v[c + n // 2:c + n] = wild
+    got = ops.mha_packed_fwd(q, k, v, i32(cq), i32(ck))
+    for c, n, m in zip(cq, lens_q, lens_k):
+        assert (got[c:c + n - m] == 0).all()
+        assert torch.isfinite(got[c:c + n - m + m // 2]).all()
+
+
 def test_decode_unseen_keys_reach_nothing(ops):
     """Keys before the window, in the tile where it starts, hold NaN."""
     q, k, v = randn(2, 4, 128, seed=1), randn(40, 2, 16, 128, seed=2), randn(40, 2, 16, 128, seed=3)
