@@ -470,8 +470,8 @@ void packed_fwd_kernel(const PackedArgs a) {
 
   // A tile that a border crosses multiplies the V of its unseen keys by a P of 0, which
   // makes NaN of what is not finite. So rows of finite weights with such values look at
-  // the unseen keys of those tiles, and where one of them, and no seen one, holds a value
-  // that is not finite in a column, that column is formed again from the seen keys alone.
+  // the unseen keys of those tiles, and where one of them holds a value that is not finite
+  // in a column, and no seen one a NaN, that column is formed again from the seen keys alone.
   const uint64_t odds = __builtin_amdgcn_ballot_w64(odd && mine && l < INFINITY);
   uint32_t rows = (uint32_t)(odds | odds >> 32);
   if (rows) {
@@ -501,9 +501,9 @@ void packed_fwd_kernel(const PackedArgs a) {
         for (int j = base; j < min(base + kTile, lk); ++j)
 #pragma unroll
           for (int c = 0; c < C; ++c) {
-            const bool wild = !(__builtin_fabsf(num(vz[(int64_t)j * z.v_ts + lane + 64 * c])) < INFINITY);
-            unseen[c] |= wild && !sees(j);
-            known[c] |= wild && sees(j);
+            const float x = num(vz[(int64_t)j * z.v_ts + lane + 64 * c]);
+            unseen[c] |= !(__builtin_fabsf(x) < INFINITY) && !sees(j);
+            known[c] |= x != x && sees(j);
           }
       }
 #pragma unroll

@@ -439,6 +439,22 @@ def test_packed_rows_that_see_nothing_stay_0(ops, wild, d, H, lens_q, lens_k):
         assert torch.isfinite(got[c:c + n - m + m // 2]).all()
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("wild", [NAN, -math.inf])
+def test_packed_seen_infinity_beside_unseen_values(ops, d, wild):
+    """An infinity that a row sees is its result, whatever unseen keys of the tile hold there."""
+    n = 200
+    q, k, v = randn(n, 2, d, seed=1), randn(n, 2, d, seed=2), randn(n, 2, d, seed=3)
+    v[130, :, 5], v[150, :, 5] = math.inf, wild
+    v[140, :, 6], v[150, :, 6] = NAN, wild
+    got = ops.mha_packed_fwd(q, k, v, i32([0, n]), i32([0, n]))
+    assert torch.isfinite(got[:130]).all()
+    assert (got[130:150, :, 5] == math.inf).all() and got[150:, :, 5].isnan().all()
+    assert torch.isfinite(got[:140, :, 6]).all() and got[140:, :, 6].isnan().all()
+    rest = [c for c in range(d) if c not in (5, 6)]
+    assert torch.isfinite(got[:, :, rest]).all()
+
+
 def test_decode_unseen_keys_reach_nothing(ops):
     """Keys before the window, in the tile where it starts, hold NaN."""
     q, k, v = randn(2, 4, 128, seed=1), randn(40, 2, 16, 128, seed=2), randn(40, 2, 16, 128, seed=3)
