@@ -72,6 +72,8 @@ Device device_info() {
 // Launches; the error is the launch's own, whatever an earlier call left behind.
 template <class A>
 int run(const Err& err, const char* what, void (*kernel)(const A), int64_t grid, int threads, size_t lds, hipStream_t st, A& a) {
+  // (a launch counts its threads in 32 bits)
+  if (grid * threads >= (1LL << 32)) return err.fail(MI355_SERVE_EINVAL, "%s: problem too large: %lld workgroups", what, (long long)grid);
   void* args[] = {&a};
   const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(kernel), dim3((unsigned)grid), dim3((unsigned)threads), args, lds, st);
   if (e == hipSuccess) return MI355_SERVE_OK;
@@ -188,7 +190,6 @@ int packed_fwd(const mi355_packed_params* p, hipStream_t st, const Err& err) {
     a.fold = dev.cus % heads == 0 && total > dev.cus ? dev.cus / heads : 0;
     if (a.fold) a.levels = 4;
   }
-  if (total >= (1LL << 31)) return err.fail(MI355_SERVE_EINVAL, "problem too large: %lld workgroups", (long long)total);
   int rc = MI355_SERVE_OK;
   by_type(p->d, p->dtype == MI355_SERVE_BF16, [&](auto d, auto bf) {
     by_scores(p->softcap > 0.f, p->slopes != nullptr, [&](auto cap, auto bias) {
@@ -280,8 +281,6 @@ int paged_decode(const mi355_decode_params* p, hipStream_t st, const Err& err) {
   a.part_ml = (float*)((char*)p->workspace + pl.ml);
   a.part_o = (float*)((char*)p->workspace + pl.o);
   const int64_t total = pl.grid;
-  if (total >= (1LL << 31) || (int64_t)p->b * p->h >= (1LL << 31))
-    return err.fail(MI355_SERVE_EINVAL, "problem too large: %lld workgroups", (long long)total);
   int rc = MI355_SERVE_OK;
   by_type(p->d, p->dtype == MI355_SERVE_BF16, [&](auto d, auto bf) {
     constexpr int D = decltype(d)::value;

@@ -221,6 +221,10 @@ std::tuple<Tensor, Tensor> rope_paged_store(const Tensor& q, const Tensor& k, co
   at::assert_no_internal_overlap(k_cache);   // written in place
   at::assert_no_internal_overlap(v_cache);
   at::assert_no_overlap(k_cache, v_cache);
+  for (const Tensor* x : {&q, &k, &v}) {
+    at::assert_no_overlap(k_cache, *x);
+    at::assert_no_overlap(v_cache, *x);
+  }
   check_groups(H, Hk);
   check_head_dim(d);
   TORCH_CHECK(T <= (1 << 30) && P <= INT_MAX && page <= INT_MAX, "too many tokens or pages");

@@ -758,7 +758,21 @@ def test_refusals_rope(ops):
     refused("single memory location", f, q, k, k, pos, freq, slots, kc[:1].expand(3, 2, 16, 64), vc)
     refused("overlap|same memory|single memory", f, q, k, k, pos, freq, slots, kc, kc)
     refused("amplitude", f, q, k, k, pos, freq, slots, kc, vc, amplitude=NAN)
+    inner = kc.view(-1)[: T * 2 * 64].view(T, 2, 64)
+    refused("overlap|same memory|single memory", f, q, inner, k, pos, freq, slots, kc, vc)
+    refused("overlap|same memory|single memory", f, q, k, inner, pos, freq, slots, kc, vc)
     refused("forward only", f, q, k.clone().requires_grad_(), k, pos, freq, slots, kc, vc)
+
+
+def test_refusals_of_launches_past_32_bits(ops):
+    """2^24 workgroups of 256 threads are more than a launch counts."""
+    T = 2 ** 24
+    row, pos = randn(1, 1, 64), torch.zeros(T, dtype=torch.int32, device="cuda")
+    freq, c = ops.rotary_frequencies(64, device="cuda")[0], torch.zeros(2, 1, 1, 16, 64, dtype=torch.bfloat16, device="cuda")
+    x = row.expand(T, 1, 64)
+    refused("too large", ops.rope_paged_store, x, x, x, pos, freq, pos.long(), c[0], c[1])
+    t = torch.zeros(1, 1, dtype=torch.int32, device="cuda").expand(T, 1)
+    refused("too large", ops.mha_paged_decode, x, c[0], c[1], t, pos)
 
 
 def test_refusals_layout(ops):
