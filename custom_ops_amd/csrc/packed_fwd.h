@@ -274,12 +274,23 @@ void packed_fwd_kernel(const PackedArgs a) {
     const uint8_t* v8 = reinterpret_cast<const uint8_t*>(tV);
     // u: scores up to the factor c2. Capped: tanh z = 1 − 2 / (e^{2z} + 1), and the
     // 1 cancels in the softmax, so u = −1 / (e^{2z} + 1) with c2 = 2·softcap·log2(e).
-    // Where all of the wave's |z| are below 1/2 it is (tanh z − 1) / 2 with tanh z / z as
-    // a polynomial in z² (least squares in Chebyshev nodes, off by 6·10^-7): 5 operations
-    // of 4 cycles a score, where the two transcendental ones take 16 each.
+    // Where |z| is below 1/2 it is (tanh z − 1) / 2 with tanh z / z as a polynomial in z²
+    // (least squares in Chebyshev nodes, off by 6·10^-7): 5 operations of 4 cycles a score,
+    // where the two transcendental ones take 16 each. The two forms differ in their last
+    // bits, so no score of an unseen key may choose: the whole wave chooses together on a
+    // tile that all of its rows see, each lane by the scores its row sees on the others.
     float u[16 * NKB];   // key 32·(c / 16) + c % 16, from the lane's first
 #pragma unroll
     for (int c = 0; c < 16 * NKB; ++c) u[c] = s[c / 16][c % 16];
+    // Only a tile that a border crosses hides scores: a bit for each key of the lane, and
+    // two operations a score (a compare with each border takes four and the scalar unit's)
+    auto crossed = [&]() { return base + kTile > pre && (base + kTile > w_hi0 || base < w_lo1); };
+    auto hidden_of = [&](int b) {   // of the lane's 16 keys
+      const int first = base + b * 32 + g * 16;
+      auto below = [&](int x) { return (1u << min(max(x - first, 0), 16)) - 1u; };   // keys before x
+      return (int)~((below(hi) & ~below(lo)) | below(pl));
+    };
+    auto hides = [](int hidden, int i) { return (uint32_t)__builtin_amdgcn_sbfe(hidden, i, 1); };   // all ones where hidden
     if constexpr (CAP) {
       const float x0 = (float)(ia - base - g * 16);
       auto biased = [&](int c, float x) {
@@ -288,9 +299,19 @@ void packed_fwd_kernel(const PackedArgs a) {
       bool small = false;
       if constexpr (D == 128) {   // (d = 64 has no registers for the choice at 4 waves a SIMD)
         float big = 0.f;
+        if (crossed()) {
 #pragma unroll
-        for (int c = 0; c < 16 * NKB; ++c) big = fmaxf(big, __builtin_fabsf(u[c]));
-        small = __builtin_amdgcn_ballot_w64(big > a.tanh_lim) == 0;
+          for (int b = 0; b < NKB; ++b) {
+            const int hidden = hidden_of(b);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) big = fmaxf(big, __uint_as_float(__float_as_uint(u[b * 16 + i]) & 0x7fffffffu & ~hides(hidden, i)));
+          }
+          small = !(big > a.tanh_lim);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 16 * NKB; ++c) big = fmaxf(big, __builtin_fabsf(u[c]));
+          small = __builtin_amdgcn_ballot_w64(big > a.tanh_lim) == 0;
+        }
       }
       if (small) {
 #pragma unroll
@@ -304,18 +325,13 @@ void packed_fwd_kernel(const PackedArgs a) {
         for (int c = 0; c < 16 * NKB; ++c) u[c] = biased(c, __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(u[c] * a.u_scale)));
       }
     }
-    // Only a tile that a border crosses hides scores: a bit for each key of the lane, and
-    // two operations a score (a compare with each border takes four and the scalar unit's)
-    const bool full = base + kTile <= pre || (base + kTile <= w_hi0 && base >= w_lo1);
-    if (!full) {
+    if (crossed()) {
 #pragma unroll
       for (int b = 0; b < NKB; ++b) {
-        const int first = base + b * 32 + g * 16;   // the lane's 16 keys
-        auto below = [&](int x) { return (1u << min(max(x - first, 0), 16)) - 1u; };   // keys before x
-        const int hidden = (int)~((below(hi) & ~below(lo)) | below(pl));
+        const int hidden = hidden_of(b);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const uint32_t h = (uint32_t)__builtin_amdgcn_sbfe(hidden, i, 1);   // all ones where hidden
+          const uint32_t h = hides(hidden, i);
           float& x = u[b * 16 + i];
           x = __uint_as_float((h & 0xff800000u) | (~h & __float_as_uint(x)));
         }
