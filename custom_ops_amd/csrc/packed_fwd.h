@@ -204,7 +204,8 @@ void packed_fwd_kernel(const PackedArgs a) {
         const int tile = tile_at(i * KG + j), left = lk - tile * kTile;
         issue(kb, a.k_ts, k_off, tile, sKV[st] + j * kElems);
         issue(vb, a.v_ts, v_off, tile, sKV[2 + st] + j * kElems);
-        // V rows behind the last key, which the DMA leaves as they are, meet a P of 0
+        // V rows behind the last key are 0, since they meet a P of 0. They lie outside the
+        // resource (V's rows do not overlap: v_ts >= D), so the DMA brings nothing of them
         if (left < kTile)
           for (int x = left * UPR + tid; x < kTile * UPR; x += 64 * WAVES)
             reinterpret_cast<u32x4*>(sKV[2 + st] + j * kElems)[x] = u32x4{0u, 0u, 0u, 0u};

@@ -134,12 +134,14 @@ Tensor mha_packed_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const T
   c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
   Tensor out = fresh(q, {Tq, H, d}, q.scalar_type());
   if (out.numel() == 0) return out;
-  p.q = q.data_ptr(); p.k = k.data_ptr(); p.v = v.data_ptr(); p.o = out.data_ptr();
+  // rows of v that overlap in memory, as of one row expanded over the tokens, get their own
+  const Tensor vr = Tk > 1 && v.stride(0) < d ? v.clone(at::MemoryFormat::Contiguous) : v;
+  p.q = q.data_ptr(); p.k = k.data_ptr(); p.v = vr.data_ptr(); p.o = out.data_ptr();
   p.cu_q = cu_q.data_ptr<int>(); p.cu_k = cu_k.data_ptr<int>();
   p.prefix_lens = prefix_lens.has_value() && n > 0 ? prefix_lens->data_ptr<int>() : nullptr;
   p.q_token_stride = step(q, 0); p.q_head_stride = step(q, 1);
   p.k_token_stride = step(k, 0); p.k_head_stride = step(k, 1);
-  p.v_token_stride = step(v, 0); p.v_head_stride = step(v, 1);
+  p.v_token_stride = step(vr, 0); p.v_head_stride = step(vr, 1);
   p.o_token_stride = H * d; p.o_head_stride = d;
   p.total_q = (int)Tq; p.total_k = (int)Tk; p.n_seqs = (int)n;
   p.h = (int)H; p.h_k = (int)Hk; p.d = (int)d; p.dtype = type_of(q);

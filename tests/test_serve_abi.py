@@ -1,0 +1,11 @@
+"""CPU tests of what the serving operators' C entry points refuse beside tests/test_serve.py:
+layouts and sizes that their kernels cannot serve."""
+import pytest
+
+from tests.test_serve import EINVAL, PACKED, Packed, call, lib, make  # noqa: F401  (lib: a fixture)
+
+@pytest.mark.parametrize("stride", [0, 8, 56])
+def test_values_that_overlap(lib, stride):   # noqa: F811
+    """More than one row of V has to lie apart: a tile's rows behind the last key are outside the memory it reads."""
+    rc, err = call(lib, "mi355_packed_fwd", make(Packed, PACKED, v_ts=stride))
+    assert rc == EINVAL and "overlap" in err, (rc, err)
