@@ -146,6 +146,8 @@ int packed_fwd(const mi355_packed_params* p, hipStream_t st, const Err& err) {
     if (s < 0 || s >= kMaxRowStride) return err.fail(MI355_SERVE_EINVAL, "token strides must be in 0 .. 2^24 elements");
   // (a tile's rows behind the last key must lie behind the last row's end)
   if (p->total_k > 1 && p->v_token_stride < p->d) return err.fail(MI355_SERVE_EINVAL, "v's rows must not overlap: its token stride must be at least d");
+  // (a wave stores 32 rows: those behind a sequence's last must lie behind that row's end)
+  if (p->total_q > 1 && p->o_token_stride < p->d) return err.fail(MI355_SERVE_EINVAL, "o's rows must not overlap: its token stride must be at least d");
   const Device dev = device_info();
   if (!dev.gfx950) return err.fail(MI355_SERVE_EDEVICE, "mi355_serve: current HIP device is not gfx950 (MI355X)");
 
@@ -159,7 +161,9 @@ int packed_fwd(const mi355_packed_params* p, hipStream_t st, const Err& err) {
   a.cu_q = p->cu_q; a.cu_k = p->cu_k; a.prefix = p->prefix_lens; a.slopes = p->slopes;
   a.q_ts = p->q_token_stride; a.q_hs = p->q_head_stride; a.k_ts = p->k_token_stride; a.k_hs = p->k_head_stride;
   a.v_ts = p->total_k > 1 ? p->v_token_stride : p->d;   // (never stepped over)
-  a.v_hs = p->v_head_stride; a.o_ts = p->o_token_stride; a.o_hs = p->o_head_stride;
+  a.v_hs = p->v_head_stride;
+  a.o_ts = p->total_q > 1 ? p->o_token_stride : p->d;
+  a.o_hs = p->o_head_stride;
   a.tq = p->total_q; a.tk = p->total_k; a.n = p->n_seqs; a.h = p->h; a.ratio = p->h / p->h_k;
   a.causal = p->causal != 0; a.window = window_of(p->window);
   // A workgroup's shape: 4 waves of 32 rows (two workgroups on a CU); 8 waves, 4 of rows

@@ -54,7 +54,7 @@ enum { MI355_SERVE_FP16 = 0, MI355_SERVE_BF16 = 1 };
  * cu_k[n] .. cu_k[n+1]-1 of k and v, are sequence n; offsets ascend. Rows of o in
  * no sequence are set to 0. Layouts: q, o [total_q, h, d]; k, v [total_k, h_k, d];
  * innermost stride 1, 16-byte aligned bases, other strides multiples of 8 elements,
- * token strides below 2^24 and, of v with more than one token, at least d.
+ * token strides below 2^24 and, of v and o with more than one token, at least d.
  */
 typedef struct mi355_packed_params {
   const void* q;

@@ -67,3 +67,25 @@ def test_keys_and_values_overlap(ops, T, step, d):
     cu = [0, T // 3, T]
     want, tol = ref.packed(q, k, v, cu, cu)
     ref.check(ops.mha_packed_fwd(q, k, v, i32(cu), i32(cu)), want, tol)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_one_row_of_any_stride(ops, d):
+    """Through the C entry: the output of a single row is that row, whatever its token stride."""
+    import ctypes
+
+    from custom_ops_amd import build
+    from tests.test_serve import Packed, call, make
+    q, k, v = randn(1, 4, d, seed=1), randn(40, 2, d, seed=2), randn(40, 2, d, seed=3)
+    cq, ck = i32([0, 1]), i32([0, 40])
+    want = ops.mha_packed_fwd(q, k, v, cq, ck)
+    lib = ctypes.CDLL(build.SERVE_LIB_PATH)
+    for o_ts in (0, 8, 4 * d):
+        out = torch.full_like(q, 3.0)
+        torch.cuda.synchronize()
+        rc = call(lib, "mi355_packed_fwd", make(Packed, dict(
+            q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), o=out.data_ptr(), cu_q=cq.data_ptr(), cu_k=ck.data_ptr(), q_ts=4 * d, q_hs=d,
+            k_ts=2 * d, k_hs=d, v_ts=2 * d, v_hs=d, o_ts=o_ts, o_hs=d, total_q=1, total_k=40, n_seqs=1, h=4, h_k=2, d=d, dtype=1, causal=1,
+            window=0, scale=1.0 / d ** 0.5, softcap=0.0)))
+        torch.cuda.synchronize()
+        assert rc == (0, "") and torch.equal(out, want), (o_ts, rc)

@@ -9,3 +9,10 @@ def test_values_that_overlap(lib, stride):   # noqa: F811
     """More than one row of V has to lie apart: a tile's rows behind the last key are outside the memory it reads."""
     rc, err = call(lib, "mi355_packed_fwd", make(Packed, PACKED, v_ts=stride))
     assert rc == EINVAL and "overlap" in err, (rc, err)
+
+
+@pytest.mark.parametrize("stride", [0, 8, 56])
+def test_outputs_that_overlap(lib, stride):   # noqa: F811
+    """A wave stores 32 rows, those behind a sequence's last one outside the memory it may write."""
+    rc, err = call(lib, "mi355_packed_fwd", make(Packed, PACKED, o_ts=stride))
+    assert rc == EINVAL and "overlap" in err, (rc, err)
