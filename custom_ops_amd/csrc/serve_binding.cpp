@@ -48,12 +48,6 @@ void* stream_of(const Tensor& x) {
 
 void finish(int rc, const char* err) { TORCH_CHECK(rc == 0, err); }
 
-// There is no backward pass: a call that autograd would have to follow is refused.
-void check_no_grad(std::initializer_list<const Tensor*> xs) {
-  if (!at::GradMode::is_enabled()) return;
-  for (const Tensor* x : xs) TORCH_CHECK(!x->requires_grad(), "forward only: call it under torch.no_grad() or on detached tensors");
-}
-
 void check_gpu(const Tensor& x, const Tensor& like, const char* name) {
   TORCH_CHECK(x.is_cuda(), name, " must be a CUDA tensor");
   TORCH_CHECK(x.device() == like.device(), "all tensors must be on the same device (", name, " is not on q's)");
@@ -90,7 +84,6 @@ void check_ints(const Tensor& x, const Tensor& q, const char* name, at::ScalarTy
 const float* slopes_of(const Maybe& s, const Tensor& q, int64_t heads) {
   if (!s.has_value()) return nullptr;
   check_gpu(*s, q, "slopes");
-  check_no_grad({&*s});
   TORCH_CHECK(s->scalar_type() == at::kFloat, "slopes must be float32");
   TORCH_CHECK(s->dim() == 1 && s->size(0) == heads && s->is_contiguous(), "slopes must be contiguous with ", heads, " elements");
   return s->data_ptr<float>();
@@ -110,7 +103,6 @@ void check_head_dim(int64_t d) { TORCH_CHECK(d == 64 || d == 128, "Only head_dim
 Tensor mha_packed_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu_q, const Tensor& cu_k, bool causal,
                       std::optional<double> scale, double softcap, int64_t window, const Maybe& slopes, const Maybe& prefix_lens) {
   check_half(q);
-  check_no_grad({&q, &k, &v});
   check_rows(q, q, "q", 3);
   check_rows(k, q, "k", 3);
   check_rows(v, q, "v", 3);
@@ -156,7 +148,6 @@ Tensor mha_packed_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const T
 Tensor mha_paged_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table, const Tensor& kv_lens,
                         std::optional<double> scale, double softcap, int64_t window, const Maybe& slopes) {
   check_half(q);
-  check_no_grad({&q, &k_cache, &v_cache});
   check_rows(q, q, "q", 3);
   check_rows(k_cache, q, "k_cache", 4);
   check_rows(v_cache, q, "v_cache", 4);
@@ -208,7 +199,6 @@ std::tuple<Tensor, Tensor> rope_paged_store(const Tensor& q, const Tensor& k, co
                                             const Tensor& slot_map, const Tensor& k_cache, const Tensor& v_cache, bool interleaved,
                                             double amplitude) {
   check_half(q);
-  check_no_grad({&q, &k, &v, &k_cache, &v_cache, &inv_freq});
   check_rows(q, q, "q", 3);
   check_rows(k, q, "k", 3);
   check_rows(v, q, "v", 3);
@@ -298,6 +288,37 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> paged_layout(const Te
   return {kv_lens, cu, positions, slots, table, counts};
 }
 
+// ── autograd ──────────────────────────────────────────────────────────────────
+// There is no derivative, so the Autograd key refuses a call that needs one, backward
+// (an input that requires a gradient while gradients are recorded) or forward (an input
+// with a tangent). It does so for every kind of tensor, before the fake kernels that
+// tracing calls in place of these.
+void refuse_derivative(const Tensor& x) {
+  if (!x.defined()) return;
+  TORCH_CHECK(!(x.requires_grad() && at::GradMode::is_enabled()) && !x._fw_grad(/*level=*/0).defined(),
+              "forward only: call it under torch.no_grad() or on detached tensors");
+}
+void refuse_derivative(const Maybe& x) {
+  if (x.has_value()) refuse_derivative(*x);
+}
+template <class T> void refuse_derivative(const T&) {}
+
+constexpr char kPackedName[] = "recsys_ops::mha_packed_fwd", kDecodeName[] = "recsys_ops::mha_paged_decode",
+               kRopeName[] = "recsys_ops::rope_paged_store";
+
+template <const char* Name, class F> struct Gate;
+template <const char* Name, class R, class... A> struct Gate<Name, R(A...)> {
+  static const c10::TypedOperatorHandle<R(A...)>& op() {
+    static const auto handle = c10::Dispatcher::singleton().findSchemaOrThrow(Name, "").template typed<R(A...)>();
+    return handle;
+  }
+  static R autograd(c10::DispatchKeySet keys, A... args) {
+    (refuse_derivative(args), ...);
+    at::AutoDispatchBelowAutograd below;
+    return op().redispatch(keys & c10::after_autograd_keyset, args...);
+  }
+};
+
 }  // namespace
 
 extern "C" __attribute__((used, visibility("default"))) const char mi355_ops_stamp[] = MI355_OPS_STAMP;
@@ -318,14 +339,12 @@ extern "C" int mi355_serve_connect(void* handle) {
     static torch::Library lib(torch::Library::IMPL, "recsys_ops", c10::DispatchKey::CUDA, __FILE__, __LINE__);
     static const bool once = (lib.impl("mha_packed_fwd", &mha_packed_fwd), lib.impl("mha_paged_decode", &mha_paged_decode),
                               lib.impl("rope_paged_store", &rope_paged_store), lib.impl("paged_layout", &paged_layout), true);
-    // nothing to record: without this every call goes through autograd's boxed
-    // fallback (check_no_grad refuses what would need it)
     static torch::Library autograd(torch::Library::IMPL, "recsys_ops", c10::DispatchKey::Autograd, __FILE__, __LINE__);
-    static const bool once_more = [] {
-      for (const char* name : {"mha_packed_fwd", "mha_paged_decode", "rope_paged_store", "paged_layout"})
-        autograd.impl(name, torch::CppFunction::makeFallthrough());
-      return true;
-    }();
+    static const bool once_more = (autograd.impl("mha_packed_fwd", &Gate<kPackedName, decltype(mha_packed_fwd)>::autograd),
+                                   autograd.impl("mha_paged_decode", &Gate<kDecodeName, decltype(mha_paged_decode)>::autograd),
+                                   autograd.impl("rope_paged_store", &Gate<kRopeName, decltype(rope_paged_store)>::autograd),
+                                   // whole numbers only: nothing to refuse
+                                   autograd.impl("paged_layout", torch::CppFunction::makeFallthrough()), true);
     (void)once;
     (void)once_more;
   } catch (const std::exception&) {
