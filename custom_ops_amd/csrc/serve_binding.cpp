@@ -319,6 +319,21 @@ template <const char* Name, class R, class... A> struct Gate<Name, R(A...)> {
   }
 };
 
+// The caches' version counters move, so that autograd notices a cache that it saved for
+// another operator. (Inference tensors have none.)
+std::tuple<Tensor, Tensor> rope_paged_store_inplace(c10::DispatchKeySet keys, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& positions,
+                                                    const Tensor& inv_freq, const Tensor& slot_map, const Tensor& k_cache, const Tensor& v_cache,
+                                                    bool interleaved, double amplitude) {
+  auto out = [&] {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return Gate<kRopeName, decltype(rope_paged_store)>::op().redispatch(keys & c10::after_ADInplaceOrView_keyset, q, k, v, positions, inv_freq, slot_map,
+                                                                        k_cache, v_cache, interleaved, amplitude);
+  }();
+  for (const Tensor* x : {&k_cache, &v_cache})
+    if (!x->is_inference()) x->unsafeGetTensorImpl()->bump_version();
+  return out;
+}
+
 }  // namespace
 
 extern "C" __attribute__((used, visibility("default"))) const char mi355_ops_stamp[] = MI355_OPS_STAMP;
@@ -345,8 +360,11 @@ extern "C" int mi355_serve_connect(void* handle) {
                                    autograd.impl("rope_paged_store", &Gate<kRopeName, decltype(rope_paged_store)>::autograd),
                                    // whole numbers only: nothing to refuse
                                    autograd.impl("paged_layout", torch::CppFunction::makeFallthrough()), true);
+    static torch::Library inplace(torch::Library::IMPL, "recsys_ops", c10::DispatchKey::ADInplaceOrView, __FILE__, __LINE__);
+    static const bool once_again = (inplace.impl("rope_paged_store", &rope_paged_store_inplace), true);
     (void)once;
     (void)once_more;
+    (void)once_again;
   } catch (const std::exception&) {
     return 1;
   }

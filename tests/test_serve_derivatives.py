@@ -103,3 +103,46 @@ def test_layout_takes_no_gradients(o):
     n = torch.zeros(4, dtype=torch.int32, device="meta")
     t = torch.zeros(4, 6, dtype=torch.int32, device="meta")
     assert o.paged_layout(n, n, t, n, 16, 11)[0].shape == (4,)
+
+
+# ── caches written in place ───────────────────────────────────────────────────
+
+@pytest.mark.parametrize("mode", ["grad", "no_grad", "inference"])
+def test_cache_versions_move(o, mode):
+    kc, vc = (torch.ones(5, 2, 16, 64, device="meta") for _ in range(2))
+    view = kc[1:3]
+    with {"grad": torch.enable_grad, "no_grad": torch.no_grad, "inference": torch.inference_mode}[mode]():
+        for n in (1, 2):
+            rope(o, "meta", kc=kc, vc=vc)
+            assert kc._version == n and vc._version == n and view._version == n
+
+
+def test_a_saved_cache_is_noticed(o):
+    w = torch.ones(64, device="meta", requires_grad=True)
+    for which in ("kc", "vc"):
+        cache = torch.ones(5, 2, 16, 64, device="meta")
+        y = (w * cache).sum()
+        rope(o, "meta", **{which: cache})
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+
+
+def test_inference_caches(o):
+    """Made in inference mode, they are written there and outside."""
+    with torch.inference_mode():
+        kc, vc = (torch.ones(5, 2, 16, 64, device="meta") for _ in range(2))
+        rope(o, "meta", kc=kc, vc=vc)
+    with torch.no_grad():
+        rope(o, "meta", kc=kc, vc=vc)
+
+
+def test_traced_writes_stay(o):
+    """A compiled step that writes the caches and returns nothing of them still writes them."""
+    from torch._dynamo.testing import CompileCounterWithBackend
+    seen = CompileCounterWithBackend("aot_eager")
+    kc, vc = (torch.ones(5, 2, 16, 64, device="meta") for _ in range(2))
+    f = torch.compile(lambda q, a, b: rope(o, "meta", q=q, kc=a, vc=b) * 2, backend=seen, fullgraph=True)
+    with torch.no_grad():
+        f(torch.ones(9, 4, 64, device="meta"), kc, vc)
+    assert kc._version > 0 and vc._version > 0
+    assert any("rope_paged_store" in str(n.target) for g in seen.graphs for n in g.graph.nodes)
