@@ -342,6 +342,8 @@ int paged_layout(const mi355_layout_params* p, hipStream_t st, const Err& err) {
   if (!p) return err.fail(MI355_SERVE_EINVAL, "params must not be NULL");
   if (p->n < 0 || p->n > MI355_SERVE_MAX_REQUESTS) return err.fail(MI355_SERVE_EINVAL, "at most %d requests", MI355_SERVE_MAX_REQUESTS);
   if (p->table_cols < 0 || p->n_free < 0 || p->max_tokens < 0) return err.fail(MI355_SERVE_EINVAL, "negative dimension");
+  // (a wave steps over a row of the table with 32-bit columns)
+  if (p->table_cols > kMaxRows) return err.fail(MI355_SERVE_EINVAL, "block_table must have at most 2^30 columns");
   if (p->page_size < 1) return err.fail(MI355_SERVE_EINVAL, "page_size must be positive");
   if (!p->cu_new || !p->counts || (p->n > 0 && (!p->seq_lens || !p->new_lens || !p->kv_lens)) ||
       (p->n > 0 && p->table_cols > 0 && (!p->block_table || !p->table)) || (p->n_free > 0 && !p->free_pages) ||

@@ -174,7 +174,7 @@ typedef struct mi355_layout_params {
   int32_t* table;             /* [n, table_cols], contiguous */
   int32_t* counts;            /* [3] */
   int64_t table_stride;       /* of block_table */
-  int32_t n, table_cols, n_free, page_size, max_tokens; /* page_size >= 1 */
+  int32_t n, table_cols, n_free, page_size, max_tokens; /* page_size >= 1, table_cols <= 2^30 */
 } mi355_layout_params;
 
 #define MI355_SERVE_MAX_REQUESTS 8192 /* n of mi355_paged_layout */

@@ -2,7 +2,7 @@
 layouts and sizes that their kernels cannot serve."""
 import pytest
 
-from tests.test_serve import EINVAL, PACKED, Packed, call, lib, make  # noqa: F401  (lib: a fixture)
+from tests.test_serve import EINVAL, LAYOUT, PACKED, Layout, Packed, call, lib, make  # noqa: F401  (lib: a fixture)
 
 @pytest.mark.parametrize("stride", [0, 8, 56])
 def test_values_that_overlap(lib, stride):   # noqa: F811
@@ -16,3 +16,10 @@ def test_outputs_that_overlap(lib, stride):   # noqa: F811
     """A wave stores 32 rows, those behind a sequence's last one outside the memory it may write."""
     rc, err = call(lib, "mi355_packed_fwd", make(Packed, PACKED, o_ts=stride))
     assert rc == EINVAL and "overlap" in err, (rc, err)
+
+
+@pytest.mark.parametrize("cols", [2 ** 30 + 1, 2 ** 31 - 256, 2 ** 31 - 1])
+def test_tables_too_wide(lib, cols):   # noqa: F811
+    """Columns are counted in 32 bits, 256 at a step: near 2^31 the count would turn negative."""
+    rc, err = call(lib, "mi355_paged_layout", make(Layout, LAYOUT, n=1, cols=cols))
+    assert rc == EINVAL and "2^30 columns" in err, (rc, err)
