@@ -303,6 +303,8 @@ int paged_decode(const mi355_decode_params* p, hipStream_t st, const Err& err) {
 int rope_store(const mi355_rope_params* p, hipStream_t st, const Err& err) {
   if (!p) return err.fail(MI355_SERVE_EINVAL, "params must not be NULL");
   if (int rc = check_heads(err, p->h, p->h_k, p->d, p->dtype)) return rc;
+  // (a workgroup counts its token's 16-element units in 32 bits)
+  if ((int64_t)p->h + 2 * (int64_t)p->h_k > (1 << 27)) return err.fail(MI355_SERVE_EINVAL, "at most 2^27 heads of q, k and v together");
   if (p->t < 0 || p->num_pages < 0 || p->t > kMaxRows) return err.fail(MI355_SERVE_EINVAL, "t and num_pages must be in 0 .. 2^30");
   if (p->rot < 0 || p->rot > p->d || p->rot % 16) return err.fail(MI355_SERVE_EINVAL, "rot must be a multiple of 16 in 0 .. head_dim");
   if (p->page_size < 1) return err.fail(MI355_SERVE_EINVAL, "page_size must be positive");
