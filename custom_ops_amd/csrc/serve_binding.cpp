@@ -18,8 +18,10 @@
 
 #include <dlfcn.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
+#include <cstdlib>
 #include <initializer_list>
 #include <tuple>
 
@@ -195,6 +197,33 @@ Tensor mha_paged_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_
   return out;
 }
 
+// Whether two tensors of the same sizes and strides share an element: their distance is a
+// sum of steps d_i·stride_i with |d_i| < size_i. Strides are taken from the largest, so
+// each d_i has two candidates at most; dimensions that do not nest count as apart.
+bool share(const Tensor& a, const Tensor& b) {
+  const int64_t n = a.dim();
+  if (a.numel() == 0 || a.strides() != b.strides() || !a.is_alias_of(b)) return false;
+  int64_t order[8], reach[9] = {};
+  if (n > 8) return false;
+  for (int64_t i = 0; i < n; ++i) order[i] = i;
+  std::sort(order, order + n, [&](int64_t x, int64_t y) { return a.stride(x) > a.stride(y); });
+  for (int64_t i = n - 1; i >= 0; --i) {
+    if (a.size(order[i]) > 1 && reach[i + 1] >= a.stride(order[i])) return false;
+    reach[i] = reach[i + 1] + (a.size(order[i]) - 1) * a.stride(order[i]);
+  }
+  auto meets = [&](auto& self, int64_t dist, int64_t i) -> bool {
+    if (std::abs(dist) > reach[i]) return false;
+    if (i == n) return true;
+    const int64_t s = a.stride(order[i]), most = a.size(order[i]) - 1;
+    if (most == 0) return self(self, dist, i + 1);
+    const int64_t d = dist / s;   // towards 0: the other candidate is one further
+    for (int64_t x : {d, dist < 0 ? d - 1 : d + 1})
+      if (std::abs(x) <= most && self(self, dist - x * s, i + 1)) return true;
+    return false;
+  };
+  return meets(meets, b.storage_offset() - a.storage_offset(), 0);
+}
+
 std::tuple<Tensor, Tensor> rope_paged_store(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& positions, const Tensor& inv_freq,
                                             const Tensor& slot_map, const Tensor& k_cache, const Tensor& v_cache, bool interleaved,
                                             double amplitude) {
@@ -213,6 +242,7 @@ std::tuple<Tensor, Tensor> rope_paged_store(const Tensor& q, const Tensor& k, co
   at::assert_no_internal_overlap(k_cache);   // written in place
   at::assert_no_internal_overlap(v_cache);
   at::assert_no_overlap(k_cache, v_cache);
+  TORCH_CHECK(!share(k_cache, v_cache), "k_cache and v_cache must not overlap");
   for (const Tensor* x : {&q, &k, &v}) {
     at::assert_no_overlap(k_cache, *x);
     at::assert_no_overlap(v_cache, *x);
