@@ -53,6 +53,22 @@ SERVE_SRC = os.path.join(PKG_DIR, "csrc", "serve.hip")   # the serving operators
 SERVE_LIB_PATH = os.path.join(PKG_DIR, "libmi355_serve.so")
 
 
+def sources_of(src: str) -> list:
+    """The files of this package that a compilation of ``src`` reads: itself and what it
+    includes, from csrc/ and include/, in order of their names."""
+    found, todo = set(), [src]
+    while todo:
+        path = todo.pop()
+        if path in found:
+            continue
+        found.add(path)
+        with open(path, encoding="utf-8") as f:
+            names = re.findall(r'^\s*#\s*include\s+"([^"]+)"', f.read(), re.M)
+        for d in (os.path.dirname(src), INCLUDE):
+            todo += [p for p in (os.path.join(d, n) for n in names) if os.path.exists(p)]
+    return sorted(found, key=os.path.basename)
+
+
 def compile_checked(out_path: str, flags=None, verbose: bool = False, src: str = SRC) -> str:
     """Compile ``src`` into ``out_path`` (atomically) after checking the device
     assembly of that same compilation; raise RuntimeError on either failure."""

@@ -355,9 +355,7 @@ class FAOps:
     # offline build
     def _provenance(self, targets: list, extra: list) -> dict:
         h = hashlib.sha256()
-        csrc = Path(self._source()).parent
-        for src in [Path(self._source()), *sorted(csrc.glob("*.h")), *sorted(csrc.glob("*.inc")),
-                    *sorted(Path(_build.INCLUDE).glob("*.h"))]:
+        for src in map(Path, _build.sources_of(self._source())):
             h.update(src.name.encode() + b"\0" + src.read_bytes())
         flags = [f for f in _build.HIPCC_FLAGS if not f.startswith("--offload-arch=")] + extra
         try:
