@@ -6,8 +6,8 @@
 // the cosine and sine of position·inv_freq. Bound: bytes; q, k and v are read once
 // and each output is written once.
 //
-//  * A workgroup serves TOK tokens: its threads first form each (token, pair)'s
-//    cosine and sine once, for all heads. The angle is a 64-bit product, reduced
+//  * A workgroup serves a token: its threads first form each pair's cosine and sine
+//    once, for all heads. The angle is a 64-bit product, reduced
 //    to half turns in 64 bits: in 32 bits position 10^6 is off by 0.06 radians.
 //  * Then a thread turns 16 elements at a time: two 16-byte chunks that hold 8
 //    whole pairs, chunks (j, j + rot/16) of a head, or (2j, 2j + 1) interleaved.
@@ -30,32 +30,26 @@ struct RopeArgs {
   float amplitude;
 };
 
-template <int D, bool BF16, bool INTER, int TOK>
+template <int D, bool BF16, bool INTER>
 __global__ __launch_bounds__(256) void rope_store_kernel(const RopeArgs a) {
   typedef typename Elt<BF16>::v8 V8;
   constexpr int U = D / 16;   // units of two chunks per head
-  __shared__ float sC[TOK][D / 2], sS[TOK][D / 2];
-  const int t0 = blockIdx.x * TOK, tid = threadIdx.x;
-  const int pairs = a.rot / 2;
-  for (int x = tid; x < TOK * pairs; x += 256) {
-    const int tok = x / pairs, i = x - tok * pairs;
-    if (t0 + tok < a.t) {
-      constexpr double kInvPi = 0.31830988618379067154;
-      const double half = (double)a.positions[t0 + tok] * a.inv_freq[i] * kInvPi;   // half turns
-      float s, c;
-      sincospif((float)(half - 2.0 * rint(half * 0.5)), &s, &c);
-      sC[tok][i] = c * a.amplitude;
-      sS[tok][i] = s * a.amplitude;
-    }
+  __shared__ float sC[D / 2], sS[D / 2];
+  const int64_t t = blockIdx.x;
+  const int tid = threadIdx.x;
+  if (tid < a.rot / 2) {
+    constexpr double kInvPi = 0.31830988618379067154;
+    const double half = (double)a.positions[t] * a.inv_freq[tid] * kInvPi;   // half turns
+    float s, c;
+    sincospif((float)(half - 2.0 * rint(half * 0.5)), &s, &c);
+    sC[tid] = c * a.amplitude;
+    sS[tid] = s * a.amplitude;
   }
   __syncthreads();
   const int heads = a.h + 2 * a.hk, units = heads * U;
   const int ru = a.rot / 16;   // units that turn
-  for (int x = tid; x < TOK * units; x += 256) {
-    const int tok = x / units, y = x - tok * units;
-    const int head = y / U, j = y % U;
-    const int64_t t = t0 + tok;
-    if (t >= a.t) break;
+  for (int x = tid; x < units; x += 256) {
+    const int head = x / U, j = x % U;
     const uint16_t* src;
     if (head < a.h) src = a.q + t * a.q_ts + head * a.q_hs;
     else if (head < a.h + a.hk) src = a.k + t * a.k_ts + (head - a.h) * a.k_hs;
@@ -65,8 +59,8 @@ __global__ __launch_bounds__(256) void rope_store_kernel(const RopeArgs a) {
     u32x4 lo = *reinterpret_cast<const u32x4*>(src + c0 * 8), hi = *reinterpret_cast<const u32x4*>(src + c1 * 8);
     if (turns) {
       const f32x8 xl = __builtin_convertvector(bitcast<V8>(lo), f32x8), xh = __builtin_convertvector(bitcast<V8>(hi), f32x8);
-      const float* cs = &sC[tok][j * 8];
-      const float* sn = &sS[tok][j * 8];
+      const float* cs = &sC[j * 8];
+      const float* sn = &sS[j * 8];
       f32x8 yl, yh;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {

@@ -335,7 +335,7 @@ int rope_store(const mi355_rope_params* p, hipStream_t st, const Err& err) {
   by_type(p->d, p->dtype == MI355_SERVE_BF16, [&](auto d, auto bf) {
     constexpr int D = decltype(d)::value;
     constexpr bool BF = decltype(bf)::value;
-    rc = run(err, "rope_paged_store", p->interleaved ? rope_store_kernel<D, BF, true, 1> : rope_store_kernel<D, BF, false, 1>, p->t, 256, 0, st, a);
+    rc = run(err, "rope_paged_store", p->interleaved ? rope_store_kernel<D, BF, true> : rope_store_kernel<D, BF, false>, p->t, 256, 0, st, a);
   });
   return rc;
 }
