@@ -279,7 +279,8 @@ void packed_fwd_kernel(const PackedArgs a) {
     // (least squares in Chebyshev nodes, off by 6·10^-7): 5 operations of 4 cycles a score,
     // where the two transcendental ones take 16 each. The two forms differ in their last
     // bits, so no score of an unseen key may choose: the whole wave chooses together on a
-    // tile that all of its rows see, each lane by the scores its row sees on the others.
+    // tile that all of its rows see, each lane by the scores its row sees on the others
+    // (4099 tokens in 3 documents with window and prefix: 57.6 us, of which that takes 2).
     float u[16 * NKB];   // key 32·(c / 16) + c % 16, from the lane's first
 #pragma unroll
     for (int c = 0; c < 16 * NKB; ++c) u[c] = s[c / 16][c % 16];

@@ -7,14 +7,18 @@ program that generates token by token needs next to it.
   * ``mha_paged_decode``  attention of one new token per request over the cache
 
 A step: ``paged_layout`` gives slots and positions, ``rope_paged_store`` fills the
-cache, then prompts attend with ``mha_packed_fwd`` (q and k as ``rope_paged_store``
-returns them, ``cu_new`` as offsets) and single tokens with ``mha_paged_decode``
-(``kv_lens`` and the table of ``paged_layout``). Nothing reads device data on the
-host, so a step can be captured into a graph.
+cache, then prompts with nothing cached attend with ``mha_packed_fwd`` (q and k as
+``rope_paged_store`` returns them, ``cu_new`` as offsets: the step's own tokens alone)
+and single tokens with ``mha_paged_decode`` (``kv_lens`` and the table of
+``paged_layout``). Several new tokens behind cached ones need their keys gathered, with
+offsets of their own as cu_k. Nothing reads device data on the host, so a step can be
+captured into a graph; from one step to the next the program drops the pages taken
+(``counts[1]``) from the front of its free ones.
 
 The kernels are HIP (csrc/serve.hip, ``libmi355_serve.so``, C ABI in
 include/mi355_serve.h); the checks and launches are csrc/serve_binding.cpp
-(``libmi355_serve_ops.so``). There is no fallback: forward only, on the GPU only.
+(``libmi355_serve_ops.so``). There is no fallback: forward only, on the GPU only; a
+call that needs a derivative is refused, while tracing too.
 Every failure of a check is a ``RuntimeError``, as of the operators of fa.py.
 """
 from __future__ import annotations

@@ -46,7 +46,8 @@ enum { MI355_SERVE_FP16 = 0, MI355_SERVE_BF16 = 1 };
  * Seen keys: j <= i where causal (always, for one token); |i − j| < window where
  * window > 0; and, whatever those say, the first prefix_lens[sequence] keys.
  * O = softmax(s over the seen keys)·V; a row that sees none gives 0. Keys that a
- * row does not see have no influence on it, whatever they hold.
+ * row does not see have no influence on it, whatever they hold. (Where one holds a
+ * V that is not finite, a column of the row can round differently in the last place.)
  */
 
 /*
