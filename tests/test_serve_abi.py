@@ -4,6 +4,7 @@ import pytest
 
 from tests.test_serve import EINVAL, LAYOUT, PACKED, ROPE, Layout, Packed, Rope, call, lib, make  # noqa: F401  (lib: a fixture)
 
+
 @pytest.mark.parametrize("stride", [0, 8, 56])
 def test_values_that_overlap(lib, stride):   # noqa: F811
     """More than one row of V has to lie apart: a tile's rows behind the last key are outside the memory it reads."""
