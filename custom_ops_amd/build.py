@@ -112,7 +112,6 @@ OPS_PATH = os.path.join(PKG_DIR, "libmi355_fa_ops.so")   # the same source, impl
 
 SERVE_BINDING_SRC = os.path.join(PKG_DIR, "csrc", "serve_binding.cpp")
 SERVE_OPS_PATH = os.path.join(PKG_DIR, "libmi355_serve_ops.so")
-_BINDING_HEADER = {TORCH_BINDING_SRC: "mi355_fa.h", SERVE_BINDING_SRC: "mi355_serve.h"}
 
 
 def ops_stamp(binding: str = TORCH_BINDING_SRC) -> str:
@@ -120,7 +119,7 @@ def ops_stamp(binding: str = TORCH_BINDING_SRC) -> str:
     and the PyTorch it runs in. The file holds this text (csrc/torch_binding.cpp)."""
     import torch
     h = hashlib.sha256()
-    for src in (binding, os.path.join(INCLUDE, _BINDING_HEADER[binding])):
+    for src in sources_of(binding):
         with open(src, "rb") as f:
             h.update(f.read())
     return f"mi355-ops {h.hexdigest()} torch {torch.__version__};"

@@ -19,8 +19,6 @@
 //    that any split of the rows can need.
 //  * K and V tiles come HBM → LDS by DMA, two stages, one barrier per tile.
 
-constexpr float kSlackLog2 = 8.f;   // the running max moves when a score passes it by this (P <= 2^8)
-
 struct PackedArgs {
   const uint16_t* q;
   const uint16_t* k;
@@ -49,16 +47,6 @@ struct RowBlock {
   int q0, lq, m0, k0, lk, pre;
 };
 
-// Inclusive sum over the wave's lanes: rows of 16 by shifts, then the rows' sums.
-__device__ __forceinline__ int wave_scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);   // row_shr:1
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // row_bcast:15 into rows 1 and 3
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);   // row_bcast:31 into rows 2 and 3
-  return x;
-}
 __device__ __forceinline__ int wave_max(int x) {   // of values >= 0, over the wave's lanes
   x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));
   x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));

@@ -42,12 +42,6 @@ struct DecodeArgs {
   float u_scale, c2, bias;       // as in PackedArgs
 };
 
-template <bool BF16>
-__device__ __forceinline__ f32x4 mfma16(typename Elt<BF16>::v8 a, typename Elt<BF16>::v8 b, f32x4 c) {
-  if constexpr (BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-  else return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-
 __device__ __forceinline__ KeySpan keys_of(const DecodeArgs& a, int len) {
   return key_span(len, (int64_t)a.cols << a.shift, a.window);
 }
