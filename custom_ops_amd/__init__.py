@@ -14,12 +14,12 @@ the library is missing, calls raise ``RuntimeError``.
 """
 from __future__ import annotations
 
-from . import _lib, fa, serve
+from . import _lib, beam, fa, serve
 from .facade import RecsysOps, resolve_backend
 from ._lib import Variant
-from .loader import CustomOpsError, FAOps, ServeOps
+from .loader import BeamOps, CustomOpsError, FAOps, ServeOps
 
-__all__ = ["ops", "RecsysOps", "CustomOpsError", "FAOps", "ServeOps", "Variant", "mha_fwd_with_mask"]
+__all__ = ["ops", "RecsysOps", "CustomOpsError", "FAOps", "ServeOps", "BeamOps", "Variant", "mha_fwd_with_mask"]
 
 _resolve_backend = resolve_backend
 

@@ -1,4 +1,4 @@
-"""Build the HIP C-ABI libraries ``libmi355_fa.so`` and ``libmi355_serve.so`` in-tree for gfx950.
+"""Build the HIP C-ABI libraries ``libmi355_fa.so``, ``libmi355_serve.so`` and ``libmi355_beam.so`` in-tree for gfx950.
 
 hipcc cross-compiles without a GPU, so this runs on any host with ROCm.
 Usage: ``python -m custom_ops_amd.build`` (or ``__graft_entry__.build()``).
@@ -51,6 +51,8 @@ def hipcc() -> str:
 
 SERVE_SRC = os.path.join(PKG_DIR, "csrc", "serve.hip")   # the serving operators' library
 SERVE_LIB_PATH = os.path.join(PKG_DIR, "libmi355_serve.so")
+BEAM_SRC = os.path.join(PKG_DIR, "csrc", "beam.hip")     # the operators' for several continuations of a prompt
+BEAM_LIB_PATH = os.path.join(PKG_DIR, "libmi355_beam.so")
 
 
 def sources_of(src: str) -> list:
@@ -69,9 +71,10 @@ def sources_of(src: str) -> list:
     return sorted(found, key=os.path.basename)
 
 
-def compile_checked(out_path: str, flags=None, verbose: bool = False, src: str = SRC) -> str:
+def compile_checked(out_path: str, flags=None, verbose: bool = False, src: str = SRC, dma: bool = True) -> str:
     """Compile ``src`` into ``out_path`` (atomically) after checking the device
-    assembly of that same compilation; raise RuntimeError on either failure."""
+    assembly of that same compilation; raise RuntimeError on either failure. ``dma``: its
+    kernels use the LDS DMA."""
     from .isa_check import missed_occupancy, violations
     flags = list(HIPCC_FLAGS if flags is None else flags)
     with tempfile.TemporaryDirectory(prefix="mi355fa-build-") as tmp:
@@ -94,7 +97,7 @@ def compile_checked(out_path: str, flags=None, verbose: bool = False, src: str =
         bad = []
         for path in asm:
             with open(path) as f:
-                bad += [f"{os.path.basename(path)}: {v}" for v in violations(f.read())]
+                bad += [f"{os.path.basename(path)}: {v}" for v in violations(f.read(), dma)]
         if bad:
             raise RuntimeError("device assembly check failed; library not installed:\n"
                                + "\n".join(bad))
@@ -112,6 +115,8 @@ OPS_PATH = os.path.join(PKG_DIR, "libmi355_fa_ops.so")   # the same source, impl
 
 SERVE_BINDING_SRC = os.path.join(PKG_DIR, "csrc", "serve_binding.cpp")
 SERVE_OPS_PATH = os.path.join(PKG_DIR, "libmi355_serve_ops.so")
+BEAM_BINDING_SRC = os.path.join(PKG_DIR, "csrc", "beam_binding.cpp")
+BEAM_OPS_PATH = os.path.join(PKG_DIR, "libmi355_beam_ops.so")
 
 
 def ops_stamp(binding: str = TORCH_BINDING_SRC) -> str:
@@ -193,12 +198,26 @@ def build_serve(verbose: bool = False) -> str:
     return out
 
 
+def build_beam_ops(path: str = BEAM_OPS_PATH, verbose: bool = False) -> str:
+    """Compile the implementation, over their library's C ABI, of the operators for several
+    continuations of a prompt."""
+    return _compile_binding(path, [f'-DMI355_OPS_STAMP="{ops_stamp(BEAM_BINDING_SRC)}"', "-ldl"], verbose, BEAM_BINDING_SRC)
+
+
+def build_beam(verbose: bool = False) -> str:
+    """Compile those operators' library and its binding; return the library's path."""
+    out = compile_checked(BEAM_LIB_PATH, verbose=verbose, src=BEAM_SRC, dma=False)
+    build_beam_ops(verbose=verbose)
+    return out
+
+
 def build(verbose: bool = False) -> str:
     """Compile the libraries (always recompiles) and the C++ torch bindings over
     them; return the attention library's path."""
     out = compile_checked(LIB_PATH, verbose=verbose)
     build_torch_binding(verbose=verbose)
     build_serve(verbose=verbose)
+    build_beam(verbose=verbose)
     return out
 
 

@@ -167,6 +167,17 @@ __device__ __forceinline__ int wave_scan(int x) {
   return x;
 }
 
+// Inclusive maximum over the wave's lanes.
+__device__ __forceinline__ int wave_max_scan(int x) {
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x111, 0xf, 0xf, false));   // (a lane without a source keeps its own)
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x112, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x114, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x118, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x142, 0xa, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x143, 0xc, 0xf, false));
+  return x;
+}
+
 // Σ of the 8 rounded P values of one MFMA operand, two per dot2 (fp32 accumulate).
 template <bool BF16>
 __device__ __forceinline__ float psum8(typename Elt<BF16>::v8 v, float acc) {

@@ -28,12 +28,12 @@ from typing import Optional
 
 import torch
 
-from . import serve
-from .loader import CustomOpsError, FAOps, ServeOps
+from . import beam, serve
+from .loader import BeamOps, CustomOpsError, FAOps, ServeOps
 
 # group name -> loader class; operator name -> group name
-GROUP_LOADERS = {"fa": FAOps, "serve": ServeOps}
-OP_GROUPS = {"mha_fwd_with_mask": "fa", **{name: "serve" for name in serve.SCHEMAS}}
+GROUP_LOADERS = {"fa": FAOps, "serve": ServeOps, "beam": BeamOps}
+OP_GROUPS = {"mha_fwd_with_mask": "fa", **{name: "serve" for name in serve.SCHEMAS}, **{name: "beam" for name in beam.SCHEMAS}}
 
 # Groups that calls naming no group stand for: the reference's. The others load by
 # name or at their operators' first call, and appear in ``ops.groups`` from then on,
@@ -89,13 +89,14 @@ class _Slot:
 
 
 class RecsysOps:
-    """Facade over the operator groups: the reference's ``fa``, and ``serve``."""
+    """Facade over the operator groups: the reference's ``fa``, ``serve`` and ``beam``."""
 
     def __init__(self, *, allow_jit: bool = True) -> None:
         self._mu = threading.RLock()
         self._slots = {name: _Slot() for name in GROUP_LOADERS}
         self._jit = _as_flag(allow_jit)
         self._serve_ops = None   # torch.ops.recsys_ops once the group "serve" is ready
+        self._beam_ops = None    # and "beam"
 
     # ── policy ──────────────────────────────────────────────────────────────
     @property
@@ -154,7 +155,7 @@ class RecsysOps:
         with self._mu:
             slot = self._slot(group)
             self.configure(allow_jit=False)
-            self._serve_ops = None
+            self._serve_ops = self._beam_ops = None
             if slot.loader is None:
                 slot.loader = GROUP_LOADERS[group](allow_jit=False)
             slot.loader.load_precompiled(library_path, metadata_path)
@@ -302,6 +303,78 @@ class RecsysOps:
         last), the new table (-1 where there is no page) and {new tokens, pages taken,
         pages wanted and not had}. Tokens without a page have the slot -1."""
         return self._serve(backend).paged_layout(seq_lens, new_lens, block_table, free_pages, page_size, max_tokens)
+
+    def _beam(self, backend: Optional[str]):
+        """The dispatcher's operators, with the group ``beam`` loaded (as ``_serve``)."""
+        if backend is not None:
+            resolve_backend(backend)
+        found = self._beam_ops
+        if found is None:
+            with self._mu:
+                resolve_backend(None)
+                self._acquire("beam")
+                found = self._beam_ops = torch.ops.recsys_ops
+        return found
+
+    def mha_shared_decode(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                          kv_lens: torch.Tensor, cu_groups: torch.Tensor, prefix_lens: torch.Tensor, scale: Optional[float] = None,
+                          softcap: float = 0.0, window: int = 0, slopes: Optional[torch.Tensor] = None,
+                          backend: Optional[str] = None) -> torch.Tensor:
+        """``mha_paged_decode`` for requests that share prefixes, which are read once for all.
+
+        Requests cu_groups[g] .. cu_groups[g+1]-1 (int32 [G+1], ascending) have their first
+        prefix_lens[g] (int32 [G]) keys in common: in the pages that block_table's row
+        cu_groups[g] names, whatever the others' rows have there. Requests of no group
+        attend to their own keys. At most 2048 requests. Other arguments and the result
+        are those of ``mha_paged_decode``."""
+        return self._beam(backend).mha_shared_decode(q, k_cache, v_cache, block_table, kv_lens, cu_groups, prefix_lens, scale, softcap,
+                                                     window, slopes)
+
+    def beam_select(self, logits: torch.Tensor, scores: torch.Tensor, k: int, finished: Optional[torch.Tensor] = None, eos: int = -1,
+                    backend: Optional[str] = None):
+        """The k best continuations of each search's beams: ``(scores, tokens, parents)``, [G,k] each.
+
+        logits [G,W,V] (fp16/bf16/fp32, W at most 256; rows may lie apart), scores [G,W]
+        float32: the beams' so far. A continuation's score is scores[g,w] + log softmax of
+        the logits at its token, formed in 64 bits; the best come first, the lowest w·V + v
+        among equals. k is at most 64. A beam that is ``finished`` ([G,W] bool) has one
+        continuation, its own score with the token ``eos``. Beams with scores that are not finite
+        (those that do not exist: -inf) or with a NaN or +inf among their logits have none,
+        tokens of -inf logits cannot be chosen; where there are fewer than k, the rest is
+        -inf, -1, -1. parents are rows g·W + w, as ``paged_fork`` takes them."""
+        return self._beam(backend).beam_select(logits, scores, k, finished, eos)
+
+    def paged_fork(self, block_table: torch.Tensor, seq_lens: torch.Tensor, parents: torch.Tensor, page_size: int, num_pages: int,
+                   held: Optional[torch.Tensor] = None, backend: Optional[str] = None):
+        """The page table in which row i continues row parents[i] of the old one.
+
+        block_table [N,M], seq_lens [N], parents [R] int32 (R at most 4096; outside 0 .. N-1, as -1: an
+        empty row). Whole pages are shared. A last, partly filled page stays with the first
+        row that has it, unless another has it as a whole one or it is in ``held`` (int32
+        page numbers that stay taken); the others get free pages, to be filled by
+        ``paged_copy``. Pages of no row are free: requests end by having no children. Returns
+        ``(table [R,M], lens [R], src [R], dst [R], free_pages [num_pages], counts [3])``:
+        the pages to copy (-1: none), the free pages left, ascending, -1 behind them, and
+        {free pages left, pages copied, pages wanted and not had}."""
+        return self._beam(backend).paged_fork(block_table, seq_lens, parents, page_size, num_pages, held)
+
+    def paged_compact(self, block_table: torch.Tensor, seq_lens: torch.Tensor, page_size: int, num_pages: int,
+                      held: Optional[torch.Tensor] = None, backend: Optional[str] = None):
+        """Moves the pages in use (of the N rows, at most 4096, and ``held``) to the front of the cache.
+
+        Returns ``(table [N,M], src, dst [num_pages // 2], remap [num_pages], free_pages
+        [num_pages], counts [2])``: the rows' pages by their new numbers, the moves for
+        ``paged_copy`` (-1 behind them), each page's new number (-1 of those not in use), the
+        free pages and {pages in use, pages moved}. Pages that stay in front keep their numbers."""
+        return self._beam(backend).paged_compact(block_table, seq_lens, page_size, num_pages, held)
+
+    def paged_copy(self, k_cache: torch.Tensor, v_cache: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
+                   backend: Optional[str] = None) -> None:
+        """Copies pages src[i] to dst[i] in both caches [pages,Hk,page_size,d], in place.
+
+        src, dst [n] int32; a pair with a number outside the cache copies nothing. The pages
+        written have to be distinct, and none of them may be read in the same call."""
+        self._beam(backend).paged_copy(k_cache, v_cache, src, dst)
 
     @staticmethod
     def rotary_frequencies(*args, **kwargs):

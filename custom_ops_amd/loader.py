@@ -1,4 +1,4 @@
-"""Deployment loading for the op groups ``fa`` and ``serve``.
+"""Deployment loading for the op groups ``fa``, ``serve`` and ``beam``.
 
 Contract kept from the reference facade (``CustomOps.build`` /
 ``load_precompiled`` / ``load``, __init__.py:654-1011, and ``FAOps``,
@@ -46,7 +46,7 @@ from typing import Callable, Optional
 
 import torch
 
-from . import _lib, build as _build, fa, serve
+from . import _lib, beam, build as _build, fa, serve
 
 ARTIFACT_FORMAT = "custom_ops_amd.artifact/2"
 GROUP_VERSION = "1"
@@ -550,16 +550,57 @@ class ServeOps(FAOps):
     def _open(self, library: Path, native: Optional[Path]) -> None:
         serve.register(str(library), str(native))
 
+    # the in-tree library, its implementation and that one's source; what compiles them
+    def _in_tree(self) -> tuple:
+        return _build.SERVE_LIB_PATH, _build.SERVE_OPS_PATH, _build.SERVE_BINDING_SRC
+
+    def _build_all(self) -> None:
+        _build.build_serve()
+
+    def _build_native(self) -> None:
+        _build.build_serve_ops()
+
     def _tree(self) -> tuple:
-        path, native = Path(_build.SERVE_LIB_PATH), Path(_build.SERVE_OPS_PATH)
+        library, implementation, source = self._in_tree()
+        path, native = Path(library), Path(implementation)
 
         def missing():
-            return not path.exists() or not _build.ops_current(str(native), _build.SERVE_BINDING_SRC)
+            return not path.exists() or not _build.ops_current(str(native), source)
         if missing():   # one process of several builds
             with open(path.parent / f".{self.so_name}.build.lock", "a") as lockf:
                 fcntl.flock(lockf, fcntl.LOCK_EX)
                 if not path.exists():
-                    _build.build_serve()
+                    self._build_all()
                 elif missing():
-                    _build.build_serve_ops()
+                    self._build_native()
         return path.resolve(strict=True), native
+
+
+class BeamOps(ServeOps):
+    """The ``beam`` op group (beam.py): no counterpart in the reference either."""
+
+    so_name = "libmi355_beam"
+    ops = dict(beam.SCHEMAS)
+    meta_ops = tuple(sorted(beam.SCHEMAS))
+    abi = beam.ABI_VERSION
+
+    def _source(self) -> str:
+        return _build.BEAM_SRC
+
+    def _compile(self, product: str, flags: list, verbose: bool) -> None:
+        _build.compile_checked(product, flags, verbose=verbose, src=_build.BEAM_SRC, dma=False)
+
+    def _compile_ops(self, product: str, verbose: bool) -> None:
+        _build.build_beam_ops(product, verbose=verbose)
+
+    def _open(self, library: Path, native: Optional[Path]) -> None:
+        beam.register(str(library), str(native))
+
+    def _in_tree(self) -> tuple:
+        return _build.BEAM_LIB_PATH, _build.BEAM_OPS_PATH, _build.BEAM_BINDING_SRC
+
+    def _build_all(self) -> None:
+        _build.build_beam()
+
+    def _build_native(self) -> None:
+        _build.build_beam_ops()
