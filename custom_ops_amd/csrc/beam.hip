@@ -126,7 +126,7 @@ int shared_decode(const mi355_shared_params* p, hipStream_t st, const Err& err) 
 }
 
 struct SelectPlan {
-  int parts, per, wide;   // wide: the steps of 8 elements a thread are of four
+  int parts, per, wide;   // wide: the steps are of kSelWide times 8 elements a thread
   size_t lists, bytes;
 };
 
@@ -134,10 +134,13 @@ SelectPlan select_plan(const mi355_select_params* p, int cus) {
   SelectPlan pl{};
   const int64_t rows = (int64_t)p->n_groups * p->beams;
   const int small = kSelThreads * 8;
-  const int64_t wanted = std::max<int64_t>(1, 4 * cus / rows);
+  // parts of a row: enough workgroups for all CUs, but no more candidates than the join holds
+  const int64_t most = (int64_t)kSelJoin * kSelEach / ((int64_t)p->beams * p->k);
+  const int64_t wanted = std::max<int64_t>(1, std::min<int64_t>(4 * cus / rows, most));
   const int64_t steps = ((int64_t)p->vocab + small - 1) / small;
-  pl.wide = steps >= 4 * wanted;
-  const int step = pl.wide ? 4 * small : small;
+  const int vectors = p->dtype == MI355_BEAM_FP32 ? kSelWide<float> : kSelWide<__bf16>;
+  pl.wide = steps >= vectors * wanted;
+  const int step = pl.wide ? vectors * small : small;
   const int64_t all = ((int64_t)p->vocab + step - 1) / step, each = (all + wanted - 1) / wanted;
   pl.per = (int)std::min<int64_t>(each * step, 1 << 30);
   pl.parts = (int)(((int64_t)p->vocab + pl.per - 1) / pl.per);
@@ -176,13 +179,15 @@ int beam_select(const mi355_select_params* p, hipStream_t st, const Err& err) {
   a.gs = p->group_stride; a.bs = p->beam_stride;
   a.groups = p->n_groups; a.beams = p->beams; a.vocab = p->vocab; a.k = p->k; a.eos = p->eos;
   a.parts = pl.parts; a.per = pl.per;
+  const uint64_t each = (uint64_t)pl.parts * p->k;
+  a.row_magic = each == 1 ? 0 : (uint32_t)(((1ull << 32) + each - 1) / each);
   const int64_t grid = (int64_t)p->n_groups * p->beams * pl.parts;
   auto go = [&](auto type) {
     typedef decltype(type) T;
-    return run(err, "beam_select", pl.wide ? select_scan_kernel<T, 4> : select_scan_kernel<T, 1>, grid, kSelThreads, 0, st, a);
+    return run(err, "beam_select", pl.wide ? select_scan_kernel<T, kSelWide<T>> : select_scan_kernel<T, 1>, grid, kSelThreads, 0, st, a);
   };
   if (int rc = p->dtype == MI355_BEAM_FP32 ? go(float{}) : p->dtype == MI355_BEAM_BF16 ? go(__bf16{}) : go(_Float16{})) return rc;
-  return run(err, "beam_select (join)", select_join_kernel, p->n_groups, kSelThreads, 0, st, a);
+  return run(err, "beam_select (join)", select_join_kernel, p->n_groups, kSelJoin, 0, st, a);
 }
 
 // What the page operators have in common.

@@ -4,26 +4,33 @@
 //
 // Order is a whole-number result: two beams' candidates that differ in the 8th digit have
 // to come out as the formula says, so the sum of exponentials is formed in 64 bits. The
-// vector unit multiplies and adds in 64 bits as fast as in 32: an exponential is 17 such
-// operations. Bound: the bytes of the logits, each read once.
+// vector unit multiplies and adds in 64 bits as fast as in 32: an exponential is 15 such
+// operations. Bound: the bytes of the logits, each read once; the exponentials take about
+// as long.
 //
 //  * Of a row's logits only the k largest can be selected (their order is that of the
 //    scores), so a workgroup that reads some of a row keeps its k largest logits beside
-//    the running maximum and sum. All elements of a step are in registers; a bound below
-//    the k-th largest comes from the lanes' maxima of 8 elements, by bisecting its bits
-//    with ballots; the few elements above it go to a list in LDS, which is ranked by
-//    counting at the end.
-//  * A second kernel, a workgroup a search, joins the parts' sums and lists.
+//    the sum. A bound below the k-th largest of the first step comes from the lanes'
+//    maxima of 8 elements, by bisecting its bits with ballots; elements that reach it go
+//    to a list in LDS, whose k-th largest is the next bound.
+//  * The next step's logits are in flight while a step computes.
+//  * A second kernel, a workgroup a search, joins the parts' sums and lists: all
+//    candidates in registers, a bound by bisection in each wave, and the few that reach it
+//    ranked by counting.
 
 constexpr int kSelThreads = 256;
 constexpr int kSelList = 1024;      // a list in LDS
 constexpr int kSelMaxK = 64;
 constexpr int kSelMaxBeams = 256;
+constexpr int kSelJoin = 1024;      // threads of the join, and candidates of a thread
+constexpr int kSelEach = 16;
+
+template <class T> constexpr int kSelWide = sizeof(T) == 2 ? 4 : 2;   // 16-byte loads of a thread at a step of a long part: 4
 
 struct SelectHead {
-  double sum;   // Σ exp(x − max)
-  float max;    // NaN: the beam has no candidates
-  int n;        // candidates listed
+  double sum;   // Σ exp(x − ref)
+  float ref;    // −infinity: nothing there; NaN: the beam has no candidates
+  int unused;
 };
 struct SelectArgs {
   const void* x;
@@ -33,10 +40,11 @@ struct SelectArgs {
   int* out_t;
   int* out_p;
   SelectHead* heads;   // [rows][parts]
-  u32x2* lists;        // [rows][parts][k]: logit's ordered bits, token; descending
+  u32x2* lists;        // [rows][parts][k]: logit's ordered bits (0: none), token
   int64_t gs, bs;
   int groups, beams, vocab, k, eos;
   int parts, per;      // parts of a row, tokens of one
+  uint32_t row_magic;  // ceil(2^32 / (parts·k)), 0 where that is 1
 };
 
 // Integers in the order of the floats, the two zeros one.
@@ -50,84 +58,67 @@ __device__ __forceinline__ float unordered(uint32_t u) {
 }
 constexpr uint32_t kLowest = 0x007fffffu;   // of −infinity
 
-// exp of t in [−700, 0], off by 10^-12 of its value: 2^n·p(t − n·ln 2), p of degree 8 fitted
-// for the least relative error on |x| <= ln(2)/2.
-__device__ __forceinline__ double exp_neg(double t) {
+// exp(t), t in [−700, 700]: 2^n·p(t − n·ln 2), p of degree 7 fitted for the least relative
+// error on |x| <= ln(2)/2, which is 4·10^-11 and changes sign 8 times: of a sum's terms most cancels.
+__device__ __forceinline__ double exp64(double t) {
   constexpr double kRound = 6755399441055744.0;   // 1.5·2^52: the sum's low word is the nearest integer
   const double u = __builtin_fma(t, 1.4426950408889634, kRound);
   const double r = __builtin_fma(u - kRound, -0.6931471805599453, t);
-  double p = 2.4727097752539182e-05;
-  p = __builtin_fma(p, r, 0.00019915434933597152);
-  p = __builtin_fma(p, r, 0.0013889178972678572);
-  p = __builtin_fma(p, r, 0.008333267008842798);
-  p = __builtin_fma(p, r, 0.04166666421728999);
-  p = __builtin_fma(p, r, 0.1666666688556212);
-  p = __builtin_fma(p, r, 0.5000000000618945);
-  p = __builtin_fma(p, r, 0.999999999980611);
-  p = __builtin_fma(p, r, 0.9999999999997615);
+  double p = 0.00019775147548215012;
+  p = __builtin_fma(p, r, 0.001394819508339855);
+  p = __builtin_fma(p, r, 0.008333561204466886);
+  p = __builtin_fma(p, r, 0.0416662252511198);
+  p = __builtin_fma(p, r, 0.16666665125072705);
+  p = __builtin_fma(p, r, 0.5000000104597899);
+  p = __builtin_fma(p, r, 1.0000000002433107);
+  p = __builtin_fma(p, r, 0.9999999999616532);
   const uint64_t n = (uint64_t)low_u32(bitcast<uint64_t>(u)) << 52;
   return bitcast<double>(bitcast<uint64_t>(p) + n);
 }
 
+// The larger one; NaN where one is NaN.
+__device__ __forceinline__ float maximum(float x, float y) { return __builtin_elementwise_maximum(x, y); }
+
+// 8 logits of a row, as loaded; behind its end −infinity.
 template <class T> struct Logits;
 template <> struct Logits<float> {
-  static __device__ __forceinline__ void load8(const void* x, int64_t i, float (&y)[8]) {
-    struct __attribute__((packed, aligned(4))) V { u32x4 a, b; };
-    const V v = *reinterpret_cast<const V*>(static_cast<const float*>(x) + i);
+  struct __attribute__((packed, aligned(4))) Raw { u32x4 a, b; };
+  static __device__ __forceinline__ Raw tail(const void* x, int64_t i, int n) {
+    Raw r;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      y[e] = bitcast<float>(v.a[e]);
-      y[4 + e] = bitcast<float>(v.b[e]);
+      const uint32_t* p = static_cast<const uint32_t*>(x) + i + e;
+      r.a[e] = e < n ? p[0] : 0xff800000u;
+      r.b[e] = e + 4 < n ? p[4] : 0xff800000u;
     }
+    return r;
   }
-  static __device__ __forceinline__ float load(const void* x, int64_t i) { return static_cast<const float*>(x)[i]; }
+  static __device__ __forceinline__ float value(const Raw& r, int e) { return bitcast<float>(e < 4 ? r.a[e % 4] : r.b[e % 4]); }
+  static __device__ __forceinline__ float one(const void* x, int64_t i) { return static_cast<const float*>(x)[i]; }
 };
-template <> struct Logits<__bf16> {
-  static __device__ __forceinline__ void load8(const void* x, int64_t i, float (&y)[8]) {
-    struct __attribute__((packed, aligned(2))) V { u32x4 a; };
-    const V v = *reinterpret_cast<const V*>(static_cast<const uint16_t*>(x) + i);
+struct __attribute__((packed, aligned(2))) HalfRaw { u32x4 a; };
+__device__ __forceinline__ HalfRaw half_tail(const void* x, int64_t i, int n, uint32_t none) {
+  HalfRaw r;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      y[2 * e] = bitcast<float>(v.a[e] << 16);
-      y[2 * e + 1] = bitcast<float>(v.a[e] & 0xffff0000u);
-    }
+  for (int e = 0; e < 4; ++e) {
+    const uint16_t* p = static_cast<const uint16_t*>(x) + i + 2 * e;
+    const uint32_t lo = 2 * e < n ? p[0] : none, hi = 2 * e + 1 < n ? p[1] : none;
+    r.a[e] = lo | hi << 16;
   }
-  static __device__ __forceinline__ float load(const void* x, int64_t i) { return bitcast<float>((uint32_t)static_cast<const uint16_t*>(x)[i] << 16); }
+  return r;
+}
+template <> struct Logits<__bf16> {
+  typedef HalfRaw Raw;
+  static __device__ __forceinline__ Raw tail(const void* x, int64_t i, int n) { return half_tail(x, i, n, 0xff80u); }
+  static __device__ __forceinline__ float one(const void* x, int64_t i) { return bitcast<float>((uint32_t)static_cast<const uint16_t*>(x)[i] << 16); }
+  static __device__ __forceinline__ float value(const Raw& r, int e) { return bitcast<float>(e % 2 ? r.a[e / 2] & 0xffff0000u : r.a[e / 2] << 16); }
 };
 template <> struct Logits<_Float16> {
-  static __device__ __forceinline__ void load8(const void* x, int64_t i, float (&y)[8]) {
-    struct __attribute__((packed, aligned(2))) V { f16x8 a; };
-    const V v = *reinterpret_cast<const V*>(static_cast<const uint16_t*>(x) + i);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = (float)v.a[e];
-  }
-  static __device__ __forceinline__ float load(const void* x, int64_t i) { return (float)static_cast<const _Float16*>(x)[i]; }
+  typedef HalfRaw Raw;
+  static __device__ __forceinline__ Raw tail(const void* x, int64_t i, int n) { return half_tail(x, i, n, 0xfc00u); }
+  static __device__ __forceinline__ float one(const void* x, int64_t i) { return (float)static_cast<const _Float16*>(x)[i]; }
+  static __device__ __forceinline__ float value(const Raw& r, int e) { return (float)bitcast<_Float16>((uint16_t)(e % 2 ? r.a[e / 2] >> 16 : r.a[e / 2])); }
 };
-
-// Ranks a list of n keys (all different) and keeps the k largest, in order. All of the
-// workgroup; the list is the same before and after for everybody.
-__device__ __forceinline__ void keep_largest(uint64_t* list, int n, int k) {
-  constexpr int E = kSelList / kSelThreads;
-  uint64_t mine[E];
-  int rank[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int i = e * kSelThreads + (int)threadIdx.x;
-    mine[e] = i < n ? list[i] : 0;
-    rank[e] = 0;
-  }
-  for (int j = 0; j < n; ++j) {
-    const uint64_t y = list[j];
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (e * kSelThreads < n) rank[e] += y > mine[e];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (e * kSelThreads + (int)threadIdx.x < n && rank[e] < k) list[rank[e]] = mine[e];
-  __syncthreads();
-}
 
 // Σ of the threads' counts, for all of the workgroup.
 __device__ __forceinline__ int count_all(int x, int* words) {
@@ -141,189 +132,288 @@ __device__ __forceinline__ int count_all(int x, int* words) {
   return sum;
 }
 
+// Of a wave's values v (E of each lane) the largest t that k of them reach, by its bits from
+// the highest to bit `low`, or a smaller one that exactly k reach (then exact is set); 0 of fewer than k.
+template <int E> __device__ __forceinline__ uint32_t bisect(const uint32_t (&v)[E], int k, int low, bool& exact) {
+  uint32_t t = 0;
+  exact = false;
+#pragma unroll 1
+  for (int bit = 31; bit >= low; --bit) {
+    const uint32_t trial = t | 1u << bit;
+    int c = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) c += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v[e] >= trial));
+    if (c >= k) t = trial;
+    if (c == k) {
+      exact = true;
+      break;
+    }
+  }
+  return t;
+}
+// f(integral_constant E) with the least power of two that E·per covers n, at most 16
+template <class F> __device__ __forceinline__ void by_count(int n, int per, F f) {
+  if (n <= per) f(std::integral_constant<int, 1>{});
+  else if (n <= 2 * per) f(std::integral_constant<int, 2>{});
+  else if (n <= 4 * per) f(std::integral_constant<int, 4>{});
+  else f(std::integral_constant<int, 16>{});
+}
+
+// The k-th largest of a list of n > k different keys (or a smaller value that only k of them
+// reach), each wave for itself.
+__device__ __forceinline__ uint64_t kth_of(const uint64_t* list, int n, int k) {
+  const int lane = threadIdx.x & 63;
+  uint64_t least = 0;
+  by_count(n, 64, [&](auto size) __attribute__((always_inline)) {
+    constexpr int E = decltype(size)::value;
+    uint32_t hi[E], lo[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const uint64_t x = e * 64 + lane < n ? list[e * 64 + lane] : 0;
+      hi[e] = high_u32(x);
+      lo[e] = low_u32(x);
+    }
+    bool exact;
+    const uint32_t h = bisect<E>(hi, k, 0, exact);
+    uint32_t l = 0;
+    if (!exact) {   // equal upper words: of those the lower
+      int above = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(hi[e] > h));
+        lo[e] = hi[e] == h ? lo[e] : 0;
+      }
+      l = bisect<E>(lo, k - above, 0, exact);
+    }
+    least = compose_u64(l, h);
+  });
+  return least;
+}
+
+// Keeps the k largest of a list of n different keys, in any order, and gives the k-th's upper
+// word (0 where there are fewer). The list is the same before and after for all threads.
+__device__ __forceinline__ uint32_t keep_largest(uint64_t* list, int& n, int k, int* count) {
+  if (n <= k) {
+    __syncthreads();
+    if (threadIdx.x == 0) *count = n;
+    __syncthreads();
+    return 0;
+  }
+  const uint64_t least = kth_of(list, n, k);
+  constexpr int E = kSelList / kSelThreads;
+  uint64_t mine[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int i = e * kSelThreads + (int)threadIdx.x;
+    mine[e] = i < n ? list[i] : 0;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) *count = 0;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (mine[e] >= least) list[atomicAdd(count, 1)] = mine[e];
+  __syncthreads();
+  n = k;
+  return high_u32(least);
+}
+
 // N·8 elements of each thread at a step.
 template <class T, int N>
-__global__ __launch_bounds__(kSelThreads) void select_scan_kernel(const SelectArgs a) {
+__global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))) void select_scan_kernel(const SelectArgs a) {
+  typedef Logits<T> L;
+  typedef typename L::Raw Raw;
   constexpr int WAVES = kSelThreads / 64, STEP = kSelThreads * 8 * N;
   __shared__ uint64_t list[kSelList];   // ordered logit, then the complement of the token: the lowest first among equals
   __shared__ int words[WAVES];
   __shared__ int count;
   __shared__ uint32_t bound;
   __shared__ double sSum[WAVES];
-  __shared__ float sMax[WAVES];
+  __shared__ float sRef[WAVES];
   const int row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
   if (a.done && a.done[row]) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6), k = a.k;
   const int64_t base = (int64_t)(row / a.beams) * a.gs + (int64_t)(row % a.beams) * a.bs;
+  const T* x = static_cast<const T*>(a.x) + base;
   const int begin = part * a.per, end = min(a.vocab, begin + a.per);
+  auto fetch = [&](int at, Raw (&r)[N]) __attribute__((always_inline)) {
+    if (at + STEP <= end) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) r[j] = *reinterpret_cast<const Raw*>(x + at + (j * kSelThreads + tid) * 8);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int i = at + (j * kSelThreads + tid) * 8;
+        if (i + 8 <= end) r[j] = *reinterpret_cast<const Raw*>(x + i);
+        else r[j] = L::tail(x, i, end - i);
+      }
+    }
+  };
+  Raw cur[N], next[N];
+  fetch(begin, cur);
   if (tid == 0) {
     count = 0;
-    bound = 0;
+    bound = kLowest + 1;   // never −infinity
   }
-  __syncthreads();
   double sum = 0.;
-  float top = -INFINITY;   // the wave's
+  float ref = -INFINITY;   // the wave's
   bool bad = false;
   int kept = 0;
   for (int at = begin; at < end; at += STEP) {
-    float x[N][8], best[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int i = at + (j * kSelThreads + tid) * 8;
-      if (i + 8 <= end) Logits<T>::load8(a.x, base + i, x[j]);
-      else
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[j][e] = i + e < end ? Logits<T>::load(a.x, base + i + e) : -INFINITY;
-    }
-    uint32_t most = 0;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      best[j] = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        best[j] = fmaxf(best[j], x[j][e]);
-        bad |= x[j][e] != x[j][e];
+    if (at + STEP < end) fetch(at + STEP, next);
+    // f(logit, token) for the thread's elements of the step, read again: for rare cases
+    auto each = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll 1
+      for (int e = 0; e < 8 * N; ++e) {
+        const int i = at + (e / 8 * kSelThreads + tid) * 8 + e % 8;
+        if (i < end) f(L::one(x, i), i);
       }
-      most = max(most, ordered(best[j]));
+    };
+    float best[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      best[j] = L::value(cur[j], 0);
+#pragma unroll
+      for (int e = 1; e < 8; ++e) best[j] = maximum(best[j], L::value(cur[j], e));   // (a NaN stays)
+      bad |= !(best[j] < INFINITY);
     }
-    const float now = unordered((uint32_t)__builtin_amdgcn_readlane(wave_max_scan((int)(most ^ 0x80000000u)), 63) ^ 0x80000000u);
-    if (now > top) {
-      if (top > -INFINITY) sum *= exp((double)top - (double)now);
-      top = now;
+    float most = best[0];
+#pragma unroll
+    for (int j = 1; j < N; ++j) most = fmaxf(most, best[j]);
+    if (__builtin_amdgcn_ballot_w64(most > ref + 300.f)) {   // (the sums' reference need not be their maximum)
+      const float top = unordered((uint32_t)__builtin_amdgcn_readlane(wave_max_scan((int)(ordered(most) ^ 0x80000000u)), 63) ^ 0x80000000u);
+      if (ref > -INFINITY) sum *= exp((double)ref - (double)top);
+      ref = top;
     }
-    if (top > -INFINITY) {
-      const double m = top;
+    if (at == begin) {
+      // At least k of the wave's elements reach t, since k maxima of 8 do, or k of its
+      // elements where there are few maxima: the largest such t, to 16 bits
+      uint32_t t = 0;
+      bool exact;
+      if (N > 1 || k <= 8) {
+        uint32_t v[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = best[j] == best[j] ? ordered(best[j]) : 0;
+        t = bisect<N>(v, k, 16, exact);
+      } else {
+        uint32_t v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = ordered(L::value(cur[0], e));
+        t = bisect<8>(v, k, 16, exact);
+      }
+      __syncthreads();
+      if (lane == 0) atomicMax(&bound, t);
+      __syncthreads();
+    }
+    const float least = unordered(bound);
+    if (__builtin_fabsf(ref) < 1e6f) {
+      const float low = ref - 700.f;
+      const double m = ref;
 #pragma unroll
       for (int j = 0; j < N; ++j)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum += exp_neg(fmax((double)x[j][e] - m, -700.));
+        for (int e = 0; e < 8; ++e) sum += exp64((double)fmaxf(L::value(cur[j], e), low) - m);
+    } else if (ref > -INFINITY) {   // (ref − 700 may be ref)
+      each([&](float y, int) { sum += exp64(fmax((double)y - (double)ref, -700.)); });
     }
-    // At least k of the wave's elements reach t, since k of the maxima of 8 do: the largest
-    // such t, to 16 bits.
-    uint32_t t = 0;
-#pragma unroll 1
-    for (int bit = 31; bit >= 16; --bit) {
-      const uint32_t trial = t | 1u << bit;
-      int n = 0;
 #pragma unroll
-      for (int j = 0; j < N; ++j) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(ordered(best[j]) >= trial));
-      if (n >= k) t = trial;
-    }
-    if (lane == 0) atomicMax(&bound, t);
-    t = max(t, bound);   // (others' bounds hold as well, seen or not)
-    t = max(t, kLowest + 1);   // never −infinity
+    for (int j = 0; j < N; ++j)
+      if (best[j] >= least) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      if (!__builtin_amdgcn_ballot_w64(ordered(best[j]) >= t)) continue;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (ordered(x[j][e]) >= t && x[j][e] == x[j][e]) {
-          const int n = atomicAdd(&count, 1);
-          if (n < kSelList) list[n] = (uint64_t)ordered(x[j][e]) << 32 | (uint32_t)~(at + (j * kSelThreads + tid) * 8 + e);
+        for (int e = 0; e < 8; ++e) {
+          const float y = L::value(cur[j], e);
+          if (y >= least) {
+            const int n = atomicAdd(&count, 1);
+            if (n < kSelList) list[n] = compose_u64(~(uint32_t)(at + (j * kSelThreads + tid) * 8 + e), ordered(y));
+          }
         }
       }
-    }
     __syncthreads();
     int n = count;
-    if (n > kSelList / 2) {
-      __syncthreads();   // all have seen it
-      if (n > kSelList) {
-        // Too many of this step, most of them equal: exactly its k largest, by their
-        // value's bits and, among those of the k-th value, by their places'
-        keep_largest(list, kept, k);
-        kept = min(kept, k);
-        uint32_t v = 0;
-        for (int bit = 31; bit >= 0; --bit) {
-          const uint32_t trial = v | 1u << bit;
-          int c = 0;
-#pragma unroll
-          for (int j = 0; j < N; ++j)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) c += ordered(x[j][e]) >= trial && x[j][e] == x[j][e];
-          if (count_all(c, words) >= k) v = trial;
-        }
-        int above = 0;
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) above += ordered(x[j][e]) > v && x[j][e] == x[j][e];
-        const int need = k - count_all(above, words);
-        int place = 0;   // `need` of the elements of value v lie at or before it
-        for (int bit = 31 - __builtin_clz(STEP); bit >= 0; --bit) {
-          const int trial = place | 1 << bit;
-          int c = 0;
-#pragma unroll
-          for (int j = 0; j < N; ++j)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) c += ordered(x[j][e]) == v && (j * kSelThreads + tid) * 8 + e < trial;
-          if (count_all(c, words) < need) place = trial;
-        }
-        if (tid == 0) count = kept;
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int i = (j * kSelThreads + tid) * 8 + e;
-            const uint32_t o = ordered(x[j][e]);
-            if (x[j][e] == x[j][e] && (o > v || (o == v && i <= place))) list[atomicAdd(&count, 1)] = (uint64_t)o << 32 | (uint32_t)~(at + i);
-          }
-        __syncthreads();
-        n = count;
+    __syncthreads();   // all have seen it
+    if (n > kSelList) {
+      // Too many of this step, most of them equal: exactly its k largest, by their
+      // value's bits and, among those of the k-th value, by their places'
+      keep_largest(list, kept, k, &count);
+      auto total = [&](auto f) __attribute__((always_inline)) {
+        int c = 0;
+        each([&](float y, int i) { c += y == y && f(ordered(y), i - at); });
+        return count_all(c, words);
+      };
+      uint32_t v = 0;
+      for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t trial = v | 1u << bit;
+        if (total([&](uint32_t o, int) { return o >= trial; }) >= k) v = trial;
       }
-      keep_largest(list, n, k);
-      n = min(n, k);
-      if (tid == 0) {
-        count = n;
-        if (n == k) bound = max(bound, (uint32_t)(list[k - 1] >> 32));
+      const int need = k - total([&](uint32_t o, int) { return o > v; });
+      int place = 0;   // `need` of the elements of value v lie at or before it
+      for (int bit = 31 - __builtin_clz(STEP); bit >= 0; --bit) {
+        const int trial = place | 1 << bit;
+        if (total([&](uint32_t o, int i) { return o == v && i < trial; }) < need) place = trial;
       }
+      each([&](float y, int i) {
+        const uint32_t o = ordered(y);
+        if (y == y && (o > v || (o == v && i - at <= place))) list[atomicAdd(&count, 1)] = compose_u64(~(uint32_t)i, o);
+      });
+      __syncthreads();
+      n = count;
+      __syncthreads();
+    }
+    // (ranked lists are the better bound: of a step that follows fewer elements reach it)
+    if (n > 2 * k || n > kSelList / 2 || at + STEP >= end) {
+      const uint32_t b = keep_largest(list, n, k, &count);
+      if (tid == 0) bound = max(bound, b);
       __syncthreads();
     }
     kept = n;
-    __syncthreads();   // nobody adds before all have seen the count
-  }
-  const int n = kept;
-  keep_largest(list, n, k);
-  const int64_t slot = blockIdx.x;
-  for (int i = tid; i < min(n, k); i += kSelThreads)
-    a.lists[slot * k + i] = u32x2{(uint32_t)(list[i] >> 32), ~(uint32_t)list[i]};
 #pragma unroll
-  for (int x = 1; x < 64; x *= 2) sum += __shfl_xor(sum, x);
+    for (int j = 0; j < N; ++j) cur[j] = next[j];
+  }
+  const int64_t slot = blockIdx.x;
+  for (int i = tid; i < k; i += kSelThreads) a.lists[slot * k + i] = i < kept ? u32x2{high_u32(list[i]), ~low_u32(list[i])} : u32x2{0u, 0u};
+#pragma unroll
+  for (int w = 1; w < 64; w *= 2) sum += __shfl_xor(sum, w);
   const bool any_bad = __builtin_amdgcn_ballot_w64(bad) != 0;
   if (lane == 0) {
     sSum[wave] = sum;
-    sMax[wave] = any_bad ? NAN : top;
+    sRef[wave] = any_bad ? NAN : ref;
   }
   __syncthreads();
-  if (tid == 0) {
-    float m = -INFINITY;
-    bool nan = false;
-    for (int w = 0; w < WAVES; ++w) {
-      m = fmaxf(m, sMax[w]);
-      nan |= !(sMax[w] < INFINITY);
-    }
-    double s = 0.;
-    for (int w = 0; w < WAVES; ++w)
-      if (sMax[w] > -INFINITY) s += sSum[w] * exp((double)sMax[w] - (double)m);
-    a.heads[slot] = SelectHead{s, nan ? NAN : m, min(n, k)};
+  if (wave == 0) {
+    const float r = sRef[lane % WAVES];
+    const double s = sSum[lane % WAVES];
+    float m = r;
+    bool nan = r != r;
+#pragma unroll
+    for (int w = 1; w < WAVES; w *= 2) m = fmaxf(m, __shfl_xor(m, w));
+    nan = __builtin_amdgcn_ballot_w64(nan) != 0;
+    double y = r > -INFINITY ? s * exp((double)r - (double)m) : 0.;
+#pragma unroll
+    for (int w = 1; w < WAVES; w *= 2) y += __shfl_xor(y, w);
+    if (lane == 0) a.heads[slot] = SelectHead{y, nan ? NAN : m, 0};
   }
 }
 
 // A search: the rows' parts together.
-__global__ __launch_bounds__(kSelThreads) void select_join_kernel(const SelectArgs a) {
-  __shared__ double base[kSelMaxBeams];    // scores[w] and the logarithm of the sum; NaN: no candidates
-  __shared__ double score[kSelList];
-  __shared__ uint32_t index[kSelList];
-  __shared__ float run[kSelMaxBeams];
-  __shared__ int count, words[kSelThreads / 64];
+__global__ __launch_bounds__(kSelJoin) void select_join_kernel(const SelectArgs a) {
+  constexpr int WAVES = kSelJoin / 64;
+  __shared__ double base[kSelMaxBeams];    // logarithm of the row's sum; infinity: finished
+  __shared__ float run[kSelMaxBeams];      // scores[w]; NaN: no candidates
+  __shared__ double score[kSelList], last[kSelList];
+  __shared__ uint32_t index[kSelList], place[kSelList];
+  __shared__ int rank[kSelList];
+  __shared__ int count, left;
   __shared__ uint32_t bound;
   const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6), k = a.k, g = blockIdx.x;
   const int64_t row0 = (int64_t)g * a.beams;
+  const int per_row = a.parts * k, entries = a.beams * per_row;
+  const u32x2* lists = a.lists + row0 * per_row;
   if (tid == 0) {
-    count = 0;
+    count = left = 0;
     bound = 0;
   }
-  for (int w = wave; w < a.beams; w += kSelThreads / 64) {
+  for (int i = tid; i < kSelList; i += kSelJoin) rank[i] = 0;
+  for (int w = wave; w < a.beams; w += WAVES) {
     const int64_t row = row0 + w;
     const float s = a.scores[row];
     const bool done = a.done && a.done[row];
@@ -332,109 +422,154 @@ __global__ __launch_bounds__(kSelThreads) void select_join_kernel(const SelectAr
     double sum = 0.;
     if (!done) {
       for (int p = lane; p < a.parts; p += 64) {
-        const float x = a.heads[row * a.parts + p].max;
-        m = fmaxf(m, x);
-        nan |= !(x < INFINITY);
-      }
-#pragma unroll
-      for (int x = 1; x < 64; x *= 2) m = fmaxf(m, __shfl_xor(m, x));
-      nan = __builtin_amdgcn_ballot_w64(nan) != 0 || m == -INFINITY;
-      for (int p = lane; p < a.parts; p += 64) {
         const SelectHead h = a.heads[row * a.parts + p];
-        if (h.max > -INFINITY) sum += h.sum * exp((double)h.max - (double)m);
+        nan |= h.ref != h.ref;
+        if (h.ref > m) {
+          sum = (m > -INFINITY ? sum * exp((double)m - (double)h.ref) : 0.) + h.sum;
+          m = h.ref;
+        } else if (h.ref > -INFINITY) sum += h.sum * exp((double)h.ref - (double)m);
       }
+      float top = m;
+#pragma unroll
+      for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
+      nan = __builtin_amdgcn_ballot_w64(nan) != 0 || top == -INFINITY;
+      sum = m > -INFINITY ? sum * exp((double)m - (double)top) : 0.;
+      m = top;
 #pragma unroll
       for (int x = 1; x < 64; x *= 2) sum += __shfl_xor(sum, x);
     }
     if (lane == 0) {
-      const bool real = s > -INFINITY && s < INFINITY && (done || !nan);
-      run[w] = real ? s : NAN;
-      base[w] = done ? INFINITY : (double)m + log(sum);   // (a finished beam: infinity)
+      run[w] = s > -INFINITY && s < INFINITY && (done || !nan) ? s : NAN;
+      base[w] = done ? INFINITY : (double)m + log(sum);
     }
   }
   __syncthreads();
-  // Candidate j of list i (its rows' parts in order), and its place w·vocab + v; false: there is none
-  const int lists = a.beams * a.parts;
-  auto candidate = [&](int i, int j, double& s, uint32_t& at) __attribute__((always_inline)) {
-    const int w = i / a.parts, p = i % a.parts;
-    if (run[w] != run[w]) return false;
-    if (base[w] == INFINITY) {
-      s = run[w];
-      at = (uint32_t)w * a.vocab + a.eos;
-      return p == 0 && j == 0;
-    }
-    const int64_t slot = (row0 + w) * a.parts + p;
-    if (j >= a.heads[slot].n) return false;
-    const u32x2 c = a.lists[slot * k + j];
-    s = (double)run[w] + ((double)unordered(c[0]) - base[w]);
-    at = (uint32_t)w * a.vocab + c[1];
-    return true;
+  // entry i of the rows' lists, one after the other; false: there is none
+  auto candidate = [&](int i, double& s, uint32_t& at) __attribute__((always_inline)) {
+    const int w = a.row_magic ? (int)__umulhi((uint32_t)i, a.row_magic) : i;
+    const u32x2 c = lists[i];   // (not written where the beam is finished, and not used)
+    const float r = run[w];
+    const double b = base[w];
+    const bool done = b == INFINITY;
+    s = done ? (double)r : (double)r + ((double)unordered(c[0]) - b);
+    at = (uint32_t)w * a.vocab + (done ? (uint32_t)a.eos : c[1]);
+    return r == r && (done ? i == w * per_row : c[0] != 0);
   };
-  // Ranks the list and keeps the k best: the highest score, the lowest place among equals
-  auto keep = [&](int n) __attribute__((always_inline)) {
-    constexpr int E = kSelList / kSelThreads;
-    double mine[E];
-    uint32_t at[E];
-    int rank[E];
+  uint32_t key[kSelEach];   // the score in 32 bits; 0: none
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int i = e * kSelThreads + tid;
-      mine[e] = i < n ? score[i] : -INFINITY;
-      at[e] = i < n ? index[i] : 0;
-      rank[e] = 0;
+  for (int e = 0; e < kSelEach; ++e) {
+    key[e] = 0;
+    if (e * kSelJoin < entries) {
+      const int i = e * kSelJoin + tid;
+      double s;
+      uint32_t at;
+      if (candidate(min(i, entries - 1), s, at) && i < entries) key[e] = ordered((float)s);
     }
-    for (int j = 0; j < n; ++j) {
-      const double y = score[j];
-      const uint32_t z = index[j];
+  }
+  uint32_t t = 0;
+  by_count(entries, kSelJoin, [&](auto size) __attribute__((always_inline)) {
+    constexpr int E = decltype(size)::value;
+    uint32_t v[E];
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (e * kSelThreads < n) rank[e] += y > mine[e] || (y == mine[e] && z < at[e]);
+    for (int e = 0; e < E; ++e) v[e] = key[e];
+    bool exact;
+    t = bisect<E>(v, k, 12, exact);
+  });
+  if (lane == 0) atomicMax(&bound, t);
+  __syncthreads();
+  t = max(bound, 1u);
+#pragma unroll
+  for (int e = 0; e < kSelEach; ++e)
+    if (key[e] >= t) {
+      const int n = atomicAdd(&count, 1);
+      if (n < kSelList) candidate(e * kSelJoin + tid, score[n], index[n]);
     }
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (e * kSelThreads + tid < n && rank[e] < k) {
-        score[rank[e]] = mine[e];
-        index[rank[e]] = at[e];
+  __syncthreads();
+  int n = count;
+  if (n > kSelList) {
+    // Too many, most of them equal: one after the other
+    double before = INFINITY;
+    uint32_t behind = 0;
+    for (int x = 0; x < k; ++x) {
+      double best = -INFINITY;
+      uint32_t where = 0xffffffffu;
+      for (int i = tid; i < entries; i += kSelJoin) {
+        double s;
+        uint32_t at;
+        if (candidate(i, s, at) && (s < before || (s == before && at > behind)) && (s > best || (s == best && at < where))) {
+          best = s;
+          where = at;
+        }
       }
-    if (tid == 0) count = min(n, k);
-    __syncthreads();
-  };
-  // Lists descend, so the candidates of rank j come after those of rank j − 1, and none
-  // are left once no list has one that reaches the bound.
-  for (int j = 0; j < k; ++j) {
-    int some = 0;
-    for (int i0 = 0; i0 < lists; i0 += kSelThreads) {
-      double s = 0.;
-      uint32_t at = 0;
-      const int i = i0 + tid;
-      const bool real = i < lists && candidate(i, j, s, at);
-      if (real && ordered((float)s) >= bound) {
-        const int n = atomicAdd(&count, 1);
-        score[n] = s;
-        index[n] = at;
-        ++some;
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {
+        const double y = __shfl_xor(best, d);
+        const uint32_t z = __shfl_xor(where, d);
+        if (y > best || (y == best && z < where)) {
+          best = y;
+          where = z;
+        }
       }
       __syncthreads();
-      const int n = count;
-      __syncthreads();   // all have seen it
-      if (n > kSelList - kSelThreads || (j == 0 && i0 + kSelThreads >= lists && n > k)) {
-        keep(n);
-        if (tid == 0 && n >= k) bound = ordered((float)score[k - 1]);
-        __syncthreads();
+      if (lane == 0) {
+        last[wave] = best;
+        place[wave] = where;
+      }
+      __syncthreads();
+#pragma unroll 1
+      for (int w = 0; w < WAVES; ++w)
+        if (last[w] > best || (last[w] == best && place[w] < where)) {
+          best = last[w];
+          where = place[w];
+        }
+      before = best;
+      behind = where;
+      if (tid == 0) {
+        score[x] = best;
+        index[x] = where;
       }
     }
-    if (count_all(some, words) == 0) break;
+    __syncthreads();
+    n = k;
+  }
+  // the k-th of the list in 32 bits, each wave for itself, and what reaches it
+  uint32_t h = 0;
+  if (n > k)
+    by_count(n, 64, [&](auto size) __attribute__((always_inline)) {
+      constexpr int E = decltype(size)::value;
+      uint32_t v[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = e * 64 + lane < n ? ordered((float)score[e * 64 + lane]) : 0;
+      bool exact;
+      h = bisect<E>(v, k, 0, exact);
+    });
+  if (tid < n && ordered((float)score[tid]) >= h) {
+    const int i = atomicAdd(&left, 1);
+    last[i] = score[tid];
+    place[i] = index[tid];
   }
   __syncthreads();
-  const int n = count;
+  // rank: a wave compares 64 of them with a share of all
+  n = left;
+  for (int i0 = 0; i0 < n; i0 += 64) {
+    const int i = min(i0 + lane, n - 1);
+    const double y = last[i];
+    const uint32_t z = place[i];
+    int better = 0;
+    for (int j = wave; j < n; j += WAVES) better += last[j] > y || (last[j] == y && place[j] < z);
+    if (i0 + lane < n && better) atomicAdd(&rank[i], better);
+  }
   __syncthreads();
-  keep(n);
-  for (int i = tid; i < k; i += kSelThreads) {
-    const bool real = i < n;
-    const int64_t o = (int64_t)g * k + i;
-    a.out_s[o] = real ? (float)score[i] : -INFINITY;
-    a.out_t[o] = real ? (int)(index[i] % (uint32_t)a.vocab) : -1;
-    a.out_p[o] = real ? (int)(row0 + index[i] / (uint32_t)a.vocab) : -1;
+  const int64_t o = (int64_t)g * k;
+  if (tid < n && rank[tid] < k) {
+    const int64_t i = o + rank[tid];
+    const uint32_t w = place[tid] / (uint32_t)a.vocab;
+    a.out_s[i] = (float)last[tid];
+    a.out_t[i] = (int)(place[tid] - w * (uint32_t)a.vocab);
+    a.out_p[i] = (int)(row0 + w);
+  }
+  if (tid >= n && tid < k) {
+    a.out_s[o + tid] = -INFINITY;
+    a.out_t[o + tid] = a.out_p[o + tid] = -1;
   }
 }
