@@ -25,10 +25,33 @@ constexpr int kSelMaxBeams = 256;
 constexpr int kSelJoin = 1024;      // threads of the join, and candidates of a thread
 constexpr int kSelEach = 16;
 
+// Σ over the wave, in all lanes.
+template <int CTRL, int ROWS> __device__ __forceinline__ double dpp_add(double x) {
+  const uint64_t b = bitcast<uint64_t>(x);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0u, low_u32(b), CTRL, ROWS, 0xf, false), hi = __builtin_amdgcn_update_dpp(0u, high_u32(b), CTRL, ROWS, 0xf, false);
+  return x + bitcast<double>(compose_u64(lo, hi));   // (a lane without a source adds 0)
+}
+__device__ __forceinline__ double wave_sum(double x) {
+  x = dpp_add<0x111, 0xf>(x);
+  x = dpp_add<0x112, 0xf>(x);
+  x = dpp_add<0x114, 0xf>(x);
+  x = dpp_add<0x118, 0xf>(x);
+  x = dpp_add<0x142, 0xa>(x);
+  x = dpp_add<0x143, 0xc>(x);
+  const uint64_t b = bitcast<uint64_t>(x);
+  return bitcast<double>(compose_u64(__builtin_amdgcn_readlane(low_u32(b), 63), __builtin_amdgcn_readlane(high_u32(b), 63)));
+}
+
 template <class T> constexpr int kSelWide = sizeof(T) == 2 ? 4 : 2;   // 16-byte loads of a thread at a step of a long part: 4
 
+// bf16 logits have few values, so a long part counts them: a bin for each of the 4096 values
+// of 2^-10 up to 64 and their negatives, of which the exponentials are taken at the end;
+// others at once. An exponential takes 14 operations in 64 bits, a count 5 and an addition in LDS.
+template <class T, int N> constexpr bool kSelBins = std::is_same_v<T, __bf16> && N > 1;
+constexpr uint32_t kBins = 4096, kBinFirst = 117u << 7;   // bits of 2^-10
+
 struct SelectHead {
-  double sum;   // Σ exp(x − ref)
+  double sum;   // 2^600·Σ exp(x − ref)
   float ref;    // −infinity: nothing there; NaN: the beam has no candidates
   int unused;
 };
@@ -58,22 +81,25 @@ __device__ __forceinline__ float unordered(uint32_t u) {
 }
 constexpr uint32_t kLowest = 0x007fffffu;   // of −infinity
 
-// exp(t), t in [−700, 700]: 2^n·p(t − n·ln 2), p of degree 7 fitted for the least relative
-// error on |x| <= ln(2)/2, which is 4·10^-11 and changes sign 8 times: of a sum's terms most cancels.
-__device__ __forceinline__ double exp64(double t) {
-  constexpr double kRound = 6755399441055744.0;   // 1.5·2^52: the sum's low word is the nearest integer
-  const double u = __builtin_fma(t, 1.4426950408889634, kRound);
-  const double r = __builtin_fma(u - kRound, -0.6931471805599453, t);
-  double p = 0.00019775147548215012;
-  p = __builtin_fma(p, r, 0.001394819508339855);
-  p = __builtin_fma(p, r, 0.008333561204466886);
-  p = __builtin_fma(p, r, 0.0416662252511198);
-  p = __builtin_fma(p, r, 0.16666665125072705);
-  p = __builtin_fma(p, r, 0.5000000104597899);
-  p = __builtin_fma(p, r, 1.0000000002433107);
-  p = __builtin_fma(p, r, 0.9999999999616532);
-  const uint64_t n = (uint64_t)low_u32(bitcast<uint64_t>(u)) << 52;
-  return bitcast<double>(bitcast<uint64_t>(p) + n);
+// 2^600·exp(x − ref), x − ref in [−415, 110]: 2^n·p(y − n) with n the whole part of
+// y = (x − ref)·log2(e) + 600 and p of degree 8, exactly 1 at 0, fitted for the least relative
+// error on [0, 1], which is 8·10^-13.
+constexpr double kExpShift = 600.;   // no term is less than 1
+constexpr float kExpLow = 415.f, kExpHigh = 100.f;
+__device__ __forceinline__ double exp_term(float x, double ref) {
+  const double y = __builtin_fma((double)x - ref, 1.4426950408889634, kExpShift);
+  const double f = __builtin_amdgcn_fract(y);
+  double p = 1.8586588623567065e-06;
+  p = __builtin_fma(p, f, 1.42173236346545e-05);
+  p = __builtin_fma(p, f, 0.00015507427260292705);
+  p = __builtin_fma(p, f, 0.0013327602242329773);
+  p = __builtin_fma(p, f, 0.00961832601697772);
+  p = __builtin_fma(p, f, 0.05550407297522302);
+  p = __builtin_fma(p, f, 0.24022651005780424);
+  p = __builtin_fma(p, f, 0.6931471804690105);
+  p = __builtin_fma(p, f, 1.);
+  const uint64_t bits = bitcast<uint64_t>(p);
+  return bitcast<double>(compose_u64(low_u32(bits), high_u32(bits) + ((uint32_t)y << 20)));
 }
 
 // The larger one; NaN where one is NaN.
@@ -138,13 +164,19 @@ template <int E> __device__ __forceinline__ uint32_t bisect(const uint32_t (&v)[
   uint32_t t = 0;
   exact = false;
 #pragma unroll 1
-  for (int bit = 31; bit >= low; --bit) {
-    const uint32_t trial = t | 1u << bit;
-    int c = 0;
+  for (int bit = 30; bit >= low; bit -= 2) {   // two at a time: the counts' latency is what it takes
+    int c[4];
 #pragma unroll
-    for (int e = 0; e < E; ++e) c += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v[e] >= trial));
-    if (c >= k) t = trial;
-    if (c == k) {
+    for (int x = 1; x < 4; ++x) {
+      c[x] = 0;
+      const uint32_t trial = t | (uint32_t)x << bit;
+#pragma unroll
+      for (int e = 0; e < E; ++e) c[x] += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v[e] >= trial));
+    }
+    const int x = c[3] >= k ? 3 : c[2] >= k ? 2 : c[1] >= k ? 1 : 0;
+    t |= (uint32_t)x << bit;
+    if (c[1] == k || c[2] == k || c[3] == k) {
+      // (the largest trial that k reach is one that exactly k reach)
       exact = true;
       break;
     }
@@ -221,6 +253,7 @@ __device__ __forceinline__ uint32_t keep_largest(uint64_t* list, int& n, int k, 
 // N·8 elements of each thread at a step.
 template <class T, int N>
 __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))) void select_scan_kernel(const SelectArgs a) {
+  constexpr bool BINS = kSelBins<T, N>;
   typedef Logits<T> L;
   typedef typename L::Raw Raw;
   constexpr int WAVES = kSelThreads / 64, STEP = kSelThreads * 8 * N;
@@ -230,8 +263,9 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
   __shared__ uint32_t bound;
   __shared__ double sSum[WAVES];
   __shared__ float sRef[WAVES];
+  __shared__ uint32_t bins[BINS ? kBins : 1];
   const int row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
-  if (a.done && a.done[row]) return;
+  const bool done = a.done && a.done[row];
   const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6), k = a.k;
   const int64_t base = (int64_t)(row / a.beams) * a.gs + (int64_t)(row % a.beams) * a.bs;
   const T* x = static_cast<const T*>(a.x) + base;
@@ -250,7 +284,10 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
     }
   };
   Raw cur[N], next[N];
-  fetch(begin, cur);
+  fetch(begin, cur);   // (before it is known whether they are needed)
+  if (done) return;
+  if constexpr (BINS)
+    for (int i = tid; i < kBins; i += kSelThreads) bins[i] = 0;   // (a barrier comes before their first use)
   if (tid == 0) {
     count = 0;
     bound = kLowest + 1;   // never −infinity
@@ -280,7 +317,7 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
     float most = best[0];
 #pragma unroll
     for (int j = 1; j < N; ++j) most = fmaxf(most, best[j]);
-    if (__builtin_amdgcn_ballot_w64(most > ref + 300.f)) {   // (the sums' reference need not be their maximum)
+    if (__builtin_amdgcn_ballot_w64(most > ref + kExpHigh)) {   // (the sums' reference need not be their maximum)
       const float top = unordered((uint32_t)__builtin_amdgcn_readlane(wave_max_scan((int)(ordered(most) ^ 0x80000000u)), 63) ^ 0x80000000u);
       if (ref > -INFINITY) sum *= exp((double)ref - (double)top);
       ref = top;
@@ -307,14 +344,42 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
     }
     const float least = unordered(bound);
     if (__builtin_fabsf(ref) < 1e6f) {
-      const float low = ref - 700.f;
+      const float low = ref - kExpLow;
       const double m = ref;
 #pragma unroll
-      for (int j = 0; j < N; ++j)
+      for (int j = 0; j < N; ++j) {
+        if constexpr (BINS) {
+          // (a bin is 4 bytes; the sign's half of them lies kBins / 2 on)
+          uint32_t to[8], most = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum += exp64((double)fmaxf(L::value(cur[j], e), low) - m);
-    } else if (ref > -INFINITY) {   // (ref − 700 may be ref)
-      each([&](float y, int) { sum += exp64(fmax((double)y - (double)ref, -700.)); });
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t w = cur[j].a[e / 2];
+            const uint32_t size = e % 2 ? w >> 16 & 0x7fffu : w & 0x7fffu;
+            to[e] = size - kBinFirst;
+            most = max(most, to[e]);
+            to[e] |= (e % 2 ? w >> 31 : w >> 15 & 1u) * (kBins / 2);
+          }
+          if (__builtin_amdgcn_ballot_w64(most >= kBins / 2) == 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) atomicAdd(&bins[to[e]], 1u);
+          } else {
+#pragma unroll 1
+            for (int e = 0; e < 8; ++e) {
+              const uint32_t w = cur[j].a[0] >> (e & 1) * 16;
+              // (the words move up, so that the loop need not be unrolled)
+              const uint32_t i = (w & 0x7fffu) - kBinFirst;
+              if (i < kBins / 2) atomicAdd(&bins[i | (w >> 15 & 1u) * (kBins / 2)], 1u);
+              else sum += exp_term(maximum(bitcast<float>(w << 16), low), m);
+              if (e & 1) cur[j].a = u32x4{cur[j].a[1], cur[j].a[2], cur[j].a[3], cur[j].a[0]};
+            }
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum += exp_term(maximum(L::value(cur[j], e), low), m);
+        }
+      }
+    } else if (ref > -INFINITY) {   // (ref − 415 may be ref)
+      each([&](float y, int) { sum += exp_term((float)fmax((double)y - (double)ref, (double)-kExpLow), 0.); });
     }
 #pragma unroll
     for (int j = 0; j < N; ++j)
@@ -371,8 +436,26 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
   }
   const int64_t slot = blockIdx.x;
   for (int i = tid; i < k; i += kSelThreads) a.lists[slot * k + i] = i < kept ? u32x2{high_u32(list[i]), ~low_u32(list[i])} : u32x2{0u, 0u};
+  if constexpr (BINS) {
+    if (lane == 0) sRef[wave] = ref;
+    __syncthreads();
+    float top = sRef[0];
 #pragma unroll
-  for (int w = 1; w < 64; w *= 2) sum += __shfl_xor(sum, w);
+    for (int w = 1; w < WAVES; ++w) top = fmaxf(top, sRef[w]);
+    if (top > -INFINITY && top < 1e6f) {   // (beside a larger one the bins' values are nothing)
+      sum = ref > -INFINITY ? sum * exp((double)ref - (double)top) : 0.;
+      ref = top;
+      for (int i = tid; i < (int)kBins; i += kSelThreads) {
+        const uint32_t c = bins[i];
+        if (__builtin_amdgcn_ballot_w64(c != 0)) {
+          const float x = bitcast<float>(((i & (kBins / 2 - 1)) + kBinFirst) << 16 | (i / (kBins / 2)) << 31);
+          sum = __builtin_fma((double)c, exp_term(fmaxf(x, top - kExpLow), top), sum);
+        }
+      }
+    }
+    __syncthreads();
+  }
+  sum = wave_sum(sum);
   const bool any_bad = __builtin_amdgcn_ballot_w64(bad) != 0;
   if (lane == 0) {
     sSum[wave] = sum;
@@ -413,15 +496,19 @@ __global__ __launch_bounds__(kSelJoin) void select_join_kernel(const SelectArgs 
     bound = 0;
   }
   for (int i = tid; i < kSelList; i += kSelJoin) rank[i] = 0;
-  for (int w = wave; w < a.beams; w += WAVES) {
-    const int64_t row = row0 + w;
+  int width = 1;   // lanes of a row, and rows of a wave: 64 / width
+  while (width < a.parts && width < 64) width *= 2;
+  for (int w0 = wave * (64 / width); w0 < a.beams; w0 += WAVES * (64 / width)) {
+    const int w = w0 + lane / width;
+    const bool real = w < a.beams;
+    const int64_t row = row0 + min(w, a.beams - 1);
     const float s = a.scores[row];
     const bool done = a.done && a.done[row];
     float m = -INFINITY;
-    bool nan = false;
+    int nan = 0;
     double sum = 0.;
-    if (!done) {
-      for (int p = lane; p < a.parts; p += 64) {
+    if (real && !done)   // (a finished row's are not written)
+      for (int p = lane % width; p < a.parts; p += width) {
         const SelectHead h = a.heads[row * a.parts + p];
         nan |= h.ref != h.ref;
         if (h.ref > m) {
@@ -429,18 +516,16 @@ __global__ __launch_bounds__(kSelJoin) void select_join_kernel(const SelectArgs 
           m = h.ref;
         } else if (h.ref > -INFINITY) sum += h.sum * exp((double)h.ref - (double)m);
       }
-      float top = m;
-#pragma unroll
-      for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
-      nan = __builtin_amdgcn_ballot_w64(nan) != 0 || top == -INFINITY;
-      sum = m > -INFINITY ? sum * exp((double)m - (double)top) : 0.;
-      m = top;
-#pragma unroll
-      for (int x = 1; x < 64; x *= 2) sum += __shfl_xor(sum, x);
+    float top = m;
+    for (int x = 1; x < width; x *= 2) {
+      top = fmaxf(top, __shfl_xor(top, x));
+      nan |= __shfl_xor(nan, x);
     }
-    if (lane == 0) {
-      run[w] = s > -INFINITY && s < INFINITY && (done || !nan) ? s : NAN;
-      base[w] = done ? INFINITY : (double)m + log(sum);
+    sum = m > -INFINITY ? sum * exp((double)m - (double)top) : 0.;
+    for (int x = 1; x < width; x *= 2) sum += __shfl_xor(sum, x);
+    if (real && lane % width == 0) {
+      run[w] = s > -INFINITY && s < INFINITY && (done || (!nan && top > -INFINITY)) ? s : NAN;
+      base[w] = done ? INFINITY : (double)top + (log(sum) - kExpShift * 0.6931471805599453);
     }
   }
   __syncthreads();
@@ -532,9 +617,9 @@ __global__ __launch_bounds__(kSelJoin) void select_join_kernel(const SelectArgs 
     __syncthreads();
     n = k;
   }
-  // the k-th of the list in 32 bits, each wave for itself, and what reaches it
+  // the k-th of the list in 32 bits, and what reaches it
   uint32_t h = 0;
-  if (n > k)
+  if (n > k && wave == 0)
     by_count(n, 64, [&](auto size) __attribute__((always_inline)) {
       constexpr int E = decltype(size)::value;
       uint32_t v[E];
@@ -543,6 +628,9 @@ __global__ __launch_bounds__(kSelJoin) void select_join_kernel(const SelectArgs 
       bool exact;
       h = bisect<E>(v, k, 0, exact);
     });
+  if (tid == 0) bound = h;
+  __syncthreads();
+  h = bound;
   if (tid < n && ordered((float)score[tid]) >= h) {
     const int i = atomicAdd(&left, 1);
     last[i] = score[tid];
