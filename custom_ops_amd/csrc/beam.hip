@@ -125,6 +125,10 @@ int shared_decode(const mi355_shared_params* p, hipStream_t st, const Err& err) 
   return rc;
 }
 
+#ifndef FILL
+#define FILL 4
+#endif
+constexpr int kSelFill = FILL;
 struct SelectPlan {
   int parts, per, wide;   // wide: the steps are of kSelWide times 8 elements a thread
   size_t lists, bytes;
@@ -136,7 +140,7 @@ SelectPlan select_plan(const mi355_select_params* p, int cus) {
   const int small = kSelThreads * 8;
   // parts of a row: enough workgroups for all CUs, but no more candidates than the join holds
   const int64_t most = (int64_t)kSelJoin * kSelEach / ((int64_t)p->beams * p->k);
-  const int64_t wanted = std::max<int64_t>(1, std::min<int64_t>(4 * cus / rows, most));
+  const int64_t wanted = std::max<int64_t>(1, std::min<int64_t>(kSelFill * cus / rows, most));
   const int64_t steps = ((int64_t)p->vocab + small - 1) / small;
   const int vectors = p->dtype == MI355_BEAM_FP32 ? kSelWide<float> : kSelWide<__bf16>;
   pl.wide = steps >= vectors * wanted;

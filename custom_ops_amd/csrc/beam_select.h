@@ -19,7 +19,8 @@
 //    ranked by counting.
 
 constexpr int kSelThreads = 256;
-constexpr int kSelList = 1024;      // a list in LDS
+constexpr int kSelList = 1024;      // candidates of the join's list
+constexpr int kSelWave = 256;       // of a wave's
 constexpr int kSelMaxK = 64;
 constexpr int kSelMaxBeams = 256;
 constexpr int kSelJoin = 1024;      // threads of the join, and candidates of a thread
@@ -146,17 +147,8 @@ template <> struct Logits<_Float16> {
   static __device__ __forceinline__ float value(const Raw& r, int e) { return (float)bitcast<_Float16>((uint16_t)(e % 2 ? r.a[e / 2] >> 16 : r.a[e / 2])); }
 };
 
-// Σ of the threads' counts, for all of the workgroup.
-__device__ __forceinline__ int count_all(int x, int* words) {
-  x = __builtin_amdgcn_readlane(wave_scan(x), 63);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) words[threadIdx.x >> 6] = x;
-  __syncthreads();
-  int sum = 0;
-#pragma unroll
-  for (int w = 0; w < kSelThreads / 64; ++w) sum += words[w];
-  return sum;
-}
+// Lanes of m before this one.
+__device__ __forceinline__ int rank_in(uint64_t m) { return __builtin_amdgcn_mbcnt_hi(high_u32(m), __builtin_amdgcn_mbcnt_lo(low_u32(m), 0)); }
 
 // Of a wave's values v (E of each lane) the largest t that k of them reach, by its bits from
 // the highest to bit `low`, or a smaller one that exactly k reach (then exact is set); 0 of fewer than k.
@@ -191,63 +183,58 @@ template <class F> __device__ __forceinline__ void by_count(int n, int per, F f)
   else f(std::integral_constant<int, 16>{});
 }
 
-// The k-th largest of a list of n > k different keys (or a smaller value that only k of them
-// reach), each wave for itself.
-__device__ __forceinline__ uint64_t kth_of(const uint64_t* list, int n, int k) {
+// Keeps the k largest of a wave's list of n different keys in LDS, n at most 64·E, in any
+// order, and gives the k-th's upper word, or a smaller one that only those k reach (0 where there are fewer).
+template <int E> __device__ __forceinline__ uint32_t keep_some(uint64_t* list, int n, int k) {
   const int lane = threadIdx.x & 63;
-  uint64_t least = 0;
-  by_count(n, 64, [&](auto size) __attribute__((always_inline)) {
-    constexpr int E = decltype(size)::value;
-    uint32_t hi[E], lo[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const uint64_t x = e * 64 + lane < n ? list[e * 64 + lane] : 0;
-      hi[e] = high_u32(x);
-      lo[e] = low_u32(x);
-    }
-    bool exact;
-    const uint32_t h = bisect<E>(hi, k, 0, exact);
-    uint32_t l = 0;
-    if (!exact) {   // equal upper words: of those the lower
-      int above = 0;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(hi[e] > h));
-        lo[e] = hi[e] == h ? lo[e] : 0;
-      }
-      l = bisect<E>(lo, k - above, 0, exact);
-    }
-    least = compose_u64(l, h);
-  });
-  return least;
-}
-
-// Keeps the k largest of a list of n different keys, in any order, and gives the k-th's upper
-// word (0 where there are fewer). The list is the same before and after for all threads.
-__device__ __forceinline__ uint32_t keep_largest(uint64_t* list, int& n, int k, int* count) {
-  if (n <= k) {
-    __syncthreads();
-    if (threadIdx.x == 0) *count = n;
-    __syncthreads();
-    return 0;
-  }
-  const uint64_t least = kth_of(list, n, k);
-  constexpr int E = kSelList / kSelThreads;
-  uint64_t mine[E];
+  uint32_t hi[E], lo[E], low[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const int i = e * kSelThreads + (int)threadIdx.x;
-    mine[e] = i < n ? list[i] : 0;
+    const uint64_t x = e * 64 + lane < n ? list[e * 64 + lane] : 0;
+    hi[e] = high_u32(x);
+    lo[e] = low_u32(x);
   }
-  __syncthreads();
-  if (threadIdx.x == 0) *count = 0;
-  __syncthreads();
+  bool exact;
+  const uint32_t h = bisect<E>(hi, k, 0, exact);
+  uint32_t l = 0;
+  if (!exact) {   // equal upper words: of those the lower
+    int above = 0;
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (mine[e] >= least) list[atomicAdd(count, 1)] = mine[e];
-  __syncthreads();
+    for (int e = 0; e < E; ++e) {
+      above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(hi[e] > h));
+      low[e] = hi[e] == h ? lo[e] : 0;
+    }
+    l = bisect<E>(low, k - above, 0, exact);
+  }
+  int at = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const bool stays = hi[e] > h || (hi[e] == h && lo[e] >= l);
+    const uint64_t m = __builtin_amdgcn_ballot_w64(stays);
+    if (stays) list[at + rank_in(m)] = compose_u64(lo[e], hi[e]);
+    at += __builtin_popcountll(m);
+  }
+  return h;
+}
+__device__ __forceinline__ uint32_t keep_largest(uint64_t* list, int& n, int k) {
+  if (n <= k) return 0;
+  const uint32_t h = n <= 64 ? keep_some<1>(list, n, k) : n <= 128 ? keep_some<2>(list, n, k) : keep_some<4>(list, n, k);
   n = k;
-  return high_u32(least);
+  return h;
+}
+
+// What k of a wave's list of n >= k reach, to 16 bits.
+__device__ __forceinline__ uint32_t some_of(const uint64_t* list, int n, int k) {
+  const int lane = threadIdx.x & 63;
+  bool exact;
+  if (n <= 64) {
+    const uint32_t v[1] = {lane < n ? high_u32(list[lane]) : 0};
+    return bisect<1>(v, k, 16, exact);
+  }
+  uint32_t v[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = e * 64 + lane < n ? high_u32(list[e * 64 + lane]) : 0;
+  return bisect<4>(v, k, 16, exact);
 }
 
 // N·8 elements of each thread at a step.
@@ -257,10 +244,10 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
   typedef Logits<T> L;
   typedef typename L::Raw Raw;
   constexpr int WAVES = kSelThreads / 64, STEP = kSelThreads * 8 * N;
-  __shared__ uint64_t list[kSelList];   // ordered logit, then the complement of the token: the lowest first among equals
-  __shared__ int words[WAVES];
-  __shared__ int count;
-  __shared__ uint32_t bound;
+  __shared__ uint64_t lists[WAVES][kSelWave];   // ordered logit, then the complement of the token: the lowest first among equals
+  __shared__ __align__(16) Raw some8[WAVES][8];
+  __shared__ int from8[WAVES][8], counts[WAVES];
+  __shared__ __align__(16) uint32_t quarter[WAVES];   // a WAVES-th of k of the wave's elements reach it
   __shared__ double sSum[WAVES];
   __shared__ float sRef[WAVES];
   __shared__ uint32_t bins[BINS ? kBins : 1];
@@ -270,34 +257,43 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
   const int64_t base = (int64_t)(row / a.beams) * a.gs + (int64_t)(row % a.beams) * a.bs;
   const T* x = static_cast<const T*>(a.x) + base;
   const int begin = part * a.per, end = min(a.vocab, begin + a.per);
+  // a whole step, and the last one
   auto fetch = [&](int at, Raw (&r)[N]) __attribute__((always_inline)) {
-    if (at + STEP <= end) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) r[j] = *reinterpret_cast<const Raw*>(x + at + (j * kSelThreads + tid) * 8);
-    } else {
+    for (int j = 0; j < N; ++j) r[j] = *reinterpret_cast<const Raw*>(x + at + (j * kSelThreads + tid) * 8);
+  };
+  auto fetch_tail = [&](int at, Raw (&r)[N]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const int i = at + (j * kSelThreads + tid) * 8;
-        if (i + 8 <= end) r[j] = *reinterpret_cast<const Raw*>(x + i);
-        else r[j] = L::tail(x, i, end - i);
-      }
+    for (int j = 0; j < N; ++j) {
+      const int i = at + (j * kSelThreads + tid) * 8;
+      if (i + 8 <= end) r[j] = *reinterpret_cast<const Raw*>(x + i);
+      else r[j] = L::tail(x, i, end - i);
     }
   };
   Raw cur[N], next[N];
-  fetch(begin, cur);   // (before it is known whether they are needed)
+  // (before it is known whether they are needed)
+  if (begin + STEP <= end) fetch(begin, cur);
+  else fetch_tail(begin, cur);
   if (done) return;
   if constexpr (BINS)
-    for (int i = tid; i < kBins; i += kSelThreads) bins[i] = 0;   // (a barrier comes before their first use)
-  if (tid == 0) {
-    count = 0;
-    bound = kLowest + 1;   // never −infinity
-  }
+    for (int i = tid; i < (int)kBins; i += kSelThreads) bins[i] = 0;
+  if (tid < WAVES) quarter[tid] = 0;
+  __syncthreads();
+  // After the first step the waves go their own ways, but that each tells what a
+  // WAVES-th of k of its elements reach: k of the workgroup's reach the least of that.
+  uint64_t* list = lists[wave];
+  const int some = (k + WAVES - 1) / WAVES;
+  auto tell = [&](uint32_t q) __attribute__((always_inline)) {
+    if (lane == 0) *const_cast<volatile uint32_t*>(&quarter[wave]) = q;
+  };
   double sum = 0.;
   float ref = -INFINITY;   // the wave's
   bool bad = false;
-  int kept = 0;
+  int n = 0, steps = 0;       // of the wave's list; done
+  uint32_t t = kLowest + 1;   // what reaches it is listed; never −infinity
   for (int at = begin; at < end; at += STEP) {
-    if (at + STEP < end) fetch(at + STEP, next);
+    const bool whole = at + 2 * STEP <= end;   // the step that follows
+    if (whole) fetch(at + STEP, next);
     // f(logit, token) for the thread's elements of the step, read again: for rare cases
     auto each = [&](auto f) __attribute__((always_inline)) {
 #pragma unroll 1
@@ -323,26 +319,17 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
       ref = top;
     }
     if (at == begin) {
-      // At least k of the wave's elements reach t, since k maxima of 8 do, or k of its
-      // elements where there are few maxima: the largest such t, to 16 bits
-      uint32_t t = 0;
+      // Of the wave's maxima of 8 elements, to 16 bits, so that it is found in 8 steps
       bool exact;
-      if (N > 1 || k <= 8) {
-        uint32_t v[N];
+      uint32_t v[N];
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = best[j] == best[j] ? ordered(best[j]) : 0;
-        t = bisect<N>(v, k, 16, exact);
-      } else {
-        uint32_t v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = ordered(L::value(cur[0], e));
-        t = bisect<8>(v, k, 16, exact);
-      }
-      __syncthreads();
-      if (lane == 0) atomicMax(&bound, t);
+      for (int j = 0; j < N; ++j) v[j] = best[j] == best[j] ? ordered(best[j]) : 0;
+      const uint32_t q = bisect<N>(v, some, 16, exact);
+      tell(q);
       __syncthreads();
     }
-    const float least = unordered(bound);
+    const u32x4 q4 = *reinterpret_cast<const volatile u32x4*>(quarter);
+    t = max(t, min(min(q4[0], q4[1]), min(q4[2], q4[3])));
     if (__builtin_fabsf(ref) < 1e6f) {
       const float low = ref - kExpLow;
       const double m = ref;
@@ -381,61 +368,70 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
     } else if (ref > -INFINITY) {   // (ref − 415 may be ref)
       each([&](float y, int) { sum += exp_term((float)fmax((double)y - (double)ref, (double)-kExpLow), 0.); });
     }
+    // Threads with an element that reaches t write their 8 down, 8 threads at a time, and
+    // each lane looks at one
+    int hits = 0, place[N];
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (best[j] >= least) {
+    for (int j = 0; j < N; ++j) {
+      const uint64_t m = __builtin_amdgcn_ballot_w64(best[j] >= unordered(t));
+      place[j] = m >> lane & 1 ? hits + rank_in(m) : -1;
+      hits += __builtin_popcountll(m);
+    }
+    uint32_t full = 0;
+    for (int p = 0; p < hits; p += 8) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float y = L::value(cur[j], e);
-          if (y >= least) {
-            const int n = atomicAdd(&count, 1);
-            if (n < kSelList) list[n] = compose_u64(~(uint32_t)(at + (j * kSelThreads + tid) * 8 + e), ordered(y));
-          }
+      for (int j = 0; j < N; ++j)
+        if ((uint32_t)(place[j] - p) < 8u) {
+          some8[wave][place[j] - p] = cur[j];
+          from8[wave][place[j] - p] = at + (j * kSelThreads + tid) * 8;
         }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // (a wave's LDS accesses stay in order)
+      const int i = lane >> 3;
+      const float y = L::one(&some8[wave][i], lane & 7);
+      const uint32_t token = from8[wave][i] + (lane & 7);
+      uint64_t m = __builtin_amdgcn_ballot_w64(i < hits - p && y >= unordered(t));
+      if (n > kSelWave - 64) {
+        full = keep_largest(list, n, k);
+        t = max(t, full);
+        m = __builtin_amdgcn_ballot_w64(i < hits - p && y >= unordered(t));
       }
-    __syncthreads();
-    int n = count;
-    __syncthreads();   // all have seen it
-    if (n > kSelList) {
-      // Too many of this step, most of them equal: exactly its k largest, by their
-      // value's bits and, among those of the k-th value, by their places'
-      keep_largest(list, kept, k, &count);
-      auto total = [&](auto f) __attribute__((always_inline)) {
-        int c = 0;
-        each([&](float y, int i) { c += y == y && f(ordered(y), i - at); });
-        return count_all(c, words);
-      };
-      uint32_t v = 0;
-      for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t trial = v | 1u << bit;
-        if (total([&](uint32_t o, int) { return o >= trial; }) >= k) v = trial;
-      }
-      const int need = k - total([&](uint32_t o, int) { return o > v; });
-      int place = 0;   // `need` of the elements of value v lie at or before it
-      for (int bit = 31 - __builtin_clz(STEP); bit >= 0; --bit) {
-        const int trial = place | 1 << bit;
-        if (total([&](uint32_t o, int i) { return o == v && i < trial; }) < need) place = trial;
-      }
-      each([&](float y, int i) {
-        const uint32_t o = ordered(y);
-        if (y == y && (o > v || (o == v && i - at <= place))) list[atomicAdd(&count, 1)] = compose_u64(~(uint32_t)i, o);
-      });
-      __syncthreads();
-      n = count;
-      __syncthreads();
+      if (m >> lane & 1) list[n + rank_in(m)] = compose_u64(~token, ordered(y));
+      n += __builtin_popcountll(m);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-    // (ranked lists are the better bound: of a step that follows fewer elements reach it)
-    if (n > 2 * k || n > kSelList / 2 || at + STEP >= end) {
-      const uint32_t b = keep_largest(list, n, k, &count);
-      if (tid == 0) bound = max(bound, b);
-      __syncthreads();
+    if (n >= 3 * k || full) {
+      full = keep_largest(list, n, k);
+      // (k of the elements up to here reach `full`, and equals come later)
+      if (full) t = max(t, full + 1);
     }
-    kept = n;
+    // after 1, 2, 4, .. steps: by then half of what is seen is new
+    ++steps;
+    if ((steps & (steps - 1)) == 0 && n >= some && at + STEP < end) tell(some_of(list, n, some));
+    if (whole) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) cur[j] = next[j];
+      for (int j = 0; j < N; ++j) cur[j] = next[j];
+    } else if (at + STEP < end) fetch_tail(at + STEP, cur);
+  }
+  // the waves' lists as one
+  if (n > 64) keep_largest(list, n, k);
+  if (lane == 0) counts[wave] = n;
+  __syncthreads();
+  if (wave == 0) {
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) {
+      const int c = counts[w];
+      const uint64_t x = lane < c ? lists[w][lane] : 0;
+      if (lane < c) list[n + lane] = x;
+      n += c;
+    }
+    keep_largest(list, n, k);
+    u32x2* out = a.lists + (int64_t)blockIdx.x * k;
+    if (lane < k) {
+      const uint64_t x = lane < n ? list[lane] : ~0ull >> 32;
+      out[lane] = u32x2{high_u32(x), ~low_u32(x)};   // (0 where there is none)
+    }
   }
   const int64_t slot = blockIdx.x;
-  for (int i = tid; i < k; i += kSelThreads) a.lists[slot * k + i] = i < kept ? u32x2{high_u32(list[i]), ~low_u32(list[i])} : u32x2{0u, 0u};
   if constexpr (BINS) {
     if (lane == 0) sRef[wave] = ref;
     __syncthreads();
