@@ -125,10 +125,6 @@ int shared_decode(const mi355_shared_params* p, hipStream_t st, const Err& err) 
   return rc;
 }
 
-#ifndef FILL
-#define FILL 4
-#endif
-constexpr int kSelFill = FILL;
 struct SelectPlan {
   int parts, per, wide;   // wide: the steps are of kSelWide times 8 elements a thread
   size_t lists, bytes;
@@ -138,9 +134,11 @@ SelectPlan select_plan(const mi355_select_params* p, int cus) {
   SelectPlan pl{};
   const int64_t rows = (int64_t)p->n_groups * p->beams;
   const int small = kSelThreads * 8;
-  // parts of a row: enough workgroups for all CUs, but no more candidates than the join holds
+  // Parts of a row: workgroups for all CUs, four on each, but one where k is large, since the
+  // join's candidates grow with both (us for one, two, four: [4 x 50 x 10007] fp32, k = 50
+  // 25.8 / 34.1 / 35.7; [64 x 8 x 128000] bf16, k = 16 71 / 71 / 60); no more than the join holds
   const int64_t most = (int64_t)kSelJoin * kSelEach / ((int64_t)p->beams * p->k);
-  const int64_t wanted = std::max<int64_t>(1, std::min<int64_t>(kSelFill * cus / rows, most));
+  const int64_t wanted = std::max<int64_t>(1, std::min<int64_t>((p->k > 32 ? 1 : 4) * cus / rows, most));
   const int64_t steps = ((int64_t)p->vocab + small - 1) / small;
   const int vectors = p->dtype == MI355_BEAM_FP32 ? kSelWide<float> : kSelWide<__bf16>;
   pl.wide = steps >= vectors * wanted;
@@ -191,7 +189,8 @@ int beam_select(const mi355_select_params* p, hipStream_t st, const Err& err) {
     return run(err, "beam_select", pl.wide ? select_scan_kernel<T, kSelWide<T>> : select_scan_kernel<T, 1>, grid, kSelThreads, 0, st, a);
   };
   if (int rc = p->dtype == MI355_BEAM_FP32 ? go(float{}) : p->dtype == MI355_BEAM_BF16 ? go(__bf16{}) : go(_Float16{})) return rc;
-  return run(err, "beam_select (join)", select_join_kernel, p->n_groups, kSelJoin, 0, st, a);
+  if (p->beams * each <= 256) return run(err, "beam_select (join)", select_join_kernel<256, 1>, p->n_groups, 256, 0, st, a);
+  return run(err, "beam_select (join)", select_join_kernel<kSelJoin, kSelEach>, p->n_groups, kSelJoin, 0, st, a);
 }
 
 // What the page operators have in common.

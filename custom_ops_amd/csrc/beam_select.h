@@ -19,11 +19,10 @@
 //    ranked by counting.
 
 constexpr int kSelThreads = 256;
-constexpr int kSelList = 1024;      // candidates of the join's list
 constexpr int kSelWave = 256;       // of a wave's
 constexpr int kSelMaxK = 64;
 constexpr int kSelMaxBeams = 256;
-constexpr int kSelJoin = 1024;      // threads of the join, and candidates of a thread
+constexpr int kSelJoin = 1024;      // threads of the join, and candidates of a thread, at most
 constexpr int kSelEach = 16;
 
 // Σ over the wave, in all lanes.
@@ -216,9 +215,20 @@ template <int E> __device__ __forceinline__ uint32_t keep_some(uint64_t* list, i
   }
   return h;
 }
+// Of 64 at most: by their ranks, so that they are in order.
+__device__ __forceinline__ uint32_t keep_few(uint64_t* list, int n, int k) {
+  const int lane = threadIdx.x & 63;
+  const uint64_t x = lane < n ? list[lane] : 0;
+  int rank = 0;
+#pragma unroll 4
+  for (int j = 0; j < n; ++j) rank += list[j] > x;
+  if (lane < n && rank < k) list[rank] = x;
+  const int last = __builtin_ctzll(__builtin_amdgcn_ballot_w64(lane < n && rank == k - 1));
+  return (uint32_t)__builtin_amdgcn_readlane(high_u32(x), last);
+}
 __device__ __forceinline__ uint32_t keep_largest(uint64_t* list, int& n, int k) {
   if (n <= k) return 0;
-  const uint32_t h = n <= 64 ? keep_some<1>(list, n, k) : n <= 128 ? keep_some<2>(list, n, k) : keep_some<4>(list, n, k);
+  const uint32_t h = n <= 64 ? keep_few(list, n, k) : n <= 128 ? keep_some<2>(list, n, k) : keep_some<4>(list, n, k);
   n = k;
   return h;
 }
@@ -247,7 +257,7 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
   __shared__ uint64_t lists[WAVES][kSelWave];   // ordered logit, then the complement of the token: the lowest first among equals
   __shared__ __align__(16) Raw some8[WAVES][8];
   __shared__ int from8[WAVES][8], counts[WAVES];
-  __shared__ __align__(16) uint32_t quarter[WAVES];   // a WAVES-th of k of the wave's elements reach it
+  __shared__ __align__(16) uint32_t quarter[WAVES];   // what a share of k of the wave's elements reach
   __shared__ double sSum[WAVES];
   __shared__ float sRef[WAVES];
   __shared__ uint32_t bins[BINS ? kBins : 1];
@@ -277,14 +287,16 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
   if (done) return;
   if constexpr (BINS)
     for (int i = tid; i < (int)kBins; i += kSelThreads) bins[i] = 0;
-  if (tid < WAVES) quarter[tid] = 0;
+  // (waves that have whole vectors of elements: the others have nothing to tell)
+  const int active = min(WAVES, max(1, (end - begin) / 512));
+  if (tid < WAVES) quarter[tid] = tid < active ? 0 : ~0u;
   __syncthreads();
-  // After the first step the waves go their own ways, but that each tells what a
-  // WAVES-th of k of its elements reach: k of the workgroup's reach the least of that.
+  // After the first step the waves go their own ways, but that each tells what its share of
+  // k of its elements reach: k of the workgroup's reach the least of that.
   uint64_t* list = lists[wave];
-  const int some = (k + WAVES - 1) / WAVES;
+  const int some = (k + active - 1) / active;
   auto tell = [&](uint32_t q) __attribute__((always_inline)) {
-    if (lane == 0) *const_cast<volatile uint32_t*>(&quarter[wave]) = q;
+    if (lane == 0 && wave < active) *const_cast<volatile uint32_t*>(&quarter[wave]) = q;
   };
   double sum = 0.;
   float ref = -INFINITY;   // the wave's
@@ -473,25 +485,31 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
   }
 }
 
-// A search: the rows' parts together.
-__global__ __launch_bounds__(kSelJoin) void select_join_kernel(const SelectArgs a) {
-  constexpr int WAVES = kSelJoin / 64;
+// A search: the rows' parts together. THREADS: 1024, or 256 where each then has one candidate
+// (4 waves meet at a barrier sooner than 16: 256 candidates 4.3 us, with 1024 threads 6.8).
+template <int THREADS, int EACH>
+__global__ __launch_bounds__(THREADS) void select_join_kernel(const SelectArgs a) {
+  constexpr int WAVES = THREADS / 64, LIST = THREADS;
   __shared__ double base[kSelMaxBeams];    // logarithm of the row's sum; infinity: finished
   __shared__ float run[kSelMaxBeams];      // scores[w]; NaN: no candidates
-  __shared__ double score[kSelList], last[kSelList];
-  __shared__ uint32_t index[kSelList], place[kSelList];
-  __shared__ int rank[kSelList];
+  __shared__ double score[LIST], last[LIST];
+  __shared__ uint32_t index[LIST], place[LIST];
+  __shared__ int rank[LIST];
   __shared__ int count, left;
   __shared__ uint32_t bound;
   const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6), k = a.k, g = blockIdx.x;
   const int64_t row0 = (int64_t)g * a.beams;
   const int per_row = a.parts * k, entries = a.beams * per_row;
   const u32x2* lists = a.lists + row0 * per_row;
+  u32x2 c[EACH];   // (a finished row's are not written, and not used)
+#pragma unroll
+  for (int e = 0; e < EACH; ++e)
+    if (e == 0 || e * THREADS < entries) c[e] = lists[min(e * THREADS + tid, entries - 1)];
   if (tid == 0) {
     count = left = 0;
     bound = 0;
   }
-  for (int i = tid; i < kSelList; i += kSelJoin) rank[i] = 0;
+  rank[tid] = 0;
   int width = 1;   // lanes of a row, and rows of a wave: 64 / width
   while (width < a.parts && width < 64) width *= 2;
   for (int w0 = wave * (64 / width); w0 < a.beams; w0 += WAVES * (64 / width)) {
@@ -526,9 +544,8 @@ __global__ __launch_bounds__(kSelJoin) void select_join_kernel(const SelectArgs 
   }
   __syncthreads();
   // entry i of the rows' lists, one after the other; false: there is none
-  auto candidate = [&](int i, double& s, uint32_t& at) __attribute__((always_inline)) {
+  auto valued = [&](int i, u32x2 c, double& s, uint32_t& at) __attribute__((always_inline)) {
     const int w = a.row_magic ? (int)__umulhi((uint32_t)i, a.row_magic) : i;
-    const u32x2 c = lists[i];   // (not written where the beam is finished, and not used)
     const float r = run[w];
     const double b = base[w];
     const bool done = b == INFINITY;
@@ -536,45 +553,48 @@ __global__ __launch_bounds__(kSelJoin) void select_join_kernel(const SelectArgs 
     at = (uint32_t)w * a.vocab + (done ? (uint32_t)a.eos : c[1]);
     return r == r && (done ? i == w * per_row : c[0] != 0);
   };
-  uint32_t key[kSelEach];   // the score in 32 bits; 0: none
+  auto candidate = [&](int i, double& s, uint32_t& at) __attribute__((always_inline)) { return valued(i, lists[i], s, at); };
+  uint32_t key[EACH];   // the score in 32 bits; 0: none
 #pragma unroll
-  for (int e = 0; e < kSelEach; ++e) {
+  for (int e = 0; e < EACH; ++e) {
     key[e] = 0;
-    if (e * kSelJoin < entries) {
-      const int i = e * kSelJoin + tid;
+    if (e == 0 || e * THREADS < entries) {
+      const int i = e * THREADS + tid;
       double s;
       uint32_t at;
-      if (candidate(min(i, entries - 1), s, at) && i < entries) key[e] = ordered((float)s);
+      if (valued(min(i, entries - 1), c[e], s, at) && i < entries) key[e] = ordered((float)s);
     }
   }
   uint32_t t = 0;
-  by_count(entries, kSelJoin, [&](auto size) __attribute__((always_inline)) {
-    constexpr int E = decltype(size)::value;
-    uint32_t v[E];
+  bool exact;
+  if constexpr (EACH == 1) t = bisect<1>(key, k, 12, exact);
+  else
+    by_count(entries, THREADS, [&](auto size) __attribute__((always_inline)) {
+      constexpr int E = decltype(size)::value;
+      uint32_t v[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = key[e];
-    bool exact;
-    t = bisect<E>(v, k, 12, exact);
-  });
+      for (int e = 0; e < E; ++e) v[e] = key[e];
+      t = bisect<E>(v, k, 12, exact);
+    });
   if (lane == 0) atomicMax(&bound, t);
   __syncthreads();
   t = max(bound, 1u);
 #pragma unroll
-  for (int e = 0; e < kSelEach; ++e)
+  for (int e = 0; e < EACH; ++e)
     if (key[e] >= t) {
       const int n = atomicAdd(&count, 1);
-      if (n < kSelList) candidate(e * kSelJoin + tid, score[n], index[n]);
+      if (n < LIST) candidate(e * THREADS + tid, score[n], index[n]);
     }
   __syncthreads();
   int n = count;
-  if (n > kSelList) {
+  if (n > LIST) {
     // Too many, most of them equal: one after the other
     double before = INFINITY;
     uint32_t behind = 0;
     for (int x = 0; x < k; ++x) {
       double best = -INFINITY;
       uint32_t where = 0xffffffffu;
-      for (int i = tid; i < entries; i += kSelJoin) {
+      for (int i = tid; i < entries; i += THREADS) {
         double s;
         uint32_t at;
         if (candidate(i, s, at) && (s < before || (s == before && at > behind)) && (s > best || (s == best && at < where))) {
@@ -613,20 +633,21 @@ __global__ __launch_bounds__(kSelJoin) void select_join_kernel(const SelectArgs 
     __syncthreads();
     n = k;
   }
-  // the k-th of the list in 32 bits, and what reaches it
+  // many: the k-th of the list in 32 bits, and what reaches it
   uint32_t h = 0;
-  if (n > k && wave == 0)
-    by_count(n, 64, [&](auto size) __attribute__((always_inline)) {
-      constexpr int E = decltype(size)::value;
-      uint32_t v[E];
+  if (n > 2 * k && n > 64) {
+    if (wave == 0)
+      by_count(n, 64, [&](auto size) __attribute__((always_inline)) {
+        constexpr int E = decltype(size)::value;
+        uint32_t v[E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[e] = e * 64 + lane < n ? ordered((float)score[e * 64 + lane]) : 0;
-      bool exact;
-      h = bisect<E>(v, k, 0, exact);
-    });
-  if (tid == 0) bound = h;
-  __syncthreads();
-  h = bound;
+        for (int e = 0; e < E; ++e) v[e] = e * 64 + lane < n ? ordered((float)score[e * 64 + lane]) : 0;
+        h = bisect<E>(v, k, 0, exact);
+      });
+    if (tid == 0) bound = h;
+    __syncthreads();
+    h = bound;
+  }
   if (tid < n && ordered((float)score[tid]) >= h) {
     const int i = atomicAdd(&left, 1);
     last[i] = score[tid];
