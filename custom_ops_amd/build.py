@@ -206,7 +206,7 @@ def build_beam_ops(path: str = BEAM_OPS_PATH, verbose: bool = False) -> str:
 
 def build_beam(verbose: bool = False) -> str:
     """Compile those operators' library and its binding; return the library's path."""
-    out = compile_checked(BEAM_LIB_PATH, verbose=verbose, src=BEAM_SRC, dma=False)
+    out = compile_checked(BEAM_LIB_PATH, verbose=verbose, src=BEAM_SRC)
     build_beam_ops(verbose=verbose)
     return out
 

@@ -47,23 +47,28 @@ size_t up(size_t x) { return (x + 255) & ~(size_t)255; }
 
 struct SharedPlan {
   int columns, groups, target, least;
-  int64_t grid;           // parts at most
+  int64_t grid;           // workgroups at most
+  int64_t own_rows, rows; // rows of partial sums: of groups' parts, and all
   size_t ml, o, bytes;    // offsets of the parts' statistics and sums in the workspace
 };
 
 SharedPlan shared_plan(const mi355_shared_params* p, int cus) {
   SharedPlan pl{};
-  const int ratio = p->h / p->h_k;
-  pl.groups = (ratio + 15) / 16;
-  pl.columns = p->n_groups > 0 && (int64_t)p->b * ratio > 16 * (int64_t)p->n_groups ? kShColumns(p->d) : 16;
+  const int64_t ratio = p->h / p->h_k;
+  pl.groups = (int)((ratio + 15) / 16);
+  // columns of a KV head that a group has on average
+  const int64_t mean = p->n_groups > 0 ? p->b * ratio / p->n_groups : 0;
+  pl.columns = mean > 64 ? 128 : mean > 32 ? 64 : 32;
   pl.target = 2 * cus;
   pl.least = 4;
   const int64_t own = (int64_t)p->b * p->h_k * pl.groups;
-  const int64_t common = p->h_k * (((int64_t)p->b * ratio + pl.columns - 1) / pl.columns + p->n_groups);
+  const int64_t common = p->h_k * ((p->b * ratio + pl.columns - 1) / pl.columns + p->n_groups);
   pl.grid = own + common + pl.target;
+  pl.own_rows = (common + pl.target) * pl.columns;
+  pl.rows = pl.own_rows + pl.grid * 16;
   pl.ml = up((size_t)(p->n_groups + p->b) * 16);
-  pl.o = pl.ml + up((size_t)pl.grid * pl.columns * 8);
-  pl.bytes = pl.o + (size_t)pl.grid * pl.columns * p->d * 4;
+  pl.o = pl.ml + up((size_t)pl.rows * 8);
+  pl.bytes = pl.o + (size_t)pl.rows * p->d * 4;
   return pl;
 }
 
@@ -88,13 +93,14 @@ int shared_decode(const mi355_shared_params* p, hipStream_t st, const Err& err) 
   if (!p->q || !p->o || !p->kv_lens || !p->cu_groups || (p->n_groups > 0 && !p->prefix_lens) || (p->table_cols > 0 && !p->block_table) ||
       (p->num_pages > 0 && (!p->k_cache || !p->v_cache)))
     return err.fail(kEinval, "tensor pointer is NULL");
-  if (!rows_ok(p->q, {p->q_batch_stride, p->q_head_stride}) || !rows_ok(p->o, {}) ||
+  if (!rows_ok(p->q, {p->q_batch_stride, p->q_head_stride}) || !rows_ok(p->o, {p->o_batch_stride, p->o_head_stride}) ||
       !rows_ok(p->k_cache, {p->k_page_stride, p->k_head_stride, p->k_row_stride}) ||
       !rows_ok(p->v_cache, {p->v_page_stride, p->v_head_stride, p->v_row_stride}))
-    return err.fail(kEinval, "q and the caches must be 16-byte aligned with strides that are multiples of 8 elements");
+    return err.fail(kEinval, "q, o and the caches must be 16-byte aligned with strides that are multiples of 8 elements");
   Device dev;
   if (int rc = device_ok(err, &dev)) return rc;
   const SharedPlan pl = shared_plan(p, dev.cus);
+  if (pl.rows > INT_MAX) return err.fail(kEinval, "too many requests and heads");
   if (int rc = workspace_ok(err, p->workspace, p->workspace_bytes, pl.bytes)) return rc;
   a.q = (const uint16_t*)p->q; a.k = (const uint16_t*)p->k_cache; a.v = (const uint16_t*)p->v_cache; a.o = (uint16_t*)p->o;
   a.table = p->block_table; a.lens = p->kv_lens; a.cu = p->cu_groups; a.prefix = p->prefix_lens; a.slopes = p->slopes;
@@ -104,7 +110,7 @@ int shared_decode(const mi355_shared_params* p, hipStream_t st, const Err& err) 
   a.q_bs = p->q_batch_stride; a.q_hs = p->q_head_stride; a.o_bs = p->o_batch_stride; a.o_hs = p->o_head_stride;
   a.kp = p->k_page_stride; a.kh = p->k_head_stride; a.kr = p->k_row_stride;
   a.vp = p->v_page_stride; a.vh = p->v_head_stride; a.vr = p->v_row_stride; a.ts = p->table_stride;
-  a.b = p->b; a.n_groups = p->n_groups; a.h = p->h; a.hk = p->h_k; a.ratio = p->h / p->h_k; a.groups = pl.groups;
+  a.b = p->b; a.n_groups = p->n_groups; a.h = p->h; a.hk = p->h_k; a.ratio = p->h / p->h_k; a.groups = pl.groups; a.columns = pl.columns; a.own_rows = (int)pl.own_rows;
   a.pages = p->num_pages; a.shift = __builtin_ctz((unsigned)p->page_size);
   a.cols = p->num_pages > 0 ? p->table_cols : 0;   // no pages: nothing is seen
   a.window = window_of(p->window);
@@ -114,13 +120,14 @@ int shared_decode(const mi355_shared_params* p, hipStream_t st, const Err& err) 
   by_type(p->d, p->dtype == MI355_BEAM_BF16, [&](auto d, auto bf) {
     constexpr int D = decltype(d)::value;
     constexpr bool BF = decltype(bf)::value;
-    auto go = [&](auto nc) {
-      constexpr int NC = decltype(nc)::value;
-      rc = run(err, "mha_shared_decode", shared_decode_kernel<D, BF, NC>, pl.grid, kShThreads, 0, st, a);
-      if (rc == kOk) rc = run(err, "mha_shared_decode (join)", shared_join_kernel<D, BF, NC>, (int64_t)p->b * p->h, 256, 0, st, a);
-    };
-    if (pl.columns > 16) go(std::integral_constant<int, kShColumns(D) / 16>{});
-    else go(std::integral_constant<int, 1>{});
+    auto go = [&](void (*kernel)(const SharedArgs)) { rc = run(err, "mha_shared_decode", kernel, pl.grid, kShThreads, 0, st, a); };
+    if (pl.columns == 128) go(shared_decode_kernel<D, BF, 4, 1, kShTiles>);
+    else if (pl.columns == 64) go(shared_decode_kernel<D, BF, 2, 2, 1>);
+    else go(shared_decode_kernel<D, BF, 1, 4, 1>);
+    if (rc != kOk) return;
+    const int64_t bh = (int64_t)p->b * p->h;
+    if (bh >= 1024) rc = run(err, "mha_shared_decode (join)", shared_join_kernel<D, BF, true>, (bh + 3) / 4, 256, 0, st, a);
+    else rc = run(err, "mha_shared_decode (join)", shared_join_kernel<D, BF, false>, bh, 256, 0, st, a);
   });
   return rc;
 }

@@ -112,6 +112,18 @@ __device__ __forceinline__ void bload16_lds(i32x4 rs, uint32_t lds_byte, uint32_
         : "memory", "m0");
 }
 
+// The same from a 64-bit address of each lane's own, for rows that lie anywhere.
+__device__ __forceinline__ void gload16_lds(const void* from, uint32_t lds_byte) {
+  const uint32_t m0v = __builtin_amdgcn_readfirstlane(lds_byte);
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, off"
+      :
+      : "s"(m0v), "v"(from)
+      : "memory", "m0");
+}
+
 // Workgroup-id remap: the hardware hands linear id L to XCD (L % 8). Give each
 // XCD a contiguous chunk of logical tile ids so neighbouring tiles share an L2.
 __device__ __forceinline__ int xcd_remap(int L, int total) {

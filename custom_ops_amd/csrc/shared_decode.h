@@ -11,19 +11,22 @@
 //  * The tiles of 32 keys that all requests of a group see whole are shared; what remains
 //    of the prefix at its ends belongs to the requests (beam_sched.h). So no column of a
 //    shared tile hides a key, and nothing of an unseen key can reach a row.
-//  * A workgroup is a part: some tiles of one unit, which is a block of 16·NC columns of a
-//    group's (KV head, requests), or a request's 16 heads of a KV head. Each of its 4
-//    waves streams every fourth tile: Sᵀ = K·Qᵀ with 16x16x32 MFMAs, K rows straight from
-//    the cache into the operand registers and used by all NC column blocks; V rows
-//    through the wave's own LDS slice, read transposed once for all NC.
+//  * Shared tiles: a workgroup is 32·RW columns by KG groups of waves that take every
+//    KG-th tile and join their sums in LDS at the end. Sᵀ = K·Qᵀ with 32x32x16 MFMAs, so
+//    that a lane holds one column's scores; K and V come from the pages to LDS by DMA, two
+//    stages, one barrier a step.
+//  * Own tiles: 16 columns, the heads of one KV head; a wave streams tiles of 32 keys, K to
+//    the operand registers, V through its own LDS slice, the next tile in flight. Four
+//    waves share a long request's; of short ones each wave has one to itself.
 //  * Lengths and offsets stay on the device: every workgroup derives the same plan from
 //    them and takes its part; workgroup 0 writes down for the join where parts lie.
 
 constexpr int kShWaves = 4;
 constexpr int kShThreads = 64 * kShWaves;
-constexpr int kShColumns(int d) { return d == 128 ? 32 : 64; }   // of a workgroup, where groups are of more than 16
 constexpr int kShMax = 2048;                   // requests, and groups
-constexpr int kShItems = 2 * kShMax / kShThreads;   // groups and requests of a thread
+constexpr int kShShort = 8;                    // tiles of a request that one wave reads by itself
+
+constexpr int kShTiles = 1;   // tiles of a step of 128 columns
 
 struct SharedArgs {
   const uint16_t* q;
@@ -35,394 +38,424 @@ struct SharedArgs {
   const int* cu;
   const int* prefix;
   const float* slopes;
-  int* rec;        // [n_groups + b][4]: first slot, parts of a unit, and of a request its group or -1
-  float* part_ml;  // [parts][16·NC][2]: max in log2 units, sum
-  float* part_o;   // [parts][16·NC][D]
+  int* rec;        // [n_groups + b][4]: row of the first part, parts of a unit; a request's group or -1; a group's first request
+  float* part_ml;  // [rows][2]: max in log2 units, sum
+  float* part_o;   // [rows][D]: `columns` rows of each group's part, then 16 of each of requests' own
   int64_t q_bs, q_hs, o_bs, o_hs, kp, kh, kr, vp, vh, vr, ts;
   int b, n_groups, h, hk, ratio;
   int groups;      // 16-head groups per KV head of a request's own keys
+  int columns;     // of a group's workgroup
+  int own_rows;    // first row of part_o of own tiles
   int pages, shift, cols, window;
   int target, least;             // parts to make, about; tiles of a part at least
   int cap;                       // scores are capped
   float u_scale, c2, bias;       // as in PackedArgs
 };
 
-// What a workgroup does.
+// 4 values rounded to the type, as 8 bytes.
+template <bool BF16> __device__ __forceinline__ void store4(uint16_t* to, f32x4 x) {
+  typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
+  typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
+  if constexpr (BF16) *reinterpret_cast<u32x2*>(to) = bitcast<u32x2>(__builtin_convertvector(x, bf16x4));
+  else *reinterpret_cast<u32x2*>(to) = bitcast<u32x2>(__builtin_convertvector(x, f16x4));
+}
+
+// What a wave does.
 struct Share {
-  int group;       // >= 0: shared tiles of it, columns from col0 on; -1: own tiles of request b
+  int kind;        // 0: nothing; 1: shared tiles of a group; 2: own tiles, four waves together; 3: own tiles, the wave alone
   int b;           // the first request of the group, or the request
   int leader;      // the row that names the prefix's pages
   int hk, col0;    // KV head; first column, or first head of the request's
   int cols;        // columns there are
   int prefix;      // keys below it: of the leader's row
-  int slot, lo, hi;   // where the part's results go; its tiles [lo, hi) of the unit's
+  int row, lo, hi; // where the part's results go (rows of part_o); its tiles [lo, hi) of the unit's
+  int alone;       // the request's only part
   OwnTiles own;    // a group's tiles: own.first + i
-  bool alone;      // the request's only part
 };
 
-// The plan. LDS: s, of kShPlan words.
-constexpr int kShPlan = 5 * kShMax + 64;
-__device__ __forceinline__ bool find_share(const SharedArgs& a, int columns, int w, int* s, Share& sh) {
+constexpr int kShWords = 7 * kShMax + 2 + 64;
+
+// The plan, by T threads (one wave, where all have little to do: no barriers). LDS: s, of
+// kShWords. Items are the groups, then the requests; an item's units have n parts each, a
+// workgroup each; short requests' units come last, four to a workgroup. What workgroup w
+// holds is left in s[0 ..]: see share_of.
+struct PlanLds {
+  int *acc, *len_of, *group_of, *least_of, *most_of, *members, *prefix, *cu;
+  __device__ __forceinline__ explicit PlanLds(int* s)
+      : acc(s), len_of(s + 64), group_of(len_of + kShMax), least_of(group_of + kShMax), most_of(least_of + kShMax), members(most_of + kShMax),
+        prefix(members + kShMax), cu(prefix + kShMax) {}
+};
+template <int T> __device__ __forceinline__ void find_share(const SharedArgs& a, int w, int* s) {
+  constexpr bool SOLO = T == 64;
+  constexpr int WAVES = T / 64;
+  auto meet = [&]() __attribute__((always_inline)) {
+    if constexpr (SOLO) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // (a wave's LDS accesses stay in order)
+    else __syncthreads();
+  };
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  int* len_of = s;                  // [b]
-  int* group_of = s + kShMax;       // [b]
-  int* least_of = s + 2 * kShMax;   // [n_groups], then tiles t0
-  int* most_of = s + 3 * kShMax;    // [n_groups], then tiles t1
-  int* members = s + 4 * kShMax;    // [n_groups]
-  int* acc = s + 5 * kShMax;        // [64]
-  const int64_t span = (int64_t)a.cols << a.shift;
-  const int cap = (int)span;
-  for (int i = tid; i < a.b; i += kShThreads) {
-    len_of[i] = min(max(a.lens[i], 0), cap);
-    group_of[i] = -1;
+  const PlanLds l(s);
+  const int cap = (int)((int64_t)a.cols << a.shift);
+  for (int i = tid; i < a.b; i += T) {
+    l.len_of[i] = min(max(a.lens[i], 0), cap);
+    l.group_of[i] = -1;
   }
-  for (int g = tid; g < a.n_groups; g += kShThreads) {
-    least_of[g] = INT_MAX;
-    most_of[g] = members[g] = 0;
-  }
-  __syncthreads();
-  // a request's group: the last one that starts at or before it, if it ends behind it
-  for (int g = tid; g < a.n_groups; g += kShThreads) {
-    const int c = a.cu[g];
-    if (c >= 0 && c < a.b) atomicMax(&group_of[c], g);
-  }
-  __syncthreads();
-  constexpr int E = kShMax / kShThreads;
-  int mine[E], top = -1;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int i = tid * E + e;
-    top = max(top, i < a.b ? group_of[i] : -1);
-    mine[e] = top;
-  }
-  const int upto = wave_max_scan(top);
-  if (lane == 63) acc[wave] = upto;
-  int before = __shfl_up(upto, 1);
-  if (lane == 0) before = -1;
-  __syncthreads();
-  for (int x = 0; x < wave; ++x) before = max(before, acc[x]);
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int i = tid * E + e;
-    if (i < a.b) {
-      int g = max(mine[e], before);
-      if (g >= 0 && i >= a.cu[g + 1]) g = -1;
-      group_of[i] = g;
-      if (g >= 0) atomicAdd(&members[g], 1);
-      if (g >= 0 && len_of[i] > 0) {
-        atomicMin(&least_of[g], len_of[i]);
-        atomicMax(&most_of[g], len_of[i]);
-      }
+  for (int g = tid; g <= a.n_groups; g += T) {
+    l.cu[g] = a.cu[g];
+    if (g < a.n_groups) {
+      l.prefix[g] = min(max(a.prefix[g], 0), cap);
+      l.least_of[g] = INT_MAX;
+      l.most_of[g] = l.members[g] = 0;
     }
   }
-  __syncthreads();
-  for (int g = tid; g < a.n_groups; g += kShThreads) {
-    const int c0 = a.cu[g], c1 = min(a.cu[g + 1], a.b);
+  if (tid < 64) l.acc[tid] = 0;
+  meet();
+  // a request's group: the last one that starts at or before it, if it ends behind it
+  for (int g = tid; g < a.n_groups; g += T) {
+    const int c = l.cu[g];
+    if (c >= 0 && c < a.b) atomicMax(&l.group_of[c], g);
+  }
+  meet();
+  const int each = (a.b + T - 1) / T, i0 = tid * each, i1 = min(i0 + each, a.b);
+  int top = -1;
+  for (int i = i0; i < i1; ++i) top = max(top, l.group_of[i]);
+  const int upto = wave_max_scan(top);
+  int before = __shfl_up(upto, 1);
+  if (lane == 0) before = -1;
+  if constexpr (!SOLO) {
+    if (lane == 63) l.acc[32 + wave] = upto;
+    meet();
+    for (int x = 0; x < wave; ++x) before = max(before, l.acc[32 + x]);
+  }
+  for (int i = i0; i < i1; ++i) {
+    before = max(before, l.group_of[i]);
+    const int g = before >= 0 && i < l.cu[before + 1] ? before : -1, n = l.len_of[i];
+    l.group_of[i] = g;
+    if (g >= 0) atomicAdd(&l.members[g], 1);
+    if (g >= 0 && n > 0) {
+      atomicMin(&l.least_of[g], n);
+      atomicMax(&l.most_of[g], n);
+    }
+  }
+  meet();
+  auto units_of = [&](int g) { return a.hk * ((int)(((int64_t)(min(l.cu[g + 1], a.b) - l.cu[g]) * a.ratio + a.columns - 1) / a.columns)); };
+  auto own_count = [&](int b) {
+    const int g = l.group_of[b];
+    return own_tiles(l.len_of[b], a.window, g >= 0 ? TileSpan{l.least_of[g], l.most_of[g]} : TileSpan{0, 0}).count;
+  };
+  const int own_units = a.hk * a.groups;
+  int64_t sum = 0;
+  for (int g = tid; g < a.n_groups; g += T) {
+    const int c0 = l.cu[g], c1 = min(l.cu[g + 1], a.b);
     TileSpan t{0, 0};
     // (offsets that do not ascend: a group that lacks some of its rows shares nothing, so
     // that groups are apart and the parts fit the grid)
-    if (c0 >= 0 && c0 < c1 && members[g] == c1 - c0 && most_of[g] > 0)
-      t = shared_tiles(min(max(a.prefix[g], 0), cap), least_of[g], most_of[g], a.window, c1 - c0);
-    least_of[g] = t.t0;
-    most_of[g] = t.t1;
+    if (c0 >= 0 && c0 < c1 && l.members[g] == c1 - c0 && l.most_of[g] > 0)
+      t = shared_tiles(l.prefix[g], l.least_of[g], l.most_of[g], a.window, c1 - c0);
+    l.least_of[g] = t.t0;
+    l.most_of[g] = t.t1;
+    if (t.t1 > t.t0) sum += (int64_t)(t.t1 - t.t0) * units_of(g);
   }
-  __syncthreads();
-  // items: the groups, then the requests
-  const int items = a.n_groups + a.b;
-  int tiles[kShItems], units[kShItems];
-  int64_t sum = 0;
-#pragma unroll
-  for (int e = 0; e < kShItems; ++e) {
-    const int i = e * kShThreads + tid;
-    tiles[e] = units[e] = 0;
-    if (i < a.n_groups) {
-      tiles[e] = most_of[i] - least_of[i];
-      if (tiles[e] > 0) units[e] = a.hk * ((int)(((int64_t)(min(a.cu[i + 1], a.b) - a.cu[i]) * a.ratio + columns - 1) / columns));
-    } else if (i < items) {
-      const int b = i - a.n_groups, g = group_of[b];
-      tiles[e] = own_tiles(len_of[b], a.window, g >= 0 ? TileSpan{least_of[g], most_of[g]} : TileSpan{0, 0}).count;
-      units[e] = a.hk * a.groups;
-    }
-    sum += (int64_t)tiles[e] * units[e];
-  }
+  meet();
+  for (int b = tid; b < a.b; b += T) sum += (int64_t)own_count(b) * own_units;
 #pragma unroll
   for (int x = 1; x < 64; x *= 2) sum += __shfl_xor(sum, x);
-  int64_t* wide = reinterpret_cast<int64_t*>(acc);
-  if (lane == 0) wide[wave] = sum;
-  __syncthreads();
-  sum = 0;
+  if constexpr (!SOLO) {
+    int64_t* wide = reinterpret_cast<int64_t*>(l.acc + 40);
+    if (lane == 0) wide[wave] = sum;
+    meet();
+    sum = 0;
 #pragma unroll
-  for (int x = 0; x < kShWaves; ++x) sum += wide[x];
+    for (int x = 0; x < WAVES; ++x) sum += wide[x];
+  }
   const int per = share_size(sum, a.target, a.least);
-  // the item that holds part w
-  int run = 0;
-#pragma unroll 1
-  for (int e = 0; e * kShThreads < items; ++e) {
-    int t = 0, u = 0;
-#pragma unroll
-    for (int x = 0; x < kShItems; ++x)
-      if (x == e) {
-        t = tiles[x];
-        u = units[x];
+  const int items = a.n_groups + a.b;
+  int parts = 0, turn = 0;   // of all items but short requests
+  for (int pass = 0; pass < 2; ++pass) {
+    int run = 0;
+    for (int e = 0; e * T < items; ++e) {
+      const int i = e * T + tid;
+      int t = 0, u = 0;
+      if (i < a.n_groups) {
+        t = l.most_of[i] - l.least_of[i];
+        u = t > 0 ? units_of(i) : 0;
+      } else if (i < items) {
+        t = own_count(i - a.n_groups);
+        u = own_units;
       }
-    const int n = share_count(t, per);
-    const int incl = wave_scan(n * u);
-    int* part = acc + 16 + (e & 1) * 4;   // (two sets, so that one barrier a step is enough)
-    if (lane == 63) part[wave] = incl;
-    __syncthreads();
-    int start = run + incl - n * u;
+      const bool small = i >= a.n_groups && t <= kShShort;
+      const int n = small ? (t > 0) : share_count(t, per), mine = small == (pass == 1) ? n * u : 0;
+      const int incl = wave_scan(mine);
+      int start = run + incl - mine;
+      if constexpr (SOLO) run += __builtin_amdgcn_readlane(incl, 63);
+      else {
+        int* part = l.acc + 48 + (turn & 1) * 4;   // (two sets, so that one barrier a step is enough)
+        if (lane == 63) part[wave] = incl;
+        meet();
+        ++turn;
 #pragma unroll
-    for (int x = 0; x < kShWaves; ++x) {
-      if (x < wave) start += part[x];
-      run += part[x];
+        for (int x = 0; x < WAVES; ++x) {
+          if (x < wave) start += part[x];
+          run += part[x];
+        }
+      }
+      if (w == 0 && i < items && small == (pass == 1)) {
+        int* r = a.rec + (int64_t)i * 4;
+        r[0] = i < a.n_groups ? start * a.columns : a.own_rows + (parts + start) * 16;
+        r[1] = n;
+        r[2] = i < a.n_groups ? -1 : l.group_of[i - a.n_groups];
+        r[3] = i < a.n_groups ? l.cu[i] : 0;
+      }
+      // s[4x]: 1 + the item of wave x, or of all; the place among its parts; parts of a unit; tiles
+      if (pass == 0) {
+        if (w >= start && w < start + mine) {
+          l.acc[0] = 1 + i;
+          l.acc[1] = w - start;
+          l.acc[2] = n;
+          l.acc[3] = t;
+          l.acc[16] = start;
+        }
+      } else
+#pragma unroll
+        for (int x = 0; x < kShWaves; ++x) {
+          const int q = (w - parts) * kShWaves + x;
+          if (q >= start && q < start + mine) {
+            l.acc[4 * x] = 1 + i;
+            l.acc[4 * x + 1] = q - start;
+            l.acc[4 * x + 2] = 1;
+            l.acc[4 * x + 3] = t;
+            l.acc[16 + x] = parts + start;
+          }
+        }
     }
-    const int i = e * kShThreads + tid;
-    if (w == 0 && i < items) {
-      int* r = a.rec + (int64_t)i * 4;
-      r[0] = start;
-      r[1] = n;
-      r[2] = i < a.n_groups ? -1 : group_of[i - a.n_groups];
-      r[3] = i < a.n_groups ? a.cu[i] : 0;
-    }
-    if (w >= start && w < start + n * u) {
-      acc[32] = i;
-      acc[33] = start;
-      acc[34] = n;
-      acc[35] = t;
-    }
+    if (pass == 0) parts = run;
+    if (w > 0 && w < parts) break;   // (the first one goes on for the records)
   }
-  if (w >= run) return false;
-  __syncthreads();
-  const int item = uni(acc[32]), start = uni(acc[33]), n = uni(acc[34]), t = uni(acc[35]);
-  const int unit = (w - start) / n, p = (w - start) % n;
-  sh.slot = w;
-  sh.lo = share_start(t, n, p);
-  sh.hi = share_start(t, n, p + 1);
-  if (item < a.n_groups) {
-    const int c0 = uni(a.cu[item]), c1 = min(uni(a.cu[item + 1]), a.b);
-    const int total = (c1 - c0) * a.ratio, blocks = (total + columns - 1) / columns;
-    sh.group = item;
-    sh.b = sh.leader = c0;
-    sh.hk = unit / blocks;
-    sh.col0 = unit % blocks * columns;
-    sh.cols = min(columns, total - sh.col0);
-    sh.own = OwnTiles{0, INT_MAX, uni(least_of[item]), INT_MAX, 0, 0};
-    sh.prefix = INT_MAX;
-    sh.alone = false;
-  } else {
-    const int b = item - a.n_groups, g = uni(group_of[b]);
-    const TileSpan sp = g >= 0 ? TileSpan{uni(least_of[g]), uni(most_of[g])} : TileSpan{0, 0};
-    sh.group = -1;
-    sh.b = b;
-    sh.leader = g >= 0 ? uni(a.cu[g]) : b;
-    sh.prefix = g >= 0 ? min(max(uni(a.prefix[g]), 0), cap) : 0;
-    sh.hk = unit / a.groups;
-    sh.col0 = unit % a.groups * 16;
-    sh.cols = min(16, a.ratio - sh.col0);
-    sh.own = own_tiles(uni(len_of[b]), a.window, sp);
-    sh.alone = n == 1 && sp.t0 == sp.t1;
-  }
-  return true;
+  if (tid == 0) l.acc[20] = parts;
 }
 
-// A part of NB blocks of 16 columns. sv: V slices of the waves. len_of: the requests' lengths in
-// LDS are gone by now, so columns read their own.
-template <int D, bool BF16, int NB, int NC>
-__device__ __forceinline__ void share_part(kernarg<SharedArgs>& a, const Share& sh, uint8_t (*sV)[kDecTile * (D * 2 + 32)], float (*sM)[16], float (*sL)[16]) {
-  typedef typename Elt<BF16>::v8 V8;
-  constexpr int KD = D / 32, DB = D / 16;
-  constexpr int kRow = D * 2 + 32;   // LDS bytes per V row: transposed reads of 16 rows touch all banks alike
-  const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
-  const int l16 = lane & 15, g = lane >> 4;
-  const int page_size = 1 << a.shift;
-  const int64_t span = (int64_t)a.cols << a.shift;
+// What the wave does, from the plan's words; all waves, before they are overwritten.
+__device__ __forceinline__ Share share_of(const SharedArgs& a, int w, int* s, int wave) {
+  const PlanLds l(s);
+  Share sh{};
+  const int parts = uni(l.acc[20]), x = w < parts ? 0 : wave, item = uni(l.acc[4 * x]) - 1;
+  if (item < 0) return sh;
+  const int place = uni(l.acc[4 * x + 1]), n = uni(l.acc[4 * x + 2]), t = uni(l.acc[4 * x + 3]), start = uni(l.acc[16 + x]);
+  const int unit = place / n, p = place - unit * n;
+  sh.lo = share_start(t, n, p);
+  sh.hi = share_start(t, n, p + 1);
+  const bool group = item < a.n_groups;
+  sh.kind = group ? 1 : w < parts ? 2 : 3;
+  const int b = group ? 0 : item - a.n_groups, g = group ? item : uni(l.group_of[b]);
+  const int c0 = g >= 0 ? uni(l.cu[g]) : b, c1 = g >= 0 ? min(uni(l.cu[g + 1]), a.b) : b;
+  const TileSpan sp = g >= 0 ? TileSpan{uni(l.least_of[g]), uni(l.most_of[g])} : TileSpan{0, 0};
+  const int width = group ? a.columns : 16, total = group ? (c1 - c0) * a.ratio : a.ratio, blocks = (total + width - 1) / width;
+  sh.b = group ? c0 : b;
+  sh.leader = c0;
+  sh.hk = unit / blocks;
+  sh.col0 = (unit - sh.hk * blocks) * width;
+  sh.cols = min(width, total - sh.col0);
+  sh.prefix = group ? INT_MAX : g >= 0 ? uni(l.prefix[g]) : 0;
+  sh.row = (group ? 0 : a.own_rows) + (start + place) * width;
+  sh.alone = !group && n == 1 && sp.t0 == sp.t1;
+  const OwnTiles own = own_tiles(uni(l.len_of[b]), a.window, sp);
+  sh.own.lo = group ? 0 : own.lo;
+  sh.own.len = group ? INT_MAX : own.len;
+  sh.own.first = group ? sp.t0 : own.first;
+  sh.own.before = group ? INT_MAX : own.before;
+  sh.own.behind = own.behind;
+  return sh;
+}
 
-  // Q: B operand, column 16·n + l16, d = 8·(4·kd + g). Column c is head c % ratio of the
-  // KV head's, of request c / ratio.
-  V8 qreg[NB][KD];
-  float bco[NB], last[NB];   // slope, and the last key of the column's request
-#pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    const int c = n * 16 + l16;
-    const bool real = c < sh.cols;
-    const int col = sh.col0 + (real ? c : 0);
-    const int b = sh.group >= 0 ? sh.b + col / a.ratio : sh.b;
-    const int h = sh.hk * a.ratio + (sh.group >= 0 ? col % a.ratio : col);
+// Own tiles: 16 columns of request sh.b, or of a group that has a bad page, streamed by W waves,
+// of which this is number `wave`; sv: the wave's V slice.
+template <int D, bool BF16> struct Stream {
+  typedef typename Elt<BF16>::v8 V8;
+  static constexpr int KD = D / 32, DB = D / 16;
+  static constexpr int kRow = D * 2 + 32;   // LDS bytes per V row: transposed reads of 16 rows touch all banks alike
+  static constexpr int kSlice = kDecTile * kRow;
+  f32x4 oacc[DB];
+  float m_run = -INFINITY, mlog2 = 0.f, l_run = 0.f;
+
+  __device__ __forceinline__ void run(kernarg<SharedArgs>& a, const Share& sh, int col0, int cols, int wave, int W, uint8_t* sv) {
+    const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+    const int page_size = 1 << a.shift;
+    const int64_t span = (int64_t)a.cols << a.shift;
+    // Q: B operand, column l16, d = 8·(4·kd + g). A group's column c is head c % ratio of the
+    // KV head's, of request c / ratio.
+    const bool mine = l16 < cols;
+    const int col = col0 + (mine ? l16 : 0);
+    const int b = sh.kind == 1 ? sh.b + col / a.ratio : sh.b, h = sh.hk * a.ratio + (sh.kind == 1 ? col % a.ratio : col);
+    V8 qreg[KD];
     const uint16_t* q = a.q + (int64_t)b * a.q_bs + (int64_t)h * a.q_hs + g * 8;
 #pragma unroll
     for (int kd = 0; kd < KD; ++kd) {
       u32x4 x = {0u, 0u, 0u, 0u};
-      if (real) x = *reinterpret_cast<const u32x4*>(q + kd * 32);
-      qreg[n][kd] = bitcast<V8>(x);
+      if (mine) x = *reinterpret_cast<const u32x4*>(q + kd * 32);
+      qreg[kd] = bitcast<V8>(x);
     }
-    bco[n] = a.slopes ? a.slopes[h] * a.bias : 0.f;
-    last[n] = a.slopes ? (float)(min(max(a.lens[b], 0), (int)span) - 1) : 0.f;
-  }
-  const float c2 = a.c2, slack = kSlackLog2 / a.c2;
-  f32x4 oacc[NB][DB];
-  float m_run[NB], mlog2[NB], l_run[NB];
+    const float bco = a.slopes ? a.slopes[h] * a.bias : 0.f;
+    const float last = a.slopes ? (float)(min(max(a.lens[b], 0), (int)span) - 1) : 0.f;   // the column's last key
+    const float c2 = a.c2, slack = kSlackLog2 / a.c2;
 #pragma unroll
-  for (int n = 0; n < NB; ++n) {
-#pragma unroll
-    for (int db = 0; db < DB; ++db) oacc[n][db] = f32x4{};
-    m_run[n] = -INFINITY;
-    mlog2[n] = l_run[n] = 0.f;
-  }
+    for (int db = 0; db < DB; ++db) oacc[db] = f32x4{};
+    m_run = -INFINITY;
+    mlog2 = l_run = 0.f;
 
-  const int* tab = a.table + (int64_t)sh.b * a.ts;
-  const int* lead = a.table + (int64_t)sh.leader * a.ts;
-  const uint16_t* kbase = a.k + (int64_t)sh.hk * a.kh + g * 8;
-  const uint16_t* vbase = a.v + (int64_t)sh.hk * a.vh + g * 8;
-  const OwnTiles own = sh.own;
-  const int end = sh.group >= 0 ? (int)min((int64_t)INT_MAX, span) : own.len, bound = max(end - 1, 0);
-  // Page numbers of the lane's keys l16 and 16 + l16 of tile i of the unit (-1: not seen).
-  // No load of the loop is conditional, or the compiler would wait for all loads in
-  // flight where the paths meet: what is behind the part's end reads what is there anyway.
-  auto entries = [&](int i, int (&e)[2]) __attribute__((always_inline)) {
-    const int t = own_tile(own, min(i, sh.hi - 1));
+    const int* tab = a.table + (int64_t)sh.b * a.ts;
+    const int* lead = a.table + (int64_t)sh.leader * a.ts;
+    const uint16_t* kbase = a.k + (int64_t)sh.hk * a.kh + g * 8;
+    const uint16_t* vbase = a.v + (int64_t)sh.hk * a.vh + g * 8;
+    const OwnTiles own = sh.own;
+    const int end = sh.kind == 1 ? (int)span : own.len, bound = max(end - 1, 0);
+    // Page numbers of the lane's keys l16 and 16 + l16 of tile i of the unit (-1: not seen).
+    // No load of the loop is conditional, or the compiler would wait for all loads in
+    // flight where the paths meet: what is behind the part's end reads what is there anyway.
+    auto entries = [&](int i, int (&e)[2]) __attribute__((always_inline)) {
+      const int t = own_tile(own, min(i, sh.hi - 1));
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int key = t * kDecTile + r * 16 + l16;
-      const int x = (key < sh.prefix ? lead : tab)[min(key, bound) >> a.shift];
-      e[r] = (i < sh.hi && key >= own.lo && key < end) ? x : -1;
-    }
-  };
-  struct Tile { u32x4 k[2][KD], v[2][KD]; bool ok[2]; };
-  auto fetch = [&](int i, const int (&e)[2], Tile& x) __attribute__((always_inline)) {
-    const int t = own_tile(own, min(i, sh.hi - 1));
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      x.ok[r] = e[r] >= 0 && e[r] < a.pages;
-      const int64_t page = x.ok[r] ? e[r] : 0;
-      const int64_t in = x.ok[r] ? (t * kDecTile + r * 16 + l16) & (page_size - 1) : 0;
-      const uint16_t* kp = kbase + page * a.kp + in * a.kr;
-      const uint16_t* vp = vbase + page * a.vp + in * a.vr;
-#pragma unroll
-      for (int kd = 0; kd < KD; ++kd) {
-        x.k[r][kd] = *reinterpret_cast<const u32x4*>(kp + kd * 32);
-        x.v[r][kd] = *reinterpret_cast<const u32x4*>(vp + kd * 32);
+      for (int r = 0; r < 2; ++r) {
+        const int key = t * kDecTile + r * 16 + l16;
+        const int x = (key < sh.prefix ? lead : tab)[min(key, bound) >> a.shift];
+        e[r] = (i < sh.hi && key >= own.lo && key < end) ? x : -1;
       }
-    }
-  };
-  uint8_t* sv = sV[wave];
-  auto compute = [&](int i, const Tile& x) __attribute__((always_inline)) {
-    const int t = own_tile(own, i);
-    const bool whole = __builtin_amdgcn_ballot_w64(x.ok[0] && x.ok[1]) == ~0ull;
+    };
+    struct Tile { u32x4 k[2][KD], v[2][KD]; bool ok[2]; };
+    auto fetch = [&](int i, const int (&e)[2], Tile& x) __attribute__((always_inline)) {
+      const int t = own_tile(own, min(i, sh.hi - 1));
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
+      for (int r = 0; r < 2; ++r) {
+        x.ok[r] = e[r] >= 0 && e[r] < a.pages;
+        const int64_t page = x.ok[r] ? e[r] : 0;
+        const int64_t in = x.ok[r] ? (t * kDecTile + r * 16 + l16) & (page_size - 1) : 0;
+        const uint16_t* kp = kbase + page * a.kp + in * a.kr;
+        const uint16_t* vp = vbase + page * a.vp + in * a.vr;
 #pragma unroll
-      for (int kd = 0; kd < KD; ++kd) {
-        u32x4 y = x.v[r][kd];
-        if (!whole && !x.ok[r]) y = u32x4{0u, 0u, 0u, 0u};   // nothing of an unseen key's V
-        *reinterpret_cast<u32x4*>(sv + (r * 16 + l16) * kRow + (kd * 4 + g) * 16) = y;
+        for (int kd = 0; kd < KD; ++kd) {
+          x.k[r][kd] = *reinterpret_cast<const u32x4*>(kp + kd * 32);
+          x.v[r][kd] = *reinterpret_cast<const u32x4*>(vp + kd * 32);
+        }
       }
-    f32x4 s[NB][2];
+    };
+    auto compute = [&](int i, const Tile& x) __attribute__((always_inline)) {
+      const int t = own_tile(own, i);
+      const bool whole = __builtin_amdgcn_ballot_w64(x.ok[0] && x.ok[1]) == ~0ull;
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
+      for (int r = 0; r < 2; ++r)
 #pragma unroll
-      for (int r = 0; r < 2; ++r) s[n][r] = f32x4{};
+        for (int kd = 0; kd < KD; ++kd) {
+          u32x4 y = x.v[r][kd];
+          if (!whole && !x.ok[r]) y = u32x4{0u, 0u, 0u, 0u};   // nothing of an unseen key's V
+          *reinterpret_cast<u32x4*>(sv + (r * 16 + l16) * kRow + (kd * 4 + g) * 16) = y;
+        }
+      f32x4 s[2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
+      for (int r = 0; r < 2; ++r) {
+        s[r] = f32x4{};
 #pragma unroll
-      for (int kd = 0; kd < KD; ++kd)
-#pragma unroll
-        for (int n = 0; n < NB; ++n) s[n][r] = mfma16<BF16>(bitcast<V8>(x.k[r][kd]), qreg[n][kd], s[n][r]);
-    // this lane: column 16·n + l16, keys 16·r + 4·g + e
-    const uint64_t ok0 = __builtin_amdgcn_ballot_w64(x.ok[0]), ok1 = __builtin_amdgcn_ballot_w64(x.ok[1]);
-    V8 p[NB];
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
+        for (int kd = 0; kd < KD; ++kd) s[r] = mfma16<BF16>(bitcast<V8>(x.k[r][kd]), qreg[kd], s[r]);
+      }
+      // this lane: column l16, keys 16·r + 4·g + e
+      const uint64_t ok0 = __builtin_amdgcn_ballot_w64(x.ok[0]), ok1 = __builtin_amdgcn_ballot_w64(x.ok[1]);
       if (a.cap) {
 #pragma unroll
-        for (int c = 0; c < 8; ++c) s[n][c / 4][c % 4] = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(s[n][c / 4][c % 4] * a.u_scale));
+        for (int c = 0; c < 8; ++c) s[c / 4][c % 4] = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(s[c / 4][c % 4] * a.u_scale));
       }
       if (a.slopes) {
-        const float back = last[n] - (float)(t * kDecTile + 4 * g);
+        const float back = last - (float)(t * kDecTile + 4 * g);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) s[n][c / 4][c % 4] = __builtin_fmaf(bco[n], back - (float)(c / 4 * 16 + c % 4), s[n][c / 4][c % 4]);
+        for (int c = 0; c < 8; ++c) s[c / 4][c % 4] = __builtin_fmaf(bco, back - (float)(c / 4 * 16 + c % 4), s[c / 4][c % 4]);
       }
       if (!whole) {
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
-          s[n][c / 4][c % 4] = (((c / 4 ? ok1 : ok0) >> (4 * g + c % 4)) & 1) ? s[n][c / 4][c % 4] : -INFINITY;
+        for (int c = 0; c < 8; ++c) s[c / 4][c % 4] = (((c / 4 ? ok1 : ok0) >> (4 * g + c % 4)) & 1) ? s[c / 4][c % 4] : -INFINITY;
       }
       float mx = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) mx = fmaxf(mx, s[n][c / 4][c % 4]);
-      if (__builtin_amdgcn_ballot_w64(mx > m_run[n] + slack)) {
+      for (int c = 0; c < 8; ++c) mx = fmaxf(mx, s[c / 4][c % 4]);
+      if (__builtin_amdgcn_ballot_w64(mx > m_run + slack)) {
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const bool need = mx > m_run[n] + slack;
-        const float alpha = need ? __builtin_amdgcn_exp2f((m_run[n] - mx) * c2) : 1.f;
-        m_run[n] = need ? mx : m_run[n];
-        mlog2[n] = m_run[n] == -INFINITY ? 0.f : m_run[n] * c2;
-        l_run[n] *= alpha;
+        const bool need = mx > m_run + slack;
+        const float alpha = need ? __builtin_amdgcn_exp2f((m_run - mx) * c2) : 1.f;
+        m_run = need ? mx : m_run;
+        mlog2 = m_run == -INFINITY ? 0.f : m_run * c2;
+        l_run *= alpha;
 #pragma unroll
-        for (int db = 0; db < DB; ++db) oacc[n][db] *= alpha;
+        for (int db = 0; db < DB; ++db) oacc[db] *= alpha;
       }
       f32x8 pf;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) pf[c] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][c / 4][c % 4], c2, -mlog2[n]));
+      for (int c = 0; c < 8; ++c) pf[c] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c / 4][c % 4], c2, -mlog2));
       // P rounded for the second product, and its sum of the rounded: normalised by their
       // own sum, the weights' errors are independent and O's about that of its own rounding
-      p[n] = __builtin_convertvector(pf, V8);
-      l_run[n] = psum8<BF16>(p[n], l_run[n]);
-    }
-    // Vᵀ: lane s of a 16-lane group reads 4 columns of row 4·g + s/4 (and 16 + that)
+      const V8 p = __builtin_convertvector(pf, V8);
+      l_run = psum8<BF16>(p, l_run);
+      // Vᵀ: lane s of a 16-lane group reads 4 columns of row 4·g + s/4 (and 16 + that)
 #pragma unroll
-    for (int db = 0; db < DB; ++db) {
-      const uint8_t* at = sv + (4 * g + l16 / 4) * kRow + (db * 16 + 4 * (l16 & 3)) * 2;
-      const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
-      const s16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 16 * kRow));
-      const V8 vt = bitcast<V8>(__builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-      for (int n = 0; n < NB; ++n) oacc[n][db] = mfma16<BF16>(vt, p[n], oacc[n][db]);
-    }
-  };
+      for (int db = 0; db < DB; ++db) {
+        const uint8_t* at = sv + (4 * g + l16 / 4) * kRow + (db * 16 + 4 * (l16 & 3)) * 2;
+        const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+        const s16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 16 * kRow));
+        oacc[db] = mfma16<BF16>(bitcast<V8>(__builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7)), p, oacc[db]);
+      }
+    };
 
-  if (sh.lo + wave < sh.hi) {
-    int t = sh.lo + wave;
-    int e0[2], e1[2];
-    Tile x0, x1;
-    entries(t, e0);
-    entries(t + kShWaves, e1);
-    fetch(t, e0, x0);
-    for (; t + kShWaves < sh.hi; t += 2 * kShWaves) {
-      entries(t + 2 * kShWaves, e0);
-      fetch(t + kShWaves, e1, x1);
-      compute(t, x0);
-      entries(t + 3 * kShWaves, e1);
-      fetch(t + 2 * kShWaves, e0, x0);
-      compute(t + kShWaves, x1);
+    if (sh.lo + wave < sh.hi) {
+      int t = sh.lo + wave;
+      int e0[2], e1[2];
+      Tile x0, x1;
+      entries(t, e0);
+      entries(t + W, e1);
+      fetch(t, e0, x0);
+      for (; t + W < sh.hi; t += 2 * W) {
+        entries(t + 2 * W, e0);
+        fetch(t + W, e1, x1);
+        compute(t, x0);
+        entries(t + 3 * W, e1);
+        fetch(t + 2 * W, e0, x0);
+        compute(t + W, x1);
+      }
+      if (t < sh.hi) compute(t, x0);
     }
-    if (t < sh.hi) compute(t, x0);
+    l_run += __shfl_xor(l_run, 16);
+    l_run += __shfl_xor(l_run, 32);
   }
 
-  // join the waves, one block of columns after the other: O in the wave's slice as fp32,
-  // [16 columns][D + 2] (the slices are free)
-  float* so = reinterpret_cast<float*>(sv);
-  static_assert(16 * (D + 2) * 4 <= kDecTile * kRow, "O fits in the V slice");
-#pragma unroll 1
-  for (int n = 0; n < NB; ++n) {
-    if (n * 16 >= sh.cols) break;
-    if (n > 0) __syncthreads();   // the last block's slices are read
+  // The wave's sums as a part, or as the result.
+  __device__ __forceinline__ void store(kernarg<SharedArgs>& a, const Share& sh) const {
+    const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+    if (l16 >= sh.cols) return;
+    if (sh.alone) {
+      const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+      uint16_t* o = a.o + (int64_t)sh.b * a.o_bs + (int64_t)(sh.hk * a.ratio + sh.col0 + l16) * a.o_hs;
 #pragma unroll
-    for (int x = 0; x < NB; ++x)
-      if (x == n) {
-        float l = l_run[x];
-        l += __shfl_xor(l, 16);
-        l += __shfl_xor(l, 32);
-        if (lane < 16) {
-          sM[wave][l16] = m_run[x] == -INFINITY ? -INFINITY : m_run[x] * c2;
-          sL[wave][l16] = l;
-        }
+      for (int db = 0; db < DB; ++db) store4<BF16>(o + db * 16 + 4 * g, l_run == 0.f ? f32x4{} : oacc[db] * inv);
+    } else {
+      const int64_t at = (int64_t)sh.row + l16;
 #pragma unroll
-        for (int db = 0; db < DB; ++db)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) so[l16 * (D + 2) + db * 16 + 4 * g + e] = oacc[x][db][e];
+      for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(a.part_o + at * D + db * 16 + 4 * g) = oacc[db];
+      if (g == 0) {
+        a.part_ml[at * 2] = m_run == -INFINITY ? -INFINITY : m_run * a.c2;
+        a.part_ml[at * 2 + 1] = l_run;
       }
+    }
+  }
+
+  // The four waves' sums as one, of columns col0 .. of the part: each wave's O in its slice as
+  // fp32, [16 columns][D + 2]. All waves; the slices are free at the end.
+  __device__ __forceinline__ void join(kernarg<SharedArgs>& a, const Share& sh, int col0, int cols, uint8_t* slices, float (*sM)[16], float (*sL)[16]) const {
+    const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6), l16 = lane & 15, g = lane >> 4;
+    float* so = reinterpret_cast<float*>(slices + wave * kSlice);
+    static_assert(16 * (D + 2) * 4 <= kSlice, "O fits in the V slice");
+    if (lane < 16) {
+      sM[wave][l16] = m_run == -INFINITY ? -INFINITY : m_run * a.c2;
+      sL[wave][l16] = l_run;
+    }
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) so[l16 * (D + 2) + db * 16 + 4 * g + e] = oacc[db][e];
     __syncthreads();
-    const int cols = min(16, sh.cols - n * 16);
     for (int x = tid; x < cols * D; x += kShThreads) {
       const int c = x / D, d = x % D;
       float m = sM[0][c];
@@ -434,7 +467,7 @@ __device__ __forceinline__ void share_part(kernarg<SharedArgs>& a, const Share& 
         const float f = sM[w][c] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(sM[w][c] - m);
         // a wave that saw nothing adds nothing; NaN sums stay
         l += sL[w][c] == 0.f ? 0.f : sL[w][c] * f;
-        acc += sL[w][c] == 0.f ? 0.f : reinterpret_cast<const float*>(sV[w])[c * (D + 2) + d] * f;
+        acc += sL[w][c] == 0.f ? 0.f : reinterpret_cast<const float*>(slices + w * kSlice)[c * (D + 2) + d] * f;
       }
       if (sh.alone) {
         const float r = l == 0.f ? 0.f : acc / l;
@@ -443,7 +476,7 @@ __device__ __forceinline__ void share_part(kernarg<SharedArgs>& a, const Share& 
         else out = bitcast<uint16_t>((_Float16)r);
         a.o[(int64_t)sh.b * a.o_bs + (int64_t)(sh.hk * a.ratio + sh.col0 + c) * a.o_hs + d] = out;
       } else {
-        const int64_t at = (int64_t)sh.slot * (16 * NC) + n * 16 + c;
+        const int64_t at = (int64_t)sh.row + col0 + c;
         a.part_o[at * D + d] = acc;
         if (d == 0) {
           a.part_ml[at * 2] = m;
@@ -451,54 +484,331 @@ __device__ __forceinline__ void share_part(kernarg<SharedArgs>& a, const Share& 
         }
       }
     }
+    __syncthreads();
+  }
+};
+
+// Shared tiles: 32·RW columns by KG key groups of TB tiles a step.
+template <int D, bool BF16, int RW, int KG, int TB>
+__device__ __forceinline__ void group_part(kernarg<SharedArgs>& a, const Share& sh, uint8_t* lds) {
+  typedef typename Elt<BF16>::v8 V8;
+  static_assert(RW * KG == kShWaves, "four waves");
+  constexpr int UPR = D / 8, KD = D / 16, DB = D / 32, kTile = 32 * TB;
+  constexpr int kElems = kTile * D;                 // of a K or V tile
+  constexpr int R = kTile / RW;                     // rows that a wave brings
+  constexpr int kLoads = R * UPR / 64, RPL = 64 / UPR;   // loads of K, of V; rows of one
+  uint16_t* sKV = reinterpret_cast<uint16_t*>(lds);   // [stage][K, V][KG][kElems]
+  const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
+  const int rw = wave % RW, kg = wave / RW, l32 = lane & 31, g = lane >> 5;
+  const int page_size = 1 << a.shift;
+
+  // the lane's column, and Q: B operand
+  const int c = rw * 32 + l32;
+  const bool mine = c < sh.cols;
+  const int col = sh.col0 + (mine ? c : 0);
+  const int b = sh.b + col / a.ratio, h = sh.hk * a.ratio + col % a.ratio;
+  const uint16_t* q = a.q + (int64_t)b * a.q_bs + (int64_t)h * a.q_hs + g * 8;
+  V8 qreg[KD];
+#pragma unroll
+  for (int kd = 0; kd < KD; ++kd) qreg[kd] = bitcast<V8>(*reinterpret_cast<const u32x4*>(q + kd * 16));
+  const float bco = a.slopes ? a.slopes[h] * a.bias : 0.f;
+  const float last = a.slopes ? (float)(min(max(a.lens[b], 0), (int)((int64_t)a.cols << a.shift)) - 1) : 0.f;   // the column's last key
+  const float c2 = a.c2, slack = kSlackLog2 / a.c2;
+
+  // steps of KG·TB tiles: key group kg has tiles first + (step·KG + kg)·TB ..
+  const int count = sh.hi - sh.lo, first = sh.own.first + sh.lo;
+  const int steps = (count + KG * TB - 1) / (KG * TB);
+  auto tiles_of = [&](int step) { return max(0, min(TB, count - (step * KG + kg) * TB)); };
+  // the lane's rows of a K and of a V tile, and its 16-byte chunk of them
+  const int* lead = a.table + (int64_t)sh.leader * a.ts;
+  const int r0 = rw * R + lane / UPR, slot = lane % UPR;
+  const uint16_t* kbase = a.k + (int64_t)sh.hk * a.kh;
+  const uint16_t* vbase = a.v + (int64_t)sh.hk * a.vh;
+  const int most = (first + count) * kDecTile - 1;   // the part's last key
+  auto k_row = [&](int i) { const int r = r0 + i * RPL; return (r & ~31) + key_perm(r & 31); };
+  auto v_row = [&](int i) { return r0 + i * RPL; };
+  struct Pages { int k[kLoads], v[kLoads]; };
+  auto entries = [&](int step, Pages& e) __attribute__((always_inline)) {
+    const int key0 = (first + (step * KG + kg) * TB) * kDecTile;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      e.k[i] = lead[min(key0 + k_row(i), most) >> a.shift];
+      e.v[i] = lead[min(key0 + v_row(i), most) >> a.shift];
+    }
+  };
+  auto issue = [&](int step, int st, const Pages& e) __attribute__((always_inline)) {
+    const int key0 = (first + (step * KG + kg) * TB) * kDecTile, rows = tiles_of(step) * 32;
+    uint16_t* tk = sKV + ((st * 2) * KG + kg) * kElems + rw * R * D;
+    uint16_t* tv = sKV + ((st * 2 + 1) * KG + kg) * kElems + rw * R * D;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      if (rw * R + i * RPL >= rows) continue;   // (whole tiles of 32 rows)
+      const int kr = k_row(i), vr = v_row(i);
+      gload16_lds(kbase + (int64_t)e.k[i] * a.kp + (int64_t)((key0 + kr) & (page_size - 1)) * a.kr + (slot ^ ((r0 + i * RPL) % UPR)) * 8,
+                  lds_addr(tk) + (uint32_t)(i * 64 * 16));
+      gload16_lds(vbase + (int64_t)e.v[i] * a.vp + (int64_t)((key0 + vr) & (page_size - 1)) * a.vr + (slot ^ v_swz<D>(vr)) * 8,
+                  lds_addr(tv) + (uint32_t)(i * 64 * 16));
+    }
+  };
+
+  uint32_t k_rd[KD], v_rd[DB];
+#pragma unroll
+  for (int kd = 0; kd < KD; ++kd) k_rd[kd] = (uint32_t)(l32 * UPR + ((2 * kd + g) ^ (l32 % UPR))) * 16u;
+  {
+    // transposed read: lane s of a 16-lane group reads 4 columns of key row 16g + s/4
+    const int s16 = lane & 15, grp = lane >> 4, r = 16 * g + s16 / 4;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+      const int d = 32 * db + 16 * (grp & 1) + 4 * (s16 & 3);
+      v_rd[db] = (uint32_t)(r * D * 2 + (((d / 8) ^ v_swz<D>(r)) * 16) + (d % 8) * 2);
+    }
+  }
+  f32x16 oacc[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) oacc[db] = f32x16{};
+  float m_run = -INFINITY, mlog2 = 0.f, l_run = 0.f;
+
+  // NT of the step's tiles at LDS tk, tv; base: the first key
+  auto compute = [&](auto nt, int base, const uint16_t* tk, const uint16_t* tv) __attribute__((always_inline)) {
+    constexpr int NT = decltype(nt)::value, kWin = 2;   // LDS operand reads in flight
+    const uint8_t* k8 = reinterpret_cast<const uint8_t*>(tk);
+    const uint8_t* v8 = reinterpret_cast<const uint8_t*>(tv);
+    f32x16 s[NT];
+    {
+      auto rd = [&](int i) { return bitcast<V8>(*reinterpret_cast<const u32x4*>(k8 + (i / KD) * 32 * D * 2 + k_rd[i % KD])); };
+      V8 win[kWin];
+#pragma unroll
+      for (int i = 0; i < kWin; ++i) win[i] = rd(i);
+#pragma unroll
+      for (int i = 0; i < NT * KD; ++i) {
+        const V8 x = win[i % kWin];
+        if (i + kWin < NT * KD) win[i % kWin] = rd(i + kWin);
+        s[i / KD] = Elt<BF16>::mfma(x, qreg[i % KD], i % KD == 0 ? f32x16{} : s[i / KD]);
+      }
+    }
+    float u[16 * NT];   // key base + 32·(c / 16) + 16·g + c % 16
+#pragma unroll
+    for (int x = 0; x < 16 * NT; ++x) u[x] = s[x / 16][x % 16];
+    if (a.cap) {
+#pragma unroll
+      for (int x = 0; x < 16 * NT; ++x) u[x] = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(u[x] * a.u_scale));
+    }
+    if (a.slopes) {
+      const float back = last - (float)(base + 16 * g);
+#pragma unroll
+      for (int x = 0; x < 16 * NT; ++x) u[x] = __builtin_fmaf(bco, back - (float)(x / 16 * 32 + x % 16), u[x]);
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < 16 * NT; ++x) mx = fmaxf(mx, u[x]);
+    mx = xhalf_max(mx);
+    const bool need = mx > m_run + slack;
+    if (__builtin_amdgcn_ballot_w64(need)) {
+      // lanes that keep their max scale by exactly 1 (also avoids -inf - -inf)
+      const float alpha = need ? __builtin_amdgcn_exp2f((m_run - mx) * c2) : 1.f;
+      m_run = need ? mx : m_run;
+      mlog2 = m_run == -INFINITY ? 0.f : m_run * c2;
+      l_run *= alpha;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) oacc[db] *= alpha;
+    }
+    constexpr int N = 2 * NT * DB;
+    auto rd = [&](int i) {
+      const int j = i / DB, db = i % DB;
+      const int o = ((j / 2) * 32 + (j % 2) * 8) * D * 2;
+      const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(v8 + v_rd[db] + o));
+      const s16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(v8 + v_rd[db] + o + 4 * D * 2));
+      return bitcast<V8>(__builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    V8 win[kWin];
+#pragma unroll
+    for (int i = 0; i < kWin; ++i) win[i] = rd(i);
+#pragma unroll
+    for (int j = 0; j < 2 * NT; ++j) {
+      f32x8 pf;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) pf[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(u[j * 8 + e], c2, -mlog2));
+      const V8 p = __builtin_convertvector(pf, V8);
+      l_run = psum8<BF16>(p, l_run);   // of the rounded P: the weights that V meets
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        const int i = j * DB + db;
+        const V8 x = win[i % kWin];
+        if (i + kWin < N) win[i % kWin] = rd(i + kWin);
+        oacc[db] = Elt<BF16>::mfma(x, p, oacc[db]);
+      }
+    }
+  };
+
+  Pages e;
+  entries(0, e);
+  issue(0, 0, e);
+  if (steps > 1) entries(1, e);
+  for (int i = 0; i < steps; ++i) {
+    wait_vmcnt<0>();   // the wave's loads of step i have landed
+    wg_barrier();      // all waves' have, and all have left the stage of step i − 1
+    if (i + 1 < steps) issue(i + 1, (i + 1) & 1, e);
+    if (i + 2 < steps) entries(i + 2, e);
+    const int n = tiles_of(i), base = (first + (i * KG + kg) * TB) * kDecTile;
+    const uint16_t* tk = sKV + (((i & 1) * 2) * KG + kg) * kElems;
+    const uint16_t* tv = sKV + (((i & 1) * 2 + 1) * KG + kg) * kElems;
+    if (n == TB) compute(std::integral_constant<int, TB>{}, base, tk, tv);
+    else if (TB > 1 && n == 1) compute(std::integral_constant<int, 1>{}, base, tk, tv);
+  }
+  wait_vmcnt<0>();
+  l_run = xhalf_sum(l_run);
+  // the key groups' sums of the same columns, in the lanes that hold them
+  constexpr int kJoin = (DB * 16 + 2) * 64;   // floats of one wave
+  float* sj = reinterpret_cast<float*>(lds);
+  if constexpr (KG > 1) {
+    wg_barrier();   // the stages are free
+    if (kg > 0) {
+      float* at = sj + (rw * (KG - 1) + kg - 1) * kJoin + lane;
+      at[0] = m_run;
+      at[64] = l_run;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) at[(2 + db * 16 + x) * 64] = oacc[db][x];
+    }
+    __syncthreads();
+    if (kg > 0) return;
+#pragma unroll 1
+    for (int k = 1; k < KG; ++k) {
+      const float* at = sj + (rw * (KG - 1) + k - 1) * kJoin + lane;
+      const float mk = at[0], lk = at[64];
+      const float top = fmaxf(m_run, mk);
+      // a group that saw nothing has sums of 0 (or NaN, which stay)
+      const float f0 = m_run == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_run - top) * c2);
+      const float f1 = mk == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mk - top) * c2);
+      l_run = l_run * f0 + lk * f1;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) oacc[db][x] = oacc[db][x] * f0 + at[(2 + db * 16 + x) * 64] * f1;
+      m_run = top;
+    }
+  }
+  if (!mine) return;
+  const int64_t at = (int64_t)sh.row + c;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      *reinterpret_cast<f32x4*>(a.part_o + at * D + db * 32 + x * 8 + g * 4) = f32x4{oacc[db][4 * x], oacc[db][4 * x + 1], oacc[db][4 * x + 2], oacc[db][4 * x + 3]};
+  if (g == 0) {
+    a.part_ml[at * 2] = m_run == -INFINITY ? -INFINITY : m_run * c2;
+    a.part_ml[at * 2 + 1] = l_run;
   }
 }
 
-template <int D, bool BF16, int NC>
-__global__ __launch_bounds__(kShThreads) __attribute__((amdgpu_waves_per_eu(NC > 1 ? 1 : 2)))
+template <int D, int RW, int KG, int TB> constexpr int kShLds() {
+  const int tiles = 4 * KG * 32 * TB * D * 2, slices = kShWaves * kDecTile * (D * 2 + 32), plan = kShWords * 4;
+  return tiles > slices ? (tiles > plan ? tiles : plan) : slices > plan ? slices : plan;
+}
+
+template <int D, bool BF16, int RW, int KG, int TB>
+__global__ __launch_bounds__(kShThreads) __attribute__((amdgpu_waves_per_eu(kShLds<D, RW, KG, TB>() * 2 <= 160 * 1024 ? 2 : 1)))
 void shared_decode_kernel(const SharedArgs a) {
-  constexpr int kSlice = kDecTile * (D * 2 + 32);
-  constexpr int kBytes = kShWaves * kSlice > kShPlan * 4 ? kShWaves * kSlice : kShPlan * 4;
-  __shared__ __align__(16) uint8_t lds[kBytes];
+  __shared__ __align__(16) uint8_t lds[kShLds<D, RW, KG, TB>()];
   __shared__ float sM[kShWaves][16], sL[kShWaves][16];
-  Share sh;
-  if (!find_share(a, 16 * NC, blockIdx.x, reinterpret_cast<int*>(lds), sh)) return;
+  int* words = reinterpret_cast<int*>(lds);
+  const int wave = uni(threadIdx.x >> 6);
+  if (a.n_groups + a.b <= 128) {
+    if (wave == 0) find_share<64>(a, blockIdx.x, words);
+  } else find_share<kShThreads>(a, blockIdx.x, words);
+  __syncthreads();
+  __shared__ Share shares[kShWaves];
+  {
+    const Share sh = share_of(a, blockIdx.x, words, wave);
+    if (threadIdx.x % 64 == 0) shares[wave] = sh;
+  }
   __syncthreads();   // the plan's words are read
-  uint8_t (*sV)[kSlice] = reinterpret_cast<uint8_t (*)[kSlice]>(lds);
-  if (NC > 1 && sh.group >= 0) share_part<D, BF16, NC, NC>(reload_kernarg(a), sh, sV, sM, sL);
-  else share_part<D, BF16, 1, NC>(reload_kernarg(a), sh, sV, sM, sL);
+  // (each way reads its share and the arguments again: held from here on they would spill)
+  auto share = [&]() __attribute__((always_inline)) {
+    static_assert(sizeof(Share) % 4 == 0, "words");
+    struct Words { int x[sizeof(Share) / 4]; } x;
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(Share) / 4); ++i) x.x[i] = uni(reinterpret_cast<const int*>(&shares[wave])[i]);
+    return bitcast<Share>(x);
+  };
+  const int kind = uni(shares[wave].kind);
+  if (kind == 0) return;
+  uint8_t* sv = lds + wave * Stream<D, BF16>::kSlice;
+  if (kind == 3) {
+    kernarg<SharedArgs>& z = reload_kernarg(a);
+    const Share sh = share();
+    Stream<D, BF16> st;
+    st.run(z, sh, sh.col0, sh.cols, 0, 1, sv);
+    st.store(z, sh);
+    return;
+  }
+  if (kind == 1) {
+    kernarg<SharedArgs>& z = reload_kernarg(a);
+    const Share sh = share();
+    // a page outside the cache hides its keys, which only the stream can
+    const int* lead = z.table + (int64_t)sh.leader * z.ts;
+    const int p0 = ((sh.own.first + sh.lo) * kDecTile) >> z.shift, p1 = ((sh.own.first + sh.hi) * kDecTile - 1) >> z.shift;
+    bool bad = false;
+    for (int p = p0 + (int)threadIdx.x % 64; p <= p1; p += 64) bad |= lead[p] < 0 || lead[p] >= z.pages;
+    if (__builtin_amdgcn_ballot_w64(bad) == 0) {
+      group_part<D, BF16, RW, KG, TB>(z, sh, lds);
+      return;
+    }
+  }
+#pragma unroll 1
+  for (int c = 0; c < uni(shares[wave].cols); c += 16) {
+    kernarg<SharedArgs>& z = reload_kernarg(a);
+    const Share sh = share();
+    const int cols = min(16, sh.cols - c);
+    Stream<D, BF16> st;
+    st.run(z, sh, sh.col0 + c, cols, wave, kShWaves, sv);
+    st.join(reload_kernarg(a), share(), c, cols, lds, sM, sL);
+  }
+}
+
+// The parts of (request, head) bh: its group's and its own.
+struct Parts {
+  int shared, own;     // how many
+  int at0, at1;        // rows of the first ones; steps from one to the next: columns, 16
+};
+__device__ __forceinline__ Parts parts_of(const SharedArgs& a, int b, int h) {
+  const int hk = h / a.ratio, n = h - hk * a.ratio;
+  const int* rec = a.rec + (int64_t)(a.n_groups + b) * 4;
+  Parts p{0, rec[1], 0, 0};
+  const int group = rec[2];
+  p.at1 = rec[0] + (hk * a.groups + n / 16) * p.own * 16 + n % 16;
+  if (group >= 0 && a.lens[b] > 0 && a.cols > 0) {
+    const int* r = a.rec + (int64_t)group * 4;
+    const int first = r[3], end = min(a.cu[group + 1], a.b);
+    const int blocks = ((end - first) * a.ratio + a.columns - 1) / a.columns, col = (b - first) * a.ratio + n;
+    p.shared = r[1];
+    p.at0 = r[0] + (hk * blocks + col / a.columns) * p.shared * a.columns + col % a.columns;
+  }
+  return p;
 }
 
 // One workgroup per (request, head): its group's parts and its own, weighted by
 // 2^(m_s − m). Its 256 threads are 1024 / D rows of D / 4 threads; a row takes every so
 // many parts, 8 of them in flight, with a running max; the rows' sums are joined in LDS.
-template <int D, bool BF16>
-__device__ __forceinline__ void shared_join(const SharedArgs& a, int columns) {
-  constexpr int TPR = D / 4, ROWS = 256 / TPR, J = 8;
-  __shared__ float sAcc[ROWS][D], sMax[ROWS], sSum[ROWS];
-  const int b = blockIdx.x / a.h, h = blockIdx.x % a.h, tid = threadIdx.x;
-  const int hk = h / a.ratio, n = h - hk * a.ratio;
-  const int* rec = a.rec + (int64_t)(a.n_groups + b) * 4;
-  const int own_parts = uni(rec[1]), group = uni(rec[2]);
-  const int own_at = uni(rec[0]) + (hk * a.groups + n / 16) * own_parts;
-  int parts0 = 0, at0 = 0, col = 0;
-  const int64_t span = (int64_t)a.cols << a.shift;
-  if (group >= 0 && a.lens[b] > 0 && span > 0) {
-    const int* r = a.rec + (int64_t)group * 4;
-    parts0 = uni(r[1]);
-    const int first = uni(r[3]), end = min(uni(a.cu[group + 1]), a.b);
-    const int blocks = ((end - first) * a.ratio + columns - 1) / columns;
-    col = (b - first) * a.ratio + n;
-    at0 = uni(r[0]) + (hk * blocks + col / columns) * parts0;
-    col %= columns;
-  }
-  const int parts = parts0 + own_parts;
-  if (parts0 == 0 && own_parts == 1) return;   // written by its one part
-  auto at = [&](int s) { return s < parts0 ? (int64_t)(at0 + s) * columns + col : (int64_t)(own_at + s - parts0) * columns + n % 16; };
+// Where there are many (request, head), a wave each is enough (ROWS = 256 / D).
+template <int D, bool BF16, bool MANY>
+__global__ __launch_bounds__(256) void shared_join_kernel(const SharedArgs a) {
+  constexpr int TPR = D / 4, ROWS = (MANY ? 64 : 256) / TPR, J = MANY ? 4 : 8, GROUPS = MANY ? 4 : 1;
+  __shared__ float sAcc[GROUPS][ROWS][D], sMax[GROUPS][ROWS], sSum[GROUPS][ROWS];
+  const int who = MANY ? uni(threadIdx.x >> 6) : 0, tid = MANY ? threadIdx.x & 63 : threadIdx.x;
+  const int64_t bh = (int64_t)blockIdx.x * GROUPS + who;
+  const bool real = bh < (int64_t)a.b * a.h;
+  const int b = real ? (int)(bh / a.h) : 0, h = real ? (int)(bh % a.h) : 0;
+  const Parts pt = parts_of(a, b, h);
+  const int parts = pt.shared + pt.own;
+  const bool written = !real || (pt.shared == 0 && pt.own == 1);   // by its one part
+  if (!MANY && written) return;
+  auto at = [&](int s) { return s < pt.shared ? (int64_t)pt.at0 + (int64_t)s * a.columns : (int64_t)pt.at1 + (int64_t)(s - pt.shared) * 16; };
   const int row = tid / TPR, c = tid % TPR;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
-  for (int s0 = row; s0 < parts; s0 += ROWS * J) {
+  for (int s0 = row; s0 < (written ? 0 : parts); s0 += ROWS * J) {
     float ms[J], ls[J];
     f32x4 x[J];
 #pragma unroll
@@ -528,30 +838,27 @@ __device__ __forceinline__ void shared_join(const SharedArgs& a, int columns) {
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) sAcc[row][c * 4 + i] = acc[i];
+  for (int i = 0; i < 4; ++i) sAcc[who][row][c * 4 + i] = acc[i];
   if (c == 0) {
-    sMax[row] = m;
-    sSum[row] = l;
+    sMax[who][row] = m;
+    sSum[who][row] = l;
   }
   __syncthreads();
-  if (tid < D) {
-    float top = sMax[0];
+  if (tid < TPR && !written) {
+    float top = sMax[who][0];
 #pragma unroll
-    for (int r = 1; r < ROWS; ++r) top = fmaxf(top, sMax[r]);
-    float y = 0.f, t = 0.f;
+    for (int r = 1; r < ROWS; ++r) top = fmaxf(top, sMax[who][r]);
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+    float t = 0.f;
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-      const float f = sMax[r] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(sMax[r] - top);
-      y += sSum[r] == 0.f ? 0.f : sAcc[r][tid] * f;
-      t += sSum[r] == 0.f ? 0.f : sSum[r] * f;
+      const float f = sMax[who][r] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(sMax[who][r] - top);
+      t += sSum[who][r] == 0.f ? 0.f : sSum[who][r] * f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] += sSum[who][r] == 0.f ? 0.f : sAcc[who][r][c * 4 + i] * f;
     }
-    const float r = t == 0.f ? 0.f : y / t;
-    uint16_t out;
-    if constexpr (BF16) out = bitcast<uint16_t>((__bf16)r);
-    else out = bitcast<uint16_t>((_Float16)r);
-    a.o[(int64_t)b * a.o_bs + (int64_t)h * a.o_hs + tid] = out;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = t == 0.f ? 0.f : y[i] / t;
+    store4<BF16>(a.o + (int64_t)b * a.o_bs + (int64_t)h * a.o_hs + c * 4, y);
   }
 }
-
-template <int D, bool BF16, int NC>
-__global__ __launch_bounds__(256) void shared_join_kernel(const SharedArgs a) { shared_join<D, BF16>(a, 16 * NC); }

@@ -588,7 +588,7 @@ class BeamOps(ServeOps):
         return _build.BEAM_SRC
 
     def _compile(self, product: str, flags: list, verbose: bool) -> None:
-        _build.compile_checked(product, flags, verbose=verbose, src=_build.BEAM_SRC, dma=False)
+        _build.compile_checked(product, flags, verbose=verbose, src=_build.BEAM_SRC)
 
     def _compile_ops(self, product: str, verbose: bool) -> None:
         _build.build_beam_ops(product, verbose=verbose)
