@@ -33,6 +33,7 @@ namespace {
 
 static_assert(kShMax == MI355_BEAM_MAX_REQUESTS && kPgRows == MI355_BEAM_MAX_ROWS, "limits of the C ABI");
 constexpr int kMaxKeys = 1 << 30;
+constexpr int64_t kMaxRowStride = 1 << 24;
 
 int device_ok(const Err& err, Device* dev) {
   *dev = device_info();
@@ -46,7 +47,7 @@ int workspace_ok(const Err& err, const void* ws, size_t have, size_t need) {
 size_t up(size_t x) { return (x + 255) & ~(size_t)255; }
 
 struct SharedPlan {
-  int columns, groups, target, least;
+  int columns, groups, target, least, wave_least;
   int64_t grid;           // workgroups at most
   int64_t own_rows, rows; // rows of partial sums: of groups' parts, and all
   size_t ml, o, bytes;    // offsets of the parts' statistics and sums in the workspace
@@ -61,11 +62,12 @@ SharedPlan shared_plan(const mi355_shared_params* p, int cus) {
   pl.columns = mean > 64 ? 128 : mean > 32 ? 64 : 32;
   pl.target = 2 * cus;
   pl.least = 4;
+  pl.wave_least = 2;
   const int64_t own = (int64_t)p->b * p->h_k * pl.groups;
   const int64_t common = p->h_k * ((p->b * ratio + pl.columns - 1) / pl.columns + p->n_groups);
-  pl.grid = own + common + pl.target;
+  pl.grid = pl.target + common + (own + 3) / 4 + 1;
   pl.own_rows = (common + pl.target) * pl.columns;
-  pl.rows = pl.own_rows + pl.grid * 16;
+  pl.rows = pl.own_rows + (4 * (int64_t)pl.target + own) * 16;
   pl.ml = up((size_t)(p->n_groups + p->b) * 16);
   pl.o = pl.ml + up((size_t)pl.rows * 8);
   pl.bytes = pl.o + (size_t)pl.rows * p->d * 4;
@@ -97,6 +99,9 @@ int shared_decode(const mi355_shared_params* p, hipStream_t st, const Err& err) 
       !rows_ok(p->k_cache, {p->k_page_stride, p->k_head_stride, p->k_row_stride}) ||
       !rows_ok(p->v_cache, {p->v_page_stride, p->v_head_stride, p->v_row_stride}))
     return err.fail(kEinval, "q, o and the caches must be 16-byte aligned with strides that are multiples of 8 elements");
+  // (a lane's offset from its tile's rows is of 32 bits)
+  if (p->k_row_stride < 0 || p->v_row_stride < 0 || p->k_row_stride >= kMaxRowStride || p->v_row_stride >= kMaxRowStride)
+    return err.fail(kEinval, "the caches' row strides must be in 0 .. 2^24 elements");
   Device dev;
   if (int rc = device_ok(err, &dev)) return rc;
   const SharedPlan pl = shared_plan(p, dev.cus);
@@ -114,7 +119,7 @@ int shared_decode(const mi355_shared_params* p, hipStream_t st, const Err& err) 
   a.pages = p->num_pages; a.shift = __builtin_ctz((unsigned)p->page_size);
   a.cols = p->num_pages > 0 ? p->table_cols : 0;   // no pages: nothing is seen
   a.window = window_of(p->window);
-  a.target = pl.target; a.least = pl.least;
+  a.target = pl.target; a.least = pl.least; a.wave_least = pl.wave_least; a.col_shift = __builtin_ctz((unsigned)pl.columns);
   a.cap = p->softcap > 0.f;
   int rc = kOk;
   by_type(p->d, p->dtype == MI355_BEAM_BF16, [&](auto d, auto bf) {

@@ -42,15 +42,17 @@ MI355_HD inline OwnTiles own_tiles(int len, int window, TileSpan s) {
 }
 MI355_HD inline int own_tile(const OwnTiles& o, int i) { return i < o.before ? o.first + i : o.behind + i - o.before; }
 
-// Tiles of a part where `sum` tiles are read and about `target` parts wanted; at most
-// target parts, and a remainder for each unit, come of it.
-MI355_HD inline int share_size(int64_t sum, int target, int least) {
-  const int64_t per = (sum + target - 1) / target;
-  return (int)(per > least ? per : least);
-}
+// Tiles of a group's part where all tiles of all units are `sum` and about `target` workgroups
+// wanted, each of which takes as many; of a request's, which one wave of four takes. At
+// most target workgroups, and one for each group's unit and each four of the requests', come of it.
+MI355_HD inline int share_size(int64_t sum, int target, int least) { return imax((int)((double)sum / target) + 1, least); }
+MI355_HD inline int wave_share_size(int per, int least) { return imax((per + 3) / 4, least); }
 MI355_HD inline int share_count(int tiles, int per) { return (tiles + per - 1) / per; }   // 0 of no tiles
 // Part p of n takes tiles [share_start(p), share_start(p + 1)).
-MI355_HD inline int share_start(int tiles, int n, int p) { return (int)((int64_t)tiles * p / n); }
+MI355_HD inline int share_start(int tiles, int n, int p) {
+  const int each = tiles / n, more = tiles - each * n;
+  return p * each + imin(p, more);
+}
 
 }  // namespace mi355fa
 

@@ -124,6 +124,20 @@ __device__ __forceinline__ void gload16_lds(const void* from, uint32_t lds_byte)
       : "memory", "m0");
 }
 
+// And from a base that all lanes share, with an offset of their own.
+__device__ __forceinline__ void gload16_lds(const void* base, uint32_t off, uint32_t lds_byte) {
+  const uint64_t b = reinterpret_cast<uint64_t>(base);
+  const uint64_t s = compose_u64(__builtin_amdgcn_readfirstlane(low_u32(b)), __builtin_amdgcn_readfirstlane(high_u32(b)));
+  const uint32_t m0v = __builtin_amdgcn_readfirstlane(lds_byte);
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, %2"
+      :
+      : "s"(m0v), "v"(off), "s"(s)
+      : "memory", "m0");
+}
+
 // Workgroup-id remap: the hardware hands linear id L to XCD (L % 8). Give each
 // XCD a contiguous chunk of logical tile ids so neighbouring tiles share an L2.
 __device__ __forceinline__ int xcd_remap(int L, int total) {

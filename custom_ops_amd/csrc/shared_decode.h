@@ -15,16 +15,14 @@
 //    KG-th tile and join their sums in LDS at the end. Sᵀ = K·Qᵀ with 32x32x16 MFMAs, so
 //    that a lane holds one column's scores; K and V come from the pages to LDS by DMA, two
 //    stages, one barrier a step.
-//  * Own tiles: 16 columns, the heads of one KV head; a wave streams tiles of 32 keys, K to
-//    the operand registers, V through its own LDS slice, the next tile in flight. Four
-//    waves share a long request's; of short ones each wave has one to itself.
+//  * Own tiles: 16 columns, the heads of one KV head; a wave by itself streams tiles of 32
+//    keys, K to the operand registers, V through its own LDS slice, the next tile in flight.
 //  * Lengths and offsets stay on the device: every workgroup derives the same plan from
 //    them and takes its part; workgroup 0 writes down for the join where parts lie.
 
 constexpr int kShWaves = 4;
 constexpr int kShThreads = 64 * kShWaves;
-constexpr int kShMax = 2048;                   // requests, and groups
-constexpr int kShShort = 8;                    // tiles of a request that one wave reads by itself
+constexpr int kShMax = 1024;                   // requests, and groups
 
 constexpr int kShTiles = 1;   // tiles of a step of 128 columns
 
@@ -47,7 +45,8 @@ struct SharedArgs {
   int columns;     // of a group's workgroup
   int own_rows;    // first row of part_o of own tiles
   int pages, shift, cols, window;
-  int target, least;             // parts to make, about; tiles of a part at least
+  int target, least, wave_least; // workgroups wanted; tiles of a group's part at least, of a request's
+  int col_shift;                 // log2 of columns
   int cap;                       // scores are capped
   float u_scale, c2, bias;       // as in PackedArgs
 };
@@ -62,7 +61,7 @@ template <bool BF16> __device__ __forceinline__ void store4(uint16_t* to, f32x4 
 
 // What a wave does.
 struct Share {
-  int kind;        // 0: nothing; 1: shared tiles of a group; 2: own tiles, four waves together; 3: own tiles, the wave alone
+  int kind;        // 0: nothing; 1: shared tiles of a group; 2: own tiles, the wave by itself
   int b;           // the first request of the group, or the request
   int leader;      // the row that names the prefix's pages
   int hk, col0;    // KV head; first column, or first head of the request's
@@ -76,9 +75,8 @@ struct Share {
 constexpr int kShWords = 7 * kShMax + 2 + 64;
 
 // The plan, by T threads (one wave, where all have little to do: no barriers). LDS: s, of
-// kShWords. Items are the groups, then the requests; an item's units have n parts each, a
-// workgroup each; short requests' units come last, four to a workgroup. What workgroup w
-// holds is left in s[0 ..]: see share_of.
+// kShWords. Units of groups have parts that take a workgroup each; behind them come the
+// requests' own, four to a workgroup. What workgroup w holds is left in s[0 ..]: see share_of.
 struct PlanLds {
   int *acc, *len_of, *group_of, *least_of, *most_of, *members, *prefix, *cu;
   __device__ __forceinline__ explicit PlanLds(int* s)
@@ -137,7 +135,7 @@ template <int T> __device__ __forceinline__ void find_share(const SharedArgs& a,
     }
   }
   meet();
-  auto units_of = [&](int g) { return a.hk * ((int)(((int64_t)(min(l.cu[g + 1], a.b) - l.cu[g]) * a.ratio + a.columns - 1) / a.columns)); };
+  auto units_of = [&](int g) { return a.hk * (((min(l.cu[g + 1], a.b) - l.cu[g]) * a.ratio + a.columns - 1) >> a.col_shift); };
   auto own_count = [&](int b) {
     const int g = l.group_of[b];
     return own_tiles(l.len_of[b], a.window, g >= 0 ? TileSpan{l.least_of[g], l.most_of[g]} : TileSpan{0, 0}).count;
@@ -167,70 +165,68 @@ template <int T> __device__ __forceinline__ void find_share(const SharedArgs& a,
 #pragma unroll
     for (int x = 0; x < WAVES; ++x) sum += wide[x];
   }
-  const int per = share_size(sum, a.target, a.least);
-  const int items = a.n_groups + a.b;
-  int parts = 0, turn = 0;   // of all items but short requests
-  for (int pass = 0; pass < 2; ++pass) {
+  const int per = share_size(sum, a.target, a.least), wave_per = wave_share_size(per, a.wave_least);
+  int turn = 0;
+  // f(item, tiles, parts of a unit, units, start) over items, in order; returns all parts
+  auto scan = [&](int items, auto size, auto f) __attribute__((always_inline)) {
     int run = 0;
-    for (int e = 0; e * T < items; ++e) {
-      const int i = e * T + tid;
-      int t = 0, u = 0;
-      if (i < a.n_groups) {
-        t = l.most_of[i] - l.least_of[i];
-        u = t > 0 ? units_of(i) : 0;
-      } else if (i < items) {
-        t = own_count(i - a.n_groups);
-        u = own_units;
-      }
-      const bool small = i >= a.n_groups && t <= kShShort;
-      const int n = small ? (t > 0) : share_count(t, per), mine = small == (pass == 1) ? n * u : 0;
-      const int incl = wave_scan(mine);
-      int start = run + incl - mine;
+    for (int e = 0; e < items; e += T) {
+      const int i = e + tid;
+      int t = 0, n = 0, u = 0;
+      if (i < items) size(i, t, n, u);
+      const int incl = wave_scan(n * u);
+      int start = run + incl - n * u;
       if constexpr (SOLO) run += __builtin_amdgcn_readlane(incl, 63);
       else {
-        int* part = l.acc + 48 + (turn & 1) * 4;   // (two sets, so that one barrier a step is enough)
+        int* part = l.acc + 48 + (turn++ & 1) * 4;   // (two sets, so that one barrier a step is enough)
         if (lane == 63) part[wave] = incl;
         meet();
-        ++turn;
 #pragma unroll
         for (int x = 0; x < WAVES; ++x) {
           if (x < wave) start += part[x];
           run += part[x];
         }
       }
-      if (w == 0 && i < items && small == (pass == 1)) {
-        int* r = a.rec + (int64_t)i * 4;
-        r[0] = i < a.n_groups ? start * a.columns : a.own_rows + (parts + start) * 16;
-        r[1] = n;
-        r[2] = i < a.n_groups ? -1 : l.group_of[i - a.n_groups];
-        r[3] = i < a.n_groups ? l.cu[i] : 0;
-      }
-      // s[4x]: 1 + the item of wave x, or of all; the place among its parts; parts of a unit; tiles
-      if (pass == 0) {
-        if (w >= start && w < start + mine) {
-          l.acc[0] = 1 + i;
-          l.acc[1] = w - start;
-          l.acc[2] = n;
-          l.acc[3] = t;
-          l.acc[16] = start;
-        }
-      } else
+      if (i < items) f(i, t, n, u, start);
+    }
+    return run;
+  };
+  // s[4x]: 1 + the item of wave x, or of all four; the place among its parts; parts of a unit; tiles
+  auto holds = [&](int x, int item, int place, int n, int t, int start) __attribute__((always_inline)) {
+    l.acc[4 * x] = 1 + item;
+    l.acc[4 * x + 1] = place;
+    l.acc[4 * x + 2] = n;
+    l.acc[4 * x + 3] = t;
+    l.acc[16 + x] = start;
+  };
+  const int parts = scan(
+      a.n_groups,
+      [&](int g, int& t, int& n, int& u) {
+        t = l.most_of[g] - l.least_of[g];
+        n = share_count(t, per);
+        u = t > 0 ? units_of(g) : 0;
+      },
+      [&](int g, int t, int n, int u, int start) {
+        if (w == 0) *reinterpret_cast<i32x4*>(a.rec + (int64_t)g * 4) = i32x4{start << a.col_shift, n, -1, l.cu[g]};
+        if (w >= start && w < start + n * u) holds(0, g, w - start, n, t, start);
+      });
+  if (tid == 0) l.acc[20] = parts;
+  if (w > 0 && w < parts) return;   // (the first one goes on for the records)
+  scan(
+      a.b,
+      [&](int b, int& t, int& n, int& u) {
+        t = own_count(b);
+        n = share_count(t, wave_per);
+        u = own_units;
+      },
+      [&](int b, int t, int n, int u, int start) {
+        if (w == 0) *reinterpret_cast<i32x4*>(a.rec + (int64_t)(a.n_groups + b) * 4) = i32x4{a.own_rows + start * 16, n, l.group_of[b], 0};
 #pragma unroll
         for (int x = 0; x < kShWaves; ++x) {
           const int q = (w - parts) * kShWaves + x;
-          if (q >= start && q < start + mine) {
-            l.acc[4 * x] = 1 + i;
-            l.acc[4 * x + 1] = q - start;
-            l.acc[4 * x + 2] = 1;
-            l.acc[4 * x + 3] = t;
-            l.acc[16 + x] = parts + start;
-          }
+          if (q >= start && q < start + n * u) holds(x, a.n_groups + b, q - start, n, t, start);
         }
-    }
-    if (pass == 0) parts = run;
-    if (w > 0 && w < parts) break;   // (the first one goes on for the records)
-  }
-  if (tid == 0) l.acc[20] = parts;
+      });
 }
 
 // What the wave does, from the plan's words; all waves, before they are overwritten.
@@ -240,18 +236,18 @@ __device__ __forceinline__ Share share_of(const SharedArgs& a, int w, int* s, in
   const int parts = uni(l.acc[20]), x = w < parts ? 0 : wave, item = uni(l.acc[4 * x]) - 1;
   if (item < 0) return sh;
   const int place = uni(l.acc[4 * x + 1]), n = uni(l.acc[4 * x + 2]), t = uni(l.acc[4 * x + 3]), start = uni(l.acc[16 + x]);
-  const int unit = place / n, p = place - unit * n;
+  const int unit = (int)((uint32_t)place / (uint32_t)n), p = place - unit * n;
   sh.lo = share_start(t, n, p);
   sh.hi = share_start(t, n, p + 1);
   const bool group = item < a.n_groups;
-  sh.kind = group ? 1 : w < parts ? 2 : 3;
+  sh.kind = group ? 1 : 2;
   const int b = group ? 0 : item - a.n_groups, g = group ? item : uni(l.group_of[b]);
   const int c0 = g >= 0 ? uni(l.cu[g]) : b, c1 = g >= 0 ? min(uni(l.cu[g + 1]), a.b) : b;
   const TileSpan sp = g >= 0 ? TileSpan{uni(l.least_of[g]), uni(l.most_of[g])} : TileSpan{0, 0};
-  const int width = group ? a.columns : 16, total = group ? (c1 - c0) * a.ratio : a.ratio, blocks = (total + width - 1) / width;
+  const int shift = group ? a.col_shift : 4, width = 1 << shift, total = group ? (c1 - c0) * a.ratio : a.ratio, blocks = (total + width - 1) >> shift;
   sh.b = group ? c0 : b;
   sh.leader = c0;
-  sh.hk = unit / blocks;
+  sh.hk = (int)((uint32_t)unit / (uint32_t)blocks);
   sh.col0 = (unit - sh.hk * blocks) * width;
   sh.cols = min(width, total - sh.col0);
   sh.prefix = group ? INT_MAX : g >= 0 ? uni(l.prefix[g]) : 0;
@@ -469,28 +465,27 @@ template <int D, bool BF16> struct Stream {
         l += sL[w][c] == 0.f ? 0.f : sL[w][c] * f;
         acc += sL[w][c] == 0.f ? 0.f : reinterpret_cast<const float*>(slices + w * kSlice)[c * (D + 2) + d] * f;
       }
-      if (sh.alone) {
-        const float r = l == 0.f ? 0.f : acc / l;
-        uint16_t out;
-        if constexpr (BF16) out = bitcast<uint16_t>((__bf16)r);
-        else out = bitcast<uint16_t>((_Float16)r);
-        a.o[(int64_t)sh.b * a.o_bs + (int64_t)(sh.hk * a.ratio + sh.col0 + c) * a.o_hs + d] = out;
-      } else {
-        const int64_t at = (int64_t)sh.row + col0 + c;
-        a.part_o[at * D + d] = acc;
-        if (d == 0) {
-          a.part_ml[at * 2] = m;
-          a.part_ml[at * 2 + 1] = l;
-        }
+      const int64_t at = (int64_t)sh.row + col0 + c;
+      a.part_o[at * D + d] = acc;
+      if (d == 0) {
+        a.part_ml[at * 2] = m;
+        a.part_ml[at * 2 + 1] = l;
       }
     }
     __syncthreads();
   }
 };
 
-// Shared tiles: 32·RW columns by KG key groups of TB tiles a step.
+template <int D, int RW, int KG, int TB> constexpr int kShLds() {
+  const int stages = 4 * KG * 32 * TB * D * 2, sums = (RW * KG * 16 * (D / 32) * 64 + RW * KG * 2 * 64 + 1) * 4, tiles = stages > sums || KG == 1 ? stages : sums,
+            slices = kShWaves * kDecTile * (D * 2 + 32), plan = kShWords * 4;
+  return tiles > slices ? (tiles > plan ? tiles : plan) : slices > plan ? slices : plan;
+}
+
+// Shared tiles: 32·RW columns by KG key groups of TB tiles a step. True if a page was none of
+// the cache's: nothing is done then.
 template <int D, bool BF16, int RW, int KG, int TB>
-__device__ __forceinline__ void group_part(kernarg<SharedArgs>& a, const Share& sh, uint8_t* lds) {
+__device__ __forceinline__ bool group_part(kernarg<SharedArgs>& a, const Share& sh, uint8_t* lds) {
   typedef typename Elt<BF16>::v8 V8;
   static_assert(RW * KG == kShWaves, "four waves");
   constexpr int UPR = D / 8, KD = D / 16, DB = D / 32, kTile = 32 * TB;
@@ -519,35 +514,57 @@ __device__ __forceinline__ void group_part(kernarg<SharedArgs>& a, const Share& 
   const int count = sh.hi - sh.lo, first = sh.own.first + sh.lo;
   const int steps = (count + KG * TB - 1) / (KG * TB);
   auto tiles_of = [&](int step) { return max(0, min(TB, count - (step * KG + kg) * TB)); };
-  // the lane's rows of a K and of a V tile, and its 16-byte chunk of them
+  // The wave's rows of the LDS tiles: load i brings rows rw·R + i·RPL .., of K the keys π(row).
+  // 4 rows of K are 4 keys that follow one another in a page, and RPL rows of V are so too, so
+  // that their page is the same for all lanes, which add an offset of their own (of d = 64,
+  // K's 8 rows are two such runs, 16 keys apart: one page where it has 32 rows, else an address each).
   const int* lead = a.table + (int64_t)sh.leader * a.ts;
-  const int r0 = rw * R + lane / UPR, slot = lane % UPR;
+  const int q4 = lane / UPR, slot = lane % UPR;
   const uint16_t* kbase = a.k + (int64_t)sh.hk * a.kh;
   const uint16_t* vbase = a.v + (int64_t)sh.hk * a.vh;
   const int most = (first + count) * kDecTile - 1;   // the part's last key
-  auto k_row = [&](int i) { const int r = r0 + i * RPL; return (r & ~31) + key_perm(r & 31); };
-  auto v_row = [&](int i) { return r0 + i * RPL; };
-  struct Pages { int k[kLoads], v[kLoads]; };
-  auto entries = [&](int step, Pages& e) __attribute__((always_inline)) {
-    const int key0 = (first + (step * KG + kg) * TB) * kDecTile;
+  const bool two = RPL == 8 && a.shift < 5;          // K's loads reach into two pages
+  // Offsets of the lane from where the tile starts in a page (of fewer than 32 rows: from the page)
+  const int in_page = page_size - 1;
+  auto k_key = [&](int i) { const int r = rw * R + i * RPL; return (r & ~31) + key_perm(r & 31); };
+  uint32_t k_off[kLoads], v_off[kLoads];
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      e.k[i] = lead[min(key0 + k_row(i), most) >> a.shift];
-      e.v[i] = lead[min(key0 + v_row(i), most) >> a.shift];
-    }
-  };
-  auto issue = [&](int step, int st, const Pages& e) __attribute__((always_inline)) {
-    const int key0 = (first + (step * KG + kg) * TB) * kDecTile, rows = tiles_of(step) * 32;
+  for (int i = 0; i < kLoads; ++i) {
+    const int r = rw * R + i * RPL;
+    k_off[i] = (uint32_t)(((k_key(i) & in_page & 31) + key_perm((r + q4) & 31) - key_perm(r & 31)) * (int)a.kr + (slot ^ ((r + q4) % UPR)) * 8) * 2u;
+    v_off[i] = (uint32_t)(((r & in_page & 31) + q4) * (int)a.vr + (slot ^ v_swz<D>(q4)) * 8) * 2u;
+  }
+  // The page numbers of a step's loads: of K's in lanes 0 .., then of V's. (Scalar loads would hold
+  // up the LDS operand reads, whose counter they share.) A page outside the cache is read as
+  // page 0, and all of it done again at the end.
+  static_assert(2 * kLoads <= 64, "a lane each");
+  const int of = lane < kLoads ? lane : min(lane - kLoads, kLoads - 1), of_row = rw * R + of * RPL;
+  const int of_key = lane < kLoads ? (of_row & ~31) + key_perm(of_row & 31) : of_row;
+  bool bad = false;
+  auto entries = [&](int step) { return lead[min((first + (step * KG + kg) * TB) * kDecTile + of_key, most) >> a.shift]; };
+  auto issue = [&](int step, int st, int e) __attribute__((always_inline)) {
+    static_assert(32 % R == 0, "a wave's rows are of one tile");
+    if (rw * R >= tiles_of(step) * 32) return;
+    const bool none = (uint32_t)e >= (uint32_t)a.pages;
+    bad |= none;
+    e = none ? 0 : e;
+    const int key0 = (first + (step * KG + kg) * TB) * kDecTile, at = (key0 + (rw * R & ~31)) & in_page;   // (0 of small pages)
+    const uint16_t* kb = kbase + (int64_t)at * a.kr;
+    const uint16_t* vb = vbase + (int64_t)at * a.vr;
     uint16_t* tk = sKV + ((st * 2) * KG + kg) * kElems + rw * R * D;
     uint16_t* tv = sKV + ((st * 2 + 1) * KG + kg) * kElems + rw * R * D;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      if (rw * R + i * RPL >= rows) continue;   // (whole tiles of 32 rows)
-      const int kr = k_row(i), vr = v_row(i);
-      gload16_lds(kbase + (int64_t)e.k[i] * a.kp + (int64_t)((key0 + kr) & (page_size - 1)) * a.kr + (slot ^ ((r0 + i * RPL) % UPR)) * 8,
-                  lds_addr(tk) + (uint32_t)(i * 64 * 16));
-      gload16_lds(vbase + (int64_t)e.v[i] * a.vp + (int64_t)((key0 + vr) & (page_size - 1)) * a.vr + (slot ^ v_swz<D>(vr)) * 8,
-                  lds_addr(tv) + (uint32_t)(i * 64 * 16));
+      if (two) {   // (its own page for each lane)
+        const int r = rw * R + i * RPL, key = key0 + (r & ~31) + key_perm((r + q4) & 31);
+        int x = lead[min(key, most) >> a.shift];
+        const bool nx = (uint32_t)x >= (uint32_t)a.pages;
+        bad |= nx;
+        x = nx ? 0 : x;
+        gload16_lds(kbase + (int64_t)x * a.kp + (int64_t)(key & in_page) * a.kr + (slot ^ ((r + q4) % UPR)) * 8, lds_addr(tk) + (uint32_t)(i * 64 * 16));
+      } else
+        gload16_lds(kb + (int64_t)__builtin_amdgcn_readlane(e, i) * a.kp, k_off[i], lds_addr(tk) + (uint32_t)(i * 64 * 16));
+      gload16_lds(vb + (int64_t)__builtin_amdgcn_readlane(e, kLoads + i) * a.vp, v_off[i], lds_addr(tv) + (uint32_t)(i * 64 * 16));
     }
   };
 
@@ -640,15 +657,14 @@ __device__ __forceinline__ void group_part(kernarg<SharedArgs>& a, const Share& 
     }
   };
 
-  Pages e;
-  entries(0, e);
+  int e = entries(0);
   issue(0, 0, e);
-  if (steps > 1) entries(1, e);
+  e = entries(1);
   for (int i = 0; i < steps; ++i) {
     wait_vmcnt<0>();   // the wave's loads of step i have landed
     wg_barrier();      // all waves' have, and all have left the stage of step i − 1
     if (i + 1 < steps) issue(i + 1, (i + 1) & 1, e);
-    if (i + 2 < steps) entries(i + 2, e);
+    e = entries(i + 2);
     const int n = tiles_of(i), base = (first + (i * KG + kg) * TB) * kDecTile;
     const uint16_t* tk = sKV + (((i & 1) * 2) * KG + kg) * kElems;
     const uint16_t* tv = sKV + (((i & 1) * 2 + 1) * KG + kg) * kElems;
@@ -657,54 +673,64 @@ __device__ __forceinline__ void group_part(kernarg<SharedArgs>& a, const Share& 
   }
   wait_vmcnt<0>();
   l_run = xhalf_sum(l_run);
-  // the key groups' sums of the same columns, in the lanes that hold them
-  constexpr int kJoin = (DB * 16 + 2) * 64;   // floats of one wave
-  float* sj = reinterpret_cast<float*>(lds);
-  if constexpr (KG > 1) {
-    wg_barrier();   // the stages are free
-    if (kg > 0) {
-      float* at = sj + (rw * (KG - 1) + kg - 1) * kJoin + lane;
-      at[0] = m_run;
-      at[64] = l_run;
-#pragma unroll
-      for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int x = 0; x < 16; ++x) at[(2 + db * 16 + x) * 64] = oacc[db][x];
-    }
-    __syncthreads();
-    if (kg > 0) return;
-#pragma unroll 1
-    for (int k = 1; k < KG; ++k) {
-      const float* at = sj + (rw * (KG - 1) + k - 1) * kJoin + lane;
-      const float mk = at[0], lk = at[64];
-      const float top = fmaxf(m_run, mk);
-      // a group that saw nothing has sums of 0 (or NaN, which stay)
-      const float f0 = m_run == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_run - top) * c2);
-      const float f1 = mk == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mk - top) * c2);
-      l_run = l_run * f0 + lk * f1;
-#pragma unroll
-      for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int x = 0; x < 16; ++x) oacc[db][x] = oacc[db][x] * f0 + at[(2 + db * 16 + x) * 64] * f1;
-      m_run = top;
-    }
-  }
-  if (!mine) return;
   const int64_t at = (int64_t)sh.row + c;
+  // The key groups' sums of the same columns, which the same lanes hold: group x of their waves
+  // forms the x-th share of the 16·DB sums, and the others hand theirs over in LDS.
+  constexpr int OWN = 16 * DB / KG, kSums = KG > 1 ? RW * KG * 16 * DB * 64 : 0;
+  float* sj = reinterpret_cast<float*>(lds);   // [RW][KG shares][KG][OWN][64], then [RW][KG][2][64]
+  float* sml = sj + kSums;
+  static_assert((kSums + RW * KG * 2 * 64 + 1) * 4 <= kShLds<D, RW, KG, TB>(), "sums fit");
+  uint32_t* flag = reinterpret_cast<uint32_t*>(sml + RW * KG * 2 * 64);
+  wg_barrier();   // the stages are free
+  if (tid == 0) *flag = 0;
+  if constexpr (KG > 1) {
 #pragma unroll
-  for (int db = 0; db < DB; ++db)
+    for (int x = 0; x < KG; ++x)
+      if (x != kg)
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
-      *reinterpret_cast<f32x4*>(a.part_o + at * D + db * 32 + x * 8 + g * 4) = f32x4{oacc[db][4 * x], oacc[db][4 * x + 1], oacc[db][4 * x + 2], oacc[db][4 * x + 3]};
-  if (g == 0) {
-    a.part_ml[at * 2] = m_run == -INFINITY ? -INFINITY : m_run * c2;
+        for (int y = 0; y < OWN; ++y) sj[(((rw * KG + x) * KG + kg) * OWN + y) * 64 + lane] = oacc[(x * OWN + y) / 16][(x * OWN + y) % 16];
+    sml[((rw * KG + kg) * 2) * 64 + lane] = m_run;
+    sml[((rw * KG + kg) * 2 + 1) * 64 + lane] = l_run;
+  }
+  __syncthreads();
+  if (__builtin_amdgcn_ballot_w64(bad) && lane == 0) atomicOr(flag, 1u);
+  float f[KG], m = m_run;
+  if constexpr (KG > 1) {
+    float l = 0.f;
+#pragma unroll
+    for (int x = 0; x < KG; ++x) m = fmaxf(m, f[x] = sml[((rw * KG + x) * 2) * 64 + lane]);
+#pragma unroll
+    for (int x = 0; x < KG; ++x) {
+      // a group that saw nothing has sums of 0 (or NaN, which stay)
+      f[x] = f[x] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((f[x] - m) * c2);
+      l += sml[((rw * KG + x) * 2 + 1) * 64 + lane] * f[x];
+    }
+    l_run = l;
+  } else f[0] = 1.f;
+#pragma unroll
+  for (int x = 0; x < KG; ++x)
+    if (x == kg) {
+      float y[OWN];
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) {
+        y[i] = oacc[(x * OWN + i) / 16][(x * OWN + i) % 16] * f[x];
+#pragma unroll
+        for (int z = 0; z < KG; ++z)
+          if (z != x) y[i] += sj[(((rw * KG + x) * KG + z) * OWN + i) * 64 + lane] * f[z];
+      }
+      if (mine)
+#pragma unroll
+        for (int i = 0; i < OWN; i += 4) {
+          const int e = x * OWN + i;   // sum e of the lane is that of d = 32·(e / 16) + 8·(e % 16 / 4) + 4·g + e % 4
+          *reinterpret_cast<f32x4*>(a.part_o + at * D + e / 16 * 32 + e % 16 / 4 * 8 + g * 4) = f32x4{y[i], y[i + 1], y[i + 2], y[i + 3]};
+        }
+    }
+  if (mine && kg == 0 && g == 0) {
+    a.part_ml[at * 2] = m == -INFINITY ? -INFINITY : m * c2;
     a.part_ml[at * 2 + 1] = l_run;
   }
-}
-
-template <int D, int RW, int KG, int TB> constexpr int kShLds() {
-  const int tiles = 4 * KG * 32 * TB * D * 2, slices = kShWaves * kDecTile * (D * 2 + 32), plan = kShWords * 4;
-  return tiles > slices ? (tiles > plan ? tiles : plan) : slices > plan ? slices : plan;
+  __syncthreads();
+  return *flag != 0;
 }
 
 template <int D, bool BF16, int RW, int KG, int TB>
@@ -735,7 +761,7 @@ void shared_decode_kernel(const SharedArgs a) {
   const int kind = uni(shares[wave].kind);
   if (kind == 0) return;
   uint8_t* sv = lds + wave * Stream<D, BF16>::kSlice;
-  if (kind == 3) {
+  if (kind == 2) {
     kernarg<SharedArgs>& z = reload_kernarg(a);
     const Share sh = share();
     Stream<D, BF16> st;
@@ -743,19 +769,9 @@ void shared_decode_kernel(const SharedArgs a) {
     st.store(z, sh);
     return;
   }
-  if (kind == 1) {
-    kernarg<SharedArgs>& z = reload_kernarg(a);
-    const Share sh = share();
-    // a page outside the cache hides its keys, which only the stream can
-    const int* lead = z.table + (int64_t)sh.leader * z.ts;
-    const int p0 = ((sh.own.first + sh.lo) * kDecTile) >> z.shift, p1 = ((sh.own.first + sh.hi) * kDecTile - 1) >> z.shift;
-    bool bad = false;
-    for (int p = p0 + (int)threadIdx.x % 64; p <= p1; p += 64) bad |= lead[p] < 0 || lead[p] >= z.pages;
-    if (__builtin_amdgcn_ballot_w64(bad) == 0) {
-      group_part<D, BF16, RW, KG, TB>(z, sh, lds);
-      return;
-    }
-  }
+  if (!group_part<D, BF16, RW, KG, TB>(reload_kernarg(a), share(), lds)) return;
+  // a page outside the cache hides its keys, which only the stream can
+  __syncthreads();
 #pragma unroll 1
   for (int c = 0; c < uni(shares[wave].cols); c += 16) {
     kernarg<SharedArgs>& z = reload_kernarg(a);

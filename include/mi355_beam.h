@@ -51,7 +51,7 @@ enum { MI355_BEAM_FP16 = 0, MI355_BEAM_BF16 = 1, MI355_BEAM_FP32 = 2 };
  * request that sees none gives 0. Keys that are not seen have no influence.
  * Layouts: q, o [b, h, d]; caches [num_pages, h_k, page_size, d]; block_table
  * [b, table_cols]; innermost stride 1, 16-byte aligned bases, other strides multiples of
- * 8 elements. A page number outside the cache hides that page's keys; kv_lens and
+ * 8 elements, the caches' row strides below 2^24. A page number outside the cache hides that page's keys; kv_lens and
  * prefix_lens past table_cols·page_size (2^30 at most) count as that.
  */
 typedef struct mi355_shared_params {
@@ -78,7 +78,7 @@ typedef struct mi355_shared_params {
   size_t workspace_bytes;
 } mi355_shared_params;
 
-#define MI355_BEAM_MAX_REQUESTS 2048
+#define MI355_BEAM_MAX_REQUESTS 1024
 
 int mi355_shared_decode(const mi355_shared_params* p, void* stream, char* err, size_t errlen);
 

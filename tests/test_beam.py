@@ -61,11 +61,11 @@ def lib():
 @pytest.mark.parametrize("name,cls,base,bad,text", [
     *[("mi355_shared_decode", Shared, SHARED, bad, text) for bad, text in [
         (dict(dtype=2), "float16 or bfloat16"), (dict(d=96), "head_dim"), (dict(h=3), "divisible"), (dict(h_k=0), "divisible"), (dict(b=-1), "requests"),
-        (dict(b=2049), "2048 requests"), (dict(groups=-1), "groups"), (dict(groups=2049), "groups"), (dict(h=2 ** 17), "heads"), (dict(cols=-1), "negative"),
+        (dict(b=1025), "1024 requests"), (dict(groups=-1), "groups"), (dict(groups=1025), "groups"), (dict(h=2 ** 17), "heads"), (dict(cols=-1), "negative"),
         (dict(num_pages=-1), "negative"), (dict(page_size=4), "page_size"), (dict(page_size=48), "page_size"), (dict(page_size=2048), "page_size"),
         (dict(cols=2 ** 27), "2\\^30 keys"), (dict(window=-1), "window"), (dict(scale=0.0), "scale"), (dict(scale=math.nan), "scale"),
         (dict(softcap=1001.0), "softcap"), (dict(lens=0), "NULL"), (dict(cu=0), "NULL"), (dict(prefix=0), "NULL"), (dict(table=0), "NULL"), (dict(v=0), "NULL"),
-        (dict(q=4104), "16-byte"), (dict(kr=68), "multiples of 8")]],
+        (dict(q=4104), "16-byte"), (dict(kr=68), "multiples of 8"), (dict(kr=2 ** 24), "row strides"), (dict(vr=-64), "row strides"), (dict(o_hs=68), "multiples of 8")]],
     *[("mi355_beam_select", Select, SELECT, bad, text) for bad, text in [
         (dict(dtype=3), "float32"), (dict(groups=-1), "beams"), (dict(beams=0), "beams"), (dict(beams=257), "beams"), (dict(vocab=0), "vocab"),
         (dict(vocab=2 ** 30), "vocab"), (dict(groups=2 ** 30), "vocab"), (dict(k=0), "k must"), (dict(k=65), "k must"), (dict(done=4096, eos=-1), "eos"),
@@ -104,7 +104,7 @@ def test_workspaces(lib):
         assert f(None) == 0
         return f(ctypes.addressof(make(cls, base, **kw)))
 
-    for b, g, h, hk, d in ((1, 1, 4, 4, 128), (67, 9, 40, 2, 64), (2048, 2048, 8, 8, 128), (2048, 1, 64, 1, 64), (5, 0, 8, 8, 64)):
+    for b, g, h, hk, d in ((1, 1, 4, 4, 128), (67, 9, 40, 2, 64), (1024, 1024, 8, 8, 128), (1024, 1, 64, 1, 64), (5, 0, 8, 8, 64)):
         units = b * hk * -(-(h // hk) // 16)   # of own keys, 16 heads each
         assert size(*CALLS[0], b=b, groups=g, h=h, h_k=hk, d=d) >= (units + 1) * 16 * (d + 2) * 4 + (b + g) * 16
     assert size(*CALLS[0], b=0) == 0 and size(*CALLS[0], d=96) == 0

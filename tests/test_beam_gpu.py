@@ -235,7 +235,7 @@ def test_shared_empty(ops):
 def test_shared_most_requests(ops):
     """The most requests a call takes, in groups of all sizes."""
     r = random.Random(2)
-    groups, left = [], 2048
+    groups, left = [], 1024
     while left:
         n = min(left, r.choice([1, 2, 3, 17, 90]))
         groups.append((r.choice([0, 33, 64, 90]), n))
@@ -243,7 +243,7 @@ def test_shared_most_requests(ops):
     x = batch(14, groups, 12, 2, 1, 64, 16, torch.bfloat16)
     out = ops.mha_shared_decode(x["q"], x["kc"], x["vc"], x["table"], ints(x["lens"]), ints(x["cu"]), ints(x["prefix"]))
     b = ops.mha_paged_decode(x["q"], x["kc"], x["vc"], x["table"], ints(x["lens"]))
-    pick = list(range(0, 2048, 67))
+    pick = list(range(0, 1024, 37))
     for i in pick:
         g = next(g for g in range(len(groups)) if x["cu"][g] <= i < x["cu"][g + 1])
         y = dict(x, q=x["q"][i:i + 1], table=x["table"][i:i + 1], lens=[x["lens"][i]], cu=[0], prefix=[])
@@ -614,9 +614,9 @@ def test_refusals(ops):
                       (dict(backend="tilelang"), "tilelang")]:
         with pytest.raises(RuntimeError, match=text):
             ops.mha_shared_decode(**{**good, **bad})
-    many = torch.zeros(2049, 4, 64, dtype=torch.bfloat16, device="cuda")
-    with pytest.raises(RuntimeError, match="2048 requests"):
-        ops.mha_shared_decode(many, x["kc"], x["vc"], x["table"][:1].expand(2049, -1), ints([0] * 2049), ints([0]), ints([]))
+    many = torch.zeros(1025, 4, 64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError, match="1024 requests"):
+        ops.mha_shared_decode(many, x["kc"], x["vc"], x["table"][:1].expand(1025, -1), ints([0] * 1025), ints([0]), ints([]))
     lx, s = logits_of(1, 2, 3, 50, torch.float32)
     done = torch.zeros(2, 3, dtype=torch.bool, device="cuda")
     good = dict(logits=lx, scores=s, k=3)

@@ -52,25 +52,29 @@ int main() {
   }
   REQUIRE(own_tiles(1 << 30, kNoWindow, TileSpan{0, 0}).count == 1 << 25);
   for (int round = 0; round < 4000; ++round) {
-    const int items = pick(1, 60), target = pick(1, 1024), least = pick(1, 16);
+    const int items = pick(1, 60), groups = pick(0, items), target = pick(1, 1024), least = pick(1, 16), wave_least = pick(1, 4);
     std::vector<int> tiles(items), units(items);
-    int64_t sum = 0, all = 0, parts = 0;
+    int64_t sum = 0, of_groups = 0, of_requests = 0, units_g = 0, units_r = 0;
     for (int i = 0; i < items; ++i) {
       tiles[i] = pick(0, 3) ? pick(0, 3000) : pick(0, 3) ? 0 : 1 << pick(0, 25);
       units[i] = pick(1, 64);
       sum += (int64_t)tiles[i] * units[i];
-      all += units[i];
+      (i < groups ? units_g : units_r) += units[i];
     }
-    const int per = share_size(sum, target, least);
-    REQUIRE(per >= least);
+    const int per = share_size(sum, target, least), wave_per = wave_share_size(per, wave_least);
+    REQUIRE(per >= least && wave_per >= wave_least);
     for (int i = 0; i < items; ++i) {
-      const int n = share_count(tiles[i], per);
-      parts += (int64_t)n * units[i];
+      const int size = i < groups ? per : wave_per, n = share_count(tiles[i], size);
+      (i < groups ? of_groups : of_requests) += (int64_t)n * units[i];
       REQUIRE((n == 0) == (tiles[i] == 0));
-      for (int p = 0; p < n; ++p) REQUIRE(share_start(tiles[i], n, p) < share_start(tiles[i], n, p + 1) && share_start(tiles[i], n, p + 1) - share_start(tiles[i], n, p) <= per);
+      for (int p = 0; p < n; ++p) {
+        const int a = share_start(tiles[i], n, p), b = share_start(tiles[i], n, p + 1);
+        REQUIRE(a < b && b - a <= size);
+      }
       if (n) REQUIRE(share_start(tiles[i], n, 0) == 0 && share_start(tiles[i], n, n) == tiles[i]);
     }
-    REQUIRE(parts <= target + all);
+    REQUIRE(of_groups + (of_requests + 3) / 4 <= target + units_g + (units_r + 3) / 4 + 1);
+    REQUIRE(of_groups <= target + units_g && of_requests <= 4 * (int64_t)target + units_r);   // rows of partial sums
   }
   printf("ok\n");
   return 0;
