@@ -60,7 +60,11 @@ SharedPlan shared_plan(const mi355_shared_params* p, int cus) {
   // columns of a KV head that a group has on average
   const int64_t mean = p->n_groups > 0 ? p->b * ratio / p->n_groups : 0;
   pl.columns = mean > 64 ? 128 : mean > 32 ? 64 : 32;
-  pl.target = 2 * cus;
+  auto per_cu = [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    return pl.columns == 128 ? kShPerCu<D, 4, 1, kShTiles>() : pl.columns == 64 ? kShPerCu<D, 2, 2, 1>() : kShPerCu<D, 1, 4, 1>();
+  };
+  pl.target = cus * (p->d == 64 ? per_cu(std::integral_constant<int, 64>{}) : per_cu(std::integral_constant<int, 128>{}));
   pl.least = 4;
   pl.wave_least = 2;
   const int64_t own = (int64_t)p->b * p->h_k * pl.groups;

@@ -54,6 +54,26 @@ MI355_HD inline int share_start(int tiles, int n, int p) {
   return p * each + imin(p, more);
 }
 
+// Place `place` of an item's parts, of heads · blocks units of n parts each: the blocks of one
+// part of one head read the same tiles, and are 8 places apart, on one XCD.
+struct UnitPart {
+  int hk, block, part;
+};
+MI355_HD inline UnitPart unit_part(int place, int n, int heads, int blocks) {
+  const uint32_t all = (uint32_t)(heads * n), whole = all & ~7u, x = (uint32_t)place;
+  uint32_t item, block;
+  if (x < whole * blocks) {
+    const uint32_t eight = x >> 3;
+    item = eight / blocks * 8 + (x & 7);
+    block = eight % blocks;
+  } else {
+    const uint32_t rest = all - whole, y = x - whole * blocks;
+    item = whole + y % rest;
+    block = y / rest;
+  }
+  return {(int)(item / (uint32_t)n), (int)block, (int)(item % (uint32_t)n)};
+}
+
 }  // namespace mi355fa
 
 #endif  // MI355_BEAM_SCHED_H

@@ -247,6 +247,7 @@ template <int D> __device__ __forceinline__ int v_swz(int r) {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 
 }  // namespace mi355fa
 

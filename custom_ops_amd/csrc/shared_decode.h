@@ -236,22 +236,22 @@ __device__ __forceinline__ Share share_of(const SharedArgs& a, int w, int* s, in
   const int parts = uni(l.acc[20]), x = w < parts ? 0 : wave, item = uni(l.acc[4 * x]) - 1;
   if (item < 0) return sh;
   const int place = uni(l.acc[4 * x + 1]), n = uni(l.acc[4 * x + 2]), t = uni(l.acc[4 * x + 3]), start = uni(l.acc[16 + x]);
-  const int unit = (int)((uint32_t)place / (uint32_t)n), p = place - unit * n;
-  sh.lo = share_start(t, n, p);
-  sh.hi = share_start(t, n, p + 1);
   const bool group = item < a.n_groups;
   sh.kind = group ? 1 : 2;
   const int b = group ? 0 : item - a.n_groups, g = group ? item : uni(l.group_of[b]);
   const int c0 = g >= 0 ? uni(l.cu[g]) : b, c1 = g >= 0 ? min(uni(l.cu[g + 1]), a.b) : b;
   const TileSpan sp = g >= 0 ? TileSpan{uni(l.least_of[g]), uni(l.most_of[g])} : TileSpan{0, 0};
   const int shift = group ? a.col_shift : 4, width = 1 << shift, total = group ? (c1 - c0) * a.ratio : a.ratio, blocks = (total + width - 1) >> shift;
+  const UnitPart at = unit_part(place, n, a.hk, blocks);
+  sh.lo = share_start(t, n, at.part);
+  sh.hi = share_start(t, n, at.part + 1);
   sh.b = group ? c0 : b;
   sh.leader = c0;
-  sh.hk = (int)((uint32_t)unit / (uint32_t)blocks);
-  sh.col0 = (unit - sh.hk * blocks) * width;
+  sh.hk = at.hk;
+  sh.col0 = at.block * width;
   sh.cols = min(width, total - sh.col0);
   sh.prefix = group ? INT_MAX : g >= 0 ? uni(l.prefix[g]) : 0;
-  sh.row = (group ? 0 : a.own_rows) + (start + place) * width;
+  sh.row = (group ? 0 : a.own_rows) + (start + (at.hk * blocks + at.block) * n + at.part) * width;
   sh.alone = !group && n == 1 && sp.t0 == sp.t1;
   const OwnTiles own = own_tiles(uni(l.len_of[b]), a.window, sp);
   sh.own.lo = group ? 0 : own.lo;
@@ -476,8 +476,12 @@ template <int D, bool BF16> struct Stream {
   }
 };
 
+// Stages of the DMA, and pages whose numbers are held in LDS.
+template <int KG, int TB> constexpr int kShStages() { return KG * TB == 1 ? 4 : 2; }
+constexpr int kShPages = 1024;
+
 template <int D, int RW, int KG, int TB> constexpr int kShLds() {
-  const int stages = 4 * KG * 32 * TB * D * 2, sums = (RW * KG * 16 * (D / 32) * 64 + RW * KG * 2 * 64 + 1) * 4, tiles = stages > sums || KG == 1 ? stages : sums,
+  const int stages = kShStages<KG, TB>() * 2 * KG * 32 * TB * D * 2 + kShPages * 4, sums = (RW * KG * 16 * (D / 32) * 64 + RW * KG * 2 * 64 + 1) * 4, tiles = stages > sums ? stages : sums,
             slices = kShWaves * kDecTile * (D * 2 + 32), plan = kShWords * 4;
   return tiles > slices ? (tiles > plan ? tiles : plan) : slices > plan ? slices : plan;
 }
@@ -488,7 +492,7 @@ template <int D, bool BF16, int RW, int KG, int TB>
 __device__ __forceinline__ bool group_part(kernarg<SharedArgs>& a, const Share& sh, uint8_t* lds) {
   typedef typename Elt<BF16>::v8 V8;
   static_assert(RW * KG == kShWaves, "four waves");
-  constexpr int UPR = D / 8, KD = D / 16, DB = D / 32, kTile = 32 * TB;
+  constexpr int UPR = D / 8, KD = D / 16, DB = D / 32, kTile = 32 * TB, S = kShStages<KG, TB>();
   constexpr int kElems = kTile * D;                 // of a K or V tile
   constexpr int R = kTile / RW;                     // rows that a wave brings
   constexpr int kLoads = R * UPR / 64, RPL = 64 / UPR;   // loads of K, of V; rows of one
@@ -506,8 +510,8 @@ __device__ __forceinline__ bool group_part(kernarg<SharedArgs>& a, const Share& 
   V8 qreg[KD];
 #pragma unroll
   for (int kd = 0; kd < KD; ++kd) qreg[kd] = bitcast<V8>(*reinterpret_cast<const u32x4*>(q + kd * 16));
-  const float bco = a.slopes ? a.slopes[h] * a.bias : 0.f;
-  const float last = a.slopes ? (float)(min(max(a.lens[b], 0), (int)((int64_t)a.cols << a.shift)) - 1) : 0.f;   // the column's last key
+  float bco = a.slopes ? a.slopes[h] * a.bias : 0.f;
+  float last = a.slopes ? (float)(min(max(a.lens[b], 0), (int)((int64_t)a.cols << a.shift)) - 1) : 0.f;   // the column's last key
   const float c2 = a.c2, slack = kSlackLog2 / a.c2;
 
   // steps of KG·TB tiles: key group kg has tiles first + (step·KG + kg)·TB ..
@@ -534,37 +538,59 @@ __device__ __forceinline__ bool group_part(kernarg<SharedArgs>& a, const Share& 
     k_off[i] = (uint32_t)(((k_key(i) & in_page & 31) + key_perm((r + q4) & 31) - key_perm(r & 31)) * (int)a.kr + (slot ^ ((r + q4) % UPR)) * 8) * 2u;
     v_off[i] = (uint32_t)(((r & in_page & 31) + q4) * (int)a.vr + (slot ^ v_swz<D>(q4)) * 8) * 2u;
   }
-  // The page numbers of a step's loads: of K's in lanes 0 .., then of V's. (Scalar loads would hold
-  // up the LDS operand reads, whose counter they share.) A page outside the cache is read as
-  // page 0, and all of it done again at the end.
+  // Page numbers in LDS, kShPages from page `held` on. (Loads of the loop's own would make it
+  // wait for the DMA issued before them.) A page outside the cache is read as page 0, and all of
+  // it done again at the end.
+  int* pages = reinterpret_cast<int*>(lds + S * 2 * KG * kElems * 2);
+  const int last_page = most >> a.shift;
+  int held = (first * kDecTile) >> a.shift;
+  bool bad = false;
+  auto fill = [&]() {
+#pragma unroll
+    for (int x = 0; x < kShPages / kShThreads; ++x) {
+      const int at = x * kShThreads + tid;
+      if (held + x * kShThreads > last_page) break;
+      const int page = lead[min(held + at, last_page)];
+      const bool none = (uint32_t)page >= (uint32_t)a.pages;
+      bad |= none;
+      pages[at] = none ? 0 : page;
+    }
+    wg_barrier();
+  };
+  // Where a step's loads start: those of K in lanes 0 .., then V's.
   static_assert(2 * kLoads <= 64, "a lane each");
   const int of = lane < kLoads ? lane : min(lane - kLoads, kLoads - 1), of_row = rw * R + of * RPL;
   const int of_key = lane < kLoads ? (of_row & ~31) + key_perm(of_row & 31) : of_row;
-  bool bad = false;
-  auto entries = [&](int step) { return lead[min((first + (step * KG + kg) * TB) * kDecTile + of_key, most) >> a.shift]; };
-  auto issue = [&](int step, int st, int e) __attribute__((always_inline)) {
+  const bool of_k = lane < kLoads;
+  const uint64_t of_base = reinterpret_cast<uint64_t>(of_k ? kbase : vbase), of_page = (uint64_t)(of_k ? a.kp : a.vp) * 2, of_step = (uint64_t)(of_k ? a.kr : a.vr) * 2;
+  auto key_of = [&](int step) { return (first + (step * KG + kg) * TB) * kDecTile; };
+  auto entries = [&](int step) __attribute__((always_inline)) {
+    const int behind = min((first + min(step + 1, steps) * KG * TB) * kDecTile - 1, most) >> a.shift;   // the step's last page
+    if (behind - held >= kShPages) {   // (all waves come here, of step after step)
+      wg_barrier();
+      held = min((first + step * KG * TB) * kDecTile, most) >> a.shift;
+      fill();
+    }
+    // (of small pages the tile starts at 0, and the lane's key is in its offset)
+    const int key0 = key_of(step), page = pages[(min(key0 + of_key, most) >> a.shift) - held];
+    return of_base + (uint64_t)(uint32_t)page * of_page + (uint64_t)(uint32_t)((key0 + (rw * R & ~31)) & in_page) * of_step;
+  };
+  const uint32_t lds0 = lds_addr(sKV);
+  auto issue = [&](int step, int st, uint64_t e) __attribute__((always_inline)) {
     static_assert(32 % R == 0, "a wave's rows are of one tile");
     if (rw * R >= tiles_of(step) * 32) return;
-    const bool none = (uint32_t)e >= (uint32_t)a.pages;
-    bad |= none;
-    e = none ? 0 : e;
-    const int key0 = (first + (step * KG + kg) * TB) * kDecTile, at = (key0 + (rw * R & ~31)) & in_page;   // (0 of small pages)
-    const uint16_t* kb = kbase + (int64_t)at * a.kr;
-    const uint16_t* vb = vbase + (int64_t)at * a.vr;
-    uint16_t* tk = sKV + ((st * 2) * KG + kg) * kElems + rw * R * D;
-    uint16_t* tv = sKV + ((st * 2 + 1) * KG + kg) * kElems + rw * R * D;
+    const uint32_t tk = lds0 + (uint32_t)(((st * 2) * KG + kg) * kElems + rw * R * D) * 2u, tv = tk + KG * kElems * 2u;
+    const uint32_t lo = low_u32(e), hi = high_u32(e);
+    auto base = [&](int x) { return reinterpret_cast<const uint8_t*>(compose_u64(__builtin_amdgcn_readlane(lo, x), __builtin_amdgcn_readlane(hi, x))); };
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       if (two) {   // (its own page for each lane)
-        const int r = rw * R + i * RPL, key = key0 + (r & ~31) + key_perm((r + q4) & 31);
-        int x = lead[min(key, most) >> a.shift];
-        const bool nx = (uint32_t)x >= (uint32_t)a.pages;
-        bad |= nx;
-        x = nx ? 0 : x;
-        gload16_lds(kbase + (int64_t)x * a.kp + (int64_t)(key & in_page) * a.kr + (slot ^ ((r + q4) % UPR)) * 8, lds_addr(tk) + (uint32_t)(i * 64 * 16));
+        const int r = rw * R + i * RPL, key = key_of(step) + (r & ~31) + key_perm((r + q4) & 31);
+        const int x = pages[(min(key, most) >> a.shift) - held];
+        gload16_lds(kbase + (int64_t)x * a.kp + (int64_t)(key & in_page) * a.kr + (slot ^ ((r + q4) % UPR)) * 8, tk + (uint32_t)(i * 64 * 16));
       } else
-        gload16_lds(kb + (int64_t)__builtin_amdgcn_readlane(e, i) * a.kp, k_off[i], lds_addr(tk) + (uint32_t)(i * 64 * 16));
-      gload16_lds(vb + (int64_t)__builtin_amdgcn_readlane(e, kLoads + i) * a.vp, v_off[i], lds_addr(tv) + (uint32_t)(i * 64 * 16));
+        gload16_lds(base(i), k_off[i], tk + (uint32_t)(i * 64 * 16));
+      gload16_lds(base(kLoads + i), v_off[i], tv + (uint32_t)(i * 64 * 16));
     }
   };
 
@@ -586,13 +612,11 @@ __device__ __forceinline__ bool group_part(kernarg<SharedArgs>& a, const Share& 
   float m_run = -INFINITY, mlog2 = 0.f, l_run = 0.f;
 
   // NT of the step's tiles at LDS tk, tv; base: the first key
-  auto compute = [&](auto nt, int base, const uint16_t* tk, const uint16_t* tv) __attribute__((always_inline)) {
+  auto compute = [&](auto nt, int base, uint32_t tk, uint32_t tv) __attribute__((always_inline)) {
     constexpr int NT = decltype(nt)::value, kWin = 2;   // LDS operand reads in flight
-    const uint8_t* k8 = reinterpret_cast<const uint8_t*>(tk);
-    const uint8_t* v8 = reinterpret_cast<const uint8_t*>(tv);
     f32x16 s[NT];
     {
-      auto rd = [&](int i) { return bitcast<V8>(*reinterpret_cast<const u32x4*>(k8 + (i / KD) * 32 * D * 2 + k_rd[i % KD])); };
+      auto rd = [&](int i) { return bitcast<V8>(*(const lds_u32x4*)(tk + k_rd[i % KD] + (i / KD) * 32 * D * 2)); };
       V8 win[kWin];
 #pragma unroll
       for (int i = 0; i < kWin; ++i) win[i] = rd(i);
@@ -633,8 +657,8 @@ __device__ __forceinline__ bool group_part(kernarg<SharedArgs>& a, const Share& 
     auto rd = [&](int i) {
       const int j = i / DB, db = i % DB;
       const int o = ((j / 2) * 32 + (j % 2) * 8) * D * 2;
-      const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(v8 + v_rd[db] + o));
-      const s16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(v8 + v_rd[db] + o + 4 * D * 2));
+      const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tv + v_rd[db] + o));
+      const s16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tv + v_rd[db] + o + 4 * D * 2));
       return bitcast<V8>(__builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
     };
     V8 win[kWin];
@@ -657,17 +681,33 @@ __device__ __forceinline__ bool group_part(kernarg<SharedArgs>& a, const Share& 
     }
   };
 
-  int e = entries(0);
-  issue(0, 0, e);
-  e = entries(1);
+  fill();
+  // Q and the slopes are here (they were asked for before the pages): were it left to their first
+  // use, every step would wait for all loads in flight
+#pragma unroll
+  for (int kd = 0; kd < KD; ++kd) {
+    u32x4 x = bitcast<u32x4>(qreg[kd]);
+    asm volatile("" : "+v"(x));
+    qreg[kd] = bitcast<V8>(x);
+  }
+  asm volatile("" : "+v"(bco), "+v"(last));
+  uint64_t e = entries(0);
+#pragma unroll
+  for (int x = 0; x < S - 1; ++x) {
+    if (x < steps) issue(x, x, e);
+    e = entries(x + 1);
+  }
+  int st = 0;
   for (int i = 0; i < steps; ++i) {
-    wait_vmcnt<0>();   // the wave's loads of step i have landed
+    // the wave's loads of step i have landed; of the steps behind it only the last one's count is not known
+    if (S > 2 && i + S - 2 < steps - (KG * TB > 1)) wait_vmcnt<(S - 2) * 2 * kLoads>();
+    else wait_vmcnt<0>();
     wg_barrier();      // all waves' have, and all have left the stage of step i − 1
-    if (i + 1 < steps) issue(i + 1, (i + 1) & 1, e);
-    e = entries(i + 2);
+    if (i + S - 1 < steps) issue(i + S - 1, st == 0 ? S - 1 : st - 1, e);
+    e = entries(i + S);
     const int n = tiles_of(i), base = (first + (i * KG + kg) * TB) * kDecTile;
-    const uint16_t* tk = sKV + (((i & 1) * 2) * KG + kg) * kElems;
-    const uint16_t* tv = sKV + (((i & 1) * 2 + 1) * KG + kg) * kElems;
+    const uint32_t tk = lds0 + (uint32_t)(((st * 2) * KG + kg) * kElems) * 2u, tv = tk + KG * kElems * 2u;
+    st = st + 1 == S ? 0 : st + 1;
     if (n == TB) compute(std::integral_constant<int, TB>{}, base, tk, tv);
     else if (TB > 1 && n == 1) compute(std::integral_constant<int, 1>{}, base, tk, tv);
   }
@@ -733,8 +773,11 @@ __device__ __forceinline__ bool group_part(kernarg<SharedArgs>& a, const Share& 
   return *flag != 0;
 }
 
+// Workgroups that a CU holds.
+template <int D, int RW, int KG, int TB> constexpr int kShPerCu() { return kShLds<D, RW, KG, TB>() <= 78 * 1024 ? 2 : 1; }
+
 template <int D, bool BF16, int RW, int KG, int TB>
-__global__ __launch_bounds__(kShThreads) __attribute__((amdgpu_waves_per_eu(kShLds<D, RW, KG, TB>() * 2 <= 160 * 1024 ? 2 : 1)))
+__global__ __launch_bounds__(kShThreads) __attribute__((amdgpu_waves_per_eu(kShPerCu<D, RW, KG, TB>())))
 void shared_decode_kernel(const SharedArgs a) {
   __shared__ __align__(16) uint8_t lds[kShLds<D, RW, KG, TB>()];
   __shared__ float sM[kShWaves][16], sL[kShWaves][16];

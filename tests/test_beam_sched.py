@@ -76,6 +76,17 @@ int main() {
     REQUIRE(of_groups + (of_requests + 3) / 4 <= target + units_g + (units_r + 3) / 4 + 1);
     REQUIRE(of_groups <= target + units_g && of_requests <= 4 * (int64_t)target + units_r);   // rows of partial sums
   }
+  for (int round = 0; round < 4000; ++round) {   // a unit's parts: each once, eight at a time next to those of the other blocks
+    const int n = pick(1, 40), heads = pick(1, 9), blocks = pick(1, 9), all = heads * n;
+    std::vector<int> seen(all * blocks, 0);
+    for (int x = 0; x < all * blocks; ++x) {
+      const UnitPart u = unit_part(x, n, heads, blocks);
+      REQUIRE(u.hk >= 0 && u.hk < heads && u.block >= 0 && u.block < blocks && u.part >= 0 && u.part < n);
+      REQUIRE(!seen[(u.hk * blocks + u.block) * n + u.part]++);
+      const int item = u.hk * n + u.part;
+      if (item < all / 8 * 8) REQUIRE(x % 8 == item % 8 && x / (8 * blocks) == item / 8);
+    }
+  }
   printf("ok\n");
   return 0;
 }
