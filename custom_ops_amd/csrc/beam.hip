@@ -47,7 +47,7 @@ int workspace_ok(const Err& err, const void* ws, size_t have, size_t need) {
 size_t up(size_t x) { return (x + 255) & ~(size_t)255; }
 
 struct SharedPlan {
-  int columns, groups, target, least, wave_least;
+  int columns, groups, target;
   int64_t grid;           // workgroups at most
   int64_t own_rows, rows; // rows of partial sums: of groups' parts, and all
   size_t ml, o, bytes;    // offsets of the parts' statistics and sums in the workspace
@@ -64,15 +64,14 @@ SharedPlan shared_plan(const mi355_shared_params* p, int cus) {
     constexpr int D = decltype(d)::value;
     return pl.columns == 128 ? kShPerCu<D, 4, 1, kShTiles>() : pl.columns == 64 ? kShPerCu<D, 2, 2, 1>() : kShPerCu<D, 1, 4, 1>();
   };
-  pl.target = cus * (p->d == 64 ? per_cu(std::integral_constant<int, 64>{}) : per_cu(std::integral_constant<int, 128>{}));
-  pl.least = 4;
-  pl.wave_least = 2;
+  const int slots = cus * (p->d == 64 ? per_cu(std::integral_constant<int, 64>{}) : per_cu(std::integral_constant<int, 128>{}));
   const int64_t own = (int64_t)p->b * p->h_k * pl.groups;
   const int64_t common = p->h_k * ((p->b * ratio + pl.columns - 1) / pl.columns + p->n_groups);
-  pl.grid = pl.target + common + (own + 3) / 4 + 1;
+  pl.target = slots - (int)(common < slots ? common / 2 : slots / 2);   // groups' units end with a part that is not whole
+  pl.grid = pl.target + common + 1;
   pl.own_rows = (common + pl.target) * pl.columns;
-  pl.rows = pl.own_rows + (4 * (int64_t)pl.target + own) * 16;
-  pl.ml = up((size_t)(p->n_groups + p->b) * 16);
+  pl.rows = pl.own_rows + (4 * (int64_t)(pl.target + 1) + own) * 16;
+  pl.ml = up((size_t)(p->n_groups + p->b + 1) * 16);
   pl.o = pl.ml + up((size_t)pl.rows * 8);
   pl.bytes = pl.o + (size_t)pl.rows * p->d * 4;
   return pl;
@@ -88,6 +87,10 @@ int shared_check(const mi355_shared_params* p, const Err& err) {
     return err.fail(kEinval, "page_size must be a power of two in 8 .. 1024");
   if ((int64_t)p->table_cols * p->page_size > kMaxKeys) return err.fail(kEinval, "block_table must span at most 2^30 keys");
   if (!window_ok(p->window)) return err.fail(kEinval, "window must be 0 (none) or positive");
+  // (places of tiles among a request's are of 32 bits, and so is a workgroup's share of all)
+  const int64_t tiles = (int64_t)p->table_cols * p->page_size / kDecTile + 1;
+  const int64_t own = p->h > 0 ? p->h_k * (int64_t)((p->h / p->h_k + 15) / 16) * tiles : 0;
+  if (own > 1 << 30 || own * p->b > (int64_t)1 << 35) return err.fail(kEinval, "too many requests, heads and keys");
   return kOk;
 }
 
@@ -123,7 +126,7 @@ int shared_decode(const mi355_shared_params* p, hipStream_t st, const Err& err) 
   a.pages = p->num_pages; a.shift = __builtin_ctz((unsigned)p->page_size);
   a.cols = p->num_pages > 0 ? p->table_cols : 0;   // no pages: nothing is seen
   a.window = window_of(p->window);
-  a.target = pl.target; a.least = pl.least; a.wave_least = pl.wave_least; a.col_shift = __builtin_ctz((unsigned)pl.columns);
+  a.target = pl.target; a.col_shift = __builtin_ctz((unsigned)pl.columns);
   a.cap = p->softcap > 0.f;
   int rc = kOk;
   by_type(p->d, p->dtype == MI355_BEAM_BF16, [&](auto d, auto bf) {

@@ -36,7 +36,8 @@ struct SharedArgs {
   const int* cu;
   const int* prefix;
   const float* slopes;
-  int* rec;        // [n_groups + b][4]: row of the first part, parts of a unit; a request's group or -1; a group's first request
+  int* rec;        // [n_groups + b + 1][4]: of groups the row of the first part, parts of a unit, first request;
+                   // of requests the first wave, its tiles before, tiles of a unit, group or -1; last the wave's tiles
   float* part_ml;  // [rows][2]: max in log2 units, sum
   float* part_o;   // [rows][D]: `columns` rows of each group's part, then 16 of each of requests' own
   int64_t q_bs, q_hs, o_bs, o_hs, kp, kh, kr, vp, vh, vr, ts;
@@ -45,7 +46,7 @@ struct SharedArgs {
   int columns;     // of a group's workgroup
   int own_rows;    // first row of part_o of own tiles
   int pages, shift, cols, window;
-  int target, least, wave_least; // workgroups wanted; tiles of a group's part at least, of a request's
+  int target;                    // workgroups wanted
   int col_shift;                 // log2 of columns
   int cap;                       // scores are capped
   float u_scale, c2, bias;       // as in PackedArgs
@@ -140,7 +141,7 @@ template <int T> __device__ __forceinline__ void find_share(const SharedArgs& a,
     const int g = l.group_of[b];
     return own_tiles(l.len_of[b], a.window, g >= 0 ? TileSpan{l.least_of[g], l.most_of[g]} : TileSpan{0, 0}).count;
   };
-  const int own_units = a.hk * a.groups;
+  const int own_units = a.hk * a.groups, weight = own_weight(a.columns);
   int64_t sum = 0;
   for (int g = tid; g < a.n_groups; g += T) {
     const int c0 = l.cu[g], c1 = min(l.cu[g + 1], a.b);
@@ -151,10 +152,15 @@ template <int T> __device__ __forceinline__ void find_share(const SharedArgs& a,
       t = shared_tiles(l.prefix[g], l.least_of[g], l.most_of[g], a.window, c1 - c0);
     l.least_of[g] = t.t0;
     l.most_of[g] = t.t1;
-    if (t.t1 > t.t0) sum += (int64_t)(t.t1 - t.t0) * units_of(g);
+    if (t.t1 > t.t0) sum += (int64_t)(t.t1 - t.t0) * units_of(g) * (a.columns / 32);
   }
   meet();
-  for (int b = tid; b < a.b; b += T) sum += (int64_t)own_count(b) * own_units;
+  int* counts = l.members;
+  for (int b = tid; b < a.b; b += T) {
+    const int g = l.group_of[b], n = own_tiles(l.len_of[b], a.window, g >= 0 ? TileSpan{l.least_of[g], l.most_of[g]} : TileSpan{0, 0}).count;
+    counts[b] = n;
+    sum += (int64_t)n * own_units * weight;
+  }
 #pragma unroll
   for (int x = 1; x < 64; x *= 2) sum += __shfl_xor(sum, x);
   if constexpr (!SOLO) {
@@ -165,101 +171,129 @@ template <int T> __device__ __forceinline__ void find_share(const SharedArgs& a,
 #pragma unroll
     for (int x = 0; x < WAVES; ++x) sum += wide[x];
   }
-  const int per = share_size(sum, a.target, a.least), wave_per = wave_share_size(per, a.wave_least);
+  const int steps = share_steps(sum, a.target), per = share_size(steps, kShWaves * 32 / a.columns), wave_per = wave_share_size(steps, weight);
   int turn = 0;
-  // f(item, tiles, parts of a unit, units, start) over items, in order; returns all parts
-  auto scan = [&](int items, auto size, auto f) __attribute__((always_inline)) {
-    int run = 0;
-    for (int e = 0; e < items; e += T) {
-      const int i = e + tid;
-      int t = 0, n = 0, u = 0;
-      if (i < items) size(i, t, n, u);
-      const int incl = wave_scan(n * u);
-      int start = run + incl - n * u;
-      if constexpr (SOLO) run += __builtin_amdgcn_readlane(incl, 63);
-      else {
-        int* part = l.acc + 48 + (turn++ & 1) * 4;   // (two sets, so that one barrier a step is enough)
-        if (lane == 63) part[wave] = incl;
-        meet();
+  // The sum over the threads before this one (and, of all, in `run`); 64 bits as two halves that cannot overflow.
+  auto scan = [&](int64_t x, int64_t& run) __attribute__((always_inline)) {
+    const int lo = (int)x & 0xfffff, hi = (int)(x >> 20), slo = wave_scan(lo), shi = wave_scan(hi);
+    int64_t start = run + ((int64_t)(shi - hi) << 20) + (slo - lo);
+    const int64_t all = ((int64_t)__builtin_amdgcn_readlane(shi, 63) << 20) + __builtin_amdgcn_readlane(slo, 63);
+    if constexpr (SOLO) run += all;
+    else {
+      int64_t* part = reinterpret_cast<int64_t*>(l.acc + 48 + (turn++ & 1) * 8);   // (two sets, so that one barrier a step is enough)
+      if (lane == 63) part[wave] = all;
+      meet();
 #pragma unroll
-        for (int x = 0; x < WAVES; ++x) {
-          if (x < wave) start += part[x];
-          run += part[x];
-        }
+      for (int x = 0; x < WAVES; ++x) {
+        if (x < wave) start += part[x];
+        run += part[x];
       }
-      if (i < items) f(i, t, n, u, start);
     }
-    return run;
+    return start;
   };
-  // s[4x]: 1 + the item of wave x, or of all four; the place among its parts; parts of a unit; tiles
-  auto holds = [&](int x, int item, int place, int n, int t, int start) __attribute__((always_inline)) {
-    l.acc[4 * x] = 1 + item;
-    l.acc[4 * x + 1] = place;
-    l.acc[4 * x + 2] = n;
-    l.acc[4 * x + 3] = t;
-    l.acc[16 + x] = start;
-  };
-  const int parts = scan(
-      a.n_groups,
-      [&](int g, int& t, int& n, int& u) {
-        t = l.most_of[g] - l.least_of[g];
-        n = share_count(t, per);
-        u = t > 0 ? units_of(g) : 0;
-      },
-      [&](int g, int t, int n, int u, int start) {
-        if (w == 0) *reinterpret_cast<i32x4*>(a.rec + (int64_t)g * 4) = i32x4{start << a.col_shift, n, -1, l.cu[g]};
-        if (w >= start && w < start + n * u) holds(0, g, w - start, n, t, start);
-      });
-  if (tid == 0) l.acc[20] = parts;
+  int64_t run = 0;
+  for (int e = 0; e < a.n_groups; e += T) {
+    const int g = e + tid;
+    const bool real = g < a.n_groups;
+    const int t = real ? l.most_of[g] - l.least_of[g] : 0, n = share_count(t, per), all = t > 0 ? n * units_of(g) : 0;
+    const int start = (int)scan(all, run);
+    if (real && w == 0) *reinterpret_cast<i32x4*>(a.rec + (int64_t)g * 4) = i32x4{start << a.col_shift, n, l.cu[g], 0};
+    if (w >= start && w < start + all) {
+      l.acc[0] = 1 + g;
+      l.acc[1] = w - start;
+      l.acc[2] = n;
+      l.acc[3] = start;
+    }
+  }
+  const int parts = (int)run;
+  if (tid == 0) {
+    l.acc[16] = parts;
+    l.acc[17] = wave_per;
+    if (w == 0) a.rec[(int64_t)(a.n_groups + a.b) * 4] = wave_per;
+  }
   if (w > 0 && w < parts) return;   // (the first one goes on for the records)
-  scan(
-      a.b,
-      [&](int b, int& t, int& n, int& u) {
-        t = own_count(b);
-        n = share_count(t, wave_per);
-        u = own_units;
-      },
-      [&](int b, int t, int n, int u, int start) {
-        if (w == 0) *reinterpret_cast<i32x4*>(a.rec + (int64_t)(a.n_groups + b) * 4) = i32x4{a.own_rows + start * 16, n, l.group_of[b], 0};
+  run = 0;
+  for (int e = 0; e < a.b; e += T) {
+    const int b = e + tid;
+    const bool real = b < a.b;
+    const int64_t all = real ? (int64_t)counts[b] * own_units : 0, start = scan(all, run);
+    if (real && w == 0) {
+      const WaveTile at = wave_tile(start, wave_per);
+      *reinterpret_cast<i32x4*>(a.rec + (int64_t)(a.n_groups + b) * 4) = i32x4{at.wave, at.before, counts[b], l.group_of[b]};
+    }
 #pragma unroll
-        for (int x = 0; x < kShWaves; ++x) {
-          const int q = (w - parts) * kShWaves + x;
-          if (q >= start && q < start + n * u) holds(x, a.n_groups + b, q - start, n, t, start);
-        }
-      });
+    for (int x = 0; x < kShWaves; ++x) {
+      const int64_t from = ((int64_t)(w - parts) * kShWaves + x) * wave_per;
+      if (w >= parts && from >= start && from < start + all) {
+        l.acc[4 * x] = 1 + b;
+        l.acc[4 * x + 1] = (int)(from - start);
+      }
+    }
+  }
 }
 
-// What the wave does, from the plan's words; all waves, before they are overwritten.
-__device__ __forceinline__ Share share_of(const SharedArgs& a, int w, int* s, int wave) {
+// A group's part, from the plan's words; all waves, before they are overwritten.
+__device__ __forceinline__ Share group_share(const SharedArgs& a, int* s) {
   const PlanLds l(s);
   Share sh{};
-  const int parts = uni(l.acc[20]), x = w < parts ? 0 : wave, item = uni(l.acc[4 * x]) - 1;
-  if (item < 0) return sh;
-  const int place = uni(l.acc[4 * x + 1]), n = uni(l.acc[4 * x + 2]), t = uni(l.acc[4 * x + 3]), start = uni(l.acc[16 + x]);
-  const bool group = item < a.n_groups;
-  sh.kind = group ? 1 : 2;
-  const int b = group ? 0 : item - a.n_groups, g = group ? item : uni(l.group_of[b]);
-  const int c0 = g >= 0 ? uni(l.cu[g]) : b, c1 = g >= 0 ? min(uni(l.cu[g + 1]), a.b) : b;
-  const TileSpan sp = g >= 0 ? TileSpan{uni(l.least_of[g]), uni(l.most_of[g])} : TileSpan{0, 0};
-  const int shift = group ? a.col_shift : 4, width = 1 << shift, total = group ? (c1 - c0) * a.ratio : a.ratio, blocks = (total + width - 1) >> shift;
+  const int g = uni(l.acc[0]) - 1, place = uni(l.acc[1]), n = uni(l.acc[2]), start = uni(l.acc[3]);
+  const int c0 = uni(l.cu[g]), c1 = min(uni(l.cu[g + 1]), a.b), total = (c1 - c0) * a.ratio, blocks = (total + a.columns - 1) >> a.col_shift;
+  const int t0 = uni(l.least_of[g]), t = uni(l.most_of[g]) - t0;
   const UnitPart at = unit_part(place, n, a.hk, blocks);
+  sh.kind = 1;
+  sh.b = sh.leader = c0;
+  sh.hk = at.hk;
+  sh.col0 = at.block * a.columns;
+  sh.cols = min(a.columns, total - sh.col0);
+  sh.prefix = INT_MAX;
+  sh.row = (start + (at.hk * blocks + at.block) * n + at.part) << a.col_shift;
   sh.lo = share_start(t, n, at.part);
   sh.hi = share_start(t, n, at.part + 1);
-  sh.b = group ? c0 : b;
-  sh.leader = c0;
-  sh.hk = at.hk;
-  sh.col0 = at.block * width;
-  sh.cols = min(width, total - sh.col0);
-  sh.prefix = group ? INT_MAX : g >= 0 ? uni(l.prefix[g]) : 0;
-  sh.row = (group ? 0 : a.own_rows) + (start + (at.hk * blocks + at.block) * n + at.part) * width;
-  sh.alone = !group && n == 1 && sp.t0 == sp.t1;
-  const OwnTiles own = own_tiles(uni(l.len_of[b]), a.window, sp);
-  sh.own.lo = group ? 0 : own.lo;
-  sh.own.len = group ? INT_MAX : own.len;
-  sh.own.first = group ? sp.t0 : own.first;
-  sh.own.before = group ? INT_MAX : own.before;
-  sh.own.behind = own.behind;
+  sh.own = OwnTiles{0, INT_MAX, t0, INT_MAX, 0, 0};
   return sh;
+}
+
+// A wave's own tiles: from tile `off` of request b's (all its units', one behind another) on.
+struct Walk {
+  int b, off, left, number;   // left: tiles; number: of the wave
+};
+// The tiles that follow as far as they are of one unit; false: none do.
+__device__ __forceinline__ bool own_share(const SharedArgs& a, int* s, Walk& w, Share& sh) {
+  const PlanLds l(s);
+  if (w.b < 0 || w.left <= 0) return false;
+  const int lane = threadIdx.x & 63, own_units = a.hk * a.groups;
+  int count = uni(l.members[w.b]);
+  if (w.off == count * own_units) {   // the next request that has some
+    w.off = count = 0;
+    for (int b = w.b + 1; b < a.b; b += 64) {
+      const int i = min(b + lane, a.b - 1), n = l.members[i];
+      const uint64_t has = __builtin_amdgcn_ballot_w64(n > 0 && b + lane < a.b);
+      if (has) {
+        const int first = __builtin_ctzll(has);
+        w.b = b + first;
+        count = __builtin_amdgcn_readlane(n, first);
+        break;
+      }
+    }
+    if (count == 0) return false;
+  }
+  const int unit = (int)((uint32_t)w.off / (uint32_t)count), g = uni(l.group_of[w.b]);
+  const TileSpan sp = g >= 0 ? TileSpan{uni(l.least_of[g]), uni(l.most_of[g])} : TileSpan{0, 0};
+  sh.kind = 2;
+  sh.b = w.b;
+  sh.leader = g >= 0 ? uni(l.cu[g]) : w.b;
+  sh.hk = (int)((uint32_t)unit / (uint32_t)a.groups);
+  sh.col0 = (unit - sh.hk * a.groups) * 16;
+  sh.cols = min(16, a.ratio - sh.col0);
+  sh.prefix = g >= 0 ? uni(l.prefix[g]) : 0;
+  sh.row = a.own_rows + (w.number + w.b * own_units + unit) * 16;
+  sh.lo = w.off - unit * count;
+  sh.hi = min(count, sh.lo + w.left);
+  sh.alone = sh.lo == 0 && sh.hi == count && sp.t0 == sp.t1;
+  sh.own = own_tiles(uni(l.len_of[w.b]), a.window, sp);
+  w.off += sh.hi - sh.lo;
+  w.left -= sh.hi - sh.lo;
+  return true;
 }
 
 // Own tiles: 16 columns of request sh.b, or of a group that has a bad page, streamed by W waves,
@@ -481,9 +515,9 @@ template <int KG, int TB> constexpr int kShStages() { return KG * TB == 1 ? 4 : 
 constexpr int kShPages = 1024;
 
 template <int D, int RW, int KG, int TB> constexpr int kShLds() {
-  const int stages = kShStages<KG, TB>() * 2 * KG * 32 * TB * D * 2 + kShPages * 4, sums = (RW * KG * 16 * (D / 32) * 64 + RW * KG * 2 * 64 + 1) * 4, tiles = stages > sums ? stages : sums,
-            slices = kShWaves * kDecTile * (D * 2 + 32), plan = kShWords * 4;
-  return tiles > slices ? (tiles > plan ? tiles : plan) : slices > plan ? slices : plan;
+  const int stages = kShStages<KG, TB>() * 2 * KG * 32 * TB * D * 2 + kShPages * 4, sums = (RW * KG * 16 * (D / 32) * 64 + RW * KG * 2 * 64 + 1) * 4,
+            own = kShWords * 4 + kShWaves * kDecTile * (D * 2 + 32);
+  return stages > sums ? (stages > own ? stages : own) : sums > own ? sums : own;
 }
 
 // Shared tiles: 32·RW columns by KG key groups of TB tiles a step. True if a page was none of
@@ -781,19 +815,18 @@ __global__ __launch_bounds__(kShThreads) __attribute__((amdgpu_waves_per_eu(kShP
 void shared_decode_kernel(const SharedArgs a) {
   __shared__ __align__(16) uint8_t lds[kShLds<D, RW, KG, TB>()];
   __shared__ float sM[kShWaves][16], sL[kShWaves][16];
+  __shared__ Share shares[kShWaves];
   int* words = reinterpret_cast<int*>(lds);
   const int wave = uni(threadIdx.x >> 6);
   if (a.n_groups + a.b <= 128) {
     if (wave == 0) find_share<64>(a, blockIdx.x, words);
   } else find_share<kShThreads>(a, blockIdx.x, words);
   __syncthreads();
-  __shared__ Share shares[kShWaves];
-  {
-    const Share sh = share_of(a, blockIdx.x, words, wave);
+  // (each way keeps its share in LDS, and reads it and the arguments again: held from here on they would spill)
+  auto keep = [&](const Share& sh) __attribute__((always_inline)) {
     if (threadIdx.x % 64 == 0) shares[wave] = sh;
-  }
-  __syncthreads();   // the plan's words are read
-  // (each way reads its share and the arguments again: held from here on they would spill)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  };
   auto share = [&]() __attribute__((always_inline)) {
     static_assert(sizeof(Share) % 4 == 0, "words");
     struct Words { int x[sizeof(Share) / 4]; } x;
@@ -801,17 +834,24 @@ void shared_decode_kernel(const SharedArgs a) {
     for (int i = 0; i < (int)(sizeof(Share) / 4); ++i) x.x[i] = uni(reinterpret_cast<const int*>(&shares[wave])[i]);
     return bitcast<Share>(x);
   };
-  const int kind = uni(shares[wave].kind);
-  if (kind == 0) return;
-  uint8_t* sv = lds + wave * Stream<D, BF16>::kSlice;
-  if (kind == 2) {
-    kernarg<SharedArgs>& z = reload_kernarg(a);
-    const Share sh = share();
-    Stream<D, BF16> st;
-    st.run(z, sh, sh.col0, sh.cols, 0, 1, sv);
-    st.store(z, sh);
+  uint8_t* slices = lds + kShWords * 4;
+  const int parts = uni(words[16]), number = ((int)blockIdx.x - parts) * kShWaves + wave;
+  if (number >= 0) {
+    Walk at{uni(words[4 * wave]) - 1, uni(words[4 * wave + 1]), uni(words[17]), number};
+    Share next{};
+#pragma unroll 1
+    while (own_share(a, words, at, next)) {
+      keep(next);
+      kernarg<SharedArgs>& z = reload_kernarg(a);
+      const Share sh = share();
+      Stream<D, BF16> st;
+      st.run(z, sh, sh.col0, sh.cols, 0, 1, slices + wave * Stream<D, BF16>::kSlice);
+      st.store(z, sh);
+    }
     return;
   }
+  keep(group_share(a, words));
+  __syncthreads();   // the plan's words are read
   if (!group_part<D, BF16, RW, KG, TB>(reload_kernarg(a), share(), lds)) return;
   // a page outside the cache hides its keys, which only the stream can
   __syncthreads();
@@ -821,8 +861,8 @@ void shared_decode_kernel(const SharedArgs a) {
     const Share sh = share();
     const int cols = min(16, sh.cols - c);
     Stream<D, BF16> st;
-    st.run(z, sh, sh.col0 + c, cols, wave, kShWaves, sv);
-    st.join(reload_kernarg(a), share(), c, cols, lds, sM, sL);
+    st.run(z, sh, sh.col0 + c, cols, wave, kShWaves, slices + wave * Stream<D, BF16>::kSlice);
+    st.join(reload_kernarg(a), share(), c, cols, slices, sM, sL);
   }
 }
 
@@ -833,13 +873,18 @@ struct Parts {
 };
 __device__ __forceinline__ Parts parts_of(const SharedArgs& a, int b, int h) {
   const int hk = h / a.ratio, n = h - hk * a.ratio;
-  const int* rec = a.rec + (int64_t)(a.n_groups + b) * 4;
-  Parts p{0, rec[1], 0, 0};
-  const int group = rec[2];
-  p.at1 = rec[0] + (hk * a.groups + n / 16) * p.own * 16 + n % 16;
+  const i32x4 rec = *reinterpret_cast<const i32x4*>(a.rec + (int64_t)(a.n_groups + b) * 4);
+  const uint32_t per = a.rec[(int64_t)(a.n_groups + a.b) * 4];
+  Parts p{0, 0, 0, 0};
+  const int count = rec[2], group = rec[3], unit = hk * a.groups + n / 16;
+  if (count > 0) {
+    const uint32_t from = (uint32_t)rec[1] + (uint32_t)(unit * count), w0 = from / per, w1 = (from + (uint32_t)count - 1) / per;
+    p.own = (int)(w1 - w0) + 1;
+    p.at1 = a.own_rows + (rec[0] + (int)w0 + b * a.hk * a.groups + unit) * 16 + n % 16;
+  }
   if (group >= 0 && a.lens[b] > 0 && a.cols > 0) {
     const int* r = a.rec + (int64_t)group * 4;
-    const int first = r[3], end = min(a.cu[group + 1], a.b);
+    const int first = r[2], end = min(a.cu[group + 1], a.b);
     const int blocks = ((end - first) * a.ratio + a.columns - 1) / a.columns, col = (b - first) * a.ratio + n;
     p.shared = r[1];
     p.at0 = r[0] + (hk * blocks + col / a.columns) * p.shared * a.columns + col % a.columns;

@@ -52,29 +52,44 @@ int main() {
   }
   REQUIRE(own_tiles(1 << 30, kNoWindow, TileSpan{0, 0}).count == 1 << 25);
   for (int round = 0; round < 4000; ++round) {
-    const int items = pick(1, 60), groups = pick(0, items), target = pick(1, 1024), least = pick(1, 16), wave_least = pick(1, 4);
+    const int items = pick(1, 60), groups = pick(0, items), target = pick(128, 1024), ways = 1 << pick(0, 2), weight = own_weight(128 / ways);
     std::vector<int> tiles(items), units(items);
-    int64_t sum = 0, of_groups = 0, of_requests = 0, units_g = 0, units_r = 0;
+    int64_t sum = 0, of_groups = 0, own = 0, units_g = 0, units_r = 0;
     for (int i = 0; i < items; ++i) {
       tiles[i] = pick(0, 3) ? pick(0, 3000) : pick(0, 3) ? 0 : 1 << pick(0, 25);
       units[i] = pick(1, 64);
-      sum += (int64_t)tiles[i] * units[i];
+      sum += (int64_t)tiles[i] * units[i] * (i < groups ? 4 / ways : weight);
       (i < groups ? units_g : units_r) += units[i];
     }
-    const int per = share_size(sum, target, least), wave_per = wave_share_size(per, wave_least);
-    REQUIRE(per >= least && wave_per >= wave_least);
+    const int steps = share_steps(sum, target), per = share_size(steps, ways), wave_per = wave_share_size(steps, weight);
+    REQUIRE(steps >= 1 && per >= 4 && per >= steps * ways && wave_per >= 2 && wave_per * weight >= steps);
+    int last = -1, unit = 0;   // of requests: the last part's row
     for (int i = 0; i < items; ++i) {
-      const int size = i < groups ? per : wave_per, n = share_count(tiles[i], size);
-      (i < groups ? of_groups : of_requests) += (int64_t)n * units[i];
-      REQUIRE((n == 0) == (tiles[i] == 0));
-      for (int p = 0; p < n; ++p) {
-        const int a = share_start(tiles[i], n, p), b = share_start(tiles[i], n, p + 1);
-        REQUIRE(a < b && b - a <= size);
+      if (i < groups) {
+        const int n = share_count(tiles[i], per);
+        of_groups += (int64_t)n * units[i];
+        REQUIRE((n == 0) == (tiles[i] == 0));
+        for (int p = 0; p < n; ++p) {
+          const int a = share_start(tiles[i], n, p), b = share_start(tiles[i], n, p + 1);
+          REQUIRE(a < b && b - a <= per);
+        }
+        if (n) REQUIRE(share_start(tiles[i], n, 0) == 0 && share_start(tiles[i], n, n) == tiles[i]);
+        continue;
       }
-      if (n) REQUIRE(share_start(tiles[i], n, 0) == 0 && share_start(tiles[i], n, n) == tiles[i]);
+      const WaveTile at = wave_tile(own, wave_per);
+      REQUIRE(at.wave == own / wave_per && at.before == own % wave_per);
+      for (int u = 0; u < units[i]; ++u, ++unit) {
+        if (tiles[i] == 0) continue;
+        const uint32_t from = (uint32_t)at.before + (uint32_t)u * (uint32_t)tiles[i];
+        const int first = at.wave + (int)(from / wave_per) + unit, end = at.wave + (int)((from + (uint32_t)tiles[i] - 1) / wave_per) + unit;
+        REQUIRE(first > last && end >= first);   // a part's row is its own
+        last = end;
+      }
+      own += (int64_t)tiles[i] * units[i];
     }
-    REQUIRE(of_groups + (of_requests + 3) / 4 <= target + units_g + (units_r + 3) / 4 + 1);
-    REQUIRE(of_groups <= target + units_g && of_requests <= 4 * (int64_t)target + units_r);   // rows of partial sums
+    const int64_t waves = (own + wave_per - 1) / wave_per;
+    REQUIRE(of_groups + (waves + 3) / 4 <= target + units_g + 1);
+    REQUIRE(of_groups <= target + units_g && last < waves + units_r && waves <= 4 * ((int64_t)target + 1));   // rows of partial sums
   }
   for (int round = 0; round < 4000; ++round) {   // a unit's parts: each once, eight at a time next to those of the other blocks
     const int n = pick(1, 40), heads = pick(1, 9), blocks = pick(1, 9), all = heads * n;
