@@ -45,7 +45,7 @@ MI355_HD inline int own_tile(const OwnTiles& o, int i) { return i < o.before ? o
 // A workgroup's steps where `sum` waves' tiles are to be read (a group's tile by a wave for each
 // 32 columns, a request's own as own_weight of them) and about `target` workgroups of four waves
 // wanted; a group's part of them, whose waves take `ways` tiles a step, of at least 4 tiles; and
-// a wave's own tiles, of at least 2. At most target + 1 workgroups, and one for each group's
+// a wave's own tiles. At most target + 1 workgroups, and one for each group's
 // unit, come of it.
 // An own tile costs more than a shared one: a wave waits for each unit's first. Measured, for
 // weights of 1, 2, 3, 4, 6: 9 groups of 32 columns 35.4, 28.2, 31.3, 32.2, 40.2 us, one of 1020
@@ -53,7 +53,7 @@ MI355_HD inline int own_tile(const OwnTiles& o, int i) { return i < o.before ? o
 MI355_HD inline int own_weight(int columns) { return imax(columns / 32, 2); }
 MI355_HD inline int share_steps(int64_t sum, int target) { return (int)((double)sum / (4.0 * target)) + 1; }
 MI355_HD inline int share_size(int steps, int ways) { return imax(steps * ways, 4); }
-MI355_HD inline int wave_share_size(int steps, int weight) { return imax((steps + weight - 1) / weight, 2); }
+MI355_HD inline int wave_share_size(int steps, int weight) { return imax((steps + weight - 1) / weight, 1); }
 MI355_HD inline int share_count(int tiles, int per) { return (tiles + per - 1) / per; }   // 0 of no tiles
 // Part p of n takes tiles [share_start(p), share_start(p + 1)).
 MI355_HD inline int share_start(int tiles, int n, int p) {

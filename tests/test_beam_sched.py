@@ -62,7 +62,7 @@ int main() {
       (i < groups ? units_g : units_r) += units[i];
     }
     const int steps = share_steps(sum, target), per = share_size(steps, ways), wave_per = wave_share_size(steps, weight);
-    REQUIRE(steps >= 1 && per >= 4 && per >= steps * ways && wave_per >= 2 && wave_per * weight >= steps);
+    REQUIRE(steps >= 1 && per >= 4 && per >= steps * ways && wave_per >= 1 && wave_per * weight >= steps);
     int last = -1, unit = 0;   // of requests: the last part's row
     for (int i = 0; i < items; ++i) {
       if (i < groups) {
