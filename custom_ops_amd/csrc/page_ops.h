@@ -4,12 +4,14 @@
 // Which pages are in use follows from the table alone: a bit a page. The first kernel's
 // workgroups each take some rows, set the bits of their pages in LDS and write their
 // bitmaps down; the second's all join the bitmaps, so that each has the whole, and form
-// the running count of bits from which a page's rank, and the page of a rank, follow.
+// the running count of bits from which a page's rank, and the page of a rank, follow. Few
+// rows are one workgroup's, which does both.
 // Bound: the bytes of the tables, and for small ones two launches.
 
 constexpr int kPgThreads = 1024;
 constexpr int kPgRows = 4096;            // rows of a fork: a bit each, and a hash of their last pages
 constexpr int kPgHash = 2 * kPgRows;
+constexpr int kPgColumns = 256;          // of a row, that a wave compacts at once
 
 struct PageArgs {
   const int* table_in;
@@ -26,7 +28,7 @@ struct PageArgs {
   uint32_t* maps;        // [marks][2][words]: pages of any kind; of whole ones and held
   int64_t ts;
   int n, r, cols, pages, page, n_held;
-  int words;             // of a bitmap: pages / 32, up
+  int words;             // of a bitmap: pages / 32, up to a multiple of 4
   int marks;             // workgroups of the first kernel
 };
 
@@ -40,52 +42,72 @@ __device__ __forceinline__ int old_row(const PageArgs& a, int i, int& len) {
   return real ? row : -1;
 }
 
-// Rows of each workgroup: marks of their pages, and for a fork the new table.
-template <bool FORK>
-__global__ __launch_bounds__(kPgThreads) void page_mark_kernel(const PageArgs a) {
-  extern __shared__ uint32_t bits[];   // [2][words]
-  uint32_t* any = bits;
-  uint32_t* whole = bits + a.words;
-  const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6), wgs = gridDim.x;
-  for (int i = tid; i < 2 * a.words; i += kPgThreads) bits[i] = 0;
-  __syncthreads();
-  if (blockIdx.x == 0)
+// Marks of the pages of rows first, first + step, .. (a wave each) and of the held ones, for a
+// fork of whole ones apart, and of a fork the new table. Bitmaps: cleared, of whole ones behind any.
+template <bool FORK> __device__ __forceinline__ void mark_rows(const PageArgs& a, uint32_t* any, uint32_t* whole, int first, int step, bool held) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
+  if (held)
     for (int i = tid; i < a.n_held; i += kPgThreads) {
       const int p = a.held[i];
       if (p >= 0 && p < a.pages) {
         atomicOr(&any[p >> 5], 1u << (p & 31));
-        atomicOr(&whole[p >> 5], 1u << (p & 31));
+        if (FORK) atomicOr(&whole[p >> 5], 1u << (p & 31));
       }
     }
-  // a wave a row
-  for (int i = blockIdx.x * (kPgThreads / 64) + wave; i < a.r; i += wgs * (kPgThreads / 64)) {
+  for (int i = first + wave; i < a.r; i += step) {
     int len;
     const int row = old_row(a, i, len);
     const int used = (int)(((int64_t)len + a.page - 1) / a.page), full = len / a.page;
     const int* from = a.table_in + (int64_t)max(row, 0) * a.ts;
     int* to = a.table + (int64_t)i * a.cols;
-    for (int c = lane; c < (FORK ? a.cols : used); c += 64) {
-      int p = c < used ? from[c] : -1;
-      if (p >= a.pages) p = -1;
-      if (p >= 0) {
-        atomicOr(&any[p >> 5], 1u << (p & 31));
-        if (FORK && c < full) atomicOr(&whole[p >> 5], 1u << (p & 31));
+    for (int c0 = lane; c0 < (FORK ? a.cols : used); c0 += 256) {
+      int p[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[e] = c0 + e * 64 < used ? from[c0 + e * 64] : -1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int c = c0 + e * 64, x = p[e] >= 0 && p[e] < a.pages ? p[e] : -1;
+        if (x >= 0) {
+          atomicOr(&any[x >> 5], 1u << (x & 31));
+          if (FORK && c < full) atomicOr(&whole[x >> 5], 1u << (x & 31));
+        }
+        if (FORK && c < a.cols) to[c] = x;
       }
-      if (FORK) to[c] = p < 0 ? -1 : p;
     }
   }
   __syncthreads();
+}
+
+template <bool FORK>
+__global__ __launch_bounds__(kPgThreads) void page_mark_kernel(const PageArgs a) {
+  extern __shared__ __align__(16) uint32_t bits[];   // [2][words]
+  const int tid = threadIdx.x;
+  for (int i = tid; i < (FORK ? 2 : 1) * a.words; i += kPgThreads) bits[i] = 0;
+  __syncthreads();
+  mark_rows<FORK>(a, bits, bits + a.words, blockIdx.x * (kPgThreads / 64), gridDim.x * (kPgThreads / 64), blockIdx.x == 0);
   uint32_t* out = a.maps + (int64_t)blockIdx.x * 2 * a.words;
   for (int i = tid; i < (FORK ? 2 : 1) * a.words; i += kPgThreads) out[i] = bits[i];
 }
 
-// The bitmap of all workgroups.
+// The bitmap of all workgroups: a thread takes 16 bytes of every so many of them, 16 asked for at once.
 __device__ __forceinline__ void joined(const PageArgs& a, int which, uint32_t* bits) {
-  for (int i = threadIdx.x; i < a.words; i += kPgThreads) {
-    uint32_t x = 0;
-#pragma unroll 8
-    for (int m = 0; m < a.marks; ++m) x |= a.maps[((int64_t)m * 2 + which) * a.words + i];
-    bits[i] = x;
+  for (int i = threadIdx.x; i < a.words; i += kPgThreads) bits[i] = 0;
+  __syncthreads();
+  const int quads = a.words / 4, ways = max(1, min(kPgThreads / quads, a.marks));
+  for (int x = threadIdx.x; x < quads * ways; x += kPgThreads) {
+    const int m0 = (int)((uint32_t)x / (uint32_t)quads), q = x - m0 * quads;
+    const u32x4* from = reinterpret_cast<const u32x4*>(a.maps + (int64_t)which * a.words) + q;
+    u32x4 y = {0u, 0u, 0u, 0u};
+    for (int m = m0; m < a.marks; m += 16 * ways) {
+      u32x4 z[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) z[e] = from[(int64_t)min(m + e * ways, a.marks - 1) * 2 * quads];   // (the last one's bits belong in all)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) y |= z[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (y[e]) atomicOr(&bits[q * 4 + e], y[e]);
   }
   __syncthreads();
 }
@@ -122,36 +144,71 @@ __device__ __forceinline__ int ranks(const uint32_t* bits, int* before, int word
 __device__ __forceinline__ int rank_of(const uint32_t* bits, const int* before, int p) {
   return before[p >> 5] + __builtin_popcount(bits[p >> 5] & ((1u << (p & 31)) - 1u));
 }
-// The page of the j-th clear bit (j below their number).
-__device__ __forceinline__ int clear_of(const uint32_t* bits, const int* before, int words, int j) {
-  int lo = 0, hi = words - 1;   // the last word with at most j clear bits below it
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (32 * mid - before[mid] <= j) lo = mid;
-    else hi = mid - 1;
+// Where every 64th clear bit lies: the word of the (64·i)-th in start[i], and behind the last
+// one the last word (a bitmap's words / 2 + 1 of them). All threads.
+__device__ __forceinline__ void clear_index(const uint32_t* bits, const int* before, int words, uint16_t* start) {
+  const int all = 32 * words - before[words - 1] - __builtin_popcount(bits[words - 1]);
+  for (int i = threadIdx.x; i < words; i += kPgThreads) {
+    const int c0 = 32 * i - before[i], c1 = c0 + 32 - __builtin_popcount(bits[i]), at = (c0 + 63) / 64;
+    if (at * 64 < c1) start[at] = (uint16_t)i;   // (32 at most: one, if any)
   }
-  uint32_t x = ~bits[lo];
-  for (int left = j - (32 * lo - before[lo]); left > 0; --left) x &= x - 1;
-  return 32 * lo + __builtin_ctz(x);
+  if (threadIdx.x == 0) start[(all + 63) / 64] = (uint16_t)(words - 1);
+  __syncthreads();
+}
+// j: in, which clear bit of [0, their number); out, its page. N at once, so that their steps wait
+// for LDS together.
+template <int N> __device__ __forceinline__ void clear_of(const uint32_t* bits, const int* before, const uint16_t* start, int (&j)[N]) {
+  int lo[N], hi[N];   // the last word with at most j clear bits below it is of [lo, hi]
+  bool more = false;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    lo[e] = start[j[e] >> 6];
+    hi[e] = start[(j[e] >> 6) + 1];
+    more |= lo[e] < hi[e];
+  }
+  while (__builtin_amdgcn_ballot_w64(more)) {
+    more = false;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int mid = (lo[e] + hi[e] + 1) / 2;
+      const bool up = 32 * mid - before[mid] <= j[e];
+      lo[e] = up ? mid : lo[e];
+      hi[e] = up || lo[e] == hi[e] ? hi[e] : mid - 1;
+      more |= lo[e] < hi[e];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+  // the bit of its word by halves
+    uint32_t x = ~bits[lo[e]];
+    int left = j[e] - (32 * lo[e] - before[lo[e]]), at = 0;
+#pragma unroll
+    for (int half = 16; half; half /= 2) {
+      const int low = __builtin_popcount(x & ((1u << half) - 1u));
+      const bool up = left >= low;
+      left -= up ? low : 0;
+      at += up ? half : 0;
+      x >>= up ? half : 0;
+    }
+    j[e] = 32 * lo[e] + at;
+  }
 }
 
 // What a fork adds to the table: pages for the rows that cannot keep their last one. All
 // workgroups find the same; the first writes the rows' results, each its share of the free pages.
+// ONE: the only workgroup, which marks the rows itself.
+template <bool ONE>
 __global__ __launch_bounds__(kPgThreads) void page_fork_kernel(const PageArgs a) {
-  extern __shared__ uint32_t bits[];   // [words] of whole pages, then of any; beside it a hash, then [words] ranks
+  extern __shared__ __align__(16) uint32_t bits[];   // [words] of whole pages, then of any; beside it a hash, then [words] ranks and where to look for clear bits
   __shared__ uint32_t wants[kPgRows / 32];
   __shared__ int wants_before[kPgRows / 32], sums[kPgThreads / 64];
   int* key = reinterpret_cast<int*>(bits + a.words);
   int* low = key + kPgHash;
   int* before = key;
+  uint16_t* start = reinterpret_cast<uint16_t*>(before + a.words);
+  uint32_t* any = ONE ? bits + a.words + 2 * kPgHash : bits;
   const int tid = threadIdx.x;
-  for (int i = tid; i < kPgHash; i += kPgThreads) {
-    key[i] = -1;
-    low[i] = INT_MAX;
-  }
-  for (int i = tid; i < kPgRows / 32; i += kPgThreads) wants[i] = 0;
-  joined(a, 1, bits);
-  // each row's last page, if it is partly filled: the lowest row of those that have it so
+  // each row's last page, if it is partly filled (asked for first, and met behind the bitmaps)
   constexpr int E = kPgRows / kPgThreads;
   int page[E], place[E], col[E];
 #pragma unroll
@@ -166,9 +223,24 @@ __global__ __launch_bounds__(kPgThreads) void page_fork_kernel(const PageArgs a)
       if (len % a.page) {
         col[e] = len / a.page;
         page[e] = a.table_in[(int64_t)row * a.ts + col[e]];
-        if (page[e] >= a.pages) page[e] = -1;
       }
     }
+  }
+  for (int i = tid; i < kPgHash; i += kPgThreads) {
+    key[i] = -1;
+    low[i] = INT_MAX;
+  }
+  for (int i = tid; i < kPgRows / 32; i += kPgThreads) wants[i] = 0;
+  if constexpr (ONE) {
+    for (int i = tid; i < a.words; i += kPgThreads) any[i] = bits[i] = 0;
+    __syncthreads();
+    mark_rows<true>(a, any, bits, 0, kPgThreads / 64, true);
+  } else joined(a, 1, bits);
+  // the lowest row of those that have a page so
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int i = e * kPgThreads + tid;
+    if (page[e] >= a.pages) page[e] = -1;
     if (page[e] >= 0) {
       uint32_t h = ((uint32_t)page[e] * 2654435761u) >> 19;   // 13 bits
       for (;;) {
@@ -189,9 +261,10 @@ __global__ __launch_bounds__(kPgThreads) void page_fork_kernel(const PageArgs a)
   }
   __syncthreads();
   const int wanted = ranks(wants, wants_before, kPgRows / 32, sums);
-  joined(a, 0, bits);
-  const int used = ranks(bits, before, a.words, sums), left = a.pages - used, taken = min(wanted, left);
+  if constexpr (!ONE) joined(a, 0, any);
+  const int used = ranks(any, before, a.words, sums), left = a.pages - used, taken = min(wanted, left);
   if (blockIdx.x == 0) {
+    clear_index(any, before, a.words, start);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int i = e * kPgThreads + tid;
@@ -200,8 +273,10 @@ __global__ __launch_bounds__(kPgThreads) void page_fork_kernel(const PageArgs a)
       if (wants[i >> 5] >> (i & 31) & 1) {
         const int nth = rank_of(wants, wants_before, i);
         if (nth < left) {
+          int x[1] = {nth};
+          clear_of(any, before, start, x);
           from = page[e];
-          to = clear_of(bits, before, a.words, nth);
+          to = x[0];
         }
         a.table[(int64_t)i * a.cols + col[e]] = to;
       }
@@ -215,29 +290,73 @@ __global__ __launch_bounds__(kPgThreads) void page_fork_kernel(const PageArgs a)
     }
   }
   for (int p = blockIdx.x * kPgThreads + tid; p < a.pages; p += gridDim.x * kPgThreads) {
-    if (!(bits[p >> 5] >> (p & 31) & 1)) {
-      const int nth = p - rank_of(bits, before, p) - taken;
+    if (!(any[p >> 5] >> (p & 31) & 1)) {
+      const int nth = p - rank_of(any, before, p) - taken;
       if (nth >= 0) a.free_pages[nth] = p;
     }
     if (p >= left - taken) a.free_pages[p] = -1;
   }
 }
 
-// The new numbers, the moves, and the table by them; each workgroup its shares.
+// The new numbers, the moves, and the table by them; each workgroup its shares. ONE: as above.
+template <bool ONE>
 __global__ __launch_bounds__(kPgThreads) void page_compact_kernel(const PageArgs a) {
-  extern __shared__ uint32_t bits[];   // [words], [words] ranks
+  extern __shared__ __align__(16) uint32_t bits[];   // [words], [words] ranks, and where to look for clear bits
   __shared__ int sums[kPgThreads / 64];
   int* before = reinterpret_cast<int*>(bits + a.words);
   const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
-  joined(a, 0, bits);
+  // Rows of the table, kPgColumns columns a wave at once; the first are asked for before others' bitmaps.
+  const int chunks = (a.cols + kPgColumns - 1) / kPgColumns, units = a.n * chunks, step = gridDim.x * (kPgThreads / 64);
+  int w = blockIdx.x * (kPgThreads / 64) + wave, p[kPgColumns / 64];
+  auto load = [&]() __attribute__((always_inline)) {
+    if (w >= units) return;
+    const int i = (int)((uint32_t)w / (uint32_t)chunks), c0 = (w - i * chunks) * kPgColumns + lane;
+    int len;
+    old_row(a, i, len);
+    const int held = (int)(((int64_t)len + a.page - 1) / a.page);
+#pragma unroll
+    for (int e = 0; e < kPgColumns / 64; ++e) {
+      const int c = c0 + e * 64;
+      p[e] = c < held ? a.table_in[(int64_t)i * a.ts + c] : -1;
+    }
+  };
+  auto next = [&]() __attribute__((always_inline)) {
+    w += step;
+    load();
+  };
+  if constexpr (ONE) {
+    for (int i = tid; i < a.words; i += kPgThreads) bits[i] = 0;
+    __syncthreads();
+    mark_rows<false>(a, bits, nullptr, 0, kPgThreads / 64, true);
+    load();   // (from the cache by now)
+  } else {
+    load();
+    joined(a, 0, bits);
+  }
   const int used = ranks(bits, before, a.words, sums);
+  uint16_t* start = reinterpret_cast<uint16_t*>(before + a.words);
+  clear_index(bits, before, a.words, start);
   const int stay = used < a.pages ? rank_of(bits, before, used) : used, moved = used - stay;   // pages below `used`
-  auto number = [&](int p) {
-    if (!(bits[p >> 5] >> (p & 31) & 1)) return -1;
-    return p < used ? p : clear_of(bits, before, a.words, rank_of(bits, before, p) - stay);
+  // The new numbers of N pages (-1: none): those below `used` stay, the others fill the gaps there.
+  auto numbers = [&](auto& p) __attribute__((always_inline)) {
+    constexpr int N = sizeof(p) / sizeof(int);
+    int j[N];
+    bool gap = false;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      if (p[e] < 0 || p[e] >= a.pages || !(bits[p[e] >> 5] >> (p[e] & 31) & 1)) p[e] = -1;
+      j[e] = p[e] < used ? 0 : rank_of(bits, before, p[e]) - stay;
+      gap |= p[e] >= used;
+    }
+    if (!__builtin_amdgcn_ballot_w64(gap)) return;
+    clear_of(bits, before, start, j);
+#pragma unroll
+    for (int e = 0; e < N; ++e) p[e] = p[e] < used ? p[e] : j[e];
   };
   for (int p = blockIdx.x * kPgThreads + tid; p < a.pages; p += gridDim.x * kPgThreads) {
-    const int to = number(p);
+    int x[1] = {p};
+    numbers(x);
+    const int to = x[0];
     a.remap[p] = to;
     if (p >= used && to >= 0) {
       const int j = rank_of(bits, before, p) - stay;
@@ -251,13 +370,13 @@ __global__ __launch_bounds__(kPgThreads) void page_compact_kernel(const PageArgs
     a.counts[0] = used;
     a.counts[1] = moved;
   }
-  for (int i = blockIdx.x * (kPgThreads / 64) + wave; i < a.n; i += gridDim.x * (kPgThreads / 64)) {
-    int len;
-    old_row(a, i, len);
-    const int held = (int)(((int64_t)len + a.page - 1) / a.page);
-    for (int c = lane; c < a.cols; c += 64) {
-      const int p = c < held ? a.table_in[(int64_t)i * a.ts + c] : -1;
-      a.table[(int64_t)i * a.cols + c] = p >= 0 && p < a.pages ? number(p) : -1;
+  for (; w < units; next()) {
+    numbers(p);
+    const int i = (int)((uint32_t)w / (uint32_t)chunks), c0 = (w - i * chunks) * kPgColumns + lane;
+#pragma unroll
+    for (int e = 0; e < kPgColumns / 64; ++e) {
+      const int c = c0 + e * 64;
+      if (c < a.cols) a.table[(int64_t)i * a.cols + c] = p[e];
     }
   }
 }
