@@ -304,18 +304,19 @@ __global__ __launch_bounds__(kPgThreads) void page_compact_kernel(const PageArgs
   extern __shared__ __align__(16) uint32_t bits[];   // [words], [words] ranks, and where to look for clear bits
   __shared__ int sums[kPgThreads / 64];
   int* before = reinterpret_cast<int*>(bits + a.words);
+  constexpr int C = ONE ? 64 : kPgColumns;   // (few rows are bound by the code they fetch)
   const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
-  // Rows of the table, kPgColumns columns a wave at once; the first are asked for before others' bitmaps.
-  const int chunks = (a.cols + kPgColumns - 1) / kPgColumns, units = a.n * chunks, step = gridDim.x * (kPgThreads / 64);
-  int w = blockIdx.x * (kPgThreads / 64) + wave, p[kPgColumns / 64];
+  // Rows of the table, C columns a wave at once; the first are asked for before others' bitmaps.
+  const int chunks = (a.cols + C - 1) / C, units = a.n * chunks, step = gridDim.x * (kPgThreads / 64);
+  int w = blockIdx.x * (kPgThreads / 64) + wave, p[C / 64];
   auto load = [&]() __attribute__((always_inline)) {
     if (w >= units) return;
-    const int i = (int)((uint32_t)w / (uint32_t)chunks), c0 = (w - i * chunks) * kPgColumns + lane;
+    const int i = (int)((uint32_t)w / (uint32_t)chunks), c0 = (w - i * chunks) * C + lane;
     int len;
     old_row(a, i, len);
     const int held = (int)(((int64_t)len + a.page - 1) / a.page);
 #pragma unroll
-    for (int e = 0; e < kPgColumns / 64; ++e) {
+    for (int e = 0; e < C / 64; ++e) {
       const int c = c0 + e * 64;
       p[e] = c < held ? a.table_in[(int64_t)i * a.ts + c] : -1;
     }
@@ -372,9 +373,9 @@ __global__ __launch_bounds__(kPgThreads) void page_compact_kernel(const PageArgs
   }
   for (; w < units; next()) {
     numbers(p);
-    const int i = (int)((uint32_t)w / (uint32_t)chunks), c0 = (w - i * chunks) * kPgColumns + lane;
+    const int i = (int)((uint32_t)w / (uint32_t)chunks), c0 = (w - i * chunks) * C + lane;
 #pragma unroll
-    for (int e = 0; e < kPgColumns / 64; ++e) {
+    for (int e = 0; e < C / 64; ++e) {
       const int c = c0 + e * 64;
       if (c < a.cols) a.table[(int64_t)i * a.cols + c] = p[e];
     }
