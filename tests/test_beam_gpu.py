@@ -252,6 +252,98 @@ def test_shared_most_requests(ops):
         check(b[i:i + 1], want, tol)
 
 
+# Columns of a KV head of a group of 5: a workgroup of 32, 64 or 128 of them.
+@pytest.mark.parametrize("H", [8, 16, 32])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("page", [8, 16, 32, 128])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_shared_shapes(ops, H, d, page, dtype):
+    x = batch(H + d + page, [(330, 5), (140, 5)], 60, H, 2, d, page, DT[dtype], alone=1)
+    shared(ops, x)
+    slopes = torch.tensor([2.0 ** (-8 * (h + 1) / H) for h in range(H)], device="cuda")
+    shared(ops, x, softcap=20.0, window=250, slopes=slopes)
+
+
+@pytest.mark.parametrize("H", [8, 16, 32])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("page", [8, 64])
+def test_shared_bad_pages_of_shapes(ops, H, d, page):
+    """In the first group's prefix, in the other's only for one request."""
+    x = batch(H + d, [(330, 5), (200, 5)], 60, H, 2, d, page, torch.bfloat16)
+    x["table"][0, 2], x["table"][7, 200 // page] = -1, 10 ** 6
+    shared(ops, x)
+    shared(ops, x, softcap=15.0, window=290)
+
+
+def means(x, lens, cu, prefix):
+    """O where all scores are equal: the mean of V, [B, Hk, d]."""
+    page, out = x["vc"].shape[2], []
+    for b, n in enumerate(lens):
+        g = next((i for i in range(len(prefix)) if cu[i] <= b < cu[i + 1]), None)
+        j = torch.arange(n, device="cuda")
+        row = torch.where(j < (0 if g is None else prefix[g]), 0 if g is None else cu[g], b)
+        at = x["table"][row, j // page].long() * page + j % page
+        times = torch.bincount(at, minlength=x["vc"].shape[0] * page).double()
+        v = x["vc"].double().transpose(1, 2).reshape(len(times), -1)
+        out.append(times @ v / n)
+    return torch.stack(out).reshape(len(lens), x["vc"].shape[1], -1)
+
+
+@pytest.mark.parametrize("ratio,B,Hk,prefix", [(1, 2, 32, 80000), (16, 3, 32, 280000), (16, 8, 32, 260000)])
+def test_shared_long_parts(ops, ratio, B, Hk, prefix):
+    """Parts of more pages than the kernel holds the numbers of at once; V are small integers and all
+    scores equal, so that 32-bit sums are exact and what is read shows."""
+    g, page, P, d = gen(B), 8, 300, 128
+    lens = [prefix + 100 * b + 1 for b in range(B)]
+    table = torch.randint(0, P // 2, (B, max(lens) // page + 1), generator=g, device="cuda").int()
+    table[:, 3 * table.shape[1] // 4:] += P // 2
+    vc = torch.randint(-3, 4, (P, Hk, page, d), generator=g, device="cuda").bfloat16()
+    vc[P // 2:] += 5
+    kc = torch.randn(P, Hk, page, d, generator=g, device="cuda").bfloat16()
+    q = torch.zeros(B, Hk * ratio, d, dtype=torch.bfloat16, device="cuda")
+    out = ops.mha_shared_decode(q, kc, vc, table, ints(lens), ints([0, B]), ints([prefix]))
+    want = means(dict(vc=vc, table=table), lens, [0, B], [prefix])
+    got = out.double().view(B, Hk, ratio, d)
+    # the sums are exact (below 2^24), their quotient and its rounding are not; 1/l is of one ulp
+    check(got, want[:, :, None].expand_as(got), (2.0 ** -9 * 2 + 2.0 ** -21) * want[:, :, None].abs().expand_as(got))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lens", [[700] * 9, [3, 0, 0, 2100, 0, 33, 1, 0, 900], [0] * 8 + [5000], [5000] + [0] * 8])
+def test_shared_own_keys_only(ops, d, lens):
+    """No groups: requests of very different lengths, whose keys are one sequence for the kernel's waves."""
+    x = batch(21, [(5000, 1)] * 9, 1, 6, 3, d, 64, torch.float16)
+    x["lens"], x["cu"], x["prefix"] = lens, [0], []
+    shared(ops, x)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_shared_plan_of_many(ops, d):
+    """More requests and groups than one wave plans."""
+    groups = [(70 + i % 50, 1 + i % 4) for i in range(60)]
+    x = batch(15, groups, 40, 2, 1, d, 16, torch.bfloat16, alone=9)
+    x["lens"][3] = x["lens"][17] = 0
+    shared(ops, x)
+
+
+@pytest.mark.parametrize("d,H", [(64, 4), (128, 32)])
+def test_shared_past_32_bits(ops, d, H):
+    """Pages that lie more than 4 GiB apart, and prefixes whose keys reach past them."""
+    x = batch(16, [(200, 5)], 60, H, 2, d, 16, torch.bfloat16)
+    want = shared(ops, x)
+    P, Hk, page, _ = x["kc"].shape
+    stride = (1 << 33) // P // 8 * 8
+    far = []
+    for c in (x["kc"], x["vc"]):
+        buf = torch.empty(stride * P, dtype=c.dtype, device="cuda")
+        y = buf.as_strided((P, Hk, page, d), (stride, page * d, d, 1))
+        y.copy_(c)
+        far.append(y)
+    assert far[0].stride(0) * (P - 1) > 1 << 32
+    out = ops.mha_shared_decode(x["q"], *far, x["table"], ints(x["lens"]), ints(x["cu"]), ints(x["prefix"]))
+    assert torch.equal(out, want)
+
+
 # ── selection ─────────────────────────────────────────────────────────────────
 
 def logits_of(seed, G, W, V, dtype, spread=3.0):
@@ -470,7 +562,7 @@ def compact(ops, table, seq, page, P, held=None):
 
 
 @pytest.mark.parametrize("page", [1, 16, 1000])
-@pytest.mark.parametrize("N,M,P", [(1, 1, 1), (1, 1, 2), (4, 6, 40), (4, 6, 10), (9, 7, 32), (60, 33, 3000), (300, 20, 70001), (3, 500, 1300), (50, 40, 1 << 19)])
+@pytest.mark.parametrize("N,M,P", [(1, 1, 1), (1, 1, 2), (4, 6, 40), (4, 6, 10), (9, 7, 32), (60, 33, 3000), (300, 20, 70001), (3, 500, 1300), (50, 40, 1 << 19), (40, 700, 30000), (17, 300, 2048)])
 def test_compact(ops, page, N, M, P):
     table, seq = pool(N + M, N, M, page, P)
     compact(ops, table, seq, page, P)
