@@ -71,10 +71,9 @@ def sources_of(src: str) -> list:
     return sorted(found, key=os.path.basename)
 
 
-def compile_checked(out_path: str, flags=None, verbose: bool = False, src: str = SRC, dma: bool = True) -> str:
+def compile_checked(out_path: str, flags=None, verbose: bool = False, src: str = SRC) -> str:
     """Compile ``src`` into ``out_path`` (atomically) after checking the device
-    assembly of that same compilation; raise RuntimeError on either failure. ``dma``: its
-    kernels use the LDS DMA."""
+    assembly of that same compilation; raise RuntimeError on either failure."""
     from .isa_check import missed_occupancy, violations
     flags = list(HIPCC_FLAGS if flags is None else flags)
     with tempfile.TemporaryDirectory(prefix="mi355fa-build-") as tmp:
@@ -97,7 +96,7 @@ def compile_checked(out_path: str, flags=None, verbose: bool = False, src: str =
         bad = []
         for path in asm:
             with open(path) as f:
-                bad += [f"{os.path.basename(path)}: {v}" for v in violations(f.read(), dma)]
+                bad += [f"{os.path.basename(path)}: {v}" for v in violations(f.read())]
         if bad:
             raise RuntimeError("device assembly check failed; library not installed:\n"
                                + "\n".join(bad))

@@ -62,7 +62,7 @@ SharedPlan shared_plan(const mi355_shared_params* p, int cus) {
   pl.columns = mean > 64 ? 128 : mean > 32 ? 64 : 32;
   auto per_cu = [&](auto d) {
     constexpr int D = decltype(d)::value;
-    return pl.columns == 128 ? kShPerCu<D, 4, 1, kShTiles>() : pl.columns == 64 ? kShPerCu<D, 2, 2, 1>() : kShPerCu<D, 1, 4, 1>();
+    return pl.columns == 128 ? kShPerCu<D, 4, 1>() : pl.columns == 64 ? kShPerCu<D, 2, 2>() : kShPerCu<D, 1, 4>();
   };
   const int slots = cus * (p->d == 64 ? per_cu(std::integral_constant<int, 64>{}) : per_cu(std::integral_constant<int, 128>{}));
   const int64_t own = (int64_t)p->b * p->h_k * pl.groups;
@@ -133,9 +133,9 @@ int shared_decode(const mi355_shared_params* p, hipStream_t st, const Err& err) 
     constexpr int D = decltype(d)::value;
     constexpr bool BF = decltype(bf)::value;
     auto go = [&](void (*kernel)(const SharedArgs)) { rc = run(err, "mha_shared_decode", kernel, pl.grid, kShThreads, 0, st, a); };
-    if (pl.columns == 128) go(shared_decode_kernel<D, BF, 4, 1, kShTiles>);
-    else if (pl.columns == 64) go(shared_decode_kernel<D, BF, 2, 2, 1>);
-    else go(shared_decode_kernel<D, BF, 1, 4, 1>);
+    if (pl.columns == 128) go(shared_decode_kernel<D, BF, 4, 1>);
+    else if (pl.columns == 64) go(shared_decode_kernel<D, BF, 2, 2>);
+    else go(shared_decode_kernel<D, BF, 1, 4>);
     if (rc != kOk) return;
     const int64_t bh = (int64_t)p->b * p->h;
     if (bh >= 1024) rc = run(err, "mha_shared_decode (join)", shared_join_kernel<D, BF, true>, (bh + 3) / 4, 256, 0, st, a);

@@ -9,14 +9,18 @@
 // as long.
 //
 //  * Of a row's logits only the k largest can be selected (their order is that of the
-//    scores), so a workgroup that reads some of a row keeps its k largest logits beside
-//    the sum. A bound below the k-th largest of the first step comes from the lanes'
-//    maxima of 8 elements, by bisecting its bits with ballots; elements that reach it go
-//    to a list in LDS, whose k-th largest is the next bound.
+//    scores), so each wave that reads some of a row keeps the k largest of them beside the
+//    sum, in a list of its own in LDS. A bound below the k-th largest of the first step comes
+//    from the lanes' maxima, by bisecting bits with ballots; waves tell each other theirs, and
+//    only elements that reach it are listed.
 //  * The next step's logits are in flight while a step computes.
+//  * bf16 logits are counted by value and their exponentials taken once a value.
 //  * A second kernel, a workgroup a search, joins the parts' sums and lists: all
 //    candidates in registers, a bound by bisection in each wave, and the few that reach it
 //    ranked by counting.
+// Measured in a graph: one search of 4 beams, 32000 tokens, bf16: 9.6 us (scan 5.6, join 4.3);
+// 4 of 50 beams, k 50, 10007 tokens, fp32: 26; 64 of 8, k 16, 128000 tokens, bf16: 60, of which the
+// scan 57 for 131 MB (2.3 TB/s): counting and listing, not the bytes.
 
 constexpr int kSelThreads = 256;
 constexpr int kSelWave = 256;       // of a wave's

@@ -6,7 +6,11 @@
 // bitmaps down; the second's all join the bitmaps, so that each has the whole, and form
 // the running count of bits from which a page's rank, and the page of a rank, follow. Few
 // rows are one workgroup's, which does both.
-// Bound: the bytes of the tables, and for small ones two launches.
+// Bound: a launch, and the waits that follow one another. Measured in a graph: a fork of 4 rows 5.0
+// us, of 512 with 512 columns and 49000 pages 14.9 (marks 5.0, the rest 10.2: two bitmaps joined,
+// two running counts, a hash of the last pages); compacting 8 rows 5.1 us, 500 of 257 columns over
+// 84000 pages 15.5 (marks 4.2, the rest 12.1, of which joining the bitmaps 2.9, the counts 1.6, the
+// table's searches 1.8). A bit a page in LDS needs no clearing between calls, as one map in memory would.
 
 constexpr int kPgThreads = 1024;
 constexpr int kPgRows = 4096;            // rows of a fork: a bit each, and a hash of their last pages
@@ -394,7 +398,8 @@ struct CopyArgs {
 };
 
 // A wave copies a piece of one page of one cache: kCopyUnits 16-byte units, all loaded
-// before any is stored. Bound: bytes, read and written.
+// before any is stored. Bound: bytes, read and written (2000 pages of 8 heads, 64 rows of 128: 213
+// us, 4.9 TB/s; 67 small ones 2.7 us).
 constexpr int kCopyLoads = 4, kCopyUnits = 64 * kCopyLoads, kCopyThreads = 256;
 __global__ __launch_bounds__(kCopyThreads) void page_copy_kernel(const CopyArgs a) {
   const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);

@@ -13,18 +13,26 @@
 //    shared tile hides a key, and nothing of an unseen key can reach a row.
 //  * Shared tiles: a workgroup is 32·RW columns by KG groups of waves that take every
 //    KG-th tile and join their sums in LDS at the end. Sᵀ = K·Qᵀ with 32x32x16 MFMAs, so
-//    that a lane holds one column's scores; K and V come from the pages to LDS by DMA, two
-//    stages, one barrier a step.
+//    that a lane holds one column's scores; K and V come from the pages to LDS by DMA, of
+//    128 columns (64 KB of LDS) four stages, else two, one barrier a step. The shape follows
+//    from the columns a group has on average: fewer than a workgroup's are idle products,
+//    more groups of waves fewer barriers a tile.
 //  * Own tiles: 16 columns, the heads of one KV head; a wave by itself streams tiles of 32
 //    keys, K to the operand registers, V through its own LDS slice, the next tile in flight.
+//    All requests' own tiles are one sequence, cut into waves of equal length wherever that
+//    falls, so that every workgroup runs at once.
 //  * Lengths and offsets stay on the device: every workgroup derives the same plan from
-//    them and takes its part; workgroup 0 writes down for the join where parts lie.
+//    them and takes its part; workgroup 0 writes down for the join where parts lie. (A plan
+//    by a kernel of its own would cost a launch, 2.1 us, and the wait for it.)
+// Measured in a graph, with the join: 9 groups, 67 requests of 16 heads of 128 on 4 KV
+// heads, prefixes to 4099 keys, capped: 28 us (65 MB: 13.9 us); one group of 256 requests,
+// 8192 keys: 48 us (74 MB, 17 GFLOP), of which plan and first loads take 8, the shared tiles
+// 26 (17 % of the matrix units' time; vector and scalar work of two waves a SIMD and the
+// wait for LDS and for each other fill the rest), the join 8; 4 requests, 300 keys of 64: 13.1 us.
 
 constexpr int kShWaves = 4;
 constexpr int kShThreads = 64 * kShWaves;
 constexpr int kShMax = 1024;                   // requests, and groups
-
-constexpr int kShTiles = 1;   // tiles of a step of 128 columns
 
 struct SharedArgs {
   const uint16_t* q;
@@ -511,24 +519,24 @@ template <int D, bool BF16> struct Stream {
 };
 
 // Stages of the DMA, and pages whose numbers are held in LDS.
-template <int KG, int TB> constexpr int kShStages() { return KG * TB == 1 ? 4 : 2; }
+template <int KG> constexpr int kShStages() { return KG == 1 ? 4 : 2; }
 constexpr int kShPages = 1024;
 
-template <int D, int RW, int KG, int TB> constexpr int kShLds() {
-  const int stages = kShStages<KG, TB>() * 2 * KG * 32 * TB * D * 2 + kShPages * 4, sums = (RW * KG * 16 * (D / 32) * 64 + RW * KG * 2 * 64 + 1) * 4,
+template <int D, int RW, int KG> constexpr int kShLds() {
+  const int stages = kShStages<KG>() * 2 * KG * kDecTile * D * 2 + kShPages * 4, sums = (RW * KG * 16 * (D / 32) * 64 + RW * KG * 2 * 64 + 1) * 4,
             own = kShWords * 4 + kShWaves * kDecTile * (D * 2 + 32);
   return stages > sums ? (stages > own ? stages : own) : sums > own ? sums : own;
 }
 
-// Shared tiles: 32·RW columns by KG key groups of TB tiles a step. True if a page was none of
+// Shared tiles: 32·RW columns by KG key groups of a tile a step. True if a page was none of
 // the cache's: nothing is done then.
-template <int D, bool BF16, int RW, int KG, int TB>
+template <int D, bool BF16, int RW, int KG>
 __device__ __forceinline__ bool group_part(kernarg<SharedArgs>& a, const Share& sh, uint8_t* lds) {
   typedef typename Elt<BF16>::v8 V8;
   static_assert(RW * KG == kShWaves, "four waves");
-  constexpr int UPR = D / 8, KD = D / 16, DB = D / 32, kTile = 32 * TB, S = kShStages<KG, TB>();
-  constexpr int kElems = kTile * D;                 // of a K or V tile
-  constexpr int R = kTile / RW;                     // rows that a wave brings
+  constexpr int UPR = D / 8, KD = D / 16, DB = D / 32, S = kShStages<KG>();
+  constexpr int kElems = kDecTile * D;              // of a K or V tile
+  constexpr int R = kDecTile / RW;                  // rows that a wave brings
   constexpr int kLoads = R * UPR / 64, RPL = 64 / UPR;   // loads of K, of V; rows of one
   uint16_t* sKV = reinterpret_cast<uint16_t*>(lds);   // [stage][K, V][KG][kElems]
   const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
@@ -548,10 +556,10 @@ __device__ __forceinline__ bool group_part(kernarg<SharedArgs>& a, const Share& 
   float last = a.slopes ? (float)(min(max(a.lens[b], 0), (int)((int64_t)a.cols << a.shift)) - 1) : 0.f;   // the column's last key
   const float c2 = a.c2, slack = kSlackLog2 / a.c2;
 
-  // steps of KG·TB tiles: key group kg has tiles first + (step·KG + kg)·TB ..
+  // steps of KG tiles: key group kg has tile first + step·KG + kg, if it is there
   const int count = sh.hi - sh.lo, first = sh.own.first + sh.lo;
-  const int steps = (count + KG * TB - 1) / (KG * TB);
-  auto tiles_of = [&](int step) { return max(0, min(TB, count - (step * KG + kg) * TB)); };
+  const int steps = (count + KG - 1) / KG;
+  auto there = [&](int step) { return step * KG + kg < count; };
   // The wave's rows of the LDS tiles: load i brings rows rw·R + i·RPL .., of K the keys π(row).
   // 4 rows of K are 4 keys that follow one another in a page, and RPL rows of V are so too, so
   // that their page is the same for all lanes, which add an offset of their own (of d = 64,
@@ -564,13 +572,12 @@ __device__ __forceinline__ bool group_part(kernarg<SharedArgs>& a, const Share& 
   const bool two = RPL == 8 && a.shift < 5;          // K's loads reach into two pages
   // Offsets of the lane from where the tile starts in a page (of fewer than 32 rows: from the page)
   const int in_page = page_size - 1;
-  auto k_key = [&](int i) { const int r = rw * R + i * RPL; return (r & ~31) + key_perm(r & 31); };
-  uint32_t k_off[kLoads], v_off[kLoads];
+    uint32_t k_off[kLoads], v_off[kLoads];
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
     const int r = rw * R + i * RPL;
-    k_off[i] = (uint32_t)(((k_key(i) & in_page & 31) + key_perm((r + q4) & 31) - key_perm(r & 31)) * (int)a.kr + (slot ^ ((r + q4) % UPR)) * 8) * 2u;
-    v_off[i] = (uint32_t)(((r & in_page & 31) + q4) * (int)a.vr + (slot ^ v_swz<D>(q4)) * 8) * 2u;
+    k_off[i] = (uint32_t)(((key_perm(r) & in_page) + key_perm(r + q4) - key_perm(r)) * (int)a.kr + (slot ^ ((r + q4) % UPR)) * 8) * 2u;
+    v_off[i] = (uint32_t)(((r & in_page) + q4) * (int)a.vr + (slot ^ v_swz<D>(q4)) * 8) * 2u;
   }
   // Page numbers in LDS, kShPages from page `held` on. (Loads of the loop's own would make it
   // wait for the DMA issued before them.) A page outside the cache is read as page 0, and all of
@@ -594,32 +601,31 @@ __device__ __forceinline__ bool group_part(kernarg<SharedArgs>& a, const Share& 
   // Where a step's loads start: those of K in lanes 0 .., then V's.
   static_assert(2 * kLoads <= 64, "a lane each");
   const int of = lane < kLoads ? lane : min(lane - kLoads, kLoads - 1), of_row = rw * R + of * RPL;
-  const int of_key = lane < kLoads ? (of_row & ~31) + key_perm(of_row & 31) : of_row;
+  const int of_key = lane < kLoads ? key_perm(of_row) : of_row;
   const bool of_k = lane < kLoads;
   const uint64_t of_base = reinterpret_cast<uint64_t>(of_k ? kbase : vbase), of_page = (uint64_t)(of_k ? a.kp : a.vp) * 2, of_step = (uint64_t)(of_k ? a.kr : a.vr) * 2;
-  auto key_of = [&](int step) { return (first + (step * KG + kg) * TB) * kDecTile; };
+  auto key_of = [&](int step) { return (first + step * KG + kg) * kDecTile; };
   auto entries = [&](int step) __attribute__((always_inline)) {
-    const int behind = min((first + min(step + 1, steps) * KG * TB) * kDecTile - 1, most) >> a.shift;   // the step's last page
+    const int behind = min((first + min(step + 1, steps) * KG) * kDecTile - 1, most) >> a.shift;   // the step's last page
     if (behind - held >= kShPages) {   // (all waves come here, of step after step)
       wg_barrier();
-      held = min((first + step * KG * TB) * kDecTile, most) >> a.shift;
+      held = min((first + step * KG) * kDecTile, most) >> a.shift;
       fill();
     }
     // (of small pages the tile starts at 0, and the lane's key is in its offset)
     const int key0 = key_of(step), page = pages[(min(key0 + of_key, most) >> a.shift) - held];
-    return of_base + (uint64_t)(uint32_t)page * of_page + (uint64_t)(uint32_t)((key0 + (rw * R & ~31)) & in_page) * of_step;
+    return of_base + (uint64_t)(uint32_t)page * of_page + (uint64_t)(uint32_t)(key0 & in_page) * of_step;
   };
   const uint32_t lds0 = lds_addr(sKV);
   auto issue = [&](int step, int st, uint64_t e) __attribute__((always_inline)) {
-    static_assert(32 % R == 0, "a wave's rows are of one tile");
-    if (rw * R >= tiles_of(step) * 32) return;
+    if (!there(step)) return;
     const uint32_t tk = lds0 + (uint32_t)(((st * 2) * KG + kg) * kElems + rw * R * D) * 2u, tv = tk + KG * kElems * 2u;
     const uint32_t lo = low_u32(e), hi = high_u32(e);
     auto base = [&](int x) { return reinterpret_cast<const uint8_t*>(compose_u64(__builtin_amdgcn_readlane(lo, x), __builtin_amdgcn_readlane(hi, x))); };
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       if (two) {   // (its own page for each lane)
-        const int r = rw * R + i * RPL, key = key_of(step) + (r & ~31) + key_perm((r + q4) & 31);
+        const int r = rw * R + i * RPL, key = key_of(step) + key_perm(r + q4);
         const int x = pages[(min(key, most) >> a.shift) - held];
         gload16_lds(kbase + (int64_t)x * a.kp + (int64_t)(key & in_page) * a.kr + (slot ^ ((r + q4) % UPR)) * 8, tk + (uint32_t)(i * 64 * 16));
       } else
@@ -645,37 +651,37 @@ __device__ __forceinline__ bool group_part(kernarg<SharedArgs>& a, const Share& 
   for (int db = 0; db < DB; ++db) oacc[db] = f32x16{};
   float m_run = -INFINITY, mlog2 = 0.f, l_run = 0.f;
 
-  // NT of the step's tiles at LDS tk, tv; base: the first key
-  auto compute = [&](auto nt, int base, uint32_t tk, uint32_t tv) __attribute__((always_inline)) {
-    constexpr int NT = decltype(nt)::value, kWin = 2;   // LDS operand reads in flight
-    f32x16 s[NT];
+  // The tile at LDS tk, tv; base: its first key
+  auto compute = [&](int base, uint32_t tk, uint32_t tv) __attribute__((always_inline)) {
+    constexpr int kWin = 2;   // LDS operand reads in flight
+    f32x16 s;
     {
-      auto rd = [&](int i) { return bitcast<V8>(*(const lds_u32x4*)(tk + k_rd[i % KD] + (i / KD) * 32 * D * 2)); };
+      auto rd = [&](int i) { return bitcast<V8>(*(const lds_u32x4*)(tk + k_rd[i])); };
       V8 win[kWin];
 #pragma unroll
       for (int i = 0; i < kWin; ++i) win[i] = rd(i);
 #pragma unroll
-      for (int i = 0; i < NT * KD; ++i) {
+      for (int i = 0; i < KD; ++i) {
         const V8 x = win[i % kWin];
-        if (i + kWin < NT * KD) win[i % kWin] = rd(i + kWin);
-        s[i / KD] = Elt<BF16>::mfma(x, qreg[i % KD], i % KD == 0 ? f32x16{} : s[i / KD]);
+        if (i + kWin < KD) win[i % kWin] = rd(i + kWin);
+        s = Elt<BF16>::mfma(x, qreg[i], i == 0 ? f32x16{} : s);
       }
     }
-    float u[16 * NT];   // key base + 32·(c / 16) + 16·g + c % 16
+    float u[16];   // key base + 16·g + x
 #pragma unroll
-    for (int x = 0; x < 16 * NT; ++x) u[x] = s[x / 16][x % 16];
+    for (int x = 0; x < 16; ++x) u[x] = s[x];
     if (a.cap) {
 #pragma unroll
-      for (int x = 0; x < 16 * NT; ++x) u[x] = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(u[x] * a.u_scale));
+      for (int x = 0; x < 16; ++x) u[x] = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(u[x] * a.u_scale));
     }
     if (a.slopes) {
       const float back = last - (float)(base + 16 * g);
 #pragma unroll
-      for (int x = 0; x < 16 * NT; ++x) u[x] = __builtin_fmaf(bco, back - (float)(x / 16 * 32 + x % 16), u[x]);
+      for (int x = 0; x < 16; ++x) u[x] = __builtin_fmaf(bco, back - (float)x, u[x]);
     }
     float mx = -INFINITY;
 #pragma unroll
-    for (int x = 0; x < 16 * NT; ++x) mx = fmaxf(mx, u[x]);
+    for (int x = 0; x < 16; ++x) mx = fmaxf(mx, u[x]);
     mx = xhalf_max(mx);
     const bool need = mx > m_run + slack;
     if (__builtin_amdgcn_ballot_w64(need)) {
@@ -687,10 +693,10 @@ __device__ __forceinline__ bool group_part(kernarg<SharedArgs>& a, const Share& 
 #pragma unroll
       for (int db = 0; db < DB; ++db) oacc[db] *= alpha;
     }
-    constexpr int N = 2 * NT * DB;
+    constexpr int N = 2 * DB;
     auto rd = [&](int i) {
       const int j = i / DB, db = i % DB;
-      const int o = ((j / 2) * 32 + (j % 2) * 8) * D * 2;
+      const int o = j * 8 * D * 2;
       const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tv + v_rd[db] + o));
       const s16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tv + v_rd[db] + o + 4 * D * 2));
       return bitcast<V8>(__builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -699,7 +705,7 @@ __device__ __forceinline__ bool group_part(kernarg<SharedArgs>& a, const Share& 
 #pragma unroll
     for (int i = 0; i < kWin; ++i) win[i] = rd(i);
 #pragma unroll
-    for (int j = 0; j < 2 * NT; ++j) {
+    for (int j = 0; j < 2; ++j) {
       f32x8 pf;
 #pragma unroll
       for (int e = 0; e < 8; ++e) pf[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(u[j * 8 + e], c2, -mlog2));
@@ -733,17 +739,15 @@ __device__ __forceinline__ bool group_part(kernarg<SharedArgs>& a, const Share& 
   }
   int st = 0;
   for (int i = 0; i < steps; ++i) {
-    // the wave's loads of step i have landed; of the steps behind it only the last one's count is not known
-    if (S > 2 && i + S - 2 < steps - (KG * TB > 1)) wait_vmcnt<(S - 2) * 2 * kLoads>();
+    // the wave's loads of step i have landed; with four stages, each step has one tile
+    if (S > 2 && i + S - 2 < steps) wait_vmcnt<(S - 2) * 2 * kLoads>();
     else wait_vmcnt<0>();
     wg_barrier();      // all waves' have, and all have left the stage of step i − 1
     if (i + S - 1 < steps) issue(i + S - 1, st == 0 ? S - 1 : st - 1, e);
     e = entries(i + S);
-    const int n = tiles_of(i), base = (first + (i * KG + kg) * TB) * kDecTile;
     const uint32_t tk = lds0 + (uint32_t)(((st * 2) * KG + kg) * kElems) * 2u, tv = tk + KG * kElems * 2u;
     st = st + 1 == S ? 0 : st + 1;
-    if (n == TB) compute(std::integral_constant<int, TB>{}, base, tk, tv);
-    else if (TB > 1 && n == 1) compute(std::integral_constant<int, 1>{}, base, tk, tv);
+    if (there(i)) compute(key_of(i), tk, tv);
   }
   wait_vmcnt<0>();
   l_run = xhalf_sum(l_run);
@@ -753,7 +757,7 @@ __device__ __forceinline__ bool group_part(kernarg<SharedArgs>& a, const Share& 
   constexpr int OWN = 16 * DB / KG, kSums = KG > 1 ? RW * KG * 16 * DB * 64 : 0;
   float* sj = reinterpret_cast<float*>(lds);   // [RW][KG shares][KG][OWN][64], then [RW][KG][2][64]
   float* sml = sj + kSums;
-  static_assert((kSums + RW * KG * 2 * 64 + 1) * 4 <= kShLds<D, RW, KG, TB>(), "sums fit");
+  static_assert((kSums + RW * KG * 2 * 64 + 1) * 4 <= kShLds<D, RW, KG>(), "sums fit");
   uint32_t* flag = reinterpret_cast<uint32_t*>(sml + RW * KG * 2 * 64);
   wg_barrier();   // the stages are free
   if (tid == 0) *flag = 0;
@@ -808,12 +812,12 @@ __device__ __forceinline__ bool group_part(kernarg<SharedArgs>& a, const Share& 
 }
 
 // Workgroups that a CU holds.
-template <int D, int RW, int KG, int TB> constexpr int kShPerCu() { return kShLds<D, RW, KG, TB>() <= 78 * 1024 ? 2 : 1; }
+template <int D, int RW, int KG> constexpr int kShPerCu() { return kShLds<D, RW, KG>() <= 78 * 1024 ? 2 : 1; }
 
-template <int D, bool BF16, int RW, int KG, int TB>
-__global__ __launch_bounds__(kShThreads) __attribute__((amdgpu_waves_per_eu(kShPerCu<D, RW, KG, TB>())))
+template <int D, bool BF16, int RW, int KG>
+__global__ __launch_bounds__(kShThreads) __attribute__((amdgpu_waves_per_eu(kShPerCu<D, RW, KG>())))
 void shared_decode_kernel(const SharedArgs a) {
-  __shared__ __align__(16) uint8_t lds[kShLds<D, RW, KG, TB>()];
+  __shared__ __align__(16) uint8_t lds[kShLds<D, RW, KG>()];
   __shared__ float sM[kShWaves][16], sL[kShWaves][16];
   __shared__ Share shares[kShWaves];
   int* words = reinterpret_cast<int*>(lds);
@@ -852,7 +856,7 @@ void shared_decode_kernel(const SharedArgs a) {
   }
   keep(group_share(a, words));
   __syncthreads();   // the plan's words are read
-  if (!group_part<D, BF16, RW, KG, TB>(reload_kernarg(a), share(), lds)) return;
+  if (!group_part<D, BF16, RW, KG>(reload_kernarg(a), share(), lds)) return;
   // a page outside the cache hides its keys, which only the stream can
   __syncthreads();
 #pragma unroll 1

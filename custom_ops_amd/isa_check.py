@@ -81,11 +81,10 @@ def sgpr_spills_in_mfma_span(text: str, name: str) -> list:
     return bad
 
 
-def violations(text: str, dma: bool = True) -> list:
-    """Human-readable list of every violated property (empty when clean). ``dma``: the
-    library's kernels use the LDS DMA."""
+def violations(text: str) -> list:
+    """Human-readable list of every violated property (empty when clean)."""
     out = []
-    if dma and ";;#ASMSTART" not in text:
+    if ";;#ASMSTART" not in text:
         out.append("the LDS DMA inline assembly is missing")
     m0 = [c for c in code_outside_asm(text) if re.search(r"\bm0\b", c)]
     if m0:

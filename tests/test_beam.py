@@ -260,7 +260,7 @@ def test_traced_copies_stay(o):
 
 def test_sealed_deployment(lib, tmp_path, monkeypatch):
     from custom_ops_amd.loader import BeamOps
-    monkeypatch.setattr(build, "compile_checked", lambda out, flags, verbose=False, src=None, dma=True: shutil.copy2(build.BEAM_LIB_PATH, out))
+    monkeypatch.setattr(build, "compile_checked", lambda out, flags, verbose=False, src=None: shutil.copy2(build.BEAM_LIB_PATH, out))
     path = BeamOps().build(tmp_path)
     md = json.loads(open(str(path) + ".json").read())
     assert set(md["contract"]["schemas"]) == {f"recsys_ops::{n}" for n in beam.SCHEMAS}
