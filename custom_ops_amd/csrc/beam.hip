@@ -68,6 +68,9 @@ SharedPlan shared_plan(const mi355_shared_params* p, int cus) {
   const int64_t own = (int64_t)p->b * p->h_k * pl.groups;
   const int64_t common = p->h_k * ((p->b * ratio + pl.columns - 1) / pl.columns + p->n_groups);
   pl.target = slots - (int)(common < slots ? common / 2 : slots / 2);   // groups' units end with a part that is not whole
+  // (no more than the tables' tiles keep busy: a workgroup without any still plans)
+  const int64_t most = (own + common * (pl.columns / 32)) * ((int64_t)p->table_cols * p->page_size / kDecTile + 1);
+  if (most < 4 * (int64_t)pl.target) pl.target = (int)((most + 3) / 4);
   pl.grid = pl.target + common + 1;
   pl.own_rows = (common + pl.target) * pl.columns;
   pl.rows = pl.own_rows + (4 * (int64_t)(pl.target + 1) + own) * 16;

@@ -51,8 +51,10 @@ enum { MI355_BEAM_FP16 = 0, MI355_BEAM_BF16 = 1, MI355_BEAM_FP32 = 2 };
  * request that sees none gives 0. Keys that are not seen have no influence.
  * Layouts: q, o [b, h, d]; caches [num_pages, h_k, page_size, d]; block_table
  * [b, table_cols]; innermost stride 1, 16-byte aligned bases, other strides multiples of
- * 8 elements, the caches' row strides below 2^24. A page number outside the cache hides that page's keys; kv_lens and
- * prefix_lens past table_cols·page_size (2^30 at most) count as that.
+ * 8 elements, the caches' row strides below 2^24. A page number outside the cache hides
+ * that page's keys; kv_lens and prefix_lens past table_cols·page_size (2^30 at most) count
+ * as that. Tiles of 32 keys that a table spans, for each KV head and 16 of its heads: at
+ * most 2^30 of a request and 2^35 of all.
  */
 typedef struct mi355_shared_params {
   const void* q;

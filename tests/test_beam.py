@@ -63,7 +63,8 @@ def lib():
         (dict(dtype=2), "float16 or bfloat16"), (dict(d=96), "head_dim"), (dict(h=3), "divisible"), (dict(h_k=0), "divisible"), (dict(b=-1), "requests"),
         (dict(b=1025), "1024 requests"), (dict(groups=-1), "groups"), (dict(groups=1025), "groups"), (dict(h=2 ** 17), "heads"), (dict(cols=-1), "negative"),
         (dict(num_pages=-1), "negative"), (dict(page_size=4), "page_size"), (dict(page_size=48), "page_size"), (dict(page_size=2048), "page_size"),
-        (dict(cols=2 ** 27), "2\\^30 keys"), (dict(window=-1), "window"), (dict(scale=0.0), "scale"), (dict(scale=math.nan), "scale"),
+        (dict(cols=2 ** 27), "2\\^30 keys"),
+        (dict(cols=2 ** 26, h=64, h_k=64), "too many requests, heads and keys"), (dict(cols=2 ** 26, b=1024), "too many requests, heads and keys"), (dict(window=-1), "window"), (dict(scale=0.0), "scale"), (dict(scale=math.nan), "scale"),
         (dict(softcap=1001.0), "softcap"), (dict(lens=0), "NULL"), (dict(cu=0), "NULL"), (dict(prefix=0), "NULL"), (dict(table=0), "NULL"), (dict(v=0), "NULL"),
         (dict(q=4104), "16-byte"), (dict(kr=68), "multiples of 8"), (dict(kr=2 ** 24), "row strides"), (dict(vr=-64), "row strides"), (dict(o_hs=68), "multiples of 8")]],
     *[("mi355_beam_select", Select, SELECT, bad, text) for bad, text in [
