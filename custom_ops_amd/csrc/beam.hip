@@ -48,7 +48,7 @@ size_t up(size_t x) { return (x + 255) & ~(size_t)255; }
 
 struct SharedPlan {
   int columns, groups, target;
-  int64_t grid;           // workgroups at most
+  int64_t common, grid;   // parts of groups that are not whole, workgroups: at most
   int64_t own_rows, rows; // rows of partial sums: of groups' parts, and all
   size_t ml, o, bytes;    // offsets of the parts' statistics and sums in the workspace
 };
@@ -57,7 +57,10 @@ SharedPlan shared_plan(const mi355_shared_params* p, int cus) {
   SharedPlan pl{};
   const int64_t ratio = p->h / p->h_k;
   pl.groups = (int)((ratio + 15) / 16);
-  // columns of a KV head that a group has on average
+  // Columns of a workgroup, from those that a group has of a KV head on average. Measured (d 128, 4 KV
+  // heads, prefixes of 4099 keys), us a call with 32, 64, 128: 29 columns 27.9, 28.0, 29.4; 40 columns
+  // 33.0, 29.8, 30.2 (120 requests) and 23.3, 23.0, 23.3 (40); 186 columns 39.9, 31.0, 31.0; 1020 of one
+  // group 136.9, 55.8, 47.4.
   const int64_t mean = p->n_groups > 0 ? p->b * ratio / p->n_groups : 0;
   pl.columns = mean > 64 ? 128 : mean > 32 ? 64 : 32;
   auto per_cu = [&](auto d) {
@@ -66,7 +69,7 @@ SharedPlan shared_plan(const mi355_shared_params* p, int cus) {
   };
   const int slots = cus * (p->d == 64 ? per_cu(std::integral_constant<int, 64>{}) : per_cu(std::integral_constant<int, 128>{}));
   const int64_t own = (int64_t)p->b * p->h_k * pl.groups;
-  const int64_t common = p->h_k * ((p->b * ratio + pl.columns - 1) / pl.columns + p->n_groups);
+  const int64_t common = pl.common = p->h_k * ((p->b * ratio + pl.columns - 1) / pl.columns + p->n_groups);
   pl.target = slots - (int)(common < slots ? common / 2 : slots / 2);   // groups' units end with a part that is not whole
   // (no more than the tables' tiles keep busy: a workgroup without any still plans)
   const int64_t most = (own + common * (pl.columns / 32)) * ((int64_t)p->table_cols * p->page_size / kDecTile + 1);
@@ -140,8 +143,11 @@ int shared_decode(const mi355_shared_params* p, hipStream_t st, const Err& err) 
     else if (pl.columns == 64) go(shared_decode_kernel<D, BF, 2, 2>);
     else go(shared_decode_kernel<D, BF, 1, 4>);
     if (rc != kOk) return;
+    // A wave joins a row, or a workgroup where that leaves the card idle and a row has many parts (about
+    // target / common). Measured, us a call by waves and by workgroups: 32 rows of 8 parts 11.7, 13.0; 640 of
+    // 18 22.4, 23.0; 512 of 31 21.5, 20.3; 336 of 63 20.7, 19.9; 1072 of 3 27.8, 29.4; 4096 of 14 47.3, 55.3.
     const int64_t bh = (int64_t)p->b * p->h;
-    if (bh >= 1024) rc = run(err, "mha_shared_decode (join)", shared_join_kernel<D, BF, true>, (bh + 3) / 4, 256, 0, st, a);
+    if (bh >= 1024 || pl.target <= 24 * pl.common) rc = run(err, "mha_shared_decode (join)", shared_join_kernel<D, BF, true>, (bh + 3) / 4, 256, 0, st, a);
     else rc = run(err, "mha_shared_decode (join)", shared_join_kernel<D, BF, false>, bh, 256, 0, st, a);
   });
   return rc;
