@@ -46,7 +46,8 @@ MI355_HD inline int own_tile(const OwnTiles& o, int i) { return i < o.before ? o
 // 32 columns, a request's own as own_weight of them) and about `target` workgroups of four waves
 // wanted; a group's part of them, whose waves take `ways` tiles a step, of at least 4 tiles; and
 // a wave's own tiles. At most target + 1 workgroups, and one for each group's
-// unit, come of it.
+// unit, come of it. (At least 2, 4, 8 tiles: 4 requests of 300 keys 11.7, 11.7, 12.5 us, 21 of 4099
+// keys 21.8, 19.5, 21.5.)
 // An own tile costs more than a shared one: a wave waits for each unit's first. Measured, for
 // weights of 1, 2, 3, 4, 6: 9 groups of 32 columns 35.4, 28.2, 31.3, 32.2, 40.2 us, one of 1020
 // columns 80, 56, 48.2, 47.8, 51.9 us.
