@@ -156,28 +156,16 @@ int shared_decode(const mi355_shared_params* p, hipStream_t st, const Err& err) 
 }
 
 struct SelectPlan {
-  int parts, per, wide;   // wide: the steps are of kSelWide times 8 elements a thread
+  SelectSplit split;
   size_t lists, bytes;
 };
 
 SelectPlan select_plan(const mi355_select_params* p, int cus) {
   SelectPlan pl{};
   const int64_t rows = (int64_t)p->n_groups * p->beams;
-  const int small = kSelThreads * 8;
-  // Parts of a row: workgroups for all CUs, four on each, but one where k is large, since the
-  // join's candidates grow with both (us for one, two, four: [4 x 50 x 10007] fp32, k = 50
-  // 25.8 / 34.1 / 35.7; [64 x 8 x 128000] bf16, k = 16 71 / 71 / 60); no more than the join holds
-  const int64_t most = (int64_t)kSelJoin * kSelEach / ((int64_t)p->beams * p->k);
-  const int64_t wanted = std::max<int64_t>(1, std::min<int64_t>((p->k > 32 ? 1 : 4) * cus / rows, most));
-  const int64_t steps = ((int64_t)p->vocab + small - 1) / small;
-  const int vectors = p->dtype == MI355_BEAM_FP32 ? kSelWide<float> : kSelWide<__bf16>;
-  pl.wide = steps >= vectors * wanted;
-  const int step = pl.wide ? vectors * small : small;
-  const int64_t all = ((int64_t)p->vocab + step - 1) / step, each = (all + wanted - 1) / wanted;
-  pl.per = (int)std::min<int64_t>(each * step, 1 << 30);
-  pl.parts = (int)(((int64_t)p->vocab + pl.per - 1) / pl.per);
-  pl.lists = up((size_t)rows * pl.parts * sizeof(SelectHead));
-  pl.bytes = pl.lists + (size_t)rows * pl.parts * p->k * 8;
+  pl.split = select_split(rows, p->beams, p->vocab, p->k, p->dtype == MI355_BEAM_FP32 ? kSelWide<float> : kSelWide<__bf16>, cus);
+  pl.lists = up((size_t)rows * pl.split.parts * sizeof(SelectHead));
+  pl.bytes = pl.lists + (size_t)rows * pl.split.parts * p->k * 8;
   return pl;
 }
 
@@ -210,13 +198,13 @@ int beam_select(const mi355_select_params* p, hipStream_t st, const Err& err) {
   a.lists = (u32x2*)((char*)p->workspace + pl.lists);
   a.gs = p->group_stride; a.bs = p->beam_stride;
   a.groups = p->n_groups; a.beams = p->beams; a.vocab = p->vocab; a.k = p->k; a.eos = p->eos;
-  a.parts = pl.parts; a.per = pl.per;
-  const uint64_t each = (uint64_t)pl.parts * p->k;
+  a.parts = pl.split.parts; a.per = pl.split.per;
+  const uint64_t each = (uint64_t)pl.split.parts * p->k;
   a.row_magic = each == 1 ? 0 : (uint32_t)(((1ull << 32) + each - 1) / each);
-  const int64_t grid = (int64_t)p->n_groups * p->beams * pl.parts;
+  const int64_t grid = (int64_t)p->n_groups * p->beams * pl.split.parts;
   auto go = [&](auto type) {
     typedef decltype(type) T;
-    return run(err, "beam_select", pl.wide ? select_scan_kernel<T, kSelWide<T>> : select_scan_kernel<T, 1>, grid, kSelThreads, 0, st, a);
+    return run(err, "beam_select", pl.split.wide ? select_scan_kernel<T, kSelWide<T>> : select_scan_kernel<T, 1>, grid, kSelThreads, 0, st, a);
   };
   if (int rc = p->dtype == MI355_BEAM_FP32 ? go(float{}) : p->dtype == MI355_BEAM_BF16 ? go(__bf16{}) : go(_Float16{})) return rc;
   if (p->beams * each <= 256) return run(err, "beam_select (join)", select_join_kernel<256, 1>, p->n_groups, 256, 0, st, a);

@@ -95,6 +95,41 @@ MI355_HD inline UnitPart unit_part(int place, int n, int heads, int blocks) {
   return {(int)(item / (uint32_t)n), (int)block, (int)(item % (uint32_t)n)};
 }
 
+// ── selection: parts of a row of logits ──────────────────────────────────────
+constexpr int kSelThreads = 256;
+constexpr int kSelCandidates = 1 << 14;   // of a search, that the join holds
+constexpr int kSelMostPer = 1 << 30;
+
+// A row's parts, of `per` tokens each but the last; wide: the steps are of `vectors` times 8 elements a
+// thread. `rows` of all searches, `beams` of one, of `vocab` tokens each, the `k` best wanted.
+struct SelectSplit {
+  int parts, per, wide;
+};
+MI355_HD inline SelectSplit select_split(int64_t rows, int beams, int vocab, int k, int vectors, int cus) {
+  const int small = kSelThreads * 8;
+  // Parts of a row: workgroups for all CUs, four on each, but one where k is large, since the
+  // join's candidates grow with both (us for one, two, four: [4 x 50 x 10007] fp32, k = 50
+  // 25.8 / 34.1 / 35.7; [64 x 8 x 128000] bf16, k = 16 71 / 71 / 60); no more than the join holds
+  const int64_t most = kSelCandidates / ((int64_t)beams * k), all_cus = (k > 32 ? 1 : 4) * (int64_t)cus / rows;
+  const int64_t wanted = imax(1, (int)(all_cus < most ? all_cus : most));
+  const int64_t steps = ((int64_t)vocab + small - 1) / small;
+  SelectSplit s;
+  s.wide = steps >= vectors * wanted;
+  const int step = s.wide ? vectors * small : small;
+  const int64_t all = ((int64_t)vocab + step - 1) / step, each = (all + wanted - 1) / wanted;
+  s.per = (int)(each * step < kSelMostPer ? each * step : kSelMostPer);
+  s.parts = (int)(((int64_t)vocab + s.per - 1) / s.per);
+  return s;
+}
+// Tokens of a part, at least one; of the last part, begin + per may be 2^31 or more.
+struct SelectSpan {
+  int begin, end;
+};
+MI355_HD inline SelectSpan select_span(int part, int per, int vocab) {
+  const int begin = part * per;
+  return {begin, vocab - begin < per ? vocab : begin + per};
+}
+
 }  // namespace mi355fa
 
 #endif  // MI355_BEAM_SCHED_H

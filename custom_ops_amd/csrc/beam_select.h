@@ -22,12 +22,12 @@
 // 4 of 50 beams, k 50, 10007 tokens, fp32: 26; 64 of 8, k 16, 128000 tokens, bf16: 60, of which the
 // scan 57 for 131 MB (2.3 TB/s): counting and listing, not the bytes.
 
-constexpr int kSelThreads = 256;
 constexpr int kSelWave = 256;       // of a wave's
 constexpr int kSelMaxK = 64;
 constexpr int kSelMaxBeams = 256;
 constexpr int kSelJoin = 1024;      // threads of the join, and candidates of a thread, at most
 constexpr int kSelEach = 16;
+static_assert(kSelJoin * kSelEach == kSelCandidates, "what the join holds");
 
 // Σ over the wave, in all lanes.
 template <int CTRL, int ROWS> __device__ __forceinline__ double dpp_add(double x) {
@@ -270,7 +270,8 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
   const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6), k = a.k;
   const int64_t base = (int64_t)(row / a.beams) * a.gs + (int64_t)(row % a.beams) * a.bs;
   const T* x = static_cast<const T*>(a.x) + base;
-  const int begin = part * a.per, end = min(a.vocab, begin + a.per);
+  const SelectSpan span = select_span(part, a.per, a.vocab);
+  const int begin = span.begin, end = span.end;
   // a whole step, and the last one
   auto fetch = [&](int at, Raw (&r)[N]) __attribute__((always_inline)) {
 #pragma unroll
@@ -279,14 +280,14 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
   auto fetch_tail = [&](int at, Raw (&r)[N]) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const int i = at + (j * kSelThreads + tid) * 8;
-      if (i + 8 <= end) r[j] = *reinterpret_cast<const Raw*>(x + i);
-      else r[j] = L::tail(x, i, end - i);
+      const int i = (j * kSelThreads + tid) * 8, left = end - at;   // (at + i may be 2^31 or more)
+      if (i + 8 <= left) r[j] = *reinterpret_cast<const Raw*>(x + at + i);
+      else r[j] = L::tail(x + at, i, left - i);
     }
   };
   Raw cur[N], next[N];
   // (before it is known whether they are needed)
-  if (begin + STEP <= end) fetch(begin, cur);
+  if (end - begin >= STEP) fetch(begin, cur);
   else fetch_tail(begin, cur);
   if (done) return;
   if constexpr (BINS)
@@ -307,15 +308,16 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
   bool bad = false;
   int n = 0, steps = 0;       // of the wave's list; done
   uint32_t t = kLowest + 1;   // what reaches it is listed; never −infinity
-  for (int at = begin; at < end; at += STEP) {
-    const bool whole = at + 2 * STEP <= end;   // the step that follows
+  for (int at = begin;; at += STEP) {
+    const int left = end - at;   // (more than 0)
+    const bool whole = left >= 2 * STEP;   // the step that follows
     if (whole) fetch(at + STEP, next);
     // f(logit, token) for the thread's elements of the step, read again: for rare cases
     auto each = [&](auto f) __attribute__((always_inline)) {
 #pragma unroll 1
       for (int e = 0; e < 8 * N; ++e) {
-        const int i = at + (e / 8 * kSelThreads + tid) * 8 + e % 8;
-        if (i < end) f(L::one(x, i), i);
+        const int i = (e / 8 * kSelThreads + tid) * 8 + e % 8;
+        if (i < left) f(L::one(x + at, i), at + i);
       }
     };
     float best[N];
@@ -404,7 +406,7 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // (a wave's LDS accesses stay in order)
       const int i = lane >> 3;
       const float y = L::one(&some8[wave][i], lane & 7);
-      const uint32_t token = from8[wave][i] + (lane & 7);
+      const uint32_t token = (uint32_t)from8[wave][i] + (lane & 7);
       uint64_t m = __builtin_amdgcn_ballot_w64(i < hits - p && y >= unordered(t));
       if (n > kSelWave - 64) {
         full = keep_largest(list, n, k);
@@ -422,11 +424,12 @@ __global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))
     }
     // after 1, 2, 4, .. steps: by then half of what is seen is new
     ++steps;
-    if ((steps & (steps - 1)) == 0 && n >= some && at + STEP < end) tell(some_of(list, n, some));
+    if (left <= STEP) break;
+    if ((steps & (steps - 1)) == 0 && n >= some) tell(some_of(list, n, some));
     if (whole) {
 #pragma unroll
       for (int j = 0; j < N; ++j) cur[j] = next[j];
-    } else if (at + STEP < end) fetch_tail(at + STEP, cur);
+    } else fetch_tail(at + STEP, cur);
   }
   // the waves' lists as one
   if (n > 64) keep_largest(list, n, k);
