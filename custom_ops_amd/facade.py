@@ -336,8 +336,8 @@ class RecsysOps:
 
         logits [G,W,V] (fp16/bf16/fp32, W at most 256; rows may lie apart), scores [G,W]
         float32: the beams' so far. A continuation's score is scores[g,w] + log softmax of
-        the logits at its token, formed in 64 bits; the best come first, the lowest w·V + v
-        among equals. k is at most 64. A beam that is ``finished`` ([G,W] bool) has one
+        the logits at its token, formed in 64 bits; the best come first, among equals the lowest
+        w, then the largest logit, then the lowest v. k is at most 64. A beam that is ``finished`` ([G,W] bool) has one
         continuation, its own score with the token ``eos``. Beams with scores that are not finite
         (those that do not exist: -inf) or with a NaN or +inf among their logits have none,
         tokens of -inf logits cannot be chosen; where there are fewer than k, the rest is

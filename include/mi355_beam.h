@@ -90,9 +90,10 @@ size_t mi355_shared_decode_workspace_bytes(const mi355_shared_params* p);
 /*
  * The selection of a step of beam search. Of n_groups searches of `beams` beams each:
  *   s[w, v] = scores[w] + x[w, v] − log Σ_v exp x[w, v]
- * formed in 64 bits, and of its beams·vocab values the k largest, in descending order,
- * the lowest w·vocab + v first among equals: their scores (rounded to 32 bits), tokens v
- * and parents g·beams + w. Candidates of one beam are in the order of their logits. A
+ * formed in 64 bits, and of its beams·vocab values the k largest, in descending order; among
+ * equals the lowest w first, of one w the largest logit, then the lowest v: their scores
+ * (rounded to 32 bits), tokens v and parents g·beams + w. So candidates of one beam are in
+ * the order of their logits, also where the score's 64 bits do not tell them apart. A
  * beam that is finished has one candidate, its own score with the token eos. A beam with
  * a score that is not finite, or whose logits hold a NaN or +infinity, has none; nor
  * has a logit of −infinity. Behind the candidates there are, outputs hold −infinity, −1 and −1.
