@@ -81,16 +81,16 @@ struct Share {
   OwnTiles own;    // a group's tiles: own.first + i
 };
 
-constexpr int kShWords = 7 * kShMax + 2 + 64;
+constexpr int kShWords = 8 * kShMax + 2 + 64;
 
 // The plan, by T threads (one wave, where all have little to do: no barriers). LDS: s, of
 // kShWords. Units of groups have parts that take a workgroup each; behind them come the
 // requests' own, four to a workgroup. What workgroup w holds is left in s[0 ..]: see share_of.
 struct PlanLds {
-  int *acc, *len_of, *group_of, *least_of, *most_of, *members, *prefix, *cu;
+  int *acc, *len_of, *group_of, *least_of, *most_of, *members, *prefix, *leader, *cu;
   __device__ __forceinline__ explicit PlanLds(int* s)
       : acc(s), len_of(s + 64), group_of(len_of + kShMax), least_of(group_of + kShMax), most_of(least_of + kShMax), members(most_of + kShMax),
-        prefix(members + kShMax), cu(prefix + kShMax) {}
+        prefix(members + kShMax), leader(prefix + kShMax), cu(leader + kShMax) {}
 };
 template <int T> __device__ __forceinline__ void find_share(const SharedArgs& a, int w, int* s) {
   constexpr bool SOLO = T == 64;
@@ -151,16 +151,37 @@ template <int T> __device__ __forceinline__ void find_share(const SharedArgs& a,
   };
   const int own_units = a.hk * a.groups, weight = own_weight(a.columns);
   int64_t sum = 0;
-  for (int g = tid; g < a.n_groups; g += T) {
-    const int c0 = l.cu[g], c1 = min(l.cu[g + 1], a.b);
-    TileSpan t{0, 0};
-    // (offsets that do not ascend: a group that lacks some of its rows shares nothing, so
-    // that groups are apart and the parts fit the grid)
-    if (c0 >= 0 && c0 < c1 && l.members[g] == c1 - c0 && l.most_of[g] > 0)
-      t = shared_tiles(l.prefix[g], l.least_of[g], l.most_of[g], a.window, c1 - c0);
-    l.least_of[g] = t.t0;
-    l.most_of[g] = t.t1;
-    if (t.t1 > t.t0) sum += (int64_t)(t.t1 - t.t0) * units_of(g) * (a.columns / 32);
+  for (int e = wave * 64; e < a.n_groups; e += T) {
+    const int g = e + lane;
+    bool ended = false;   // the first request, and not all
+    if (g < a.n_groups) {
+      const int c0 = l.cu[g], c1 = min(l.cu[g + 1], a.b);
+      TileSpan t{0, 0};
+      // (offsets that do not ascend: a group that lacks some of its rows shares nothing, so
+      // that groups are apart and the parts fit the grid)
+      if (c0 >= 0 && c0 < c1 && l.members[g] == c1 - c0 && l.most_of[g] > 0)
+        t = shared_tiles(l.prefix[g], l.least_of[g], l.most_of[g], a.window, c1 - c0);
+      ended = l.most_of[g] > 0 && l.len_of[c0] == 0;
+      l.leader[g] = c0;
+      l.least_of[g] = t.t0;
+      l.most_of[g] = t.t1;
+      if (t.t1 > t.t0) sum += (int64_t)(t.t1 - t.t0) * units_of(g) * (a.columns / 32);
+    }
+    // The row that names the prefix is then the first that has keys or a page: an ended
+    // request's may be kept for the prefix, but a fork leaves it empty.
+#pragma unroll 1
+    for (uint64_t left = __builtin_amdgcn_ballot_w64(ended); left; left &= left - 1) {
+      const int which = e + __builtin_ctzll(left), c0 = l.cu[which], c1 = min(l.cu[which + 1], a.b);
+#pragma unroll 1
+      for (int i0 = c0; i0 < c1; i0 += 64) {
+        const int i = min(i0 + lane, c1 - 1);
+        const uint64_t named = __builtin_amdgcn_ballot_w64(l.len_of[i] > 0 || (uint32_t)a.table[(int64_t)i * a.ts] < (uint32_t)a.pages);
+        if (named) {
+          if (lane == 0) l.leader[which] = min(i0 + __builtin_ctzll(named), c1 - 1);
+          break;
+        }
+      }
+    }
   }
   meet();
   int* counts = l.members;
@@ -249,7 +270,8 @@ __device__ __forceinline__ Share group_share(const SharedArgs& a, int* s) {
   const int t0 = uni(l.least_of[g]), t = uni(l.most_of[g]) - t0;
   const UnitPart at = unit_part(place, n, a.hk, blocks);
   sh.kind = 1;
-  sh.b = sh.leader = c0;
+  sh.b = c0;
+  sh.leader = uni(l.leader[g]);
   sh.hk = at.hk;
   sh.col0 = at.block * a.columns;
   sh.cols = min(a.columns, total - sh.col0);
@@ -289,7 +311,7 @@ __device__ __forceinline__ bool own_share(const SharedArgs& a, int* s, Walk& w, 
   const TileSpan sp = g >= 0 ? TileSpan{uni(l.least_of[g]), uni(l.most_of[g])} : TileSpan{0, 0};
   sh.kind = 2;
   sh.b = w.b;
-  sh.leader = g >= 0 ? uni(l.cu[g]) : w.b;
+  sh.leader = g >= 0 ? uni(l.leader[g]) : w.b;
   sh.hk = (int)((uint32_t)unit / (uint32_t)a.groups);
   sh.col0 = (unit - sh.hk * a.groups) * 16;
   sh.cols = min(16, a.ratio - sh.col0);

@@ -323,9 +323,10 @@ class RecsysOps:
         """``mha_paged_decode`` for requests that share prefixes, which are read once for all.
 
         Requests cu_groups[g] .. cu_groups[g+1]-1 (int32 [G+1], ascending) have their first
-        prefix_lens[g] (int32 [G]) keys in common: in the pages that block_table's row
-        cu_groups[g] names, whatever the others' rows have there. Requests of no group
-        attend to their own keys. At most 1024 requests. Other arguments and the result
+        prefix_lens[g] (int32 [G]) keys in common: in the pages that block_table's row of the
+        first of them names, whatever the others' rows have there. (Rows without a key and
+        without a page in the first column, as ``paged_fork`` leaves those of ended requests,
+        are passed over.) Requests of no group attend to their own keys. At most 1024 requests. Other arguments and the result
         are those of ``mha_paged_decode``."""
         return self._beam(backend).mha_shared_decode(q, k_cache, v_cache, block_table, kv_lens, cu_groups, prefix_lens, scale, softcap,
                                                      window, slopes)

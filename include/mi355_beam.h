@@ -40,8 +40,10 @@ enum { MI355_BEAM_FP16 = 0, MI355_BEAM_BF16 = 1, MI355_BEAM_FP32 = 2 };
 /*
  * Attention of one new token per request over a paged cache, of which requests share
  * prefixes. Requests cu_groups[g] .. cu_groups[g+1]-1 are group g (offsets ascend); the
- * first prefix_lens[g] keys of each are those that block_table's row cu_groups[g] names,
- * its others those of its own row. Requests of no group have no prefix. Key j is row
+ * first prefix_lens[g] keys of each are those that block_table's row of its first request
+ * names, its others those of its own row. (First of those that have keys, or a page of the
+ * cache in their row's first column: a row that mi355_paged_fork left empty is passed
+ * over.) Requests of no group have no prefix. Key j is row
  * j % page_size of page table[j / page_size], j < kv_lens[n]; a request's row is at its
  * last key, len - 1. Scores of key j:
  *   s = scale·q·k_j
