@@ -12,6 +12,12 @@
 
 namespace mi355fa {
 
+// ── shared decode: the plan in LDS ────────────────────────────────────────────
+constexpr int kShMax = 1024;   // requests, and groups
+// Its words: 64 of its own, eight of each request or group (one more of the offsets), in whole 16
+// bytes, since the waves' rows of V lie behind it.
+constexpr int kShWords = (64 + 8 * kShMax + 1 + 3) / 4 * 4;
+
 // ── shared decode: what a group reads once, and what is left to its requests ──
 // Tiles of kDecTile keys that every request of a group sees whole: inside the prefix,
 // of the shortest request's keys, from the longest one's window on. `least` and `most`:

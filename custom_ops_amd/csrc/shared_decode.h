@@ -32,7 +32,6 @@
 
 constexpr int kShWaves = 4;
 constexpr int kShThreads = 64 * kShWaves;
-constexpr int kShMax = 1024;                   // requests, and groups
 
 struct SharedArgs {
   const uint16_t* q;
@@ -80,8 +79,6 @@ struct Share {
   int alone;       // the request's only part
   OwnTiles own;    // a group's tiles: own.first + i
 };
-
-constexpr int kShWords = 8 * kShMax + 2 + 64;
 
 // The plan, by T threads (one wave, where all have little to do: no barriers). LDS: s, of
 // kShWords. Units of groups have parts that take a workgroup each; behind them come the
@@ -861,7 +858,8 @@ void shared_decode_kernel(const SharedArgs a) {
     for (int i = 0; i < (int)(sizeof(Share) / 4); ++i) x.x[i] = uni(reinterpret_cast<const int*>(&shares[wave])[i]);
     return bitcast<Share>(x);
   };
-  uint8_t* slices = lds + kShWords * 4;
+  uint8_t* slices = lds + kShWords * 4;   // (behind the plan, which the streams go on reading)
+  static_assert(kShWords * 4 % 16 == 0 && Stream<D, BF16>::kSlice % 16 == 0, "rows of V are stored 16 bytes at a time");
   const int parts = uni(words[16]), number = ((int)blockIdx.x - parts) * kShWaves + wave;
   if (number >= 0) {
     Walk at{uni(words[4 * wave]) - 1, uni(words[4 * wave + 1]), uni(words[17]), number};
