@@ -34,6 +34,7 @@ namespace {
 static_assert(kShMax == MI355_BEAM_MAX_REQUESTS && kPgRows == MI355_BEAM_MAX_ROWS, "limits of the C ABI");
 constexpr int kMaxKeys = 1 << 30;
 constexpr int64_t kMaxRowStride = 1 << 24;
+constexpr int64_t kMaxGrid = 1 << 24;   // workgroups of 256 threads
 
 int device_ok(const Err& err, Device* dev) {
   *dev = device_info();
@@ -85,6 +86,11 @@ SharedPlan shared_plan(const mi355_shared_params* p, int cus) {
   return pl;
 }
 
+// Whether the launches take it (they count their threads in 32 bits), and rows of sums fit theirs.
+bool shared_fits(const mi355_shared_params* p, const SharedPlan& pl) {
+  return pl.rows <= INT_MAX && pl.grid < kMaxGrid && (int64_t)p->b * p->h < 4 * (kMaxGrid - 1);
+}
+
 int shared_check(const mi355_shared_params* p, const Err& err) {
   if (!p) return err.fail(kEinval, "params must not be NULL");
   if (int rc = check_heads(err, p->h, p->h_k, p->d, p->dtype)) return rc;
@@ -120,7 +126,7 @@ int shared_decode(const mi355_shared_params* p, hipStream_t st, const Err& err) 
   Device dev;
   if (int rc = device_ok(err, &dev)) return rc;
   const SharedPlan pl = shared_plan(p, dev.cus);
-  if (pl.rows > INT_MAX) return err.fail(kEinval, "too many requests and heads");
+  if (!shared_fits(p, pl)) return err.fail(kEinval, "too many requests, groups and heads");
   if (int rc = workspace_ok(err, p->workspace, p->workspace_bytes, pl.bytes)) return rc;
   a.q = (const uint16_t*)p->q; a.k = (const uint16_t*)p->k_cache; a.v = (const uint16_t*)p->v_cache; a.o = (uint16_t*)p->o;
   a.table = p->block_table; a.lens = p->kv_lens; a.cu = p->cu_groups; a.prefix = p->prefix_lens; a.slopes = p->slopes;
@@ -174,8 +180,8 @@ int select_check(const mi355_select_params* p, const Err& err) {
   if (p->dtype != MI355_BEAM_FP16 && p->dtype != MI355_BEAM_BF16 && p->dtype != MI355_BEAM_FP32)
     return err.fail(kEinval, "logits must be float16, bfloat16 or float32");
   if (p->n_groups < 0 || p->beams < 1 || p->beams > kSelMaxBeams) return err.fail(kEinval, "beams must be in 1 .. %d", kSelMaxBeams);
-  if (p->vocab < 1 || (int64_t)p->vocab * p->beams > INT_MAX || (int64_t)p->n_groups * p->beams > INT_MAX)
-    return err.fail(kEinval, "vocab must be positive, and beams·vocab and n_groups·beams below 2^31");
+  if (p->vocab < 1 || (int64_t)p->vocab * p->beams > INT_MAX || (int64_t)p->n_groups * p->beams >= kMaxGrid)
+    return err.fail(kEinval, "vocab must be positive, beams·vocab below 2^31 and n_groups·beams below 2^24");
   if (p->k < 1 || p->k > kSelMaxK) return err.fail(kEinval, "k must be in 1 .. %d", kSelMaxK);
   if (p->finished && (p->eos < 0 || p->eos >= p->vocab)) return err.fail(kEinval, "eos must be a token of the vocabulary");
   if (p->group_stride < 0 || p->beam_stride < 0) return err.fail(kEinval, "logits' strides must not be negative");
@@ -335,7 +341,8 @@ int mi355_shared_decode(const mi355_shared_params* p, void* stream, char* err, s
 }
 size_t mi355_shared_decode_workspace_bytes(const mi355_shared_params* p) {
   if (mi355fa::shared_check(p, {nullptr, 0}) || p->b == 0 || p->h == 0) return 0;
-  return mi355fa::shared_plan(p, mi355fa::device_info().cus).bytes;
+  const mi355fa::SharedPlan pl = mi355fa::shared_plan(p, mi355fa::device_info().cus);
+  return mi355fa::shared_fits(p, pl) ? pl.bytes : 0;
 }
 
 int mi355_beam_select(const mi355_select_params* p, void* stream, char* err, size_t errlen) {

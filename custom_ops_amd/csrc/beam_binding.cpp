@@ -98,7 +98,7 @@ std::tuple<Tensor, Tensor, Tensor> beam_select(const Tensor& logits, const Tenso
   TORCH_CHECK(logits.dim() == 3, "logits must be 3D (searches, beams, vocabulary)");
   const int64_t G = logits.size(0), W = logits.size(1), V = logits.size(2);
   TORCH_CHECK(W >= 1 && W <= 256, "beams must be in 1 .. 256");
-  TORCH_CHECK(V >= 1 && V <= INT_MAX / W && G <= INT_MAX / W, "the vocabulary must not be empty, and beams·vocabulary and searches·beams below 2^31");
+  TORCH_CHECK(V >= 1 && V <= INT_MAX / W && G < ((1 << 24) + W - 1) / W, "the vocabulary must not be empty, beams·vocabulary below 2^31 and searches·beams below 2^24");
   TORCH_CHECK(V == 1 || logits.stride(2) == 1, "logits must have an innermost stride of 1");
   check_gpu(scores, logits, "scores");
   TORCH_CHECK(scores.scalar_type() == at::kFloat, "scores must be float32");

@@ -56,7 +56,8 @@ enum { MI355_BEAM_FP16 = 0, MI355_BEAM_BF16 = 1, MI355_BEAM_FP32 = 2 };
  * 8 elements, the caches' row strides below 2^24. A page number outside the cache hides
  * that page's keys; kv_lens and prefix_lens past table_cols·page_size (2^30 at most) count
  * as that. Tiles of 32 keys that a table spans, for each KV head and 16 of its heads: at
- * most 2^30 of a request and 2^35 of all.
+ * most 2^30 of a request and 2^35 of all. Workgroups are counted: b·h stays below
+ * 2^26, and h_k·n_groups + b·h / 32 about below 2^24.
  */
 typedef struct mi355_shared_params {
   const void* q;
@@ -109,7 +110,7 @@ typedef struct mi355_select_params {
   int32_t* out_tokens;
   int32_t* out_parents;
   int64_t group_stride, beam_stride; /* of logits, in elements, not negative */
-  int32_t n_groups, beams, vocab, k; /* beams 1 .. 256, k 1 .. 64; beams·vocab, n_groups·beams < 2^31 */
+  int32_t n_groups, beams, vocab, k; /* beams 1 .. 256, k 1 .. 64; beams·vocab < 2^31, n_groups·beams < 2^24 */
   int32_t eos;                /* 0 .. vocab − 1 where finished is given */
   int32_t dtype;
   void* workspace;            /* device memory, 16-byte aligned; contents need no clearing */
