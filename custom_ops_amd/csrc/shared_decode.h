@@ -142,10 +142,6 @@ template <int T> __device__ __forceinline__ void find_share(const SharedArgs& a,
   }
   meet();
   auto units_of = [&](int g) { return a.hk * (((min(l.cu[g + 1], a.b) - l.cu[g]) * a.ratio + a.columns - 1) >> a.col_shift); };
-  auto own_count = [&](int b) {
-    const int g = l.group_of[b];
-    return own_tiles(l.len_of[b], a.window, g >= 0 ? TileSpan{l.least_of[g], l.most_of[g]} : TileSpan{0, 0}).count;
-  };
   const int own_units = a.hk * a.groups, weight = own_weight(a.columns);
   int64_t sum = 0;
   for (int e = wave * 64; e < a.n_groups; e += T) {
@@ -591,7 +587,7 @@ __device__ __forceinline__ bool group_part(kernarg<SharedArgs>& a, const Share& 
   const bool two = RPL == 8 && a.shift < 5;          // K's loads reach into two pages
   // Offsets of the lane from where the tile starts in a page (of fewer than 32 rows: from the page)
   const int in_page = page_size - 1;
-    uint32_t k_off[kLoads], v_off[kLoads];
+  uint32_t k_off[kLoads], v_off[kLoads];
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
     const int r = rw * R + i * RPL;
