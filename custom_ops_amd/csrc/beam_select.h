@@ -14,15 +14,18 @@
 //    from the lanes' maxima, by bisecting bits with ballots; waves tell each other theirs, and
 //    only elements that reach it are listed.
 //  * The next step's logits are in flight while a step computes.
-//  * bf16 logits are counted by value and their exponentials taken once a value.
+//  * bf16 logits of long parts are counted by value and their exponentials taken once a value.
+//    (Eight logits of which one is 0, below 2^-10, 64 or more, or −infinity go one after the other.)
 //  * A second kernel, a workgroup a search, joins the parts' sums and lists: all
 //    candidates in registers, a bound by bisection in each wave, and the few that reach it
 //    ranked by counting.
 //  * Equal scores: a row's candidates stay in the order of their logits, so that what a part keeps
 //    and what the join takes are the same order, and results do not depend on the split.
-// Measured in a graph: one search of 4 beams, 32000 tokens, bf16: 9.6 us (scan 5.6, join 4.3);
-// 4 of 50 beams, k 50, 10007 tokens, fp32: 26; 64 of 8, k 16, 128000 tokens, bf16: 60, of which the
-// scan 57 for 131 MB (2.3 TB/s): counting and listing, not the bytes.
+// Measured in a graph: one search of 4 beams, 32000 tokens, bf16: 9.4 us (scan 5.5, join 4.0);
+// 128000 tokens 13.0, of which the join has 1008 candidates; 4 of 50 beams, k 50, 10007 tokens,
+// fp32: 26; 64 of 8, k 16, 128000 tokens, bf16: 60, of which the scan 57 for 131 MB (2.3 TB/s):
+// counting and listing, not the bytes. Of that size, normal logits 63 us in bf16, 65 in fp16, 69 in
+// fp32; a tenth of them −infinity 116, 66, 70; all equal 331, 216, 151 (one bin; all listed).
 
 constexpr int kSelWave = 256;       // of a wave's
 constexpr int kSelMaxK = 64;

@@ -326,8 +326,11 @@ class RecsysOps:
         prefix_lens[g] (int32 [G]) keys in common: in the pages that block_table's row of the
         first of them names, whatever the others' rows have there. (Rows without a key and
         without a page in the first column, as ``paged_fork`` leaves those of ended requests,
-        are passed over.) Requests of no group attend to their own keys. At most 1024 requests. Other arguments and the result
-        are those of ``mha_paged_decode``."""
+        are passed over.) Requests of no group attend to their own keys. Read once is what
+        all requests of a group with keys see: a single one shorter than the prefix leaves the
+        rest of it to each. Groups that share nothing are ``mha_paged_decode``'s, which is faster
+        there. At most 1024 requests. Other arguments and the result are those of
+        ``mha_paged_decode``."""
         return self._beam(backend).mha_shared_decode(q, k_cache, v_cache, block_table, kv_lens, cu_groups, prefix_lens, scale, softcap,
                                                      window, slopes)
 

@@ -43,7 +43,9 @@ enum { MI355_BEAM_FP16 = 0, MI355_BEAM_BF16 = 1, MI355_BEAM_FP32 = 2 };
  * first prefix_lens[g] keys of each are those that block_table's row of its first request
  * names, its others those of its own row. (First of those that have keys, or a page of the
  * cache in their row's first column: a row that mi355_paged_fork left empty is passed
- * over.) Requests of no group have no prefix. Key j is row
+ * over.) Requests of no group have no prefix. What is read once is the part of the prefix
+ * that all requests of the group with keys see: one that is shorter than the prefix, or a
+ * window that ends inside it, leaves the rest to each. Key j is row
  * j % page_size of page table[j / page_size], j < kv_lens[n]; a request's row is at its
  * last key, len - 1. Scores of key j:
  *   s = scale·q·k_j
