@@ -147,39 +147,28 @@ template <int T> __device__ __forceinline__ void find_share(const SharedArgs& a,
   auto units_of = [&](int g) { return a.hk * (((min(l.cu[g + 1], a.b) - l.cu[g]) * a.ratio + a.columns - 1) >> a.col_shift); };
   const int own_units = a.hk * a.groups, weight = own_weight(a.columns);
   int64_t sum = 0;
-  for (int e = wave * 64; e < a.n_groups; e += T) {
-    const int g = e + lane;
-    bool ended = false;   // the first request, and not all
-    if (g < a.n_groups) {
-      const int c0 = l.cu[g], c1 = min(l.cu[g + 1], a.b);
-      TileSpan t{0, 0};
-      // (offsets that do not ascend: a group that lacks some of its rows shares nothing, so
-      // that groups are apart and the parts fit the grid)
-      if (c0 >= 0 && c0 < c1 && l.members[g] == c1 - c0 && l.most_of[g] > 0)
-        t = shared_tiles(l.prefix[g], l.least_of[g], l.most_of[g], a.window, c1 - c0);
-      ended = l.most_of[g] > 0 && l.len_of[c0] == 0;
-      l.leader[g] = c0;
-      l.least_of[g] = t.t0;
-      l.most_of[g] = t.t1;
-      if (t.t1 > t.t0) sum += (int64_t)(t.t1 - t.t0) * units_of(g) * (a.columns / 32);
-    }
-    // The row that names the prefix is then the first that has keys or a page: an ended
-    // request's may be kept for the prefix, but a fork leaves it empty.
-#pragma unroll 1
-    for (uint64_t left = __builtin_amdgcn_ballot_w64(ended); left; left &= left - 1) {
-      const int which = e + __builtin_ctzll(left), c0 = l.cu[which], c1 = min(l.cu[which + 1], a.b);
-#pragma unroll 1
-      for (int i0 = c0; i0 < c1; i0 += 64) {
-        const int i = min(i0 + lane, c1 - 1);
-        const uint64_t named = __builtin_amdgcn_ballot_w64(l.len_of[i] > 0 || (uint32_t)a.table[(int64_t)i * a.ts] < (uint32_t)a.pages);
-        if (named) {
-          if (lane == 0) l.leader[which] = min(i0 + __builtin_ctzll(named), c1 - 1);
-          break;
-        }
-      }
-    }
+  for (int g = tid; g < a.n_groups; g += T) {
+    const int c0 = l.cu[g], c1 = min(l.cu[g + 1], a.b);
+    TileSpan t{0, 0};
+    // (offsets that do not ascend: a group that lacks some of its rows shares nothing, so
+    // that groups are apart and the parts fit the grid)
+    if (c0 >= 0 && c0 < c1 && l.members[g] == c1 - c0 && l.most_of[g] > 0)
+      t = shared_tiles(l.prefix[g], l.least_of[g], l.most_of[g], a.window, c1 - c0);
+    const bool ended = l.most_of[g] > 0 && l.len_of[c0] == 0;   // the first request, and not all
+    l.leader[g] = ended ? INT_MAX : c0;
+    if (ended) l.acc[36] = 1;
+    l.least_of[g] = t.t0;
+    l.most_of[g] = t.t1;
+    if (t.t1 > t.t0) sum += (int64_t)(t.t1 - t.t0) * units_of(g) * (a.columns / 32);
   }
   meet();
+  // The row that names such a group's prefix is the first that has keys or a page: an ended
+  // request's may be kept for the prefix, but a fork leaves it empty.
+  if (uni(l.acc[36]))
+    for (int i = tid; i < a.b; i += T) {
+      const int g = l.group_of[i];
+      if (g >= 0 && l.len_of[l.cu[g]] == 0 && (l.len_of[i] > 0 || (uint32_t)a.table[(int64_t)i * a.ts] < (uint32_t)a.pages)) atomicMin(&l.leader[g], i);
+    }
   int* counts = l.members;
   for (int b = tid; b < a.b; b += T) {
     const int g = l.group_of[b], n = own_tiles(l.len_of[b], a.window, g >= 0 ? TileSpan{l.least_of[g], l.most_of[g]} : TileSpan{0, 0}).count;

@@ -89,3 +89,22 @@ def test_a_fork_that_ends_the_first(ops):
         want, tol = ref.shared(q, kc, vc, table, lens.tolist(), [0], [])
         check(out, want, tol)
         assert [bool((o != 0).any()) for o in out] == [p >= 0 for p in parents]
+
+
+def test_replays_as_requests_end(ops):
+    """One captured call, replayed as requests end one after the other, with eager calls between."""
+    x = batch(8, [(200, 4), (90, 3)], 40, 8, 2, 64, 16, torch.bfloat16)
+    lens, cu, prefix = ints(x["lens"]), ints(x["cu"]), ints(x["prefix"])
+    args = (x["q"], x["kc"], x["vc"], x["table"], lens, cu, prefix)
+    ops.mha_shared_decode(*args)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = ops.mha_shared_decode(*args)
+    for row in (None, 0, 4, 1, 6, 2):
+        if row is not None:
+            end(x, [row])
+            lens.copy_(ints(x["lens"]))
+        graph.replay()
+        got = held.clone()
+        assert torch.equal(got, run(ops, x))
+        torch.cuda.synchronize()
